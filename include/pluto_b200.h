@@ -57,7 +57,8 @@ const char* pluto_build_info(void);
  * their bounded waits ran out.  SYNCHRONISES the device.  *value == 0 means healthy; otherwise
  * (site << 8) | kind with kind 1 = a bounded wait ran out, 2 = a device-side sequence length lay
  * outside the declared bound, 3 = a block-table entry lay outside the page pool, 4 = a kernel found
- * its dynamic shared memory off the boundary it needs (it returns without computing). */
+ * its dynamic shared memory off the boundary it needs (it returns without computing), 5 = a drafted
+ * token, a parent or an accepted path was out of range. */
 int pluto_kernel_status(uint32_t* value /* host */, int clear);
 
 /* Diagnostic with no counterpart in the reference: proves on the running GPU that a bounded wait
@@ -352,6 +353,126 @@ int pluto_cached_attention_step(pluto_stream_t stream, const void* q_gate, const
                                 int out_dtype, void* workspace, size_t workspace_bytes, int q_heads,
                                 int kv_heads, int head_dim, int rotary_dim, float rms_norm_epsilon,
                                 float rope_theta, int round_to_bf16);
+
+/* --------------------------------------------------------------------------------------------
+ * Decoding with drafted tokens (speculative decoding), and an 8-bit key/value cache.  The reference decodes
+ * one token at a time over an fp32 cache (src/llm/key_value_cache.h:25-57,
+ * src/llm/layers/util/cached_attention_ops.cc:308-353) and has no counterpart; names, addressing and rounding
+ * points follow pluto_qk_prepare and pluto_gqa_decode.  A step for sequences with prefix_lens[b] cached tokens:
+ *
+ *   pluto_draft_prepare     norm + RoPE of the drafts, their K/V rows to slots prefix_lens[b] + i
+ *   pluto_gqa_tree_decode   every draft attends to the cached tokens, its ancestors and itself
+ *   pluto_verify_drafts     accepts a path of the tree and draws one more token
+ *   pluto_kv_keep           moves the path's rows to the first slots; the caller adds the path's length to
+ *                           prefix_lens
+ *
+ * Drafts.  Every sequence has up to `nodes` <= 128 drafted tokens; node i is the child of parents[b][i] < i, or
+ * of the last cached token where that is -1.  parents NULL: a chain, node i the child of i - 1.  counts
+ * (optional, device int32 [batch]): sequence b has nodes 0 .. counts[b] - 1; outputs of the others are left as
+ * they were and nothing of theirs is read.  prefix_lens: device int32 [batch], each >= 0.
+ * Contents of device arrays that are out of range (a negative length or one beyond the declared bound, a slot
+ * past the sequence's pages, a page outside the pool, a parent >= i, a token >= vocab, a path that does not
+ * rise) never lead to an access out of bounds: they are reported through pluto_kernel_status (kinds 2, 3, 5) and
+ * the length is clamped, the row reads as absent, the write or move is left out, the parent taken as -1, the
+ * token refused.
+ *
+ * Caches.  One page pool per layer as in pluto_kv_cache, contiguous (page = sequence) or through a block table
+ * (num_pages must then be given); k_bases / v_bases are PLUTO_E_UNIMPLEMENTED.  dtype may be PLUTO_FP32,
+ * PLUTO_BF16 or, for the functions of this section, PLUTO_E4M3: one byte per element (strides stay in
+ * elements) and one scale byte per (token, head) row in `scales`, at element
+ *     page * page_stride + (t % page_size) * token_stride + head        (strides of pluto_kv_scales)
+ * A row x is stored with the smallest n >= -127 for which max|x| <= 448 * 2^n: scale byte n + 127 (E8M0), codes
+ * the E4M3 values nearest to x * 2^-n (ties to even).  Every value read back is exact in bf16.  A row that
+ * holds an infinity or a NaN gets scale byte 255 and reads back as NaN.  `scales` is NULL for the other two. */
+enum { PLUTO_E4M3 = 2 };
+typedef struct pluto_kv_scales {
+  uint8_t* k; /* device */
+  uint8_t* v;
+  size_t page_stride;  /* elements */
+  size_t token_stride; /* elements, >= kv_heads */
+} pluto_kv_scales;
+
+/* Writes rows of keys and values into an 8-bit cache (the append of src/llm/layers/util/cached_attention_ops.cc:73-78
+ * for this storage).  k, v: [batch, tokens, kv_heads, head_dim], fp32 or bf16, element strides for batch, token and
+ * head, head rows contiguous.  Token t of sequence b goes to slot positions[b] + t (NULL: t); counts (optional
+ * [batch]) as above, any number of tokens.  head_dim <= 256. */
+int pluto_kv8_append(pluto_stream_t stream, const void* k, const void* v, int dtype, size_t batch_stride,
+                     size_t token_stride, size_t head_stride, const pluto_kv_cache* cache /* host */,
+                     const pluto_kv_scales* scales /* host */, const int32_t* positions,
+                     const int32_t* counts, int batch, int tokens, int kv_heads, int head_dim);
+/* Reads rows of an 8-bit cache back as the values they hold; arguments as pluto_kv8_append with k, v the
+ * destination, whose rows must not overlap (the fp32 rows that src/llm/key_value_cache.h:25-57 stores). */
+int pluto_kv8_read(pluto_stream_t stream, void* k, void* v, int dtype, size_t batch_stride,
+                   size_t token_stride, size_t head_stride, const pluto_kv_cache* cache /* host */,
+                   const pluto_kv_scales* scales /* host */, const int32_t* positions,
+                   const int32_t* counts, int batch, int tokens, int kv_heads, int head_dim);
+
+/* After a verification (in the place of KeyValueCache::Advance, src/llm/key_value_cache.h:25-57): for i < accepted[b] the key and value rows (and scales) of slot prefix_lens[b] +
+ * path[b][i] move to slot prefix_lens[b] + i, in place; path is int32 [batch, nodes], rising, accepted int32
+ * [batch] in [0, nodes].  Every other slot keeps its rows.  Any of the three storage types. */
+int pluto_kv_keep(pluto_stream_t stream, const pluto_kv_cache* cache /* host */,
+                  const pluto_kv_scales* scales /* host */, const int32_t* prefix_lens, const int32_t* path,
+                  const int32_t* accepted, int batch, int nodes, int kv_heads, int head_dim);
+
+/* pluto_qk_prepare (src/llm/layers/util/cached_attention_ops.cc:30-79) for drafted tokens: q_in, k_in, v_in as there with tokens = nodes.  Node i of sequence b is
+ * rotated for position prefix_lens[b] + (number of its ancestors) and its K/V row goes to slot
+ * prefix_lens[b] + i of a cache of any storage type; queries and rows are those of pluto_qk_prepare bit for
+ * bit (8-bit rows: those of pluto_kv8_append of them).  parents NULL (a chain, or a prompt): any number of
+ * tokens; prefix_lens NULL: 0. */
+int pluto_draft_prepare(pluto_stream_t stream, const void* q_in, const void* k_in, const void* v_in,
+                        int in_dtype, size_t q_token_stride, size_t q_head_stride, const float* q_norm,
+                        const float* k_norm, const int32_t* prefix_lens, const int32_t* parents,
+                        const int32_t* counts, void* q_out, int q_out_dtype,
+                        const pluto_kv_cache* cache /* host */, const pluto_kv_scales* scales /* host */,
+                        int batch, int nodes, int q_heads, int kv_heads, int head_dim, int rotary_dim,
+                        float rms_norm_epsilon, float rope_theta, int round_to_bf16);
+
+/* Attention of the drafts over the cache (FullAttentionKernel, src/llm/layers/util/cached_attention_ops.cc:83-126, for
+ * several new tokens at once): out(i, h) = sum_t softmax(q(i, h) . k(t) / sqrt(head_dim)) v(t) over the
+ * slots t < prefix_lens[b] and those of node i's ancestors and of node i itself; then the output stage of
+ * pluto_gqa_decode (gate optional).  One node per sequence is pluto_gqa_decode with seq_lens = prefix_lens + 1.
+ *   q            [batch, nodes, q_heads, head_dim] prepared queries (q_dtype)
+ *   gate         optional; element (b, i, h, d) at gate + (b * nodes + i) * gate_token_stride + h *
+ *                gate_head_stride + d
+ *   max_prefix_len  host upper bound of prefix_lens
+ *   out          [batch, nodes, q_heads, head_dim] (out_dtype);  lse optional fp32 [batch, nodes, q_heads]
+ *   workspace    >= pluto_gqa_tree_decode_workspace_bytes(...) bytes, 16-byte aligned; overwritten, so calls that
+ *                share one are ordered on one stream
+ * What a node does not see does not reach its output, whatever it holds; a node that sees a row with an
+ * infinity or a NaN gets NaN.
+ * bf16 queries with a bf16 result over a bf16 or 8-bit cache, head_dim 64, 128 or 256, rows on 16-byte
+ * boundaries, run on the tensor cores (probabilities enter P V as bf16); everything else in fp32 arithmetic. */
+size_t pluto_gqa_tree_decode_workspace_bytes(int batch, int nodes, int q_heads, int kv_heads, int head_dim);
+int pluto_gqa_tree_decode(pluto_stream_t stream, const void* q, int q_dtype, const void* gate, int gate_dtype,
+                          size_t gate_token_stride, size_t gate_head_stride,
+                          const pluto_kv_cache* cache /* host */, const pluto_kv_scales* scales /* host */,
+                          const int32_t* prefix_lens, int max_prefix_len, const int32_t* parents,
+                          const int32_t* counts, void* out, int out_dtype, float* lse, void* workspace,
+                          size_t workspace_bytes, int batch, int nodes, int q_heads, int kv_heads,
+                          int head_dim, int round_to_bf16);
+
+/* Accepts drafted tokens against the target model's probabilities, and draws one more, from given uniform numbers
+ * in [0, 1).  (One node more than the reference's one token per step, src/llm/layers/util/cached_attention_ops.cc:308-353,
+ * is what the other functions of this section allow; which of them stay is decided here.)
+ *   target_probs [batch, nodes + 1, vocab] (dtype): row 0 follows the last cached token, row i + 1 follows node i
+ *   draft_probs  optional, chains only: row i of [batch, nodes, vocab] is what token i was drawn from; NULL:
+ *                the drafts were given, not drawn
+ *   tokens       int32 [batch, nodes];  accept_uniforms fp32 [batch, nodes];  sample_uniforms fp32 [batch]
+ * Chain: token i is accepted, if all before it were, when u_i * q(x_i) < p(x_i) (q = 1 without draft_probs); the
+ * first refused one leaves max(p - q, 0) to draw the last token from (without draft_probs: p without it).
+ * Tree: the children of the last accepted node are tried in index order; child c is accepted when
+ * u_c * (1 - sum of p over the siblings tried before it) < p(x_c), a token that was tried before never; when
+ * none is left the last token is drawn from p without the tried tokens.  After a leaf it is drawn from p.  Where
+ * nothing is left to draw from, from p itself.
+ * The drawn token is the smallest x whose running sum exceeds u * total.  Tests and sums are in double.
+ *   accepted     int32 [batch]: length of the path;  path int32 [batch, nodes]: its nodes, then -1
+ *   out_tokens   int32 [batch, nodes + 1]: the path's tokens, the drawn token (-1 where the row's sum is not
+ *                positive and finite), then -1
+ * vocab <= 1048576. */
+int pluto_verify_drafts(pluto_stream_t stream, const void* target_probs, const void* draft_probs, int dtype,
+                        const int32_t* tokens, const float* accept_uniforms, const float* sample_uniforms,
+                        const int32_t* parents, const int32_t* counts, int32_t* accepted, int32_t* path,
+                        int32_t* out_tokens, int batch, int nodes, int vocab);
 
 /* --------------------------------------------------------------------------------------------
  * Gated delta-net.

@@ -72,6 +72,14 @@ _SIGNATURES = {
     "pluto_gdn_token_step_scratch_bytes": (_sz, [_i] * 4),
     "pluto_gdn_token_step": (_i, [_vp, _vp, _i, _vp, _i, _vp, _vp, _i] + [_vp] * 7 + [_i, _vp, _sz] + [_i] * 5
                              + [_fp, _i]),
+    "pluto_kv8_append": (_i, [_vp] * 3 + [_i] + [_sz] * 3 + [_vp] * 4 + [_i] * 4),
+    "pluto_kv8_read": (_i, [_vp] * 3 + [_i] + [_sz] * 3 + [_vp] * 4 + [_i] * 4),
+    "pluto_kv_keep": (_i, [_vp] * 6 + [_i] * 4),
+    "pluto_draft_prepare": (_i, [_vp] * 4 + [_i, _sz, _sz] + [_vp] * 6 + [_i, _vp, _vp] + [_i] * 6 + [_fp, _fp, _i]),
+    "pluto_gqa_tree_decode_workspace_bytes": (_sz, [_i] * 5),
+    "pluto_gqa_tree_decode": (_i, [_vp, _vp, _i, _vp, _i, _sz, _sz, _vp, _vp, _vp, _i, _vp, _vp, _vp, _i, _vp, _vp, _sz]
+                              + [_i] * 6),
+    "pluto_verify_drafts": (_i, [_vp, _vp, _vp, _i] + [_vp] * 8 + [_i] * 3),
     "pluto_gdn_gates": (_i, [_vp] * 5 + [_i, C.c_longlong, _i, _i, _vp, _vp]),
     "pluto_gdn_conv_silu": (_i, [_vp] * 3 + [_i] * 6 + [_vp, _vp, _i]),
     "pluto_gdn_prefill": (_i, [_vp] * 4 + [_i] + [_vp] * 4 + [_i] * 7 + [_sz, _sz, _i, _fp, _i, _vp,
@@ -91,6 +99,12 @@ class KvCacheStruct(C.Structure):
     _fields_ = [("k_base", _vp), ("v_base", _vp), ("block_table", _vp), ("max_blocks", _i),
                 ("page_size", _i), ("page_stride", _sz), ("token_stride", _sz), ("dtype", _i),
                 ("num_pages", _i), ("k_bases", _vp), ("v_bases", _vp)]
+
+
+class KvScalesStruct(C.Structure):
+    """struct pluto_kv_scales of include/pluto_b200.h."""
+    _fields_ = [("k", _vp), ("v", _vp), ("page_stride", _sz), ("token_stride", _sz)]
+
 
 _lib = None
 

@@ -19,7 +19,8 @@ enum : uint32_t {
   kWaitTimeout = 1u,   // a bounded wait ran out
   kBadLength = 2u,     // a device-side sequence length lay outside the host-declared bound
   kBadPage = 3u,       // a block-table entry lay outside the page pool
-  kBadSmemBase = 4u    // dynamic shared memory did not start on the boundary a kernel without slack needs
+  kBadSmemBase = 4u,   // dynamic shared memory did not start on the boundary a kernel without slack needs
+  kBadDraft = 5u       // a drafted token, a parent or a path entry lay outside what it may be
 };
 
 // Records (site << 8) | kind if the word is still healthy; the first report wins.

@@ -231,6 +231,83 @@ struct PrepareArgs {
 };
 cudaError_t qk_prepare(cudaStream_t stream, const PrepareArgs& args);
 
+// ---- decoding with drafted tokens -----------------------------------------------------------------
+// A page pool of any of the three storage types as the kernels of this section address it (draft_rows.cuh):
+// the row of (sequence b, slot t, kv head h) starts at element
+//   page * page_stride + (t % page_size) * token_stride + h * head_dim,   page = table[b][t / page_size] or b,
+// and its scale byte (E4M3 storage) at page * scale_page + (t % page_size) * scale_token + h.
+enum : int { kStoreFp32 = 0, kStoreBf16 = 1, kStoreE4m3 = 2 };
+struct DraftPool {
+  void *k, *v;
+  uint8_t *k_scales, *v_scales;   // E4M3 only
+  const int32_t* table;
+  int max_blocks, page_size, num_pages, store;
+  size_t page_stride, token_stride, scale_page, scale_token;
+  uint32_t* status;
+};
+constexpr int kMaxDraftNodes = 128;   // drafted tokens per sequence: ancestor sets are 128 bits
+
+// kv8.cu
+struct Kv8Args {
+  DraftPool pool;
+  void *k, *v;                    // [batch, tokens, heads, dim] rows, element strides below; head rows contiguous
+  size_t batch_stride, token_stride, head_stride;
+  int is_bf16;
+  const int32_t* positions;       // optional [batch]: slot of token 0
+  const int32_t* counts;          // optional [batch]: tokens of the sequence, at most `tokens`
+  int batch, tokens, heads, dim;
+};
+cudaError_t kv8_append(cudaStream_t stream, const Kv8Args& args);
+cudaError_t kv8_read(cudaStream_t stream, const Kv8Args& args);
+struct KeepArgs {
+  DraftPool pool;
+  const int32_t *prefix, *path, *accepted;   // [batch], [batch, nodes], [batch]
+  int batch, nodes, heads, dim;
+};
+cudaError_t kv_keep(cudaStream_t stream, const KeepArgs& args);
+
+// qk_prepare.cu: the prepare step for drafted tokens (PrepareArgs without its cache): token t of sequence b
+// goes to slot positions[b] + t and has RoPE position positions[b] + its depth in the tree.
+struct DraftPrepareArgs {
+  PrepareArgs p;
+  DraftPool pool;
+  const int32_t *parents, *counts;   // optional [batch, tokens], [batch]
+};
+cudaError_t draft_prepare(cudaStream_t stream, const DraftPrepareArgs& args);
+
+// tree_decode.cu (exact), tree_decode_sm100.cu (tcgen05)
+struct TreeArgs {
+  DraftPool pool;
+  const void* q;                  // [batch, nodes, q_heads, dim]
+  int q_is_bf16;
+  const void* gate;               // optional, element (b * nodes + n) * gate_token + h * gate_head + d
+  int gate_is_bf16;
+  size_t gate_token, gate_head;
+  const int32_t* prefix;          // [batch] cached tokens before the drafts
+  int max_prefix;
+  const int32_t* parents;         // optional [batch, nodes], null: a chain
+  const int32_t* counts;          // optional [batch]
+  void* out;                      // [batch, nodes, q_heads, dim]
+  int out_is_bf16;
+  float* lse;                     // optional [batch, nodes, q_heads]
+  void* workspace;
+  int batch, nodes, q_heads, kv_heads, dim, round;
+  float scale;
+};
+cudaError_t tree_decode_exact(cudaStream_t stream, const TreeArgs& args);
+
+// verify.cu
+struct VerifyArgs {
+  const void *target, *draft;     // [batch, nodes + 1, vocab], optional [batch, nodes, vocab]
+  int is_bf16;
+  const int32_t *tokens, *parents, *counts;
+  const float *accept, *sample;   // [batch, nodes], [batch]
+  int32_t *accepted, *path, *out; // [batch], [batch, nodes], [batch, nodes + 1]
+  int batch, nodes, vocab;
+  uint32_t* status;
+};
+cudaError_t verify_drafts(cudaStream_t stream, const VerifyArgs& args);
+
 // ---- token_step.cu: one token of one sequence in one launch ----------------------------------------
 constexpr int kCachedStepTokens = 1024;   // longest context cached_step takes
 struct CachedStepArgs {

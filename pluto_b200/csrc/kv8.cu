@@ -1,0 +1,292 @@
+// The 8-bit key/value cache: rows quantised as they are written, read back as the values they hold, and the
+// rows of an accepted path moved to the front of the drafts' slots.  The reference keeps its cache in fp32
+// (src/llm/key_value_cache.h:25-57) and has none of the three.
+//
+// Append and read are streams.  A row's channels are dealt to the lanes of a sub-warp, eight consecutive
+// ones each (16 bytes of bf16 in, 8 of codes out), so the row maximum is a butterfly over at most 32 lanes
+// and no shared memory is used; a sub-warp takes the key and the value row of kRows (token, head) pairs at
+// a time, which keeps 2 * kRows loads per lane in flight.  Widths that 8 does not divide and rows off the
+// 16-byte boundary take single channels, a warp per row.
+#include "draft_rows.cuh"
+
+namespace pluto {
+namespace {
+
+constexpr int kRows = 2;
+
+struct RowAt {
+  bool live;
+  size_t data, pool, scale;   // element offsets: activation row, pool row, scale byte
+};
+
+__device__ __forceinline__ RowAt row_at(const Kv8Args& a, unsigned row, uint32_t site) {
+  RowAt r{};
+  const unsigned h = row % a.heads, token = row / a.heads, t = token % a.tokens, b = token / a.tokens;
+  if (b >= static_cast<unsigned>(a.batch) || static_cast<int>(t) >= draft_count(a.counts, b, a.tokens, a.pool.status, site)) return r;
+  const long long slot = static_cast<long long>(a.positions ? a.positions[b] : 0) + t;
+  const long long page = draft_page(a.pool, b, slot > 0x7fffffff ? -1 : static_cast<int>(slot), site);
+  if (page < 0) return r;
+  r.live = true;
+  r.data = b * a.batch_stride + t * a.token_stride + h * a.head_stride;
+  r.pool = draft_row(a.pool, page, static_cast<int>(slot)) + static_cast<size_t>(h) * a.dim;
+  r.scale = draft_scale(a.pool, page, static_cast<int>(slot)) + h;
+  return r;
+}
+
+__device__ __forceinline__ void load8(const void* p, size_t at, int is_bf16, float (&x)[8]) {
+  if (is_bf16) {
+    const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p) + at);
+    x[0] = bf16_lo(w.x); x[1] = bf16_hi(w.x); x[2] = bf16_lo(w.y); x[3] = bf16_hi(w.y);
+    x[4] = bf16_lo(w.z); x[5] = bf16_hi(w.z); x[6] = bf16_lo(w.w); x[7] = bf16_hi(w.w);
+  } else {
+    const float4* f = reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
+    const float4 u = f[0], v = f[1];
+    x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w; x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
+  }
+}
+
+// The codes of eight channels; a row that is not finite gets NaN codes.
+__device__ __forceinline__ uint2 codes8(const float (&x)[8], uint32_t byte) {
+  if (byte == 255u) return make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu);
+  const float f = e8m0_inverse(byte);
+  return make_uint2(e4m3_pair(x[0] * f, x[1] * f) | e4m3_pair(x[2] * f, x[3] * f) << 16,
+                    e4m3_pair(x[4] * f, x[5] * f) | e4m3_pair(x[6] * f, x[7] * f) << 16);
+}
+
+template <int kLanes>   // lanes per row: dim <= 8 * kLanes
+__global__ void __launch_bounds__(256) kv8_append_vec(Kv8Args a) {
+  const unsigned group = (blockIdx.x * 256u + threadIdx.x) / kLanes, lane = threadIdx.x % kLanes;
+  const int c = lane * 8;
+  float k[kRows][8], v[kRows][8];
+  RowAt at[kRows];
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    at[i] = row_at(a, group * kRows + i, 40);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) k[i][u] = v[i][u] = 0.0f;
+    if (at[i].live && c < a.dim) {
+      load8(a.k, at[i].data + c, a.is_bf16, k[i]);
+      load8(a.v, at[i].data + c, a.is_bf16, v[i]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    uint32_t km = 0u, vm = 0u;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      km = max(km, __float_as_uint(k[i][u]) & 0x7fffffffu);
+      vm = max(vm, __float_as_uint(v[i][u]) & 0x7fffffffu);
+    }
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) {
+      km = max(km, __shfl_xor_sync(0xffffffffu, km, o));
+      vm = max(vm, __shfl_xor_sync(0xffffffffu, vm, o));
+    }
+    if (!at[i].live) continue;
+    const uint32_t kb = e8m0_of(km), vb = e8m0_of(vm);
+    if (c < a.dim) {
+      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.pool.k) + at[i].pool + c) = codes8(k[i], kb);
+      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.pool.v) + at[i].pool + c) = codes8(v[i], vb);
+    }
+    if (lane == 0) {
+      a.pool.k_scales[at[i].scale] = static_cast<uint8_t>(kb);
+      a.pool.v_scales[at[i].scale] = static_cast<uint8_t>(vb);
+    }
+  }
+}
+
+__device__ __forceinline__ float load1(const void* p, size_t at, int is_bf16) {
+  return is_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[at]) : static_cast<const float*>(p)[at];
+}
+__device__ __forceinline__ void store1(void* p, size_t at, int is_bf16, float x) {
+  if (is_bf16) static_cast<__nv_bfloat16*>(p)[at] = __float2bfloat16_rn(x);
+  else static_cast<float*>(p)[at] = x;
+}
+
+__global__ void __launch_bounds__(256) kv8_append_any(Kv8Args a) {
+  const int lane = threadIdx.x % 32;
+  const RowAt at = row_at(a, (blockIdx.x * 256u + threadIdx.x) / 32, 40);
+  if (!at.live) return;
+#pragma unroll
+  for (int side = 0; side < 2; ++side) {
+    const void* in = side ? a.v : a.k;
+    uint8_t* pool = static_cast<uint8_t*>(side ? a.pool.v : a.pool.k) + at.pool;
+    uint32_t m = 0u;
+    for (int c = lane; c < a.dim; c += 32) m = max(m, __float_as_uint(load1(in, at.data + c, a.is_bf16)) & 0x7fffffffu);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const uint32_t byte = e8m0_of(m);
+    for (int c = lane; c < a.dim; c += 32)
+      pool[c] = byte == 255u ? 0x7f : static_cast<uint8_t>(e4m3_pair(load1(in, at.data + c, a.is_bf16) * e8m0_inverse(byte), 0.0f));
+    if (lane == 0) (side ? a.pool.v_scales : a.pool.k_scales)[at.scale] = static_cast<uint8_t>(byte);
+  }
+}
+
+__device__ __forceinline__ void store8(void* p, size_t at, int is_bf16, uint2 codes, float f) {
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 pair = e4m3_values((i < 2 ? codes.x : codes.y) >> (16 * (i & 1)));
+    x[2 * i] = pair.x * f;
+    x[2 * i + 1] = pair.y * f;
+  }
+  if (is_bf16) {
+    *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p) + at) =
+        make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+  } else {
+    float4* out = reinterpret_cast<float4*>(static_cast<float*>(p) + at);
+    out[0] = make_float4(x[0], x[1], x[2], x[3]);
+    out[1] = make_float4(x[4], x[5], x[6], x[7]);
+  }
+}
+
+template <int kLanes>
+__global__ void __launch_bounds__(256) kv8_read_vec(Kv8Args a) {
+  const unsigned group = (blockIdx.x * 256u + threadIdx.x) / kLanes, lane = threadIdx.x % kLanes;
+  const int c = lane * 8;
+  if (c >= a.dim) return;
+  uint2 k[kRows], v[kRows];
+  uint32_t kb[kRows], vb[kRows];
+  RowAt at[kRows];
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    at[i] = row_at(a, group * kRows + i, 41);
+    if (at[i].live) {
+      k[i] = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.pool.k) + at[i].pool + c);
+      v[i] = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.pool.v) + at[i].pool + c);
+      kb[i] = a.pool.k_scales[at[i].scale];
+      vb[i] = a.pool.v_scales[at[i].scale];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kRows; ++i)
+    if (at[i].live) {
+      store8(a.k, at[i].data + c, a.is_bf16, k[i], e8m0_value(kb[i]));
+      store8(a.v, at[i].data + c, a.is_bf16, v[i], e8m0_value(vb[i]));
+    }
+}
+
+__global__ void __launch_bounds__(256) kv8_read_any(Kv8Args a) {
+  const int lane = threadIdx.x % 32;
+  const RowAt at = row_at(a, (blockIdx.x * 256u + threadIdx.x) / 32, 41);
+  if (!at.live) return;
+  const float kf = e8m0_value(a.pool.k_scales[at.scale]), vf = e8m0_value(a.pool.v_scales[at.scale]);
+  for (int c = lane; c < a.dim; c += 32) {
+    store1(a.k, at.data + c, a.is_bf16, e4m3_value(static_cast<const uint8_t*>(a.pool.k)[at.pool + c]) * kf);
+    store1(a.v, at.data + c, a.is_bf16, e4m3_value(static_cast<const uint8_t*>(a.pool.v)[at.pool + c]) * vf);
+  }
+}
+
+// Eight channels at a time: rows and strides on 16-byte boundaries (8 bytes of codes).
+bool vector_rows(const Kv8Args& a) {
+  const size_t step = a.is_bf16 ? 8 : 4;
+  const auto aligned = [](const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; };
+  return a.dim % 8 == 0 && a.batch_stride % step == 0 && a.token_stride % step == 0 && a.head_stride % step == 0 &&
+         aligned(a.k, 16) && aligned(a.v, 16) && aligned(a.pool.k, 8) && aligned(a.pool.v, 8) &&
+         a.pool.page_stride % 8 == 0 && a.pool.token_stride % 8 == 0;
+}
+
+unsigned blocks_for(const Kv8Args& a, int lanes, int rows) {
+  const unsigned total = static_cast<unsigned>(a.batch) * a.tokens * a.heads, per_block = 256 / lanes * rows;
+  return (total + per_block - 1) / per_block;
+}
+
+// Moves the rows of an accepted path to the first slots of the drafts, in place.  A thread owns one piece
+// (16 bytes where the rows allow it, and one scale byte of E4M3 storage) of the key or value row and takes
+// the path in order, eight rows at a time, loads before stores: entry j comes from slot path[j] >= j, which
+// no earlier entry has written, so no barrier is needed.  A path that is not strictly increasing inside
+// [0, nodes) is reported and nothing of that sequence moves.
+template <typename Piece>
+__device__ __forceinline__ void move_rows(char* base, const size_t* rows, const int* path, int count, size_t at) {
+  for (int i0 = 0; i0 < count; i0 += 8) {
+    Piece x[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (i0 + u < count && path[i0 + u] != i0 + u) x[u] = *reinterpret_cast<const Piece*>(base + rows[path[i0 + u]] + at);
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (i0 + u < count && path[i0 + u] != i0 + u) *reinterpret_cast<Piece*>(base + rows[i0 + u] + at) = x[u];
+  }
+}
+
+template <typename Piece>
+__global__ void __launch_bounds__(128) kv_keep_kernel(KeepArgs a, size_t row_bytes, int element) {
+  __shared__ int path[kMaxDraftNodes], bad;
+  __shared__ size_t rows[kMaxDraftNodes], scales[kMaxDraftNodes];
+  const int b = blockIdx.y;
+  int count = a.accepted[b];
+  if (threadIdx.x == 0) bad = 0;
+  __syncthreads();
+  if (count < 0 || count > a.nodes) {
+    if (threadIdx.x == 0) report_status(a.pool.status, 42, kBadDraft);
+    return;
+  }
+  const int prefix = a.prefix[b];
+  for (int i = threadIdx.x; i < count; i += 128) {
+    const int node = a.path[static_cast<size_t>(b) * a.nodes + i];
+    path[i] = node;
+    if (node < i || node >= a.nodes || (i > 0 && node <= a.path[static_cast<size_t>(b) * a.nodes + i - 1])) bad = 1;
+  }
+  __syncthreads();
+  if (bad) {
+    if (threadIdx.x == 0) report_status(a.pool.status, 42, kBadDraft);
+    return;
+  }
+  const int last = count > 0 ? path[count - 1] : -1;   // the slots beyond it are not touched
+  for (int i = threadIdx.x; i <= last; i += 128) {
+    const long long slot = static_cast<long long>(prefix) + i;
+    const long long page = prefix < 0 || slot > 0x7fffffff ? draft_page(a.pool, b, -1, 42) : draft_page(a.pool, b, static_cast<int>(slot), 42);
+    if (page < 0) {
+      bad = 1;
+    } else {
+      rows[i] = draft_row(a.pool, page, static_cast<int>(slot)) * element;
+      if (a.pool.store == kStoreE4m3) scales[i] = draft_scale(a.pool, page, static_cast<int>(slot));
+    }
+  }
+  __syncthreads();
+  if (bad) return;
+  const size_t at = (static_cast<size_t>(blockIdx.x) * 128 + threadIdx.x) * sizeof(Piece);
+  if (at < row_bytes) {
+    move_rows<Piece>(static_cast<char*>(blockIdx.z ? a.pool.v : a.pool.k), rows, path, count, at);
+  } else if (a.pool.store == kStoreE4m3) {
+    const size_t head = at / sizeof(Piece) - (row_bytes + sizeof(Piece) - 1) / sizeof(Piece);
+    if (head < static_cast<size_t>(a.heads))
+      move_rows<uint8_t>(reinterpret_cast<char*>(blockIdx.z ? a.pool.v_scales : a.pool.k_scales), scales, path, count, head);
+  }
+}
+
+}  // namespace
+
+cudaError_t kv8_append(cudaStream_t stream, const Kv8Args& a) {
+  if (!vector_rows(a)) kv8_append_any<<<blocks_for(a, 32, 1), 256, 0, stream>>>(a);
+  else if (a.dim <= 64) kv8_append_vec<8><<<blocks_for(a, 8, kRows), 256, 0, stream>>>(a);
+  else if (a.dim <= 128) kv8_append_vec<16><<<blocks_for(a, 16, kRows), 256, 0, stream>>>(a);
+  else kv8_append_vec<32><<<blocks_for(a, 32, kRows), 256, 0, stream>>>(a);
+  return cudaGetLastError();
+}
+
+cudaError_t kv8_read(cudaStream_t stream, const Kv8Args& a) {
+  if (!vector_rows(a)) kv8_read_any<<<blocks_for(a, 32, 1), 256, 0, stream>>>(a);
+  else if (a.dim <= 64) kv8_read_vec<8><<<blocks_for(a, 8, kRows), 256, 0, stream>>>(a);
+  else if (a.dim <= 128) kv8_read_vec<16><<<blocks_for(a, 16, kRows), 256, 0, stream>>>(a);
+  else kv8_read_vec<32><<<blocks_for(a, 32, kRows), 256, 0, stream>>>(a);
+  return cudaGetLastError();
+}
+
+cudaError_t kv_keep(cudaStream_t stream, const KeepArgs& a) {
+  const int element = a.pool.store == kStoreE4m3 ? 1 : a.pool.store == kStoreBf16 ? 2 : 4;
+  const size_t row = static_cast<size_t>(a.heads) * a.dim * element;
+  const auto fits = [&](size_t n) {
+    return row % n == 0 && a.pool.page_stride * element % n == 0 && a.pool.token_stride * element % n == 0 &&
+           reinterpret_cast<uintptr_t>(a.pool.k) % n == 0 && reinterpret_cast<uintptr_t>(a.pool.v) % n == 0;
+  };
+  const size_t piece = fits(16) ? 16 : fits(4) ? 4 : 1;
+  const size_t pieces = row / piece + (a.pool.store == kStoreE4m3 ? a.heads : 0);
+  const dim3 grid(static_cast<unsigned>((pieces + 127) / 128), a.batch, 2);
+  if (piece == 16) kv_keep_kernel<uint4><<<grid, 128, 0, stream>>>(a, row, element);
+  else if (piece == 4) kv_keep_kernel<uint32_t><<<grid, 128, 0, stream>>>(a, row, element);
+  else kv_keep_kernel<uint8_t><<<grid, 128, 0, stream>>>(a, row, element);
+  return cudaGetLastError();
+}
+
+}  // namespace pluto

@@ -10,7 +10,12 @@
 // channels of every 32 * kPer (4 consecutive ones where width, rotary half and strides allow).  A
 // stream bound by HBM; a CTA per (token, head), each computing its own sines, took 60 us at 1000
 // tokens of 24 + 4 heads of 256, this 23.  Token (b, t) has RoPE position positions[b] + t.
+//
+// draft_prepare_kernel is the same step for drafted tokens: slot and RoPE position part ways in a tree (siblings
+// share a position), and the rows may go to an 8-bit cache, quantised where they are produced.  Its queries
+// and keys are those of qk_prepare_kernel bit for bit.
 #include "common.cuh"
+#include "draft_rows.cuh"
 #include "engine.h"
 #include "qk_rows.cuh"
 
@@ -124,7 +129,153 @@ __global__ void __launch_bounds__(256) qk_prepare_kernel(PrepareArgs a) {
   }
 }
 
+// kPer consecutive channels of a key or value row, in the pool's storage.
+template <int kPer>
+__device__ __forceinline__ void store_pool(void* pool, size_t at, int store, const float* v, uint32_t byte) {
+  if (store != kStoreE4m3) {
+    store_out_vec<kPer>(pool, at, store == kStoreBf16, v);
+    return;
+  }
+  uint8_t* codes = static_cast<uint8_t*>(pool) + at;
+  const float f = byte == 255u ? 0.0f : e8m0_inverse(byte);
+  if (kPer == 4)
+    *reinterpret_cast<uint32_t*>(codes) =
+        byte == 255u ? 0x7f7f7f7fu : e4m3_pair(v[0] * f, v[1] * f) | e4m3_pair(v[2] * f, v[3] * f) << 16;
+  else
+    *codes = byte == 255u ? 0x7f : static_cast<uint8_t>(e4m3_pair(v[0] * f, 0.0f));
+}
+
+template <int kPer>
+__global__ void __launch_bounds__(256) draft_prepare_kernel(DraftPrepareArgs d) {
+  __shared__ float cosine[128], sine[128];
+  __shared__ int parents[kMaxDraftNodes], depth;
+  const PrepareArgs& a = d.p;
+  const int heads = a.q_heads + a.kv_heads;
+  const int token = blockIdx.x, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int b = token / a.tokens, t = token % a.tokens;
+  if (t >= draft_count(d.counts, b, a.tokens, d.pool.status, 46)) return;
+  const int D = a.head_dim, half = a.rotary / 2, first = a.positions ? a.positions[b] : 0;
+  if (d.parents) {
+    if (static_cast<int>(threadIdx.x) <= t) parents[threadIdx.x] = d.parents[static_cast<size_t>(b) * a.tokens + threadIdx.x];
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      int n = 0;
+      for (int i = t, up; (up = parents[i]) >= 0; i = up, ++n)
+        if (up >= i) {   // taken as a first token
+          report_status(d.pool.status, 46, kBadDraft);
+          break;
+        }
+      depth = n;
+    }
+  } else if (threadIdx.x == 0) {
+    depth = t;
+  }
+  __syncthreads();
+  const int position = first + depth;
+  if (static_cast<int>(threadIdx.x) < half)
+    rotary_angle(position, threadIdx.x, a.log_theta, a.rotary, a.round, cosine[threadIdx.x], sine[threadIdx.x]);
+  __syncthreads();
+  const long long slot = static_cast<long long>(first) + t;
+  const long long page = draft_page(d.pool, b, slot < 0 || slot > 0x7fffffff ? -1 : static_cast<int>(slot), 46);
+  const size_t kv_row = page < 0 ? 0 : draft_row(d.pool, page, static_cast<int>(slot));
+  const int stride = 8 * gridDim.y;
+  for (int head = blockIdx.y * 8 + warp; head < heads; head += stride) {
+    const bool is_query = head < a.q_heads;
+    const int h = is_query ? head : head - a.q_heads;
+    const size_t dense = (static_cast<size_t>(token) * a.kv_heads + h) * D;
+    const size_t in0 = is_query ? static_cast<size_t>(token) * a.q_token + static_cast<size_t>(h) * a.q_head : dense;
+    const void* in = is_query ? a.q_in : a.k_in;
+    const float* norm = is_query ? a.q_norm : a.k_norm;
+    float x[kRowOwn], value[kRowOwn], result[kRowOwn];
+#pragma unroll
+    for (int i = 0; i < kRowOwn; i += kPer) {
+      const int c = row_channel<kPer>(i, lane);
+#pragma unroll
+      for (int u = 0; u < kPer; ++u) x[i + u] = value[i + u] = result[i + u] = 0.0f;
+      if (c < D) {
+        load_in_vec<kPer>(in, in0 + c, a.in_is_bf16, x + i);
+        if (!is_query) load_in_vec<kPer>(a.v_in, dense + c, a.in_is_bf16, value + i);
+      }
+    }
+    const float inverse = rsqrtf(row_square_sum<kPer>(x, lane) / static_cast<float>(D) + a.epsilon);
+    uint32_t k_max = 0u, v_max = 0u;
+#pragma unroll
+    for (int i = 0; i < kRowOwn; i += kPer) {
+      const int c = row_channel<kPer>(i, lane);
+      if (c >= D) continue;
+#pragma unroll
+      for (int u = 0; u < kPer; ++u) result[i + u] = rnd(x[i + u] * inverse * (1.0f + norm[c + u]), a.round);
+      if (c < a.rotary) {
+        const int partner = c < half ? c + half : c - half;
+        float p[kPer];
+        load_in_vec<kPer>(in, in0 + partner, a.in_is_bf16, p);
+#pragma unroll
+        for (int u = 0; u < kPer; ++u) {
+          float rotated = rnd(p[u] * inverse * (1.0f + norm[partner + u]), a.round);
+          if (c < half) rotated = -rotated;
+          const int f = (c < half ? c : c - half) + u;
+          result[i + u] = rotate(result[i + u], rotated, cosine[f], sine[f], a.round);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kPer; ++u) {
+        value[i + u] = rnd(value[i + u], a.round);
+        k_max = max(k_max, __float_as_uint(result[i + u]) & 0x7fffffffu);
+        v_max = max(v_max, __float_as_uint(value[i + u]) & 0x7fffffffu);
+      }
+    }
+    if (is_query) {
+#pragma unroll
+      for (int i = 0; i < kRowOwn; i += kPer) {
+        const int c = row_channel<kPer>(i, lane);
+        if (c < D) store_out_vec<kPer>(a.q_out, (static_cast<size_t>(token) * a.q_heads + h) * D + c, a.q_out_is_bf16, result + i);
+      }
+      continue;
+    }
+    if (page < 0) continue;
+    uint32_t k_byte = 0u, v_byte = 0u;
+    if (d.pool.store == kStoreE4m3) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        k_max = max(k_max, __shfl_xor_sync(0xffffffffu, k_max, o));
+        v_max = max(v_max, __shfl_xor_sync(0xffffffffu, v_max, o));
+      }
+      k_byte = e8m0_of(k_max);
+      v_byte = e8m0_of(v_max);
+      if (lane == 0) {
+        const size_t s = draft_scale(d.pool, page, static_cast<int>(slot)) + h;
+        d.pool.k_scales[s] = static_cast<uint8_t>(k_byte);
+        d.pool.v_scales[s] = static_cast<uint8_t>(v_byte);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kRowOwn; i += kPer) {
+      const int c = row_channel<kPer>(i, lane);
+      if (c >= D) continue;
+      const size_t at = kv_row + static_cast<size_t>(h) * D + c;
+      store_pool<kPer>(d.pool.k, at, d.pool.store, result + i, k_byte);
+      store_pool<kPer>(d.pool.v, at, d.pool.store, value + i, v_byte);
+    }
+  }
+}
+
 }  // namespace
+
+cudaError_t draft_prepare(cudaStream_t stream, const DraftPrepareArgs& d) {
+  const PrepareArgs& a = d.p;
+  const int tokens = a.batch * a.tokens, heads = a.q_heads + a.kv_heads;
+  const auto aligned = [](const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; };
+  const size_t in = a.in_is_bf16 ? 8 : 16, kv = d.pool.store == kStoreFp32 ? 16 : d.pool.store == kStoreBf16 ? 8 : 4;
+  // (the rule of qk_prepare below)
+  const bool vector = a.head_dim % 4 == 0 && a.rotary % 8 == 0 && a.q_token % 4 == 0 && a.q_head % 4 == 0 &&
+                      d.pool.token_stride % 4 == 0 && d.pool.page_stride % 4 == 0 && aligned(a.q_in, in) &&
+                      aligned(a.k_in, in) && aligned(a.v_in, in) && aligned(a.q_out, a.q_out_is_bf16 ? 8 : 16) &&
+                      aligned(d.pool.k, kv) && aligned(d.pool.v, kv);
+  const dim3 grid(tokens, tokens < 2 * 148 ? (heads + 7) / 8 : 1);
+  if (vector) draft_prepare_kernel<4><<<grid, 256, 0, stream>>>(d);
+  else draft_prepare_kernel<1><<<grid, 256, 0, stream>>>(d);
+  return cudaGetLastError();
+}
 
 cudaError_t qk_prepare(cudaStream_t stream, const PrepareArgs& a) {
   const int tokens = a.batch * a.tokens, heads = a.q_heads + a.kv_heads;

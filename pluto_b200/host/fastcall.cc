@@ -88,6 +88,18 @@ PyObject* kv_cache(PyObject*, PyObject* const* args, Py_ssize_t count) {
   return PyBytes_FromStringAndSize(reinterpret_cast<const char*>(&c), sizeof(c));
 }
 
+// kv_scales(k, v, page_stride, token_stride) -> bytes: struct pluto_kv_scales.
+PyObject* kv_scales(PyObject*, PyObject* const* args, Py_ssize_t count) {
+  if (count != 4) {
+    PyErr_SetString(PyExc_TypeError, "kv_scales takes 4 arguments");
+    return nullptr;
+  }
+  pluto_kv_scales s = {};
+  if (!convert(args[0], s.k) || !convert(args[1], s.v) || !convert(args[2], s.page_stride) || !convert(args[3], s.token_stride))
+    return nullptr;
+  return PyBytes_FromStringAndSize(reinterpret_cast<const char*>(&s), sizeof(s));
+}
+
 template <auto Function>
 constexpr PyMethodDef entry(const char* name) {
   return {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&Entry<Function>::fastcall)), METH_FASTCALL, nullptr};
@@ -113,6 +125,13 @@ PyMethodDef methods[] = {
     ENTRY(pluto_gqa_decode_probs),
     ENTRY(pluto_cached_attention_step),
     ENTRY(pluto_cached_attention_step_workspace_bytes),
+    ENTRY(pluto_kv8_append),
+    ENTRY(pluto_kv8_read),
+    ENTRY(pluto_kv_keep),
+    ENTRY(pluto_draft_prepare),
+    ENTRY(pluto_gqa_tree_decode),
+    ENTRY(pluto_gqa_tree_decode_workspace_bytes),
+    ENTRY(pluto_verify_drafts),
     ENTRY(pluto_gdn_token_step),
     ENTRY(pluto_gdn_token_step_scratch_bytes),
     ENTRY(pluto_gdn_gates),
@@ -135,6 +154,7 @@ PyMethodDef methods[] = {
     ENTRY(pluto_block_linear_workspace_bytes),
     ENTRY(pluto_dequantize_matrix),
     {"kv_cache", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&kv_cache)), METH_FASTCALL, nullptr},
+    {"kv_scales", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&kv_scales)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fastcall", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -16,7 +16,7 @@ from __future__ import annotations
 
 import enum
 from dataclasses import dataclass, field
-from typing import Callable, List, Optional, Sequence
+from typing import Callable, List, NamedTuple, Optional, Sequence
 
 import torch
 
@@ -365,7 +365,9 @@ class KeyValueCache:
     """Per-sequence K/V storage [capacity, kv_heads, head_dim] with a position counter
     (src/llm/key_value_cache.h:25-57).  The reference stores fp32; every value it writes is already
     bf16-rounded when rounding is on, so `dtype=torch.bfloat16` (default) holds the same numbers
-    in half the bytes.  `torch.float32` keeps the reference's storage."""
+    in half the bytes.  `torch.float32` keeps the reference's storage.  `torch.float8_e4m3fn` stores E4M3
+    codes with one power-of-two scale per (token, head) row (`key_scales()`, `value_scales()`: uint8
+    [capacity, kv_heads], the exponent plus 127): a quarter of the bytes, quantised as the rows are written."""
 
     def __init__(self, capacity, key_value_heads, head_dim, dtype, device):
         self.capacity_ = capacity
@@ -373,8 +375,13 @@ class KeyValueCache:
         self.head_dim_ = head_dim
         self.keys_ = torch.zeros((capacity, key_value_heads, head_dim), dtype=dtype, device=device)
         self.values_ = torch.zeros_like(self.keys_)
+        self.key_scales_ = self.value_scales_ = None
+        if dtype == torch.float8_e4m3fn:
+            self.key_scales_ = torch.zeros((capacity, key_value_heads), dtype=torch.uint8, device=device)
+            self.value_scales_ = torch.zeros_like(self.key_scales_)
         self.position_ = 0
         self.packed_ = None
+        self.length_ = None
 
     @staticmethod
     def Create(capacity: int, key_value_heads: int, head_dim: int,
@@ -382,8 +389,8 @@ class KeyValueCache:
         # src/llm/key_value_cache.cc:20-36
         if capacity <= 0 or key_value_heads <= 0 or head_dim <= 0:
             raise _invalid("key-value cache dimensions must be positive")
-        if dtype not in (torch.bfloat16, torch.float32):
-            raise _invalid("key-value cache stores bf16 or fp32")
+        if dtype not in (torch.bfloat16, torch.float32, torch.float8_e4m3fn):
+            raise _invalid("key-value cache stores bf16, fp32 or E4M3")
         return KeyValueCache(capacity, key_value_heads, head_dim, dtype, device)
 
     def capacity(self): return self.capacity_
@@ -392,6 +399,33 @@ class KeyValueCache:
     def position(self): return self.position_
     def keys(self): return self.keys_
     def values(self): return self.values_
+    def key_scales(self): return self.key_scales_
+    def value_scales(self): return self.value_scales_
+
+    def pool(self) -> dict:
+        """The cache as the one page of a pool, for the functions that take pools."""
+        part = lambda t: None if t is None else t.unsqueeze(0)   # noqa: E731
+        return dict(k_pool=part(self.keys_), v_pool=part(self.values_), k_scales=part(self.key_scales_),
+                    v_scales=part(self.value_scales_))
+
+    def device_position(self) -> torch.Tensor:
+        """The position as an int32 [1] device tensor, set on the current stream."""
+        if self.length_ is None or self.length_.device != self.keys_.device:
+            self.length_ = torch.empty((1,), dtype=torch.int32, device=self.keys_.device)
+        return self.length_.fill_(self.position_)
+
+    def Keep(self, path: torch.Tensor, accepted: torch.Tensor) -> int:
+        """After CachedDraftStep and a verification: the rows of the accepted path (int32 [nodes] and [1], as
+        verify_drafts returns them for one sequence) become the next rows of the cache and the position moves
+        behind them.  Reads `accepted` back, so it waits for the stream."""
+        count = int(accepted.item())
+        if count < 0 or count > path.numel():
+            raise _invalid("the accepted path is longer than its nodes")
+        if self.position_ + count > self.capacity_:
+            raise _resource_exhausted("key-value cache capacity reached")
+        kv_keep(**self.pool(), prefix_lens=self.device_position(), path=path.reshape(1, -1), accepted=accepted.reshape(1))
+        self.position_ += count
+        return count
 
     def Advance(self) -> None:
         if self.position_ >= self.capacity_:
@@ -418,6 +452,7 @@ class KeyValueCache:
 
 def kv_layout(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: Optional[torch.Tensor],
               page_size: int, page_stride: int, token_stride: int) -> "_capi.KvCacheStruct":
+    _wide_cache(k_pool)
     s = _capi.KvCacheStruct()
     s.k_base, s.v_base = k_pool.data_ptr(), v_pool.data_ptr()
     s.block_table = None if block_table is None else block_table.data_ptr()
@@ -428,8 +463,14 @@ def kv_layout(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: Optional[
     return s
 
 
+def _wide_cache(pool: torch.Tensor) -> None:
+    if pool.element_size() == 1:
+        raise _unimplemented("an 8-bit cache is attended with gqa_tree_decode and CachedAttentionStep")
+
+
 def _pack_cache(k_pool, v_pool, block_table, page_size, page_stride, token_stride) -> bytes:
     """kv_layout as the bytes the vectorcall binding takes."""
+    _wide_cache(k_pool)
     return _capi.fast().kv_cache(k_pool.data_ptr(), v_pool.data_ptr(),
                                  None if block_table is None else block_table.data_ptr(),
                                  0 if block_table is None else block_table.shape[1], page_size, page_stride,
@@ -445,6 +486,7 @@ def gqa_decode_separate_caches(q: torch.Tensor, caches, seq_lens: torch.Tensor, 
     `caches` B KeyValueCache objects of equal shape and dtype; seq_lens int32 [B]."""
     B, Hq, D = q.shape
     first = caches[0]
+    _wide_cache(first.keys())
     if len(caches) != B or any(c.keys().shape != first.keys().shape or c.keys().dtype != first.keys().dtype
                                for c in caches):
         raise _invalid("one cache per sequence, all of one shape and dtype")
@@ -533,16 +575,54 @@ def CachedAttentionStep(p: FullAttentionParameters, cache: KeyValueCache, q_gate
             raise _invalid("attention requires non-null device pointers")
     if cache.position() >= cache.capacity():
         raise _resource_exhausted("full-attention cache capacity reached")
+    if probabilities is not None:
+        _wide_cache(cache.keys())
     _cached_step(p, cache, q_gate, k, v, q_norm, k_norm, output)
     if probabilities is not None:
         _cached_probabilities(p, cache, q_gate, k, v, q_norm, k_norm, probabilities)
     cache.Advance()
 
 
+def CachedDraftStep(p: FullAttentionParameters, cache: KeyValueCache, q_gate: torch.Tensor, k: torch.Tensor,
+                    v: torch.Tensor, q_norm: torch.Tensor, k_norm: torch.Tensor, output: torch.Tensor,
+                    parents: Optional[torch.Tensor] = None) -> None:
+    """CachedAttentionStep for several drafted tokens at once: q_gate [N,Hq,2,D], k, v [N,Hkv,D], output
+    [N,Hq,D] (fp32 or bf16).  Node i is the child of parents[i] < i (int32 [N]; -1: of the last cached token;
+    None: a chain) and attends to the cached tokens, its ancestors and itself; its rotary position is that of
+    its depth.  The rows go to the slots behind the cache's position, which stays where it is: `cache.Keep`
+    moves it once a path is accepted."""
+    ValidateCachedAttention(p, cache)
+    for t in (q_gate, k, v, q_norm, k_norm, output):
+        if t is None:
+            raise _invalid("attention requires non-null device pointers")
+    n = q_gate.shape[0]
+    if n < 1 or n > 128 or q_gate.numel() != 2 * n * p.query_heads * p.head_dim or output.numel() * 2 != q_gate.numel() or \
+            k.numel() != n * p.key_value_heads * p.head_dim or v.numel() != k.numel():
+        raise _invalid("drafted tokens do not match the attention parameters")
+    if cache.position() + n > cache.capacity():
+        raise _resource_exhausted("full-attention cache capacity reached")
+    _draft_step(p, cache, q_gate.reshape(1, n, p.query_heads, 2, p.head_dim), k, v, q_norm, k_norm, output,
+                None if parents is None else parents.reshape(1, n))
+
+
+def _draft_step(p, cache, q_gate, k, v, q_norm, k_norm, output, parents=None) -> None:
+    n, hkv, d = q_gate.shape[1], p.key_value_heads, p.head_dim
+    at, pool = cache.device_position(), cache.pool()
+    queries = draft_prepare(q_gate[:, :, :, 0], k.reshape(1, n, hkv, d), v.reshape(1, n, hkv, d), q_norm, k_norm, at, **pool,
+                            rotary_dim=p.rotary_dim, rms_norm_epsilon=p.rms_norm_epsilon, rope_theta=p.rope_theta,
+                            round_to_bfloat16=p.round_to_bfloat16, parents=parents)
+    gqa_tree_decode(queries, pool["k_pool"], pool["v_pool"], at, cache.position_, parents=parents, gate=q_gate[:, :, :, 1],
+                    k_scales=pool["k_scales"], v_scales=pool["v_scales"], round_to_bfloat16=p.round_to_bfloat16,
+                    out=output.view(1, n, p.query_heads, d))
+
+
 def _cached_step(p, cache, q_gate, k, v, q_norm, k_norm, output) -> None:
     """The launches of CachedAttentionStep at the cache's position, which stays where it is.  Whether a step
     needs scratch is the library's to decide: it gets what the stream has, and where it refuses for the want
     of more (before any launch), that much is brought."""
+    if cache.key_scales_ is not None:
+        _draft_step(p, cache, q_gate.reshape(1, 1, p.query_heads, 2, p.head_dim), k, v, q_norm, k_norm, output)
+        return
     L = _capi.fast()
     position, index, stream = cache.position_, output.get_device(), _stream()
     _, scratch, size = _decode_workspaces.get((index, stream), _NO_SCRATCH)
@@ -607,6 +687,232 @@ def gqa_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, seq_
                              _ptr(seq_lens), max_seq_len, _ptr(out), _dt(out), _ptr(lse), _ptr(ws),
                              ws.numel(), B, Hq, Hkv, D, int(round_to_bfloat16)))
     return (out, lse) if want_lse else out
+
+
+# =================================================================================================
+# Decoding with drafted tokens, and the 8-bit cache
+# =================================================================================================
+class DraftVerdict(NamedTuple):
+    """What verify_drafts returns, all int32 on the device."""
+    accepted: torch.Tensor   # [B] length of the accepted path
+    path: torch.Tensor       # [B, N] its nodes, then -1
+    tokens: torch.Tensor     # [B, N + 1] its tokens, the drawn token, then -1
+
+
+_STORAGE = {torch.float32: 0, torch.bfloat16: 1, torch.float8_e4m3fn: 2}
+
+
+def _draft_pool(k_pool, v_pool, block_table, k_scales, v_scales, batch):
+    """struct pluto_kv_cache and struct pluto_kv_scales of a page pool of any storage type, as bytes."""
+    code = _STORAGE.get(k_pool.dtype)
+    if code is None or v_pool.dtype != k_pool.dtype:
+        raise _invalid("a cache pool stores fp32, bf16 or E4M3")
+    strides = k_pool.stride()
+    if (k_pool.dim() != 4 or v_pool.shape != k_pool.shape or v_pool.stride() != strides or strides[3] != 1
+            or strides[2] != k_pool.shape[3]):
+        raise _invalid("cache pools are [pages, page_size, kv_heads, head_dim] of one shape, heads contiguous")
+    if k_pool.get_device() != _device_index():
+        raise _invalid("the cache is not on the current device")
+    if block_table is None:
+        if k_pool.shape[0] < batch:
+            raise _invalid("a cache without a block table has a page for every sequence")
+    else:
+        _check_ints(block_table, (batch, block_table.shape[-1]), "block table")
+    cache = _capi.fast().kv_cache(k_pool.data_ptr(), v_pool.data_ptr(), _ptr(block_table),
+                                  0 if block_table is None else block_table.shape[1], k_pool.shape[1], strides[0], strides[1],
+                                  code, k_pool.shape[0])
+    if (code == 2) != (k_scales is not None) or (code == 2) != (v_scales is not None):
+        raise _invalid("an 8-bit cache needs its scales, and only that")
+    if code != 2:
+        return cache, None
+    if (k_scales.shape != k_pool.shape[:3] or v_scales.shape != k_scales.shape or v_scales.stride() != k_scales.stride()
+            or (k_scales.stride(2) != 1 and k_scales.shape[2] != 1) or k_scales.element_size() != 1
+            or v_scales.element_size() != 1 or k_scales.get_device() != k_pool.get_device()):
+        raise _invalid("cache scales are one byte each, [pages, page_size, kv_heads], heads contiguous")
+    return cache, _capi.fast().kv_scales(k_scales.data_ptr(), v_scales.data_ptr(), k_scales.stride(0), k_scales.stride(1))
+
+
+def _device_index() -> int:
+    return torch.cuda.current_device() if _current_device is None else _current_device()
+
+
+def _check_ints(t, shape, what: str) -> None:
+    if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous() or not t.is_cuda):
+        raise _invalid(f"{what} must be a contiguous int32 device tensor of shape {list(shape)}")
+
+
+def _check_rows(t, shape, what: str) -> None:
+    if tuple(t.shape) != tuple(shape) or t.stride(3) != 1 or t.get_device() != _device_index():
+        raise _invalid(f"{what} must be {list(shape)} on the current device, head rows contiguous")
+
+
+def _call_scratch(device: torch.device, nbytes: int) -> torch.Tensor:
+    """The stream's scratch; inside a graph capture memory of the graph's own, so that graphs neither share
+    it nor keep an address that a later, larger call replaces."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty((nbytes,), dtype=torch.uint8, device=device)
+    return _workspace(device, nbytes)
+
+
+def kv8_append(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, k_scales: torch.Tensor,
+               v_scales: torch.Tensor, positions: Optional[torch.Tensor] = None, *,
+               block_table: Optional[torch.Tensor] = None, counts: Optional[torch.Tensor] = None) -> None:
+    """Quantises rows k, v [B,T,Hkv,D] (bf16 or fp32) into the slots positions[b] + t (None: t) of an 8-bit page
+    pool [pages, page_size, Hkv, D] (float8_e4m3fn) with scales [pages, page_size, Hkv] (one byte each); with
+    `counts` int32 [B] only the first counts[b] tokens of sequence b."""
+    B, T, H, D = k.shape
+    cache, scales = _draft_pool(k_pool, v_pool, block_table, k_scales, v_scales, B)
+    if k.stride(3) != 1 or k.stride() != v.stride():
+        k, v = k.contiguous(), v.contiguous()
+    if v.shape != k.shape or v.dtype != k.dtype or k_pool.shape[2:] != k.shape[2:]:
+        raise _invalid("8-bit cache rows do not match the pool")
+    _check_rows(k, k.shape, "cache rows")
+    _check_ints(positions, (B,), "positions")
+    _check_ints(counts, (B,), "counts")
+    check(_capi.fast().pluto_kv8_append(_stream(), k.data_ptr(), v.data_ptr(), _dt(k), k.stride(0), k.stride(1), k.stride(2),
+                                        cache, scales, _ptr(positions), _ptr(counts), B, T, H, D))
+
+
+def kv8_read(k_pool: torch.Tensor, v_pool: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor,
+             positions: torch.Tensor, tokens: int, *, block_table: Optional[torch.Tensor] = None,
+             counts: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.bfloat16):
+    """(k, v) [B,tokens,Hkv,D]: the values that the slots positions[b] .. positions[b] + tokens - 1 of an 8-bit
+    pool hold (exact in bf16); with `counts` the rows from counts[b] on are zero."""
+    B, (_, _, H, D) = positions.shape[0], k_pool.shape
+    cache, scales = _draft_pool(k_pool, v_pool, block_table, k_scales, v_scales, B)
+    _check_ints(positions, (B,), "positions")
+    _check_ints(counts, (B,), "counts")
+    new = torch.empty if counts is None else torch.zeros
+    k, v = (new((B, tokens, H, D), dtype=dtype, device=k_pool.device) for _ in range(2))
+    check(_capi.fast().pluto_kv8_read(_stream(), k.data_ptr(), v.data_ptr(), _dt(k), k.stride(0), k.stride(1), k.stride(2),
+                                      cache, scales, positions.data_ptr(), _ptr(counts), B, tokens, H, D))
+    return k, v
+
+
+def kv_keep(k_pool: torch.Tensor, v_pool: torch.Tensor, prefix_lens: torch.Tensor, path: torch.Tensor,
+            accepted: torch.Tensor, *, block_table: Optional[torch.Tensor] = None, k_scales: Optional[torch.Tensor] = None,
+            v_scales: Optional[torch.Tensor] = None) -> None:
+    """After a verification: the rows of the accepted path move from slots prefix_lens[b] + path[b][i] to slots
+    prefix_lens[b] + i, in place, for i < accepted[b]; every other slot keeps its rows.  The caller then adds
+    `accepted` to its lengths.  path int32 [B,N], accepted int32 [B], as verify_drafts returns them."""
+    B, N = path.shape
+    cache, scales = _draft_pool(k_pool, v_pool, block_table, k_scales, v_scales, B)
+    _check_ints(prefix_lens, (B,), "prefix lengths")
+    _check_ints(path, (B, N), "path")
+    _check_ints(accepted, (B,), "accepted")
+    check(_capi.fast().pluto_kv_keep(_stream(), cache, scales, prefix_lens.data_ptr(), path.data_ptr(), accepted.data_ptr(), B, N,
+                                     k_pool.shape[2], k_pool.shape[3]))
+
+
+def draft_prepare(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_norm: torch.Tensor, k_norm: torch.Tensor,
+                  prefix_lens: Optional[torch.Tensor], k_pool: torch.Tensor, v_pool: torch.Tensor, *, rotary_dim: int,
+                  rms_norm_epsilon: float = 1e-6, rope_theta: float = 10000000.0, round_to_bfloat16: bool = True,
+                  parents: Optional[torch.Tensor] = None, counts: Optional[torch.Tensor] = None,
+                  block_table: Optional[torch.Tensor] = None, k_scales: Optional[torch.Tensor] = None,
+                  v_scales: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Norm and rotation of drafted tokens and the append of their K/V rows: q [B,N,Hq,D] (any token and head
+    strides), k, v [B,N,Hkv,D].  Node i of sequence b is rotated for position prefix_lens[b] + its depth and its
+    rows go to slot prefix_lens[b] + i of a pool of any storage type.  Returns the queries [B,N,Hq,D], bf16
+    when round_to_bfloat16 and fp32 otherwise.  Without `parents` (a chain, or a whole prompt) any N."""
+    B, N, Hq, D = q.shape
+    Hkv = k_pool.shape[2]
+    cache, scales = _draft_pool(k_pool, v_pool, block_table, k_scales, v_scales, B)
+    if q.stride(3) != 1 or (B > 1 and q.stride(0) != N * q.stride(1)):
+        raise _invalid("attention query must have a contiguous head dimension and batch")
+    k, v = k.contiguous(), v.contiguous()
+    _check_rows(q, (B, N, Hq, k_pool.shape[3]), "drafted queries")
+    _check_rows(k, (B, N, Hkv, D), "drafted keys")
+    _check_rows(v, (B, N, Hkv, D), "drafted values")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise _invalid("drafted queries, keys and values have one type")
+    for norm in (q_norm, k_norm):
+        if norm.dtype != torch.float32 or norm.numel() != D or not norm.is_cuda:
+            raise _invalid("Qwen attention norms must be FP32 head-width parameters on its Executor")
+    _check_ints(prefix_lens, (B,), "prefix lengths")
+    _check_ints(parents, (B, N), "parents")
+    _check_ints(counts, (B,), "counts")
+    out = torch.empty((B, N, Hq, D), dtype=torch.bfloat16 if round_to_bfloat16 else torch.float32, device=q.device)
+    check(_capi.fast().pluto_draft_prepare(
+        _stream(), q.data_ptr(), k.data_ptr(), v.data_ptr(), _dt(q), q.stride(1), q.stride(2), q_norm.data_ptr(),
+        k_norm.data_ptr(), _ptr(prefix_lens), _ptr(parents), _ptr(counts), out.data_ptr(), _dt(out), cache, scales, B, N, Hq,
+        Hkv, D, rotary_dim, rms_norm_epsilon, rope_theta, int(round_to_bfloat16)))
+    return out
+
+
+def gqa_tree_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, prefix_lens: torch.Tensor,
+                    max_prefix_len: int, *, parents: Optional[torch.Tensor] = None, counts: Optional[torch.Tensor] = None,
+                    block_table: Optional[torch.Tensor] = None, k_scales: Optional[torch.Tensor] = None,
+                    v_scales: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None,
+                    round_to_bfloat16: bool = True, out: Optional[torch.Tensor] = None,
+                    workspace: Optional[torch.Tensor] = None, want_lse: bool = False):
+    """gqa_decode for several drafted tokens per sequence, over a pool of any storage type: q [B,N,Hq,D] prepared
+    queries, node i of sequence b in slot prefix_lens[b] + i of the cache.  A node sees the cached slots below
+    prefix_lens[b], its ancestors by `parents` int32 [B,N] (None: a chain) and itself.  `counts` int32 [B]: the
+    sequence has that many nodes; the rows of the others are left as they were (zeros without `out`).  One
+    node per sequence is gqa_decode.  Returns out [B,N,Hq,D] (and lse [B,N,Hq])."""
+    B, N, Hq, D = q.shape
+    Hkv = k_pool.shape[2]
+    cache, scales = _draft_pool(k_pool, v_pool, block_table, k_scales, v_scales, B)
+    _check_rows(q, (B, N, Hq, k_pool.shape[3]), "drafted queries")
+    if not q.is_contiguous():
+        q = q.contiguous()
+    _check_ints(prefix_lens, (B,), "prefix lengths")
+    _check_ints(parents, (B, N), "parents")
+    _check_ints(counts, (B,), "counts")
+    new = torch.empty if counts is None else torch.zeros
+    if out is None:
+        out = new((B, N, Hq, D), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or not out.is_contiguous() or out.get_device() != q.get_device():
+        raise _invalid("attention output must be contiguous and of the query's shape")
+    lse = new((B, N, Hq), dtype=torch.float32, device=q.device) if want_lse else None
+    gts = ghs = 0
+    if gate is not None:
+        _check_rows(gate, q.shape, "attention gate")
+        if B > 1 and gate.stride(0) != N * gate.stride(1):
+            raise _invalid("attention gate must have a contiguous head dimension and batch")
+        gts, ghs = gate.stride(1), gate.stride(2)
+    L = _capi.fast()
+    if workspace is None:
+        workspace = _call_scratch(q.device, L.pluto_gqa_tree_decode_workspace_bytes(B, N, Hq, Hkv, D))
+    check(L.pluto_gqa_tree_decode(_stream(), q.data_ptr(), _dt(q), _ptr(gate), 0 if gate is None else _dt(gate), gts, ghs, cache,
+                                  scales, prefix_lens.data_ptr(), max_prefix_len, _ptr(parents), _ptr(counts), out.data_ptr(),
+                                  _dt(out), _ptr(lse), workspace.data_ptr(), workspace.numel() * workspace.element_size(), B, N,
+                                  Hq, Hkv, D, int(round_to_bfloat16)))
+    return (out, lse) if want_lse else out
+
+
+def verify_drafts(target_probs: torch.Tensor, tokens: torch.Tensor, accept_uniforms: torch.Tensor,
+                  sample_uniforms: torch.Tensor, *, parents: Optional[torch.Tensor] = None,
+                  counts: Optional[torch.Tensor] = None, draft_probs: Optional[torch.Tensor] = None) -> DraftVerdict:
+    """Accepts drafted tokens against the target's probabilities [B,N+1,V] (row 0 follows the last cached token, row
+    i + 1 follows node i; fp32 or bf16) and draws one more token, from given uniform numbers in [0, 1):
+    accept_uniforms fp32 [B,N], sample_uniforms fp32 [B].
+
+    A chain (parents None): token i is accepted, if all before it were, when u_i * q(x_i) < p(x_i), q row i of
+    draft_probs [B,N,V] (None: the drafts were given, q = 1); the first refused one leaves max(p - q, 0).  A
+    tree: the children of the last accepted node in index order, child c when u_c * (1 - p of the siblings tried
+    before) < p(x_c), a token tried before never; what is left is p without the tried tokens.  The drawn
+    token is the smallest x whose running sum exceeds u * total.  Tests and sums are in double."""
+    B, N = tokens.shape
+    V = target_probs.shape[2] if target_probs.dim() == 3 else 0
+    if V == 0 or tuple(target_probs.shape) != (B, N + 1, V) or not target_probs.is_contiguous():
+        raise _invalid("target probabilities must be [batch, nodes + 1, vocab], contiguous")
+    if draft_probs is not None and (tuple(draft_probs.shape) != (B, N, V) or not draft_probs.is_contiguous()
+                                    or draft_probs.dtype != target_probs.dtype or not draft_probs.is_cuda):
+        raise _invalid("draft probabilities must be [batch, nodes, vocab] of the target's type, contiguous")
+    for u, shape in ((accept_uniforms, (B, N)), (sample_uniforms, (B,))):
+        if u.dtype != torch.float32 or tuple(u.shape) != shape or not u.is_contiguous() or not u.is_cuda:
+            raise _invalid("uniform numbers must be fp32 [batch, nodes] and [batch], contiguous")
+    if target_probs.get_device() != _device_index():
+        raise _invalid("target probabilities are not on the current device")
+    _check_ints(tokens, (B, N), "drafted tokens")
+    _check_ints(parents, (B, N), "parents")
+    _check_ints(counts, (B,), "counts")
+    accepted, path, out = (torch.empty(shape, dtype=torch.int32, device=target_probs.device) for shape in ((B,), (B, N), (B, N + 1)))
+    check(_capi.fast().pluto_verify_drafts(
+        _stream(), target_probs.data_ptr(), _ptr(draft_probs), _dt(target_probs), tokens.data_ptr(), accept_uniforms.data_ptr(),
+        sample_uniforms.data_ptr(), _ptr(parents), _ptr(counts), accepted.data_ptr(), path.data_ptr(), out.data_ptr(), B, N, V))
+    return DraftVerdict(accepted, path, out)
 
 
 # =================================================================================================
@@ -857,6 +1163,7 @@ class QwenAttentionLayer(Layer):
             _cached_step(p, cache, inputs[0], inputs[1], inputs[2], self.weights_[0], self.weights_[1], output)
             cache.Advance()
             return FwdResult([output], BackwardState())
+        _wide_cache(cache.keys())
         length = cache.position_ + 1
         probabilities = torch.empty((p.query_heads, length), dtype=torch.float32, device=inputs[0].device)
         CachedAttentionStep(p, cache, inputs[0], inputs[1], inputs[2], self.weights_[0], self.weights_[1], output,
