@@ -373,7 +373,7 @@ int pluto_cached_attention_step(pluto_stream_t stream, const void* q_gate, const
  * Contents of device arrays that are out of range (a negative length or one beyond the declared bound, a slot
  * past the sequence's pages, a page outside the pool, a parent >= i, a token >= vocab, a path that does not
  * rise) never lead to an access out of bounds: they are reported through pluto_kernel_status (kinds 2, 3, 5) and
- * the length is clamped, the row reads as absent, the write or move is left out, the parent taken as -1, the
+ * the length is clamped, the row reads as zeros, the write or move is left out, the parent taken as -1, the
  * token refused.
  *
  * Caches.  One page pool per layer as in pluto_kv_cache, contiguous (page = sequence) or through a block table

@@ -147,7 +147,8 @@ int pluto_draft_prepare(pluto_stream_t stream, const void* q_in, const void* k_i
 
 size_t pluto_gqa_tree_decode_workspace_bytes(int batch, int nodes, int q_heads, int kv_heads, int head_dim) {
   if (!draft_shape(batch, nodes, q_heads, kv_heads, head_dim) || nodes > pluto::kMaxDraftNodes) return 0;
-  return 16;
+  const size_t parts = pluto::tree_decode_tc_workspace_bytes(nodes, q_heads, kv_heads, head_dim);
+  return parts > 0 ? parts : 16;
 }
 
 int pluto_gqa_tree_decode(pluto_stream_t stream, const void* q, int q_dtype, const void* gate, int gate_dtype,
@@ -177,7 +178,8 @@ int pluto_gqa_tree_decode(pluto_stream_t stream, const void* q, int q_dtype, con
   a.round = round_to_bf16;
   a.scale = 1.0f / sqrtf(static_cast<float>(head_dim));
   if (int c = take_status(&a.pool.status)) return c;
-  return pluto::report_cuda(pluto::tree_decode_exact(stream, a), "attention of drafted tokens");
+  return pluto::report_cuda(pluto::tree_decode_tc_supported(a) ? pluto::tree_decode_tc(stream, a) : pluto::tree_decode_exact(stream, a),
+                            "attention of drafted tokens");
 }
 
 int pluto_verify_drafts(pluto_stream_t stream, const void* target_probs, const void* draft_probs, int dtype,

@@ -295,6 +295,9 @@ struct TreeArgs {
   float scale;
 };
 cudaError_t tree_decode_exact(cudaStream_t stream, const TreeArgs& args);
+bool tree_decode_tc_supported(const TreeArgs& args);
+size_t tree_decode_tc_workspace_bytes(int nodes, int q_heads, int kv_heads, int dim);   // 0: no such width
+cudaError_t tree_decode_tc(cudaStream_t stream, const TreeArgs& args);
 
 // verify.cu
 struct VerifyArgs {

@@ -72,10 +72,10 @@ __global__ void __launch_bounds__(kWarps * 32) tree_decode_exact_kernel(TreeArgs
       live[j] = key < keys;
       const int slot = !live[j] ? 0 : key < prefix ? key : prefix + seen[key - prefix];
       const long long page = live[j] ? draft_page(a.pool, b, slot, 45) : -1;
-      live[j] = page >= 0;
-      const size_t at = live[j] ? draft_row(a.pool, page, slot) + static_cast<size_t>(kv_head) * D : 0;
+      const bool there = page >= 0;   // a slot without a page reads as zeros
+      const size_t at = there ? draft_row(a.pool, page, slot) + static_cast<size_t>(kv_head) * D : 0;
       float kf = 1.0f, vf = 1.0f;
-      if (live[j] && a.pool.store == kStoreE4m3) {
+      if (there && a.pool.store == kStoreE4m3) {
         const size_t s = draft_scale(a.pool, page, slot) + kv_head;
         kf = e8m0_value(a.pool.k_scales[s]);
         vf = e8m0_value(a.pool.v_scales[s]);
@@ -83,8 +83,8 @@ __global__ void __launch_bounds__(kWarps * 32) tree_decode_exact_kernel(TreeArgs
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int d = lane + 32 * i;
-        k[j][i] = live[j] && d < D ? stored(a.pool.k, at + d, a.pool.store) * kf : 0.0f;
-        v[j][i] = live[j] && d < D ? stored(a.pool.v, at + d, a.pool.store) * vf : 0.0f;
+        k[j][i] = there && d < D ? stored(a.pool.k, at + d, a.pool.store) * kf : 0.0f;
+        v[j][i] = there && d < D ? stored(a.pool.v, at + d, a.pool.store) * vf : 0.0f;
       }
     }
 #pragma unroll
@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(kWarps * 32) tree_decode_exact_kernel(TreeArgs
   for (int d = threadIdx.x; d < D; d += kWarps * 32) {
     float sum = 0.0f;
     for (int w = 0; w < kWarps; ++w) sum += acc_of[w][d] * expf(ml_of[w][0] - m_safe);
-    float value = l_all == 0.0f ? 0.0f : sum / l_all;   // every key on a bad page: zeros
+    float value = sum / l_all;
     value = tree_output(a, static_cast<size_t>(b) * a.nodes + node, head, d, value);
     if (a.out_is_bf16) static_cast<__nv_bfloat16*>(a.out)[row * D + d] = __float2bfloat16_rn(value);
     else static_cast<float*>(a.out)[row * D + d] = value;
