@@ -14,36 +14,39 @@
 // Up to 128 rows: the streams take the even and the odd key tiles and are merged at the end.  More: each
 // takes 128 rows and both read every tile.  Width 256 (O takes half of TMEM): one O, two buffers of S.
 //
-// Loading.  Eight warps fetch 16 bytes per lane from the pages into registers, up to 64 KB per SM in flight, and store
-// them as 128-byte-swizzled bf16 tiles; pages may have any size and rows any 16-byte stride.  8-bit codes
-// are widened on the way: the code's bits shifted into a bf16 are the value times 2^-120, and one packed
-// product with 2^(120 + n) gives the exact value (no rounding: see draft_rows.cuh), so what follows is one
-// kernel for both.  (Copies of raw codes through shared memory would add a third to its traffic, which
-// binds before HBM does.)
+// Loading.  Four warps copy the rows into a ring with asynchronous 16-byte copies; pages may have any size and rows any
+// 16-byte stride.  bf16 rows land as the swizzled tiles that the products read.  8-bit codes land as they are (96 KB per
+// SM in flight at width 128) and eight more warps widen them to fp16 tiles, one instruction per two codes and exact,
+// and multiply them by their row's 2^n where fp16 holds every product (-15 <= n <= 7, values from 2^-24 to 57344);
+// a tile with other rows keeps its codes and the softmax multiplies scores and weights by the rows' factors.  P then
+// carries 11 bits, over bf16 caches 8.
 //
 // Work is cut evenly over the SMs whatever the lengths: the units' key tiles, each unit with a few more for what
 // it costs besides, form one line that is cut into equal ranges, one per CTA.  A CTA walks the units of its range; one that
 // it holds whole it writes out, of the others it leaves (accumulator, maximum, sum) in the workspace, and a
 // second kernel merges a cut unit's parts in the order of the keys.  The cut follows from the lengths alone.
+#include <stddef.h>
+
 #include "draft_rows.cuh"
 
 namespace pluto {
 namespace {
 
 constexpr int kTile = 64;            // keys
-constexpr int kThreads = 640;        // warps 0-3: MMA issue; 4-11: softmax; 12-15: keys; 16-19: values
+template <bool kEight>
+constexpr int kThreads = kEight ? 768 : 512;   // warps 0-3: MMA issue; 4-11: softmax; 12-15: loads; 16-23: widening
 constexpr int kMaxCtas = 148;
 constexpr int kUnitTiles = 3;        // what a unit costs besides its tiles (query load, read-out), in tiles
 constexpr float kRescale = 8.0f;     // O is rescaled when the maximum has grown by more than 2^8
+constexpr float kSmallest = -100.0f; // exponent of the value rows from which smaller ones are taken for as large
 
+template <int D, bool kEight>
+constexpr int kStages = kEight ? (D == 64 ? 6 : D == 128 ? 3 : 2) : (D == 64 ? 10 : D == 128 ? 6 : 3);   // tiles of keys, and of values
 template <int D>
-constexpr int kStages = D == 64 ? 10 : D == 128 ? 6 : 3;
+constexpr int kRawStages = D == 64 ? 8 : D == 128 ? 6 : 2;   // key and value tiles as codes
 template <int D>
 constexpr int kTileBytes = kTile * D * 2;
-template <int D>
-constexpr int kGroupRows = D == 256 ? 128 : 256;   // rows that share one pass over the keys
-
-constexpr int group_rows(int dim) { return dim == 256 ? 128 : 256; }
+constexpr int group_rows(int dim) { return dim == 256 ? 128 : 256; }   // rows that share one pass over the keys
 
 // ---- the line of work ----------------------------------------------------------------------------------------
 struct Sequence {
@@ -156,22 +159,33 @@ struct Cursor {
 
 // ---- shared memory -------------------------------------------------------------------------------------------
 constexpr int kSegments = 8;         // of the ring
-constexpr int kSegmentReaders = 17;  // warps: MMA issue, eight softmax, eight loaders
+constexpr int kSegmentReaders = 13;  // warps: MMA issue, eight softmax, four loaders
 
-template <int D>
+template <int D, bool kEight>
 struct Shared {
+  static constexpr int kTiles = kStages<D, kEight>, kRaw = kEight ? kRawStages<D> : 1;
   uint64_t seg_full[kSegments], seg_empty[kSegments];
-  Segment seg[kSegments];
-  uint64_t k_full[kStages<D>], k_empty[kStages<D>], v_full[kStages<D>], v_empty[kStages<D>];
-  uint64_t q_full[2], s_full[2], p_full[2], pv_done[2];
+  uint64_t k_full[kTiles], k_empty[kTiles], v_full[kTiles], v_empty[kTiles];
+  uint64_t raw_k[kRaw], raw_v[kRaw], raw_scales[kRaw], raw_empty[kRaw];
+  uint64_t q_full[2], s_full[2], p_half[2], p_full[2], pv_half[2], pv_done[2];   // one phase per tile of the buffer
   uint64_t ml_full, o_read;   // the two streams' meeting points: sums written, O read
+  Segment seg[kSegments];
   uint32_t tmem;
   float2 ml[2][128];
+  // 8-bit caches: the raw tiles' scale bytes and first draft that not every node sees (-1: the range ends)
+  uint8_t k_byte[kRaw][kTile], v_byte[kRaw][kTile];
+  int draft_row[kRaw];
+  // ... and per tile whether the softmax has to apply the rows' factors; a ring of twice the stages (a tile's scores may
+  // still be read when its key stage has been refilled, but not when the next one has: that product was issued
+  // behind this tile's)
+  alignas(16) float k_factor[2 * kTiles][kTile];   // (read four at a time)
+  float v_factor[2 * kTiles][kTile];
+  int scaled[2 * kTiles], v_largest[2 * kTiles];
 };
 
 // The next segment of the range, by every lane of a warp; false at its end (or when a wait ran out).
-template <int D>
-__device__ __forceinline__ bool next_segment(Shared<D>* sh, int& n, Segment& seg, int lane, uint32_t* status) {
+template <typename S>
+__device__ __forceinline__ bool next_segment(S* sh, int& n, Segment& seg, int lane, uint32_t* status) {
   const int at = n % kSegments;
   if (!__all_sync(0xffffffffu, mbar_wait(&sh->seg_full[at], (n / kSegments) & 1, status, 61))) return false;
   seg = sh->seg[at];
@@ -181,31 +195,12 @@ __device__ __forceinline__ bool next_segment(Shared<D>* sh, int& n, Segment& seg
   return seg.rows > 0;
 }
 
-// ---- 8-bit codes to bf16 -------------------------------------------------------------------------------------
-// Two codes in the high bytes of x's halves -> sign and magnitude bits of bf16: the value times 2^-120.
-__device__ __forceinline__ uint32_t widen_pair(uint32_t x) { return (x & 0x80008000u) | ((x >> 4) & 0x07f007f0u); }
-__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
-__device__ __forceinline__ uint2 widen_word(uint32_t w, uint32_t factor) {   // four codes
-  return make_uint2(mul_bf16x2(widen_pair(__byte_perm(w, 0u, 0x1404)), factor),
-                    mul_bf16x2(widen_pair(__byte_perm(w, 0u, 0x3424)), factor));
-}
-// A row's factors as bf16 bits: 2^(120 + n) in the low half as far as bf16 holds it (n <= 7), the rest in the
-// high half (1 unless the row holds values above 57344).  255 (not finite): NaN.
-constexpr uint32_t kOne = 0x3f80u;
-__device__ __forceinline__ uint32_t widen_factors(uint32_t byte) {
-  if (byte == 255u) return kOne << 16 | 0x7fc0u;
-  return (byte > 134u ? (byte - 7u) << 7 : kOne) << 16 | (min(byte, 134u) + 120u) << 7;
-}
-
 // ---- loaders -------------------------------------------------------------------------------------------------
-__device__ __forceinline__ uint4 load_once(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool there) {   // zeros where it is not
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void arrive_behind_copies(uint64_t* bar) {   // when this thread's copies so far have landed
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 __device__ __forceinline__ bool not_finite(uint32_t pair) {
   return (pair & 0x7f80u) == 0x7f80u || (pair & 0x7f800000u) == 0x7f800000u;
@@ -213,130 +208,214 @@ __device__ __forceinline__ bool not_finite(uint32_t pair) {
 __device__ __forceinline__ bool not_finite(const uint4& v) {
   return not_finite(v.x) || not_finite(v.y) || not_finite(v.z) || not_finite(v.w);
 }
+// Where (row, piece of 8 channels) of a tile lies: 64-channel slabs of 64 rows x 128 bytes, 128-byte swizzle.
+__device__ __forceinline__ uint32_t tile_piece(uint32_t tile, int r, int piece) {
+  return tile + (piece / 8) * (kTile * 128) + r * 128 + (((piece & 7) ^ (r & 7)) << 4);
+}
 
-// One warp's sixteen rows of every tile of the keys (or values).  A lane looks after row lane % 16's address and scale
-// and copies pieces lane, lane + 32, ... of the sixteen rows.
-template <int D, bool kEight, bool kValues>
-__device__ __forceinline__ void load_tiles(const TreeArgs& a, Shared<D>* sh, uint32_t ring, int warp, int lane) {
-  constexpr int kPieces = kEight ? D / 16 : D / 8;       // 16-byte pieces of a row
-  constexpr int kLoads = kPieces / 2;                    // of sixteen rows, per lane
-  constexpr int kBuffers = 16 / kLoads;
-  constexpr int kElement = kEight ? 1 : 2;
-  uint64_t* full = kValues ? sh->v_full : sh->k_full;
-  uint64_t* empty = kValues ? sh->v_empty : sh->k_empty;
-  const char* base = static_cast<const char*>(kValues ? a.pool.v : a.pool.k);
-  const char* other = static_cast<const char*>(a.pool.v);
+__device__ __forceinline__ uint32_t load_byte(const uint8_t* p, bool there) {   // 127 where it is not
+  uint32_t v;
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\tmov.u32 %0, 127;\n\t@p ld.global.u8 %0, [%1];\n\t}"
+               : "=r"(v) : "l"(p), "r"(static_cast<uint32_t>(there)));
+  return v;
+}
 
-  uint4 raw[kBuffers][kLoads];
-  uint32_t factors[kBuffers];
+// Four warps; a warp copies every fourth half tile (32 rows of keys and of values), a lane looking after the page and the
+// scales of its row.  Nothing is used in the step that asks for it: pages are fetched one unit ahead of the
+// copies, scale bytes are passed on one unit later.
+template <int D, bool kEight>
+__device__ __forceinline__ void load_tiles(const TreeArgs& a, Shared<D, kEight>* sh, uint32_t k_ring, uint32_t v_ring, int warp, int lane) {
+  constexpr int kRing = kEight ? kRawStages<D> : kStages<D, kEight>;
+  constexpr int kElement = kEight ? 1 : 2, kBytes = kTile * D * kElement, kPieces = D * kElement / 16, kLoads = kPieces;
+  uint64_t* k_full = kEight ? sh->raw_k : sh->k_full;
+  uint64_t* v_full = kEight ? sh->raw_v : sh->v_full;
+  uint32_t* status = a.pool.status;
+  const int page_shift = (a.pool.page_size & (a.pool.page_size - 1)) == 0 ? __ffs(a.pool.page_size) - 1 : -1;
+  const int first_row = (warp & 1) * 32, own = first_row + lane;   // row of the tile
   Segment seg;
-  int tile = 0, issued = 0, stored = 0, seg_n = 0;
-  bool more = next_segment(sh, seg_n, seg, lane, a.pool.status);
-  if (more) tile = seg.tile0;
-  long long row_at = -1;     // byte offset of the lane's row of the next tile, -1: no row there
-  size_t scale_at = 0;
-  const auto locate = [&]() {
-    row_at = -1;
-    if (!more) return;
-    const int t = tile * kTile + warp * 16 + lane % 16;
-    if (t >= seg.prefix + seg.count) return;
-    const long long page = draft_page(a.pool, seg.b, t, 48);
-    if (page < 0) return;
-    row_at = static_cast<long long>((draft_row(a.pool, page, t) + static_cast<size_t>(seg.kv_head) * D) * kElement);
-    if (kEight) scale_at = draft_scale(a.pool, page, t) + seg.kv_head;
+  int seg_n = 0, n = warp >> 1, tile = 0, page = -1;   // tile number n of the range is `tile` of the segment
+  bool more = next_segment(sh, seg_n, seg, lane, status);
+  if (more) tile = seg.tile0 + n;
+  const auto settle = [&]() {
+    while (more && tile >= seg.tile1) {
+      const int beyond = tile - seg.tile1;
+      more = next_segment(sh, seg_n, seg, lane, status);
+      if (more) tile = seg.tile0 + beyond;
+    }
+    const int t = tile * kTile + own;
+    page = -1;
+    if (!more || t >= seg.prefix + seg.count) return;
+    const int block = page_shift >= 0 ? t >> page_shift : t / a.pool.page_size;
+    if (block >= (a.pool.table ? a.pool.max_blocks : 1)) report_status(status, 48, kBadLength);
+    else page = a.pool.table ? a.pool.table[static_cast<size_t>(seg.b) * a.pool.max_blocks + block] : seg.b;
   };
-  // Fetches the next tile of the range into a buffer.  Of drafts that not every node sees, a value row that is
-  // not finite must not meet the zero weights of the nodes that do not see it: it is loaded as zeros, and
-  // the key row is made NaN, which gives those that see it NaN scores and touches no other node.
-  const auto issue = [&](uint4 (&buffer)[kLoads], uint32_t& factor) {
-    const int first_draft = seg.count > 1 ? max(0, seg.prefix - tile * kTile) : kTile;   // row of the tile
-    const bool drafts = first_draft < kTile;
-    if (kEight) {
-      factor = kOne << 16;
-      if (row_at >= 0) {
-        uint32_t byte = (kValues ? a.pool.v_scales : a.pool.k_scales)[scale_at];
-        factor = widen_factors(byte);
-        if (drafts && warp * 16 + lane % 16 >= first_draft) {
-          if (kValues && byte == 255u) factor = kOne << 16;                              // zeros
-          if (!kValues && a.pool.v_scales[scale_at] == 255) factor = widen_factors(255u);
-        }
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int piece = i * 32 + lane, row = piece / kPieces;
-      const long long at = __shfl_sync(0xffffffffu, row_at, row);
-      buffer[i] = at >= 0 ? load_once(base + at + piece % kPieces * 16) : make_uint4(0u, 0u, 0u, 0u);
-    }
-    if (!kEight && drafts) {
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        const int piece = i * 32 + lane, row = piece / kPieces;
-        const long long at = __shfl_sync(0xffffffffu, row_at, row);
-        if (at < 0 || warp * 16 + row < first_draft) continue;
-        if (kValues) {
-          if (not_finite(buffer[i])) buffer[i] = make_uint4(0u, 0u, 0u, 0u);
-        } else if (not_finite(load_once(other + at + piece % kPieces * 16))) {
-          buffer[i] = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
-        }
-      }
-    }
-    ++issued;
-    if (++tile >= seg.tile1) {
-      more = next_segment(sh, seg_n, seg, lane, a.pool.status);
-      if (more) tile = seg.tile0;
-    }
-    locate();
+  settle();
+  int passed = -1;                 // slot whose scale bytes are to be passed on
+  uint32_t k_byte = 0u, v_byte = 0u;
+  const auto pass_scales = [&]() {
+    if (passed < 0) return;
+    sh->k_byte[passed][own] = static_cast<uint8_t>(k_byte);
+    sh->v_byte[passed][own] = static_cast<uint8_t>(v_byte);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh->raw_scales[passed]);
+    passed = -1;
   };
-  locate();
-#pragma unroll
-  for (int u = 0; u < kBuffers; ++u)
-    if (more) issue(raw[u], factors[u]);
-  bool ok = true;
-  while (ok && stored < issued) {
-#pragma unroll
-    for (int u = 0; u < kBuffers; ++u) {
-      if (!ok || stored >= issued) break;
-      const int stage = stored % kStages<D>, use = stored / kStages<D>;
-      if (use > 0) ok = __all_sync(0xffffffffu, mbar_wait(&empty[stage], (use - 1) & 1, a.pool.status, kValues ? 51 : 50));
-      if (!ok) break;
-      const uint32_t to = ring + stage * kTileBytes<D>;
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        const int piece = i * 32 + lane, row = piece / kPieces, c = piece % kPieces, r = warp * 16 + row;
-        const uint4 v = raw[u][i];
-        if (!kEight) {
-          sts_b32x4(to + (c / 8) * (kTile * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4), v.x, v.y, v.z, v.w);
-        } else {
-          const uint32_t both = __shfl_sync(0xffffffffu, factors[u], row);
-          const uint32_t factor = __byte_perm(both, both, 0x1010);
-          uint2 w[4] = {widen_word(v.x, factor), widen_word(v.y, factor), widen_word(v.z, factor), widen_word(v.w, factor)};
-          if ((both >> 16) != kOne) {   // values above 57344
-            const uint32_t more_factor = __byte_perm(both, both, 0x3232);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) w[k] = make_uint2(mul_bf16x2(w[k].x, more_factor), mul_bf16x2(w[k].y, more_factor));
-          }
-          // pieces 2c and 2c + 1 of the row; odd slabs store the second one first, so that eight lanes hit all banks once
-          const uint32_t slab = to + (c / 4) * (kTile * 128) + r * 128;
-          const int p0 = (2 * c) & 7, odd = (c / 4) & 1;
-          const uint32_t at0 = slab + ((p0 ^ (r & 7)) << 4), at1 = slab + (((p0 + 1) ^ (r & 7)) << 4);
-          if (odd) {
-            sts_b32x4(at1, w[2].x, w[2].y, w[3].x, w[3].y);
-            sts_b32x4(at0, w[0].x, w[0].y, w[1].x, w[1].y);
-          } else {
-            sts_b32x4(at0, w[0].x, w[0].y, w[1].x, w[1].y);
-            sts_b32x4(at1, w[2].x, w[2].y, w[3].x, w[3].y);
-          }
-        }
-      }
-      fence_proxy_async();
+  for (;; n += 2, tile += 2, settle()) {
+    const int slot = n % kRing, use = n / kRing;
+    if (!more && !kEight) break;
+    // (with two slots this unit's is the one whose scales are still to be passed on)
+    if (kEight && kRing == 2) pass_scales();
+    if (use > 0) {
+      if (!__all_sync(0xffffffffu, mbar_wait(kEight ? &sh->raw_empty[slot] : &sh->k_empty[slot], (use - 1) & 1, status, 50))) return;
+      if (!kEight && !__all_sync(0xffffffffu, mbar_wait(&sh->v_empty[slot], (use - 1) & 1, status, 51))) return;
+    }
+    if (!more) {   // the range ends, for the widening warps of this half and parity as well
+      if (first_row == 0 && lane == 0) sh->draft_row[slot] = -1;
       __syncwarp();
-      if (lane == 0) mbar_arrive(&full[stage]);
-      ++stored;
-      if (more) issue(raw[u], factors[u]);
+      if (lane == 0) mbar_arrive(&sh->raw_scales[slot]);
+      break;
+    }
+    const int t = tile * kTile + own, draft_row = seg.count > 1 ? max(0, seg.prefix - tile * kTile) : kTile;
+    long long row_at = -1;         // byte offset of the lane's row
+    size_t scale_at = 0;
+    if (t < seg.prefix + seg.count) {
+      if (page < 0 || (a.pool.table && page >= a.pool.num_pages)) {
+        report_status(status, 48, kBadPage);   // (a slot past the pages was reported as such before)
+      } else {
+        const int inside = t - (page_shift >= 0 ? t >> page_shift << page_shift : t / a.pool.page_size * a.pool.page_size);
+        row_at = static_cast<long long>((static_cast<size_t>(page) * a.pool.page_stride + static_cast<size_t>(inside) * a.pool.token_stride +
+                                         static_cast<size_t>(seg.kv_head) * D) * kElement);
+        if (kEight) scale_at = static_cast<size_t>(page) * a.pool.scale_page + static_cast<size_t>(inside) * a.pool.scale_token + seg.kv_head;
+      }
+    }
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+      const uint32_t to = (side ? v_ring : k_ring) + slot * kBytes;
+      const char* base = static_cast<const char*>(side ? a.pool.v : a.pool.k);
+#pragma unroll 4
+      for (int i = 0; i < kLoads; ++i) {
+        const int row = i * (32 / kPieces) + lane / kPieces, c = lane % kPieces, r = first_row + row;
+        const long long at = __shfl_sync(0xffffffffu, row_at, row);
+        copy16(kEight ? to + r * D + c * 16 : tile_piece(to, r, c), base + (at >= 0 ? at + c * 16 : 0), at >= 0);
+      }
+      if (kEight || draft_row >= first_row + 32) arrive_behind_copies(side ? &v_full[slot] : &k_full[slot]);
+    }
+    if (!kEight && draft_row < first_row + 32) {
+      // Drafts that not every node sees: a value row that is not finite must not meet the zero weights of those that do
+      // not see it.  It becomes zeros, and the key row NaN, which gives those that see it NaN scores and touches no
+      // other node.  (8-bit rows: their scale byte says so, when they are widened.)  A lane looks at its own copies.
+      asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll 4
+      for (int i = 0; i < kLoads; ++i) {
+        const int r = first_row + i * (32 / kPieces) + lane / kPieces, c = lane % kPieces;
+        if (r >= draft_row && not_finite(lds_b32x4(tile_piece(v_ring + slot * kBytes, r, c)))) {
+          sts_b32x4(tile_piece(v_ring + slot * kBytes, r, c), 0u, 0u, 0u, 0u);
+          sts_b32x4(tile_piece(k_ring + slot * kBytes, r, c), 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
+        }
+      }
+      mbar_arrive(&k_full[slot]);
+      mbar_arrive(&v_full[slot]);
+    }
+    if (kEight) {
+      pass_scales();
+      k_byte = load_byte(a.pool.k_scales + scale_at, row_at >= 0);
+      v_byte = load_byte(a.pool.v_scales + scale_at, row_at >= 0);
+      passed = slot;
+      if (first_row == 0 && lane == 0) sh->draft_row[slot] = draft_row;
+    }
+  }
+  if (kEight) pass_scales();
+}
+
+// ---- 8-bit codes to fp16 -------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t halves_of(uint32_t codes) {   // two codes in the low 16 bits -> two fp16
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<uint16_t>(codes)));
+  return r;
+}
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// A row's scale byte: 2^n times any of its codes is exact in fp16 for -15 <= n <= 7 (2^-24 to 57344; n = 0 stands in for
+// rows that are not finite, whose codes are NaN).
+constexpr uint32_t kHalfOne = 0x3c003c00u;
+__device__ __forceinline__ bool fits_fp16(uint32_t byte) { return byte == 255u || (byte >= 112u && byte <= 134u); }
+__device__ __forceinline__ uint32_t half_power(uint32_t byte) {
+  const uint32_t h = byte == 255u ? 0x3c00u : byte >= 113u ? (byte - 112u) << 10 : 0x200u;   // 2^-15 is subnormal
+  return h | h << 16;
+}
+
+// Eight warps: every fourth half of the key tiles, or of the value tiles, each.
+template <int D>
+__device__ __forceinline__ void widen_tiles(Shared<D, true>* sh, uint32_t raw_ring, uint32_t ring, uint32_t* status, int warp, int lane, bool values) {
+  constexpr int kTiles = kStages<D, true>, kRaw = kRawStages<D>, kPieces = D / 16, kStep = 32 / kPieces;   // rows per step
+  const int first_row = (warp & 1) * 32;
+  const int row = lane / kPieces, c = lane % kPieces;
+  // Channels 16c .. 16c + 15 are pieces 2c and 2c + 1 of the tile's row; odd slabs store the second first, so that eight lanes
+  // hit all banks once.  A step is kStep rows, so the swizzle of the two pieces repeats every 8 / kStep steps.
+  const int second = c / 4 & 1, slab = c / 4 * (kTile * 128), p0 = (2 * c + second) & 7, p1 = (2 * c + 1 - second) & 7;
+  for (int n = warp >> 1;; n += 2) {
+    const int slot = n % kRaw, stage = n % kTiles, use = n / kTiles, scale_slot = n % (2 * kTiles);
+    if (!__all_sync(0xffffffffu, mbar_wait(&sh->raw_scales[slot], (n / kRaw) & 1, status, 47))) return;
+    const int draft_row = sh->draft_row[slot];
+    if (draft_row < 0) return;
+    // the rows' factors: in the codes for all rows of the tile or for none
+    const uint32_t k[2] = {sh->k_byte[slot][lane], sh->k_byte[slot][lane + 32]}, v[2] = {sh->v_byte[slot][lane], sh->v_byte[slot][lane + 32]};
+    const bool k_fits = __all_sync(0xffffffffu, fits_fp16(k[0]) && fits_fp16(k[1]));
+    const bool v_fits = __all_sync(0xffffffffu, fits_fp16(v[0]) && fits_fp16(v[1]));
+    const uint32_t own_k = first_row ? k[1] : k[0], own_v = first_row ? v[1] : v[0];   // of row first_row + lane
+    uint32_t factor = kHalfOne;
+    if (values ? v_fits : k_fits) factor = half_power(values ? own_v : own_k);
+    // Of drafts that not every node sees, values that are not finite are stored as zeros and their keys as NaN (see above).
+    const bool hidden = own_v == 255u && first_row + lane >= draft_row;
+    if (!values && hidden) factor = 0x7fff7fffu;
+    const unsigned zeros = __ballot_sync(0xffffffffu, values && hidden);
+    if (use > 0 && !__all_sync(0xffffffffu, mbar_wait(values ? &sh->v_empty[stage] : &sh->k_empty[stage], (use - 1) & 1, status, values ? 46 : 45))) return;
+    if (!values && first_row == 0) {
+      uint32_t largest = 127u;
+      if (!k_fits || !v_fits) {
+#pragma unroll
+        for (int o = 0; o < 2; ++o) {
+          sh->k_factor[scale_slot][lane + 32 * o] = k_fits || k[o] == 255u ? 1.0f : e8m0_value(k[o]);
+          sh->v_factor[scale_slot][lane + 32 * o] = v_fits || v[o] == 255u ? 1.0f : e8m0_value(v[o]);
+        }
+        if (!v_fits) largest = __reduce_max_sync(0xffffffffu, max(v[0] == 255u ? 0u : v[0], v[1] == 255u ? 0u : v[1]));
+      }
+      if (lane == 0) {
+        sh->scaled[scale_slot] = !k_fits || !v_fits;
+        sh->v_largest[scale_slot] = static_cast<int>(largest) - 127;
+      }
+    }
+    if (!__all_sync(0xffffffffu, mbar_wait(values ? &sh->raw_v[slot] : &sh->raw_k[slot], (n / kRaw) & 1, status, 44))) return;
+    uint32_t from = raw_ring + slot * (kTile * D) + (first_row + row) * D + c * 16;
+    uint32_t to = ring + stage * kTileBytes<D> + slab + (first_row + row) * 128;
+#pragma unroll 4
+    for (int i = 0; i < 32 / kStep; ++i) {
+      const int r = i * kStep + row, swizzle = r & 7;
+      const uint32_t f = __shfl_sync(0xffffffffu, factor, r);
+      const uint64_t first = lds_b64(from + second * 8), other = lds_b64(from + 8 - second * 8);
+      uint32_t x = static_cast<uint32_t>(first), y = static_cast<uint32_t>(first >> 32);
+      uint32_t z = static_cast<uint32_t>(other), w = static_cast<uint32_t>(other >> 32);
+      if (zeros != 0u && (zeros >> r & 1u)) x = y = z = w = 0u;
+      sts_b32x4(to + ((p0 ^ swizzle) << 4), mul_f16x2(halves_of(x), f), mul_f16x2(halves_of(x >> 16), f), mul_f16x2(halves_of(y), f),
+                mul_f16x2(halves_of(y >> 16), f));
+      sts_b32x4(to + ((p1 ^ swizzle) << 4), mul_f16x2(halves_of(z), f), mul_f16x2(halves_of(z >> 16), f), mul_f16x2(halves_of(w), f),
+                mul_f16x2(halves_of(w >> 16), f));
+      from += kStep * D;
+      to += kStep * 128;
+    }
+    __syncwarp();
+    if (lane == 0) {
+      mbar_arrive(values ? &sh->v_full[stage] : &sh->k_full[stage]);
+      mbar_arrive(&sh->raw_empty[slot]);
     }
   }
 }
+
+template <int D, bool kEight>
+constexpr int kRingBytes = 2 * kStages<D, kEight> * kTileBytes<D> + (kEight ? 2 * kRawStages<D> * kTile * D : 0);
 
 // ---- output --------------------------------------------------------------------------------------------------
 struct Partials {
@@ -354,6 +433,12 @@ __device__ __forceinline__ Partials partials_of(const TreeArgs& a) {
   p.ml = static_cast<float2*>(a.workspace);
   p.acc = reinterpret_cast<float*>(p.ml + static_cast<size_t>((2 * kMaxCtas * p.rows + 1) & ~1));
   return p;
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
 }
 
 // Eight neighbouring channels of one output row.
@@ -380,24 +465,35 @@ __device__ __forceinline__ bool gate_in_pieces(const TreeArgs& a) {
 }
 
 template <int D, bool kEight>
-__global__ void __launch_bounds__(kThreads, 1) tree_decode_sm100(TreeArgs a) {
+__global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(TreeArgs a) {
   constexpr bool kOneO = D == 256;                       // one accumulator for both score buffers
   constexpr uint32_t kColO1 = D, kColS = kOneO ? 256 : 2 * D, kColQ = kColS + 128;
   static_assert(kColQ + (kOneO ? D / 2 : D) <= 512, "tensor memory");
-  constexpr uint32_t kIdescQK = umma_idesc_bf16(128, kTile, false), kIdescPV = umma_idesc_bf16(128, D, true);
+  constexpr uint32_t kBf16 = 1u << 7 | 1u << 10;   // operand types: bf16, or fp16 for 8-bit caches
+  constexpr uint32_t kIdescQK = umma_idesc_bf16(128, kTile, false) ^ (kEight ? kBf16 : 0u);
+  constexpr uint32_t kIdescPV = umma_idesc_bf16(128, D, true) ^ (kEight ? kBf16 : 0u);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  Shared<D>* sh = reinterpret_cast<Shared<D>*>(smem + 2 * kStages<D> * kTileBytes<D>);
-  const uint32_t k_ring = smem_u32(smem), v_ring = k_ring + kStages<D> * kTileBytes<D>;
+  Shared<D, kEight>* sh = reinterpret_cast<Shared<D, kEight>*>(smem + kRingBytes<D, kEight>);
+  const uint32_t k_ring = smem_u32(smem), v_ring = k_ring + kStages<D, kEight> * kTileBytes<D>;
+  const uint32_t raw_k = v_ring + kStages<D, kEight> * kTileBytes<D>, raw_v = raw_k + kRawStages<D> * kTile * D;   // 8-bit caches
   const int warp = uniform_warp_index(), lane = threadIdx.x % 32;
   pdl_launch_dependents();   // the merge may be placed as SMs free up; it waits for this grid's end
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages<D>; ++s) {
-      mbar_init(&sh->k_full[s], 4);
-      mbar_init(&sh->v_full[s], 4);
+    for (int s = 0; s < kStages<D, kEight>; ++s) {
+      mbar_init(&sh->k_full[s], kEight ? 2 : 64);
+      mbar_init(&sh->v_full[s], kEight ? 2 : 64);
       mbar_init(&sh->k_empty[s], 1);
       mbar_init(&sh->v_empty[s], 1);
+    }
+    if (kEight) {
+      for (int r = 0; r < kRawStages<D>; ++r) {
+        mbar_init(&sh->raw_k[r], 64);
+        mbar_init(&sh->raw_v[r], 64);
+        mbar_init(&sh->raw_scales[r], 2);
+        mbar_init(&sh->raw_empty[r], 4);
+      }
     }
     for (int i = 0; i < kSegments; ++i) {
       mbar_init(&sh->seg_full[i], 1);
@@ -406,7 +502,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_sm100(TreeArgs a) {
     for (int x = 0; x < 2; ++x) {
       mbar_init(&sh->q_full[x], 4);
       mbar_init(&sh->s_full[x], 1);
+      mbar_init(&sh->p_half[x], 4);
       mbar_init(&sh->p_full[x], 4);
+      mbar_init(&sh->pv_half[x], 1);
       mbar_init(&sh->pv_done[x], 1);
     }
     mbar_init(&sh->ml_full, 8);
@@ -423,10 +521,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_sm100(TreeArgs a) {
   const uint32_t tmem = sh->tmem;
   uint32_t* status = a.pool.status;
 
-  // Register file: 640 threads x 96 at launch; the issuing warpgroup gives 56 x 128 back, of which the softmax ones
-  // take 16 x 256 and the loaders 8 x 256.
+  // Register file: 512 threads x 128, nothing to move; or 768 x 80 (of 480 per thread of six warpgroups: issue 40,
+  // softmax 2 x 112, loads 56, widening 2 x 72).
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (kEight) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     if (warp == 0) {
       // ---------------------------------------------------------------- MMA issue
       int tile_n = 0, q_n[2] = {0, 0}, p_n[2] = {0, 0};   // tiles, queries and P handed over so far
@@ -441,9 +539,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_sm100(TreeArgs a) {
           ok = __all_sync(0xffffffffu, mbar_wait(&sh->q_full[x], q_n[x]++ & 1, status, 52));
         if (!ok) break;
         const auto issue_qk = [&](int i) -> bool {
-          const int x = i & 1, n = tile_n + (pair ? i >> 1 : i), stage = n % kStages<D>;
+          const int x = i & 1, n = tile_n + (pair ? i >> 1 : i), stage = n % kStages<D, kEight>;
           if (!pair || x == 0) {
-            if (!__all_sync(0xffffffffu, mbar_wait(&sh->k_full[stage], (n / kStages<D>) & 1, status, 53))) return false;
+            if (!__all_sync(0xffffffffu, mbar_wait(&sh->k_full[stage], (n / kStages<D, kEight>) & 1, status, 53))) return false;
+            fence_proxy_async();   // the loaders' stores, before the tensor cores read them
           }
           tc_fence_after();
           const uint64_t k_desc = umma_desc_sw128(k_ring + stage * kTileBytes<D>, 16, 1024);
@@ -459,19 +558,29 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_sm100(TreeArgs a) {
           return true;
         };
         const auto issue_pv = [&](int i) -> bool {
-          const int x = i & 1, j = pair ? i >> 1 : i, n = tile_n + j, stage = n % kStages<D>;
+          const int x = i & 1, j = pair ? i >> 1 : i, n = tile_n + j, stage = n % kStages<D, kEight>;
           if (!pair || x == 0) {
-            if (!__all_sync(0xffffffffu, mbar_wait(&sh->v_full[stage], (n / kStages<D>) & 1, status, 54))) return false;
+            if (!__all_sync(0xffffffffu, mbar_wait(&sh->v_full[stage], (n / kStages<D, kEight>) & 1, status, 54))) return false;
+            fence_proxy_async();
           }
-          if (!__all_sync(0xffffffffu, mbar_wait(&sh->p_full[x], p_n[x]++ & 1, status, 55))) return false;
-          tc_fence_after();
           const uint64_t v_desc = umma_desc_sw128(v_ring + stage * kTileBytes<D>, kTile * 128, 1024);
           const bool add = kOneO ? i > 0 : pair ? j > 0 : i > 1;
+          const uint32_t phase = p_n[x]++ & 1, o = tmem + (kOneO ? 0u : x * kColO1), p = tmem + kColS + x * kTile;
+          // the weights come in two halves of the tile's keys; the first half's product runs under the second's softmax
+          if (!__all_sync(0xffffffffu, mbar_wait(&sh->p_half[x], phase, status, 55))) return false;
+          tc_fence_after();
           if (elect_one()) {
 #pragma unroll
-            for (int ks = 0; ks < kTile / 16; ++ks)
-              umma_ts(tmem + (kOneO ? 0u : x * kColO1), tmem + kColS + x * kTile + ks * 8, v_desc + ks * (2048 >> 4), kIdescPV, add || ks > 0);
-            tc_commit(&sh->pv_done[kOneO ? 0 : x]);
+            for (int ks = 0; ks < kTile / 32; ++ks) umma_ts(o, p + ks * 8, v_desc + ks * (2048 >> 4), kIdescPV, add || ks > 0);
+            tc_commit(&sh->pv_half[x]);
+          }
+          __syncwarp();
+          if (!__all_sync(0xffffffffu, mbar_wait(&sh->p_full[x], phase, status, 55))) return false;
+          tc_fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int ks = kTile / 32; ks < kTile / 16; ++ks) umma_ts(o, p + ks * 8, v_desc + ks * (2048 >> 4), kIdescPV, true);
+            tc_commit(&sh->pv_done[x]);
             if (!pair || x == 1) tc_commit(&sh->v_empty[stage]);
           }
           __syncwarp();
@@ -514,14 +623,15 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_sm100(TreeArgs a) {
       }
     }
   } else if (warp < 12) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
+    if (kEight) asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
     // ------------------------------------------------------------------ softmax, one thread per row
     const int x = (warp - 4) / 4, quarter = warp & 3, row = quarter * 32 + lane, group = a.q_heads / a.kv_heads;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
     const float scale_log2 = a.scale * 1.4426950408889634f;
     const Partials parts = partials_of(a);
     const bool gate_pieces = gate_in_pieces(a);
-    int s_n[2] = {0, 0}, pv_n[2] = {0, 0}, met = 0;   // score tiles taken, products into each O, meetings of the streams
+    // tiles of the range; those of the score buffers 0 and 1; meetings of the streams
+    int tile_n = 0, tiles_0 = 0, tiles_1 = 0, met = 0;
     bool ok = true;
     int seg_n = 0;
     Segment seg;
@@ -533,10 +643,26 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_sm100(TreeArgs a) {
       const bool live = own_row < seg.rows, warp_live = (pair ? x * 128 : 0) + quarter * 32 < seg.rows;
       const int r = seg.row0 + own_row, node = r / group, head = seg.kv_head * group + r % group;
       const size_t token = static_cast<size_t>(seg.b) * a.nodes + node;
+      const uint4* q = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) + (token * a.q_heads + head) * D);
+      float row_scale = scale_log2;   // of the scores as the tensor cores return them, into powers of two
+      float q_scale = 1.0f;
+      if (kEight && warp_live) {
+        // fp16 holds the row exactly once its largest value is between 1 and 2 (what is below 2^-14 of that loses bits
+        // beyond those that the row's scores have); the scores get the power of two back
+        uint32_t largest = 0u;
+#pragma unroll 4
+        for (int i = 0; i < D / 8; ++i) {
+          const uint4 v = live ? q[i] : make_uint4(0u, 0u, 0u, 0u);
+          largest = max(largest, max(max(v.x & 0x7fffu, v.y & 0x7fffu), max(v.z & 0x7fffu, v.w & 0x7fffu)));
+          largest = max(largest, max(max(v.x & 0x7fff0000u, v.y & 0x7fff0000u), max(v.z & 0x7fff0000u, v.w & 0x7fff0000u)) >> 16);
+        }
+        const uint32_t e = min(max(largest >> 7, 2u), 252u);
+        q_scale = __uint_as_float((254u - e) << 23);
+        row_scale = scale_log2 * __uint_as_float(e << 23);
+      }
       // ---- the queries, into TMEM
       if (pair || x == 0) {
         if (warp_live) {
-          const uint4* q = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) + (token * a.q_heads + head) * D);
 #pragma unroll 1
           for (int c = 0; c < D / 64; ++c) {
             uint32_t w[32];
@@ -544,6 +670,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_sm100(TreeArgs a) {
             for (int i = 0; i < 8; ++i) {
               const uint4 v = live ? q[c * 8 + i] : make_uint4(0u, 0u, 0u, 0u);
               w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+            }
+            if (kEight) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                w[i] = pack_f16(bf16_lo(w[i]) * q_scale, bf16_hi(w[i]) * q_scale);
             }
             tmem_st32(lanes + kColQ + (pair ? x * (D / 2) : 0) + c * 32, w);
           }
@@ -573,120 +704,145 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_sm100(TreeArgs a) {
         }
       }
       // ---- the tiles of this stream
-      float m_used = -INFINITY, m_true = -INFINITY, l = 0.0f;
+      // Weights are 2^(score * row_scale - reference), reference = m_used * row_scale + v_used: for 8-bit caches v_used is
+      // the largest exponent of the value rows so far, so that a weight times its row's 2^n fits fp16.
+      float m_used = -INFINITY, m_true = -INFINITY, l = 0.0f, v_used = kEight ? kSmallest : 0.0f;
       const int step = pair || kOneO ? 1 : 2;
       int done = 0;
       for (int j = pair || kOneO ? 0 : x; j < tiles && ok; j += step, ++done) {
-        const int sb = kOneO ? j & 1 : x;
-        ok = __all_sync(0xffffffffu, mbar_wait(&sh->s_full[sb], s_n[sb]++ & 1, status, 56));
+        // A parity tells the phase that is awaited from its two neighbours only: every barrier of a buffer completes once per
+        // tile, and this tile's scores were committed behind the buffer's previous product.
+        const int sb = kOneO ? j & 1 : x, phase = ((sb ? tiles_1 : tiles_0) + (kOneO ? j >> 1 : done)) & 1;
+        ok = __all_sync(0xffffffffu, mbar_wait(&sh->s_full[sb], phase, status, 56));
         if (!ok) break;
-        if (warp_live) {
-          tc_fence_after();
-          uint32_t s[2][32];
-          const uint32_t s_at = lanes + kColS + sb * kTile;
-          tmem_ld32(s_at, s[0]);
-          tmem_ld32(s_at + 32, s[1]);
-          tmem_wait_ld();
-          const int behind = (seg.tile0 + j) * kTile - seg.prefix;   // of the drafts' first slot
-          if (behind > -kTile) {
-            const uint64_t seen = behind >= 64  ? seen_hi >> (behind - 64)
-                                  : behind > 0  ? seen_lo >> behind | seen_hi << (64 - behind)
-                                  : behind == 0 ? seen_lo
-                                                : seen_lo << -behind | ((1ull << -behind) - 1);
-            const uint32_t bits[2] = {static_cast<uint32_t>(seen), static_cast<uint32_t>(seen >> 32)};
+        const uint32_t s_at = lanes + kColS + sb * kTile;
+        const int slot = (tile_n + j) % (2 * kStages<D, kEight>);
+        const uint32_t k_factor = smem_u32(sh->k_factor[slot]), v_factor = smem_u32(sh->v_factor[slot]);
+        const bool scaled = kEight && warp_live && sh->scaled[slot] != 0;   // the rare tile with rows that fp16 does not hold
+        const float v_tile = scaled ? fmaxf(v_used, static_cast<float>(sh->v_largest[slot])) : kEight ? fmaxf(v_used, 0.0f) : v_used;
+        const int behind = (seg.tile0 + j) * kTile - seg.prefix;   // of the drafts' first slot
+        uint64_t seen = ~0ull;
+        if (behind > -kTile)
+          seen = behind >= 64  ? seen_hi >> (behind - 64)
+                 : behind > 0  ? seen_lo >> behind | seen_hi << (64 - behind)
+                 : behind == 0 ? seen_lo
+                               : seen_lo << -behind | ((1ull << -behind) - 1);
+        // Half of the tile's keys at a time, in a loop: its code then fits the instruction caches beside the other
+        // warps' (straight-line code of 64 columns took twice as long), and the first half's product starts earlier.
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+          if (warp_live) {
+            if (h == 0) tc_fence_after();
+            uint32_t s[32];
+            tmem_ld32(s_at + h * 32, s);
+            tmem_wait_ld();
+            if (scaled) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+              for (int i = 0; i < 32; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) * lds_f32(k_factor + (h * 32 + i) * 4));
+            }
+            if (behind > -kTile) {
+              const uint32_t bits = static_cast<uint32_t>(seen >> (h * 32));
 #pragma unroll
               for (int i = 0; i < 32; ++i)
-                if (!(bits[h] >> i & 1u)) s[h][i] = 0xff800000u;
-          }
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(s[h][i]), __uint_as_float(s[h][i + 1]));
-          m_true = max3(fmaxf(m_true, mx[0]), mx[1], fmaxf(mx[2], mx[3]));
-          const bool grow = (m_true - m_used) * scale_log2 > kRescale;
-          if (__any_sync(0xffffffffu, grow)) {
-            const float factor = grow ? fast_exp2((m_used - m_true) * scale_log2) : 1.0f;
-            if (grow) m_used = m_true;
-            l *= factor;
-            if (done > 0) {
-              // (with its own O the previous product has ended: this tile's scores were committed behind it)
-              if (kOneO) ok = __all_sync(0xffffffffu, mbar_wait(&sh->pv_done[0], (pv_n[0] + done - 1) & 1, status, 57));
-              if (!ok) break;
-              tc_fence_after();
-#pragma unroll 1
-              for (int c = 0; c < D / 16; ++c) {
-                uint32_t o[16];
-                const uint32_t o_at = lanes + (kOneO ? 0u : x * kColO1) + c * 16;
-                tmem_ld16(o_at, o);
-                tmem_wait_ld();
-#pragma unroll
-                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
-                tmem_st16(o_at, o);
-              }
-              tmem_wait_st();
+                if (!(bits >> i & 1u)) s[i] = 0xff800000u;
             }
-          }
-          const float m_safe = m_used == -INFINITY ? 0.0f : m_used;   // nothing seen yet
-          const uint64_t scale2 = f2_pack(scale_log2, scale_log2), neg2 = f2_pack(-m_safe * scale_log2, -m_safe * scale_log2);
-          uint64_t sum2[2] = {0ull, 0ull};
+            float mx[4] = {m_true, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
+            for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+            m_true = max3(mx[0], mx[1], fmaxf(mx[2], mx[3]));
+            const bool grow = (m_true - m_used) * row_scale > kRescale;
+            if (__any_sync(0xffffffffu, grow || v_tile > v_used)) {
+              const float factor = fast_exp2((grow ? (m_used - m_true) * row_scale : 0.0f) + (v_used - v_tile));
+              if (grow) m_used = m_true;
+              v_used = v_tile;
+              l *= factor;
+              if (done > 0 || h == 1) {
+                // every product into this O must have ended: this tile's first half, the other buffer's last tile (one O);
+                // those into an own O before this tile have
+                if (h == 1) ok = __all_sync(0xffffffffu, mbar_wait(&sh->pv_half[sb], phase, status, 57));
+                else if (kOneO) ok = __all_sync(0xffffffffu, mbar_wait(&sh->pv_done[sb ^ 1], ((sb ? tiles_0 : tiles_1) + ((j - 1) >> 1)) & 1, status, 57));
+                if (!ok) break;
+                tc_fence_after();
+#pragma unroll 1
+                for (int c = 0; c < D / 16; ++c) {
+                  uint32_t o[16];
+                  const uint32_t o_at = lanes + (kOneO ? 0u : x * kColO1) + c * 16;
+                  tmem_ld16(o_at, o);
+                  tmem_wait_ld();
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
+                  tmem_st16(o_at, o);
+                }
+                tmem_wait_st();
+              }
+            }
+            const float reference = (m_used == -INFINITY ? 0.0f : m_used * row_scale) + v_used;   // (nothing seen yet: any)
+            const uint64_t scale2 = f2_pack(row_scale, row_scale), neg2 = f2_pack(-reference, -reference);
+            uint64_t sum2[2] = {0ull, 0ull};
             uint32_t packed[16];
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
               float p0, p1;
-              f2_unpack(f2_fma(f2_pack(__uint_as_float(s[h][i]), __uint_as_float(s[h][i + 1])), scale2, neg2), p0, p1);
+              f2_unpack(f2_fma(f2_pack(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), scale2, neg2), p0, p1);
               p0 = fast_exp2(p0);
               p1 = fast_exp2(p1);
               sum2[(i >> 1) & 1] = f2_add(sum2[(i >> 1) & 1], f2_pack(p0, p1));
-              packed[i / 2] = pack_bf16(p0, p1);
+              if (kEight) {   // (kept apart from the products with the rows' factors below)
+                s[i] = __float_as_uint(p0);
+                s[i + 1] = __float_as_uint(p1);
+              } else {
+                packed[i / 2] = pack_bf16(p0, p1);
+              }
+            }
+            if (scaled) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) * lds_f32(v_factor + (h * 32 + i) * 4));
+            }
+            if (kEight) {
+#pragma unroll
+              for (int i = 0; i < 32; i += 2) packed[i / 2] = pack_f16(__uint_as_float(s[i]), __uint_as_float(s[i + 1]));
             }
             tmem_st16(s_at + h * 16, packed);
+            float a0, a1, b0, b1;
+            f2_unpack(sum2[0], a0, a1);
+            f2_unpack(sum2[1], b0, b1);
+            l += (a0 + a1) + (b0 + b1);
+            tmem_wait_st();
+            tc_fence_before();
           }
-          float a0, a1, b0, b1;
-          f2_unpack(sum2[0], a0, a1);
-          f2_unpack(sum2[1], b0, b1);
-          l += (a0 + a1) + (b0 + b1);
-          tmem_wait_st();
-          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(h ? &sh->p_full[sb] : &sh->p_half[sb]);
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh->p_full[sb]);
       }
       if (!ok) break;
       const bool merged = !pair && !kOneO;
-      const int products[2] = {merged ? (tiles + 1) / 2 : tiles, merged ? tiles / 2 : pair ? tiles : 0};
-      // A parity tells the phase that is awaited from its neighbours only, so the one before must be known to be over:
-      // this stream's last scores were committed behind its last but one product (one O: behind the last but two).
-      const int own_o = kOneO ? 0 : x;
-      pv_n[0] += products[0];
-      pv_n[1] += products[1];
-      if (kOneO && tiles > 1) ok = __all_sync(0xffffffffu, mbar_wait(&sh->pv_done[0], (pv_n[0] - 2) & 1, status, 57));
-      if (ok && done > 0) ok = __all_sync(0xffffffffu, mbar_wait(&sh->pv_done[own_o], (pv_n[own_o] - 1) & 1, status, 58));
+      tile_n += tiles;
+      tiles_0 += pair ? tiles : (tiles + 1) / 2;
+      tiles_1 += pair ? tiles : tiles / 2;
+      // this stream's last product (one O: the last tile's, which ends behind all others)
+      const int last = kOneO ? (tiles - 1) & 1 : x;
+      if (kOneO || done > 0) ok = __all_sync(0xffffffffu, mbar_wait(&sh->pv_done[last], ((last ? tiles_1 : tiles_0) - 1) & 1, status, 58));
       if (!ok) break;
       tc_fence_after();
       // ---- read-out: rows of one stream, or the two streams' halves of the keys merged, half of the channels each
-      float m = m_used, f0 = 1.0f, f1 = 0.0f;
+      float m = m_used == -INFINITY ? m_used : m_used * row_scale + v_used, f0 = 1.0f, f1 = 0.0f;   // log2 units from here
       bool both = false;
       if (merged) {
-        sh->ml[x][row] = make_float2(m_used, l);
+        sh->ml[x][row] = make_float2(m, l);
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh->ml_full);
         ok = __all_sync(0xffffffffu, mbar_wait(&sh->ml_full, met & 1, status, 59));
         // (the other stream has seen its last product end before it arrived there: this returns at once)
-        if (ok && products[1 - x] > 0)
-          ok = __all_sync(0xffffffffu, mbar_wait(&sh->pv_done[1 - x], (pv_n[1 - x] - 1) & 1, status, 58));
+        if (ok && (x == 1 || tiles > 1))
+          ok = __all_sync(0xffffffffu, mbar_wait(&sh->pv_done[1 - x], ((x ? tiles_0 : tiles_1) - 1) & 1, status, 58));
         if (!ok) break;
         tc_fence_after();
         const float2 one = sh->ml[0][row], two = sh->ml[1][row];
         both = tiles > 1;
         m = both ? fmaxf(one.x, two.x) : one.x;
         const float m_safe = m == -INFINITY ? 0.0f : m;
-        f0 = fast_exp2((one.x - m_safe) * scale_log2);
-        f1 = both ? fast_exp2((two.x - m_safe) * scale_log2) : 0.0f;
+        f0 = fast_exp2(one.x - m_safe);
+        f1 = both ? fast_exp2(two.x - m_safe) : 0.0f;
         l = both ? one.y * f0 + two.y * f1 : one.y * f0;
       }
       if (warp_live) {
@@ -725,8 +881,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_sm100(TreeArgs a) {
           __syncwarp();
         }
         if (live && (x == 0 || pair)) {
-          if (!seg.whole) parts.ml[static_cast<size_t>(slot) * parts.rows + own_row] = make_float2(m * scale_log2, l);
-          else if (a.lse) a.lse[token * a.q_heads + head] = (m == -INFINITY ? 0.0f : m * a.scale) + logf(l);
+          if (!seg.whole) parts.ml[static_cast<size_t>(slot) * parts.rows + own_row] = make_float2(m, l);
+          else if (a.lse) a.lse[token * a.q_heads + head] = (m == -INFINITY ? 0.0f : m * 0.6931471805599453f) + logf(l);
         }
         tc_fence_before();
       }
@@ -738,10 +894,17 @@ __global__ void __launch_bounds__(kThreads, 1) tree_decode_sm100(TreeArgs a) {
       }
     }
   } else {
-    // ------------------------------------------------------------------ loaders
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
-    if (warp < 16) load_tiles<D, kEight, false>(a, sh, k_ring, warp - 12, lane);
-    else load_tiles<D, kEight, true>(a, sh, v_ring, warp - 16, lane);
+    // ------------------------------------------------------------------ loads, widening
+    if (warp < 16) {
+      if (kEight) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+      load_tiles<D, kEight>(a, sh, kEight ? raw_k : k_ring, kEight ? raw_v : v_ring, warp - 12, lane);
+      asm volatile("cp.async.wait_all;" ::: "memory");   // (landed long ago unless a wait ran out)
+    } else {
+      if constexpr (kEight) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        widen_tiles<D>(sh, warp < 20 ? raw_k : raw_v, warp < 20 ? k_ring : v_ring, status, warp & 3, lane, warp >= 20);
+      }
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -826,14 +989,16 @@ __global__ void __launch_bounds__(256) tree_decode_merge(TreeArgs a, int ctas) {
 template <int D, bool kEight>
 cudaError_t launch(cudaStream_t stream, const TreeArgs& a) {
   const int rows = slot_rows(a.nodes, a.q_heads, a.kv_heads, D);
-  const long long units = static_cast<long long>(a.batch) * a.kv_heads * ((a.nodes * (a.q_heads / a.kv_heads) + kGroupRows<D> - 1) / kGroupRows<D>);
+  const long long units = static_cast<long long>(a.batch) * a.kv_heads * ((a.nodes * (a.q_heads / a.kv_heads) + group_rows(D) - 1) / group_rows(D));
   const long long tiles = units * ((static_cast<long long>(a.max_prefix) + a.nodes + kTile - 1) / kTile);
   const int ctas = static_cast<int>(tiles < kMaxCtas ? tiles : kMaxCtas);
-  constexpr int kBytes = 2 * kStages<D> * kTileBytes<D> + static_cast<int>(sizeof(Shared<D>)) + 1024;
+  constexpr int kBytes = kRingBytes<D, kEight> + static_cast<int>(sizeof(Shared<D, kEight>)) + 1024;
   static_assert(kBytes <= 227 * 1024, "shared memory");
+  using S = Shared<D, kEight>;
+  static_assert(offsetof(S, k_factor) % 16 == 0 && offsetof(S, ml) % 8 == 0 && alignof(S) == 16, "alignment");
   cudaError_t e = cudaFuncSetAttribute(tree_decode_sm100<D, kEight>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
   if (e != cudaSuccess) return e;
-  tree_decode_sm100<D, kEight><<<ctas, kThreads, kBytes, stream>>>(a);
+  tree_decode_sm100<D, kEight><<<ctas, kThreads<kEight>, kBytes, stream>>>(a);
   if ((e = cudaGetLastError()) != cudaSuccess || ctas == 1) return e;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(ctas - 1, (rows + 7) / 8);
