@@ -81,6 +81,16 @@ bool draft_shape(int batch, int nodes, int q_heads, int kv_heads, int head_dim) 
          head_dim <= 256 && batch <= 65535 && fits_int(batch, nodes, q_heads);
 }
 
+// Rows that share a KV head fit one 16-row tile of mma.sync (at width 256 half of it: registers).
+bool few_rows(int nodes, int q_heads, int kv_heads, int head_dim) { return nodes * (q_heads / kv_heads) <= (head_dim == 256 ? 8 : 16); }
+
+bool tensor_core_shape(const pluto::TreeArgs& a) {
+  const size_t element = a.pool.store == pluto::kStoreBf16 ? 2 : 1;
+  return a.q_is_bf16 && a.out_is_bf16 && a.pool.store != pluto::kStoreFp32 && (a.dim == 64 || a.dim == 128 || a.dim == 256) &&
+         aligned_to(a.q, 16) && aligned_to(a.out, 16) && aligned_to(a.pool.k, 16) && aligned_to(a.pool.v, 16) &&
+         a.pool.page_stride * element % 16 == 0 && a.pool.token_stride * element % 16 == 0;
+}
+
 }  // namespace
 
 extern "C" {
@@ -147,8 +157,9 @@ int pluto_draft_prepare(pluto_stream_t stream, const void* q_in, const void* k_i
 
 size_t pluto_gqa_tree_decode_workspace_bytes(int batch, int nodes, int q_heads, int kv_heads, int head_dim) {
   if (!draft_shape(batch, nodes, q_heads, kv_heads, head_dim) || nodes > pluto::kMaxDraftNodes) return 0;
-  const size_t parts = pluto::tree_decode_tc_workspace_bytes(nodes, q_heads, kv_heads, head_dim);
-  return parts > 0 ? parts : 16;
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256) return 16;
+  return few_rows(nodes, q_heads, kv_heads, head_dim) ? pluto::tree_decode_mma_workspace_bytes(nodes, q_heads, kv_heads, head_dim)
+                                            : pluto::tree_decode_tc_workspace_bytes(nodes, q_heads, kv_heads, head_dim);
 }
 
 int pluto_gqa_tree_decode(pluto_stream_t stream, const void* q, int q_dtype, const void* gate, int gate_dtype,
@@ -178,7 +189,9 @@ int pluto_gqa_tree_decode(pluto_stream_t stream, const void* q, int q_dtype, con
   a.round = round_to_bf16;
   a.scale = 1.0f / sqrtf(static_cast<float>(head_dim));
   if (int c = take_status(&a.pool.status)) return c;
-  return pluto::report_cuda(pluto::tree_decode_tc_supported(a) ? pluto::tree_decode_tc(stream, a) : pluto::tree_decode_exact(stream, a),
+  return pluto::report_cuda(!tensor_core_shape(a)                    ? pluto::tree_decode_exact(stream, a)
+                            : few_rows(nodes, q_heads, kv_heads, head_dim) ? pluto::tree_decode_mma(stream, a)
+                                                                 : pluto::tree_decode_tc(stream, a),
                             "attention of drafted tokens");
 }
 

@@ -1,0 +1,532 @@
+// Attention of drafted tokens over a bf16 or 8-bit cache where few rows share a KV head (nodes * query heads per KV head
+// at most 16, at width 256 at most 8): single tokens and short drafts.  Bound by HBM: the cache is read once, the
+// rows are one 16-row tile of mma.sync (m16n8k16, fp32 accumulation), and the arithmetic has to stay out of the way.
+//
+// A warp works alone: it streams its range of the line (tree_line.cuh) in steps of sixteen tokens through a ring of its
+// own in shared memory (asynchronous 16-byte copies, up to 160 KB in flight per SM), so its main loop meets no other
+// warp and no barrier.  Pages may have any size, rows any 16-byte stride.
+//
+// The codes of an 8-bit cache become MMA operands in registers, one instruction per two codes and exact.  The order of
+// the channels in a product is free as long as both operands share it, so a lane takes whole 16-byte pieces: of the
+// keys the pieces of its row, of the values the piece of its columns from four rows, paired by byte permutes.  The
+// rows' powers of two stay out of the products: a key's multiplies its scores, a value's its weights, relative to
+// the largest so far so that the products fit fp16 (P carries 11 bits).  Over bf16 caches P enters as a bf16 part and
+// its bf16 remainder, 16 bits, as in gqa_decode.cu.
+#include "tree_line.cuh"
+
+namespace pluto {
+namespace {
+
+constexpr int kTile = 16;          // tokens of a step
+constexpr int kWarps = 4;
+constexpr float kRescale = 8.0f;   // the accumulator is rescaled when the maximum has grown by more than 2^8
+constexpr float kSmallest = -100.0f;   // exponent of the value rows from which smaller ones are taken for as large
+
+template <int D, bool kEight>
+constexpr int kRowBytes = D * (kEight ? 1 : 2);
+template <int D, bool kEight>
+constexpr int kStageBytes = 2 * kTile * kRowBytes<D, kEight>;   // keys, then values
+// CTAs per SM, and steps in the ring of a warp
+template <int D, bool kEight>
+constexpr int kCtas = D == 256 && !kEight ? 1 : 2;
+template <int D, bool kEight>
+constexpr int kStages = D == 256 ? 3 : D == 128 ? (kEight ? 6 : 3) : (kEight ? 8 : 6);
+template <int D, bool kEight>
+constexpr int kWarpBytes = kStages<D, kEight> * (kStageBytes<D, kEight> + 2 * kTile);   // and two scale bytes per token
+
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool there) {   // zeros where it is not
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft>
+__device__ __forceinline__ void wait_copies() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
+}
+__device__ __forceinline__ uint32_t load_byte(const uint8_t* p, bool there) {   // 127 where it is not
+  uint32_t v;
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\tmov.u32 %0, 127;\n\t@p ld.global.u8 %0, [%1];\n\t}"
+               : "=r"(v) : "l"(p), "r"(static_cast<uint32_t>(there)));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds_b8(uint32_t at) {
+  uint32_t v;
+  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t lds_b16(uint32_t at) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts_b8(uint32_t at, uint32_t v) {
+  asm volatile("st.shared.u8 [%0], %1;" ::"r"(at), "r"(v) : "memory");
+}
+__device__ __forceinline__ uint32_t halves_of(uint32_t codes) {   // two codes in the low 16 bits -> two fp16
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<uint16_t>(codes)));
+  return r;
+}
+// d (+)= a b: rows lane / 4 (d[0], d[1]) and, unless kHalf, lane / 4 + 8
+template <bool kEight, bool kHalf>
+__device__ __forceinline__ void mma(float (&d)[kHalf ? 2 : 4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  float x = 0.0f, y = 0.0f;
+  float& d2 = kHalf ? x : d[kHalf ? 0 : 2];
+  float& d3 = kHalf ? y : d[kHalf ? 0 : 3];
+  if (kEight)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d2), "+f"(d3) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d2), "+f"(d3) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ bool not_finite(uint32_t pair) {
+  return (pair & 0x7f80u) == 0x7f80u || (pair & 0x7f800000u) == 0x7f800000u;
+}
+
+// Byte offset of 16-byte piece c of row r in a tile: pieces are exchanged within 128 bytes so that the reads below, which
+// take the same piece of several rows, hit all banks.
+template <int kBytes>
+__device__ __forceinline__ uint32_t piece_at(int r, int c) {
+  return r * kBytes + (kBytes == 64 ? (c ^ (r >> 1 & 3)) << 4 : ((c & ~7) | ((c ^ r) & 7)) << 4);
+}
+
+template <int D, bool kEight, bool kHalf>   // kHalf: at most eight rows
+__global__ void __launch_bounds__(kWarps * 32, kCtas<D, kEight>) tree_decode_mma_kernel(TreeArgs a, LineShape shape) {
+  constexpr int kBytes = kRowBytes<D, kEight>, kPieces = kBytes / 16, kS = kStages<D, kEight>;
+  constexpr int kH = kHalf ? 1 : 2;                     // rows of a lane
+  constexpr int kC = kHalf ? 2 : 4;                     // values of an accumulator block in a lane
+  constexpr int kChunks = kPieces < 4 ? 1 : kPieces / 4, kSteps = kEight ? 4 : 2;   // pieces of a key row per lane, k steps per piece
+  constexpr int kBlocks = D / 8;                        // accumulator blocks
+  static_assert(kChunks * kSteps == D / 16, "channels");
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int warp = uniform_warp_index(), lane = threadIdx.x % 32, quad = lane / 4, t4 = lane % 4;
+  const uint32_t ring = smem_u32(smem) + warp * kS * kStageBytes<D, kEight>;
+  const uint32_t scale_ring = smem_u32(smem) + kWarps * kS * kStageBytes<D, kEight> + warp * kS * 2 * kTile;
+  uint32_t* status = a.pool.status;
+  const char* k_base = static_cast<const char*>(a.pool.k);
+  const char* v_base = static_cast<const char*>(a.pool.v);
+  const int page_shift = (a.pool.page_size & (a.pool.page_size - 1)) == 0 ? __ffs(a.pool.page_size) - 1 : -1;
+  const int group = a.q_heads / a.kv_heads;
+  const float scale_log2 = a.scale * 1.4426950408889634f;
+  const Partials parts = partials_of(a, shape);
+  const bool gate_pieces = gate_in_pieces(a);
+  pdl_launch_dependents();   // the merge may be placed as SMs free up; it waits for this grid's end
+
+  const int worker = blockIdx.x * kWarps + warp;
+  Cursor cursor;
+  cursor.seek(a, shape, worker, lane);
+
+  // ---- copies: the next step to issue, kS - 1 ahead of the one that is worked on
+  Cursor ahead = cursor;
+  Segment load;
+  bool more = ahead.next(a, load);
+  int tile = more ? load.tile0 : 0, page = -1, issued = 0, passed = -1;
+  uint32_t k_byte = 0u, v_byte = 0u;
+  const auto fetch_page = [&]() {   // of row lane % 16 of the next step
+    const int t = tile * kTile + lane % 16;
+    page = -1;
+    if (!more || t >= load.prefix + load.count) return;
+    const int block = page_shift >= 0 ? t >> page_shift : t / a.pool.page_size;
+    if (block >= (a.pool.table ? a.pool.max_blocks : 1)) report_status(status, 48, kBadLength);
+    else page = a.pool.table ? a.pool.table[static_cast<size_t>(load.b) * a.pool.max_blocks + block] : load.b;
+  };
+  fetch_page();
+  const auto issue = [&]() {
+    if (kEight && passed >= 0) {   // the scale bytes asked for by the last issue have arrived meanwhile
+      if (lane < kTile) {
+        sts_b8(scale_ring + passed * 2 * kTile + lane, k_byte);
+        sts_b8(scale_ring + passed * 2 * kTile + kTile + lane, v_byte);
+      }
+      passed = -1;
+    }
+    if (more) {
+      const int t = tile * kTile + lane % 16, slot = issued % kS;
+      long long row_at = -1;
+      size_t scale_at = 0;
+      if (t < load.prefix + load.count) {
+        if (page < 0 || (a.pool.table && page >= a.pool.num_pages)) {
+          report_status(status, 48, kBadPage);   // (a slot past the pages was reported as such before)
+        } else {
+          const int inside = t - (page_shift >= 0 ? t >> page_shift << page_shift : t / a.pool.page_size * a.pool.page_size);
+          row_at = static_cast<long long>((static_cast<size_t>(page) * a.pool.page_stride + static_cast<size_t>(inside) * a.pool.token_stride +
+                                           static_cast<size_t>(load.kv_head) * D) * (kEight ? 1 : 2));
+          if (kEight) scale_at = static_cast<size_t>(page) * a.pool.scale_page + static_cast<size_t>(inside) * a.pool.scale_token + load.kv_head;
+        }
+      }
+      const uint32_t to = ring + slot * kStageBytes<D, kEight>;
+#pragma unroll
+      for (int i = 0; i < kPieces / 2; ++i) {
+        const int row = i * (32 / kPieces) + lane / kPieces, c = lane % kPieces;
+        const long long at = __shfl_sync(0xffffffffu, row_at, row);
+        const uint32_t piece = to + piece_at<kBytes>(row, c);
+        const long long from = at >= 0 ? at + c * 16 : 0;
+        copy16(piece, k_base + from, at >= 0);
+        copy16(piece + kTile * kBytes, v_base + from, at >= 0);
+      }
+      if (kEight) {
+        k_byte = load_byte(a.pool.k_scales + scale_at, row_at >= 0);
+        v_byte = load_byte(a.pool.v_scales + scale_at, row_at >= 0);
+        passed = slot;
+      }
+      ++issued;
+      if (++tile >= load.tile1) {
+        more = ahead.next(a, load);
+        if (more) tile = load.tile0;
+      }
+      fetch_page();
+    }
+    commit_copies();
+  };
+#pragma unroll 1
+  for (int i = 0; i < kS - 1; ++i) issue();
+
+  int step = 0;   // of the range
+  Segment seg;
+  while (cursor.next(a, seg)) {
+    // ---- the queries: A fragments, columns in the order of the keys' pieces
+    uint32_t qf[D / 16][kHalf ? 2 : 4];
+    float row_scale[kH];
+#pragma unroll
+    for (int h = 0; h < kH; ++h) {
+      const int r = quad + 8 * h, node = r / group, head = seg.kv_head * group + r % group;
+      const bool live = r < seg.rows;
+      const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) + ((static_cast<size_t>(seg.b) * a.nodes + node) * a.q_heads + head) * D;
+      uint32_t largest = 0u;
+#pragma unroll
+      for (int j = 0; j < kChunks; ++j) {
+        const int c = kPieces < 8 ? t4 : 2 * t4 + (j & 1) + 8 * (j >> 1);
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+          const uint2 w = live ? *reinterpret_cast<const uint2*>(q + c * (kEight ? 16 : 8) + 4 * s) : make_uint2(0u, 0u);
+          qf[j * kSteps + s][h] = w.x;
+          qf[j * kSteps + s][kH + h] = w.y;
+          largest = max(largest, max(max(w.x & 0x7fffu, w.y & 0x7fffu), max(w.x & 0x7fff0000u, w.y & 0x7fff0000u) >> 16));
+        }
+      }
+      row_scale[h] = scale_log2;
+      if (kEight) {
+        // fp16 holds the row exactly once its largest value is between 1 and 2 (what is below 2^-14 of that loses bits
+        // beyond those that the row's scores have); the scores get the power of two back
+        largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+        largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+        const uint32_t e = min(max(largest >> 7, 2u), 252u);
+        const float down = __uint_as_float((254u - e) << 23);
+        row_scale[h] = scale_log2 * __uint_as_float(e << 23);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            uint32_t& w = qf[k][u * kH + h];
+            w = pack_f16(bf16_lo(w) * down, bf16_hi(w) * down);
+          }
+      }
+    }
+    // ---- which drafts a row sees: one bit per node
+    uint32_t seen[kH] = {};
+    if (seg.tile1 * kTile > seg.prefix) {
+#pragma unroll
+      for (int h = 0; h < kH; ++h) {
+        const int r = quad + 8 * h;
+        if (r >= seg.rows) continue;
+        for (int i = r / group; i >= 0;) {
+          seen[h] |= 1u << i;
+          const int up = a.parents ? a.parents[static_cast<size_t>(seg.b) * a.nodes + i] : i - 1;
+          if (up < -1 || up >= i) report_status(status, 49, kBadDraft);   // taken as a first token's
+          i = up < i ? up : -1;
+        }
+      }
+    }
+    // Weights are 2^(score * row_scale - reference), reference = m_used + v_used: for 8-bit caches v_used is the largest
+    // exponent of the value rows seen so far, so that a weight times its row's 2^n fits fp16.
+    float m_used[kH], m_true[kH], v_used[kH], l[kH], o[kBlocks][kC];
+#pragma unroll
+    for (int h = 0; h < kH; ++h) {
+      m_used[h] = m_true[h] = -INFINITY;
+      v_used[h] = kEight ? kSmallest : 0.0f;
+      l[h] = 0.0f;
+    }
+#pragma unroll
+    for (int nb = 0; nb < kBlocks; ++nb)
+#pragma unroll
+      for (int i = 0; i < kC; ++i) o[nb][i] = 0.0f;
+
+#pragma unroll 1
+    for (int j = seg.tile0; j < seg.tile1; ++j, ++step) {
+      issue();
+      wait_copies<kS - 1>();
+      __syncwarp();
+      const int slot = step % kS;
+      const uint32_t k_tile = ring + slot * kStageBytes<D, kEight>, v_tile = k_tile + kTile * kBytes;
+      const uint32_t k_scale = scale_ring + slot * 2 * kTile, v_scale = k_scale + kTile;
+      const int behind = j * kTile - seg.prefix;   // of the drafts' first slot
+      const bool border = behind > -kTile;         // the step holds drafts, or ends the sequence
+      uint32_t hidden = 0u;                        // tokens whose value row is not finite, among drafts that not every row sees
+      if (border && seg.count > 1) {
+        // Such a row must not meet the zero weights of the rows that do not see it: it becomes zeros, and those that see
+        // it get NaN scores.
+        if (kEight) {
+          const bool bad = lane < kTile && lane + behind >= 0 && lds_b8(v_scale + lane) == 255u;
+          hidden = __ballot_sync(0xffffffffu, bad);
+        } else {
+#pragma unroll 2
+          for (int i = 0; i < kPieces / 2; ++i) {
+            const int row = i * (32 / kPieces) + lane / kPieces;
+            const uint4 w = lds_b32x4(v_tile + piece_at<kBytes>(row, lane % kPieces));
+            if (row + behind >= 0 && (not_finite(w.x) || not_finite(w.y) || not_finite(w.z) || not_finite(w.w))) hidden |= 1u << row;
+          }
+          hidden = __reduce_or_sync(0xffffffffu, hidden);
+        }
+        if (hidden) {
+#pragma unroll 1
+          for (int i = lane; i < kTile * kPieces; i += 32)
+            if (hidden >> (i / kPieces) & 1u) sts_b32x4(v_tile + piece_at<kBytes>(i / kPieces, i % kPieces), 0u, 0u, 0u, 0u);
+          __syncwarp();
+        }
+      }
+      // ---- S = Q K^T: two blocks of eight tokens, two accumulators each (the chain of products is what a step waits for)
+      float s[2][kC] = {}, s2[2][kC] = {};
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) {
+        const int c = kPieces < 8 ? t4 : 2 * t4 + (i & 1) + 8 * (i >> 1);
+#pragma unroll
+        for (int nb = 0; nb < 2; ++nb) {
+          const uint4 w = lds_b32x4(k_tile + piece_at<kBytes>(nb * 8 + quad, c));
+#pragma unroll
+          for (int k = 0; k < kSteps; ++k) {
+            uint32_t b0, b1;
+            if (kEight) {
+              const uint32_t codes = k == 0 ? w.x : k == 1 ? w.y : k == 2 ? w.z : w.w;
+              b0 = halves_of(codes);
+              b1 = halves_of(codes >> 16);
+            } else {
+              b0 = k == 0 ? w.x : w.z;
+              b1 = k == 0 ? w.y : w.w;
+            }
+            const uint32_t(&q)[kHalf ? 2 : 4] = qf[i * kSteps + k];
+            mma<kEight, kHalf>(k & 1 ? s2[nb] : s[nb], q[0], kHalf ? 0u : q[kHalf ? 0 : 1], q[kHalf ? 1 : 2], kHalf ? 0u : q[kHalf ? 0 : 3], b0, b1);
+          }
+        }
+      }
+      // ---- the tokens of this lane: nb * 8 + 2 t4 + e
+      float v_factor[2][2];
+      float v_tile_max[kH];
+#pragma unroll
+      for (int h = 0; h < kH; ++h) v_tile_max[h] = v_used[h];
+      float x[2][kC];
+#pragma unroll
+      for (int nb = 0; nb < 2; ++nb) {
+        uint32_t k2 = 0u, v2 = 0u;
+        if (kEight) {
+          k2 = lds_b16(k_scale + nb * 8 + 2 * t4);
+          v2 = lds_b16(v_scale + nb * 8 + 2 * t4);
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int token = nb * 8 + 2 * t4 + e;
+          float k_factor = 1.0f, v_power = kSmallest;
+          if (kEight) {
+            const uint32_t k = k2 >> (8 * e) & 0xffu, v = v2 >> (8 * e) & 0xffu;
+            k_factor = e8m0_value(k);
+            v_factor[nb][e] = v == 255u ? 1.0f : e8m0_value(v);   // (codes of a row that is not finite are NaN, or zeros here)
+            if (v != 255u) v_power = static_cast<float>(static_cast<int>(v) - 127);
+          }
+          if (hidden >> token & 1u) k_factor = __uint_as_float(0x7fc00000u);
+#pragma unroll
+          for (int h = 0; h < kH; ++h) {
+            float score = (s[nb][2 * h + e] + s2[nb][2 * h + e]) * row_scale[h];
+            if (kEight || border) score *= k_factor;
+            const bool sees = !border || token + behind < 0 || (token + behind < 16 && (seen[h] >> (token + behind) & 1u));
+            x[nb][2 * h + e] = sees ? score : -INFINITY;
+            if (kEight && sees) v_tile_max[h] = fmaxf(v_tile_max[h], v_power);
+          }
+        }
+      }
+      // ---- running maximum, rescaled rarely
+      bool grow[kH], any = false;
+#pragma unroll
+      for (int h = 0; h < kH; ++h) {
+        float m = fmaxf(fmaxf(x[0][2 * h], x[0][2 * h + 1]), fmaxf(x[1][2 * h], x[1][2 * h + 1]));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        m_true[h] = fmaxf(m_true[h], m);
+        if (kEight) {
+          v_tile_max[h] = fmaxf(v_tile_max[h], __shfl_xor_sync(0xffffffffu, v_tile_max[h], 1));
+          v_tile_max[h] = fmaxf(v_tile_max[h], __shfl_xor_sync(0xffffffffu, v_tile_max[h], 2));
+        }
+        grow[h] = m_true[h] - m_used[h] > kRescale;
+        any = any || grow[h] || v_tile_max[h] > v_used[h];
+      }
+      if (__any_sync(0xffffffffu, any)) {
+#pragma unroll
+        for (int h = 0; h < kH; ++h) {
+          const float factor = fast_exp2((grow[h] ? m_used[h] - m_true[h] : 0.0f) + (v_used[h] - v_tile_max[h]));
+          if (grow[h]) m_used[h] = m_true[h];
+          v_used[h] = v_tile_max[h];
+          l[h] *= factor;
+#pragma unroll
+          for (int nb = 0; nb < kBlocks; ++nb) {
+            o[nb][2 * h] *= factor;
+            o[nb][2 * h + 1] *= factor;
+          }
+        }
+      }
+      uint32_t p[2][2], rest[2][2];   // [h][tokens 0-7, 8-15]
+#pragma unroll
+      for (int h = 0; h < kH; ++h) {
+        const float reference = (m_used[h] == -INFINITY ? 0.0f : m_used[h]) + v_used[h];   // (nothing seen yet: any)
+#pragma unroll
+        for (int nb = 0; nb < 2; ++nb) {
+          float p0 = fast_exp2(x[nb][2 * h] - reference), p1 = fast_exp2(x[nb][2 * h + 1] - reference);
+          l[h] += p0 + p1;
+          if (kEight) {
+            p[h][nb] = pack_f16(p0 * v_factor[nb][0], p1 * v_factor[nb][1]);
+          } else {
+            p[h][nb] = pack_bf16(p0, p1);
+            rest[h][nb] = pack_bf16(p0 - bf16_lo(p[h][nb]), p1 - bf16_hi(p[h][nb]));
+          }
+        }
+      }
+      // ---- O += P V
+      if constexpr (kEight) {
+        // block nb of 128 channels (of 64): column n is channel 16 n + nb (8 n + nb) of the tile's rows 2 t4, 2 t4 + 1, and 8 further
+        constexpr int kWide = D == 64 ? 2 : 4;   // words of a row a lane takes
+#pragma unroll
+        for (int set = 0; set < (D == 256 ? 2 : 1); ++set) {
+          uint32_t w[4][kWide];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const int row = 2 * t4 + (u & 1) + 8 * (u >> 1);
+            if constexpr (D == 64) {
+              const uint64_t half = lds_b64(v_tile + piece_at<kBytes>(row, quad / 2) + (quad & 1) * 8);
+              w[u][0] = static_cast<uint32_t>(half);
+              w[u][1] = static_cast<uint32_t>(half >> 32);
+            } else {
+              const uint4 v = lds_b32x4(v_tile + piece_at<kBytes>(row, set * 8 + quad));
+              w[u][0] = v.x; w[u][1] = v.y; w[u][2] = v.z; w[u][3] = v.w;
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < kWide; ++k)
+#pragma unroll
+            for (int pair = 0; pair < 2; ++pair) {   // bytes 0, 1 and 2, 3 of the word
+              const uint32_t ab = __byte_perm(w[0][k], w[1][k], pair ? 0x7362 : 0x5140), cd = __byte_perm(w[2][k], w[3][k], pair ? 0x7362 : 0x5140);
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                mma<kEight, kHalf>(o[set * 16 + 4 * k + 2 * pair + e], p[0][0], kHalf ? 0u : p[kHalf ? 0 : 1][0], p[0][1],
+                                   kHalf ? 0u : p[kHalf ? 0 : 1][1], halves_of(e ? ab >> 16 : ab), halves_of(e ? cd >> 16 : cd));
+            }
+        }
+      } else {
+#pragma unroll
+        for (int np = 0; np < D / 16; ++np) {
+          uint32_t vf[4];
+          ldmatrix_x4_trans(vf, v_tile + piece_at<kBytes>((lane / 8 & 1) * 8 + lane % 8, np * 2 + lane / 16));
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            mma<kEight, kHalf>(o[2 * np + u], p[0][0], kHalf ? 0u : p[kHalf ? 0 : 1][0], p[0][1], kHalf ? 0u : p[kHalf ? 0 : 1][1], vf[2 * u], vf[2 * u + 1]);
+            mma<kEight, kHalf>(o[2 * np + u], rest[0][0], kHalf ? 0u : rest[kHalf ? 0 : 1][0], rest[0][1], kHalf ? 0u : rest[kHalf ? 0 : 1][1], vf[2 * u],
+                               vf[2 * u + 1]);
+          }
+        }
+      }
+      __syncwarp();   // the slot is free for the next issue
+    }
+
+    // ---- the unit's part, or its result
+    const int slot = 2 * worker + seg.slot;
+#pragma unroll
+    for (int h = 0; h < kH; ++h) {
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+      const int r = quad + 8 * h, node = r / group, head = seg.kv_head * group + r % group;
+      if (r >= seg.rows) continue;
+      const size_t token = static_cast<size_t>(seg.b) * a.nodes + node;
+      const float inverse = l[h] == 0.0f ? 0.0f : 1.0f / l[h];
+      const float reference = m_used[h] == -INFINITY ? -INFINITY : m_used[h] + v_used[h];
+      float* acc = parts.acc + (static_cast<size_t>(slot) * parts.rows + r) * D;
+      if constexpr (kEight) {
+        constexpr int kWidth = D == 64 ? 8 : 16;   // neighbouring channels of a column
+#pragma unroll
+        for (int set = 0; set < (D == 256 ? 2 : 1); ++set)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int b = 0; b < kWidth; b += 8) {
+              const int d = set * 128 + (2 * t4 + e) * kWidth + b;
+              float v[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) v[i] = o[set * 16 + b + i][2 * h + e];
+              if (seg.whole) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] *= inverse;
+                store_out8(a, token, head, d, v, gate_pieces);
+              } else {
+                reinterpret_cast<float4*>(acc + d)[0] = make_float4(v[0], v[1], v[2], v[3]);
+                reinterpret_cast<float4*>(acc + d)[1] = make_float4(v[4], v[5], v[6], v[7]);
+              }
+            }
+      } else {
+#pragma unroll
+        for (int nb = 0; nb < kBlocks; ++nb) {
+          const int d = nb * 8 + 2 * t4;
+          const float v0 = o[nb][2 * h], v1 = o[nb][2 * h + 1];
+          if (seg.whole)
+            *reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(a.out) + (token * a.q_heads + head) * D + d) =
+                pack_bf16(tree_output(a, token, head, d, v0 * inverse), tree_output(a, token, head, d + 1, v1 * inverse));
+          else
+            *reinterpret_cast<float2*>(acc + d) = make_float2(v0, v1);
+        }
+      }
+      if (t4 == 0) {
+        if (!seg.whole) parts.ml[static_cast<size_t>(slot) * parts.rows + r] = make_float2(reference, l[h]);
+        else if (a.lse) a.lse[token * a.q_heads + head] = (reference == -INFINITY ? 0.0f : reference * 0.6931471805599453f) + logf(l[h]);
+      }
+    }
+    __syncwarp();
+  }
+  wait_copies<0>();
+}
+
+template <int D, bool kEight>
+constexpr LineShape line_shape() {
+  return {kTile, 3, 16, 148 * kCtas<D, kEight> * kWarps};
+}
+
+template <int D, bool kEight, bool kHalf>
+cudaError_t launch_rows(cudaStream_t stream, const TreeArgs& a) {
+  constexpr LineShape shape = line_shape<D, kEight>();
+  constexpr int kBytes = kWarps * kWarpBytes<D, kEight>;
+  static_assert(kBytes * kCtas<D, kEight> <= 224 * 1024, "shared memory");
+  const long long tiles = static_cast<long long>(a.batch) * a.kv_heads * ((static_cast<long long>(a.max_prefix) + a.nodes + kTile - 1) / kTile);
+  const long long ctas = (tiles + kWarps - 1) / kWarps, most = 148 * kCtas<D, kEight>;
+  cudaError_t e = cudaFuncSetAttribute(tree_decode_mma_kernel<D, kEight, kHalf>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+  if (e != cudaSuccess) return e;
+  tree_decode_mma_kernel<D, kEight, kHalf><<<static_cast<unsigned>(ctas < most ? ctas : most), kWarps * 32, kBytes, stream>>>(a, shape);
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  return tree_decode_merge(stream, a, shape);
+}
+
+template <int D, bool kEight>
+cudaError_t launch(cudaStream_t stream, const TreeArgs& a) {
+  if constexpr (D == 256) return launch_rows<D, kEight, true>(stream, a);
+  else return a.nodes * (a.q_heads / a.kv_heads) <= 8 ? launch_rows<D, kEight, true>(stream, a) : launch_rows<D, kEight, false>(stream, a);
+}
+
+}  // namespace
+
+size_t tree_decode_mma_workspace_bytes(int nodes, int q_heads, int kv_heads, int dim) {
+  return line_workspace_bytes({kTile, 3, 16, 148 * 2 * kWarps}, nodes, q_heads, kv_heads, dim);   // (one CTA per SM needs less)
+}
+
+cudaError_t tree_decode_mma(cudaStream_t stream, const TreeArgs& a) {
+  const bool eight = a.pool.store == kStoreE4m3;
+  if (a.dim == 64) return eight ? launch<64, true>(stream, a) : launch<64, false>(stream, a);
+  if (a.dim == 128) return eight ? launch<128, true>(stream, a) : launch<128, false>(stream, a);
+  return eight ? launch<256, true>(stream, a) : launch<256, false>(stream, a);
+}
+
+}  // namespace pluto

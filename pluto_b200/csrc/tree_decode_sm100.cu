@@ -21,13 +21,10 @@
 // a tile with other rows keeps its codes and the softmax multiplies scores and weights by the rows' factors.  P then
 // carries 11 bits, over bf16 caches 8.
 //
-// Work is cut evenly over the SMs whatever the lengths: the units' key tiles, each unit with a few more for what
-// it costs besides, form one line that is cut into equal ranges, one per CTA.  A CTA walks the units of its range; one that
-// it holds whole it writes out, of the others it leaves (accumulator, maximum, sum) in the workspace, and a
-// second kernel merges a cut unit's parts in the order of the keys.  The cut follows from the lengths alone.
+// Work is cut evenly over the SMs as tree_line.cuh says, one CTA per SM.
 #include <stddef.h>
 
-#include "draft_rows.cuh"
+#include "tree_line.cuh"
 
 namespace pluto {
 namespace {
@@ -36,7 +33,7 @@ constexpr int kTile = 64;            // keys
 template <bool kEight>
 constexpr int kThreads = kEight ? 768 : 512;   // warps 0-3: MMA issue; 4-11: softmax; 12-15: loads; 16-23: widening
 constexpr int kMaxCtas = 148;
-constexpr int kUnitTiles = 3;        // what a unit costs besides its tiles (query load, read-out), in tiles
+constexpr int kUnitTiles = 3;        // query load and read-out of a unit, in tiles
 constexpr float kRescale = 8.0f;     // O is rescaled when the maximum has grown by more than 2^8
 constexpr float kSmallest = -100.0f; // exponent of the value rows from which smaller ones are taken for as large
 
@@ -47,115 +44,6 @@ constexpr int kRawStages = D == 64 ? 8 : D == 128 ? 6 : 2;   // key and value ti
 template <int D>
 constexpr int kTileBytes = kTile * D * 2;
 constexpr int group_rows(int dim) { return dim == 256 ? 128 : 256; }   // rows that share one pass over the keys
-
-// ---- the line of work ----------------------------------------------------------------------------------------
-struct Sequence {
-  int prefix, count, tiles, units;
-};
-__device__ __forceinline__ Sequence sequence_at(const TreeArgs& a, int b) {
-  Sequence s;
-  s.count = draft_count(a.counts, b, a.nodes, a.pool.status, 47);
-  s.prefix = a.prefix[b];
-  if (s.prefix < 0 || s.prefix > a.max_prefix) {
-    report_status(a.pool.status, 47, kBadLength);
-    s.prefix = s.prefix < 0 ? 0 : a.max_prefix;
-  }
-  const int rows = s.count * (a.q_heads / a.kv_heads), per = group_rows(a.dim);
-  s.tiles = (s.prefix + s.count + kTile - 1) / kTile;
-  s.units = a.kv_heads * ((rows + per - 1) / per);   // no nodes: no units
-  return s;
-}
-__device__ __forceinline__ long long weight_of(const Sequence& s) {
-  return static_cast<long long>(s.units) * (s.tiles + kUnitTiles);
-}
-
-// Where CTA c's range of the line begins, and the sequence that holds a position: by one warp.
-struct Line {
-  long long total;
-  int parts;   // CTAs that take part
-};
-__device__ __forceinline__ long long range_begin(const Line& line, int c) { return line.total * c / line.parts; }
-__device__ __forceinline__ Line measure_line(const TreeArgs& a, int ctas, int lane) {
-  long long total = 0, tiles = 0;
-  for (int b = lane; b < a.batch; b += 32) {
-    const Sequence s = sequence_at(a, b);
-    total += weight_of(s);
-    tiles += static_cast<long long>(s.units) * s.tiles;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    total += __shfl_xor_sync(0xffffffffu, total, o);
-    tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
-  }
-  return Line{total, static_cast<int>(max(1ll, min(static_cast<long long>(ctas), tiles)))};
-}
-// Sequence that holds `position` < total, and where it starts on the line.
-__device__ __forceinline__ int find_sequence(const TreeArgs& a, long long position, int lane, long long& start) {
-  long long before = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += 32) {
-    const int b = b0 + lane;
-    const long long own = b < a.batch ? weight_of(sequence_at(a, b)) : 0;
-    long long up_to = own;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long other = __shfl_up_sync(0xffffffffu, up_to, o);
-      if (lane >= o) up_to += other;
-    }
-    const unsigned holds = __ballot_sync(0xffffffffu, before + up_to > position);
-    if (holds) {
-      const int at = __ffs(holds) - 1;
-      start = before + __shfl_sync(0xffffffffu, up_to - own, at);
-      return b0 + at;
-    }
-    before += __shfl_sync(0xffffffffu, up_to, 31);
-  }
-  start = before;
-  return a.batch;
-}
-
-// A CTA's part of a unit.
-struct Segment {
-  int b, kv_head, row0, rows;      // rows: live rows of the group from row0 on (0: the range ends)
-  int prefix, count, tile0, tile1; // key tiles [tile0, tile1)
-  int whole;
-  int slot;                        // workspace slot of a partial result: 0 for a unit that began before the range
-};
-// Walks the segments of a range: one warp, which hands them to the others through a ring in shared memory.
-struct Cursor {
-  long long begin, end, start;   // of the range; start of the current unit
-  int b, unit;
-  Sequence s;
-  __device__ __forceinline__ bool next(const TreeArgs& a, Segment& out) {
-    while (start < end && b < a.batch) {
-      if (unit >= s.units) {
-        unit = 0;
-        if (++b >= a.batch) return false;
-        s = sequence_at(a, b);
-        continue;
-      }
-      const long long first = start + kUnitTiles;
-      const int tile0 = static_cast<int>(max(0ll, begin - first)), tile1 = static_cast<int>(min(static_cast<long long>(s.tiles), end - first));
-      const int own = unit;
-      const long long own_start = start;
-      ++unit;
-      start += s.tiles + kUnitTiles;
-      if (tile0 >= tile1) continue;
-      const int per = group_rows(a.dim), rows = s.count * (a.q_heads / a.kv_heads), groups = s.units / a.kv_heads;
-      out.b = b;
-      out.kv_head = own / groups;
-      out.row0 = own % groups * per;
-      out.rows = min(per, rows - out.row0);
-      out.prefix = s.prefix;
-      out.count = s.count;
-      out.tile0 = tile0;
-      out.tile1 = tile1;
-      out.whole = tile0 == 0 && tile1 == s.tiles;
-      out.slot = own_start < begin ? 0 : 1;
-      return true;
-    }
-    return false;
-  }
-};
 
 // ---- shared memory -------------------------------------------------------------------------------------------
 constexpr int kSegments = 8;         // of the ring
@@ -417,55 +305,8 @@ __device__ __forceinline__ void widen_tiles(Shared<D, true>* sh, uint32_t raw_ri
 template <int D, bool kEight>
 constexpr int kRingBytes = 2 * kStages<D, kEight> * kTileBytes<D> + (kEight ? 2 * kRawStages<D> * kTile * D : 0);
 
-// ---- output --------------------------------------------------------------------------------------------------
-struct Partials {
-  float* acc;   // [slots][rows][D]
-  float2* ml;   // [slots][rows]
-  int rows;     // rows a slot has room for
-};
-__host__ __device__ inline int slot_rows(int nodes, int q_heads, int kv_heads, int dim) {
-  const int rows = nodes * (q_heads / kv_heads);
-  return rows < group_rows(dim) ? rows : group_rows(dim);
-}
-__device__ __forceinline__ Partials partials_of(const TreeArgs& a) {
-  Partials p;
-  p.rows = slot_rows(a.nodes, a.q_heads, a.kv_heads, a.dim);
-  p.ml = static_cast<float2*>(a.workspace);
-  p.acc = reinterpret_cast<float*>(p.ml + static_cast<size_t>((2 * kMaxCtas * p.rows + 1) & ~1));
-  return p;
-}
-
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-
-// Eight neighbouring channels of one output row.
-__device__ __forceinline__ void store_out8(const TreeArgs& a, size_t token, int head, int d, const float (&x)[8], bool gate_pieces) {
-  float y[8];
-  if (a.gate != nullptr && gate_pieces) {
-    const uint4 g = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.gate) + token * a.gate_token +
-                                                    static_cast<size_t>(head) * a.gate_head + d);
-    const float gate[8] = {bf16_lo(g.x), bf16_hi(g.x), bf16_lo(g.y), bf16_hi(g.y), bf16_lo(g.z), bf16_hi(g.z), bf16_lo(g.w), bf16_hi(g.w)};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float factor = sigmoid(gate[i]);
-      y[i] = a.round ? bf16_round(x[i]) * bf16_round(factor) : x[i] * factor;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = tree_output(a, token, head, d + i, x[i]);
-  }
-  *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + (token * a.q_heads + head) * a.dim + d) =
-      make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
-}
-__device__ __forceinline__ bool gate_in_pieces(const TreeArgs& a) {
-  return a.gate_is_bf16 && a.gate_token % 8 == 0 && a.gate_head % 8 == 0 && (reinterpret_cast<uintptr_t>(a.gate) & 15u) == 0;
-}
-
 template <int D, bool kEight>
-__global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(TreeArgs a) {
+__global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(TreeArgs a, LineShape shape) {
   constexpr bool kOneO = D == 256;                       // one accumulator for both score buffers
   constexpr uint32_t kColO1 = D, kColS = kOneO ? 256 : 2 * D, kColQ = kColS + 128;
   static_assert(kColQ + (kOneO ? D / 2 : D) <= 512, "tensor memory");
@@ -592,22 +433,8 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(TreeArg
       }
     } else if (warp == 1) {
       // ---------------------------------------------------------------- the range's segments
-      const Line line = measure_line(a, gridDim.x, lane);
-      const int c = blockIdx.x;
       Cursor cursor;
-      cursor.begin = cursor.end = cursor.start = 0;
-      cursor.b = cursor.unit = 0;
-      cursor.s = Sequence{0, 0, 0, 0};
-      if (c < line.parts && line.total > 0) {
-        cursor.begin = range_begin(line, c);
-        cursor.end = range_begin(line, c + 1);
-        cursor.b = find_sequence(a, cursor.begin, lane, cursor.start);
-        if (cursor.b < a.batch) {   // straight to the unit that holds the range's begin
-          cursor.s = sequence_at(a, cursor.b);
-          cursor.unit = static_cast<int>((cursor.begin - cursor.start) / (cursor.s.tiles + kUnitTiles));
-          cursor.start += static_cast<long long>(cursor.unit) * (cursor.s.tiles + kUnitTiles);
-        }
-      }
+      cursor.seek(a, shape, blockIdx.x, lane);
       bool more = true;
       for (int n = 0; more; ++n) {
         const int at = n % kSegments;
@@ -628,7 +455,7 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(TreeArg
     const int x = (warp - 4) / 4, quarter = warp & 3, row = quarter * 32 + lane, group = a.q_heads / a.kv_heads;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
     const float scale_log2 = a.scale * 1.4426950408889634f;
-    const Partials parts = partials_of(a);
+    const Partials parts = partials_of(a, shape);
     const bool gate_pieces = gate_in_pieces(a);
     // tiles of the range; those of the score buffers 0 and 1; meetings of the streams
     int tile_n = 0, tiles_0 = 0, tiles_1 = 0, met = 0;
@@ -912,120 +739,28 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(TreeArg
   if (warp == 0) tmem_dealloc(tmem, 512);
 }
 
-// Merges the parts of the units that the line's cuts fall into, in the order of the keys.  Block (j, y): cut j + 1,
-// eight rows; it acts if its cut is the first one inside its unit.  One warp per row.
-__global__ void __launch_bounds__(256) tree_decode_merge(TreeArgs a, int ctas) {
-  __shared__ Line line;
-  __shared__ long long found_start;
-  __shared__ int found_b;
-  __shared__ float weight[8][kMaxCtas];
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, cut = blockIdx.x + 1, row = blockIdx.y * 8 + warp;
-  if (warp == 0) {   // (prefix and counts were there before the kernel that this one waits for)
-    const Line l = measure_line(a, ctas, lane);
-    long long start = 0;
-    const int b = cut < l.parts ? find_sequence(a, range_begin(l, cut), lane, start) : a.batch;
-    if (lane == 0) {
-      line = l;
-      found_b = b;
-      found_start = start;
-    }
-  }
-  __syncthreads();
-  pdl_wait();   // the parts are complete and visible from here on
-  if (cut >= line.parts || found_b >= a.batch) return;
-  const Sequence s = sequence_at(a, found_b);
-  const long long span = s.tiles + kUnitTiles;
-  const int unit = static_cast<int>((range_begin(line, cut) - found_start) / span);
-  const long long start = found_start + unit * span, end = start + span;
-  if (range_begin(line, cut) <= start || range_begin(line, cut - 1) > start) return;
-  // the CTAs that hold tiles of it
-  int first = -1, last = -1;
-  for (int c = cut - 1; c < line.parts && range_begin(line, c) < end; ++c) {
-    if (min(range_begin(line, c + 1), end) > max(range_begin(line, c), start + kUnitTiles)) {
-      if (first < 0) first = c;
-      last = c;
-    }
-  }
-  if (first == last) return;   // one CTA holds all of its tiles and has written it out
-  const int group = a.q_heads / a.kv_heads, groups = s.units / a.kv_heads, per = group_rows(a.dim);
-  const int row0 = unit % groups * per, rows = min(per, s.count * group - row0), kv_head = unit / groups;
-  if (row >= rows) return;
-  const Partials parts = partials_of(a);
-  const auto part_at = [&](int c) {
-    return static_cast<size_t>(2 * c + (start < range_begin(line, c) ? 0 : 1)) * parts.rows + row;
-  };
-  float m = -INFINITY;
-  for (int c = first + lane; c <= last; c += 32) m = fmaxf(m, parts.ml[part_at(c)].x);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const float m_safe = m == -INFINITY ? 0.0f : m;
-  for (int c = first + lane; c <= last; c += 32) weight[warp][c - first] = fast_exp2(parts.ml[part_at(c)].x - m_safe);
-  __syncwarp();
-  float l = 0.0f, acc[8] = {};
-  const int D = a.dim;
-#pragma unroll 4
-  for (int c = first; c <= last; ++c) {
-    const float w = weight[warp][c - first];
-    const size_t at = part_at(c);
-    l = fmaf(parts.ml[at].y, w, l);
-    const float* from = parts.acc + at * D + lane * 8;
-    if (lane * 8 < D) {
-      const float4 u = reinterpret_cast<const float4*>(from)[0], v = reinterpret_cast<const float4*>(from)[1];
-      acc[0] = fmaf(u.x, w, acc[0]); acc[1] = fmaf(u.y, w, acc[1]); acc[2] = fmaf(u.z, w, acc[2]); acc[3] = fmaf(u.w, w, acc[3]);
-      acc[4] = fmaf(v.x, w, acc[4]); acc[5] = fmaf(v.y, w, acc[5]); acc[6] = fmaf(v.z, w, acc[6]); acc[7] = fmaf(v.w, w, acc[7]);
-    }
-  }
-  const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
-  const int r = row0 + row, node = r / group, head = kv_head * group + r % group;
-  const size_t token = static_cast<size_t>(found_b) * a.nodes + node;
-  if (lane * 8 < D) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) acc[i] *= inverse;
-    store_out8(a, token, head, lane * 8, acc, gate_in_pieces(a));
-  }
-  if (lane == 0 && a.lse) a.lse[token * a.q_heads + head] = m_safe * 0.6931471805599453f + logf(l);
-}
+constexpr LineShape line_shape(int dim) { return {kTile, kUnitTiles, group_rows(dim), kMaxCtas}; }
 
 template <int D, bool kEight>
 cudaError_t launch(cudaStream_t stream, const TreeArgs& a) {
-  const int rows = slot_rows(a.nodes, a.q_heads, a.kv_heads, D);
-  const long long units = static_cast<long long>(a.batch) * a.kv_heads * ((a.nodes * (a.q_heads / a.kv_heads) + group_rows(D) - 1) / group_rows(D));
+  constexpr LineShape shape = line_shape(D);
+  const long long units = static_cast<long long>(a.batch) * a.kv_heads * ((a.nodes * (a.q_heads / a.kv_heads) + shape.rows - 1) / shape.rows);
   const long long tiles = units * ((static_cast<long long>(a.max_prefix) + a.nodes + kTile - 1) / kTile);
-  const int ctas = static_cast<int>(tiles < kMaxCtas ? tiles : kMaxCtas);
   constexpr int kBytes = kRingBytes<D, kEight> + static_cast<int>(sizeof(Shared<D, kEight>)) + 1024;
   static_assert(kBytes <= 227 * 1024, "shared memory");
   using S = Shared<D, kEight>;
   static_assert(offsetof(S, k_factor) % 16 == 0 && offsetof(S, ml) % 8 == 0 && alignof(S) == 16, "alignment");
   cudaError_t e = cudaFuncSetAttribute(tree_decode_sm100<D, kEight>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
   if (e != cudaSuccess) return e;
-  tree_decode_sm100<D, kEight><<<ctas, kThreads<kEight>, kBytes, stream>>>(a);
-  if ((e = cudaGetLastError()) != cudaSuccess || ctas == 1) return e;
-  cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(ctas - 1, (rows + 7) / 8);
-  config.blockDim = dim3(256);
-  config.stream = stream;
-  cudaLaunchAttribute attribute;
-  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attribute.val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = &attribute;
-  config.numAttrs = 1;
-  return cudaLaunchKernelEx(&config, tree_decode_merge, a, ctas);
+  tree_decode_sm100<D, kEight><<<static_cast<unsigned>(tiles < kMaxCtas ? tiles : kMaxCtas), kThreads<kEight>, kBytes, stream>>>(a, shape);
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  return tree_decode_merge(stream, a, shape);
 }
 
 }  // namespace
 
-bool tree_decode_tc_supported(const TreeArgs& a) {
-  const size_t element = a.pool.store == kStoreBf16 ? 2 : 1;
-  const auto aligned = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
-  return a.q_is_bf16 && a.out_is_bf16 && a.pool.store != kStoreFp32 && (a.dim == 64 || a.dim == 128 || a.dim == 256) &&
-         aligned(a.q) && aligned(a.out) && aligned(a.pool.k) && aligned(a.pool.v) && a.pool.page_stride * element % 16 == 0 &&
-         a.pool.token_stride * element % 16 == 0;
-}
-
 size_t tree_decode_tc_workspace_bytes(int nodes, int q_heads, int kv_heads, int dim) {
-  if (dim != 64 && dim != 128 && dim != 256) return 0;
-  const size_t rows = slot_rows(nodes, q_heads, kv_heads, dim);
-  return ((2 * kMaxCtas * rows + 1) & ~static_cast<size_t>(1)) * sizeof(float2) + 2 * kMaxCtas * rows * dim * sizeof(float);
+  return line_workspace_bytes(line_shape(dim), nodes, q_heads, kv_heads, dim);
 }
 
 cudaError_t tree_decode_tc(cudaStream_t stream, const TreeArgs& a) {

@@ -1,0 +1,208 @@
+// How the attention of drafted tokens is cut over the GPU, whatever the sequences' lengths.
+//
+// A unit is a (sequence, KV head, group of rows); it is a row of key tiles.  All units, each with a few tiles more for what
+// it costs besides, form one line that is cut into equal ranges, one per worker (a CTA or a warp).  A worker walks the
+// units of its range; a unit that it holds whole it writes out, of the others it leaves (accumulator, maximum, sum) in
+// one of its two workspace slots, and tree_decode_merge adds a cut unit's parts in the order of the keys.  Where the
+// line is cut follows from the lengths alone, so results repeat bit for bit.
+#pragma once
+
+#include "draft_rows.cuh"
+
+namespace pluto {
+
+struct LineShape {
+  int tile;       // keys per tile
+  int overhead;   // what a unit costs besides its tiles, in tiles
+  int rows;       // rows of a unit at most
+  int workers;    // at most
+};
+struct Sequence {
+  int prefix, count, tiles, units;
+};
+__device__ __forceinline__ Sequence sequence_at(const TreeArgs& a, const LineShape& shape, int b) {
+  Sequence s;
+  s.count = draft_count(a.counts, b, a.nodes, a.pool.status, 47);
+  s.prefix = a.prefix[b];
+  if (s.prefix < 0 || s.prefix > a.max_prefix) {
+    report_status(a.pool.status, 47, kBadLength);
+    s.prefix = s.prefix < 0 ? 0 : a.max_prefix;
+  }
+  const int rows = s.count * (a.q_heads / a.kv_heads);
+  s.tiles = (s.prefix + s.count + shape.tile - 1) / shape.tile;
+  s.units = a.kv_heads * ((rows + shape.rows - 1) / shape.rows);   // no nodes: no units
+  return s;
+}
+__device__ __forceinline__ long long weight_of(const LineShape& shape, const Sequence& s) {
+  return static_cast<long long>(s.units) * (s.tiles + shape.overhead);
+}
+
+struct Line {
+  long long total;
+  int parts;   // workers that take part: no more than there are tiles
+};
+__device__ __forceinline__ long long range_begin(const Line& line, int c) { return line.total * c / line.parts; }
+
+// The whole line, by one warp; `before`: the weight of the sequences below `upto`.
+__device__ __forceinline__ Line measure_line(const TreeArgs& a, const LineShape& shape, int lane, int upto, long long& before) {
+  long long total = 0, tiles = 0, below = 0;
+  for (int b = lane; b < a.batch; b += 32) {
+    const Sequence s = sequence_at(a, shape, b);
+    const long long weight = weight_of(shape, s);
+    total += weight;
+    tiles += static_cast<long long>(s.units) * s.tiles;
+    if (b < upto) below += weight;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    total += __shfl_xor_sync(0xffffffffu, total, o);
+    tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
+    below += __shfl_xor_sync(0xffffffffu, below, o);
+  }
+  before = below;
+  return Line{total, static_cast<int>(max(1ll, min(static_cast<long long>(shape.workers), tiles)))};
+}
+// Sequence that holds `position` < total, and where it starts on the line: by one warp.
+__device__ __forceinline__ int find_sequence(const TreeArgs& a, const LineShape& shape, long long position, int lane, long long& start) {
+  long long before = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += 32) {
+    const int b = b0 + lane;
+    const long long own = b < a.batch ? weight_of(shape, sequence_at(a, shape, b)) : 0;
+    long long up_to = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long other = __shfl_up_sync(0xffffffffu, up_to, o);
+      if (lane >= o) up_to += other;
+    }
+    const unsigned holds = __ballot_sync(0xffffffffu, before + up_to > position);
+    if (holds) {
+      const int at = __ffs(holds) - 1;
+      start = before + __shfl_sync(0xffffffffu, up_to - own, at);
+      return b0 + at;
+    }
+    before += __shfl_sync(0xffffffffu, up_to, 31);
+  }
+  start = before;
+  return a.batch;
+}
+
+// A worker's part of a unit.
+struct Segment {
+  int b, kv_head, row0, rows;      // rows: live rows of the group from row0 on (0: the range ends)
+  int prefix, count, tile0, tile1; // key tiles [tile0, tile1)
+  int whole;
+  int slot;                        // workspace slot of a partial result: 0 for a unit that began before the range
+};
+// Walks the segments of a range.
+struct Cursor {
+  LineShape shape;
+  long long begin, end, start;   // of the range; start of the current unit
+  int b, unit;
+  Sequence s;
+  // by a whole warp
+  __device__ __forceinline__ void seek(const TreeArgs& a, const LineShape& line_shape, int worker, int lane) {
+    shape = line_shape;
+    long long before;
+    const Line line = measure_line(a, shape, lane, 0, before);
+    begin = end = start = 0;
+    b = unit = 0;
+    s = Sequence{0, 0, 0, 0};
+    if (worker >= line.parts || line.total == 0) return;
+    begin = range_begin(line, worker);
+    end = range_begin(line, worker + 1);
+    b = find_sequence(a, shape, begin, lane, start);
+    if (b >= a.batch) return;
+    s = sequence_at(a, shape, b);
+    unit = static_cast<int>((begin - start) / (s.tiles + shape.overhead));   // straight to the unit that holds the begin
+    start += static_cast<long long>(unit) * (s.tiles + shape.overhead);
+  }
+  __device__ __forceinline__ bool next(const TreeArgs& a, Segment& out) {
+    while (start < end && b < a.batch) {
+      if (unit >= s.units) {
+        unit = 0;
+        if (++b >= a.batch) return false;
+        s = sequence_at(a, shape, b);
+        continue;
+      }
+      const long long first = start + shape.overhead;
+      const int tile0 = static_cast<int>(max(0ll, begin - first)), tile1 = static_cast<int>(min(static_cast<long long>(s.tiles), end - first));
+      const int own = unit;
+      const long long own_start = start;
+      ++unit;
+      start += s.tiles + shape.overhead;
+      if (tile0 >= tile1) continue;
+      const int rows = s.count * (a.q_heads / a.kv_heads), groups = s.units / a.kv_heads;
+      out.b = b;
+      out.kv_head = own / groups;
+      out.row0 = own % groups * shape.rows;
+      out.rows = min(shape.rows, rows - out.row0);
+      out.prefix = s.prefix;
+      out.count = s.count;
+      out.tile0 = tile0;
+      out.tile1 = tile1;
+      out.whole = tile0 == 0 && tile1 == s.tiles;
+      out.slot = own_start < begin ? 0 : 1;
+      return true;
+    }
+    return false;
+  }
+};
+
+// ---- the workspace: two slots per worker --------------------------------------------------------------------
+struct Partials {
+  float* acc;   // [slots][rows][D], relative to the maximum
+  float2* ml;   // [slots][rows]: maximum in powers of two, sum of the weights
+  int rows;     // rows a slot has room for
+};
+__host__ __device__ inline int slot_rows(const LineShape& shape, int nodes, int q_heads, int kv_heads) {
+  const int rows = nodes * (q_heads / kv_heads);
+  return rows < shape.rows ? rows : shape.rows;
+}
+__host__ __device__ inline size_t ml_pairs(const LineShape& shape, int rows) {   // even: the accumulators stay 16-byte aligned
+  return (2 * static_cast<size_t>(shape.workers) * rows + 1) & ~static_cast<size_t>(1);
+}
+inline size_t line_workspace_bytes(const LineShape& shape, int nodes, int q_heads, int kv_heads, int dim) {
+  const int rows = slot_rows(shape, nodes, q_heads, kv_heads);
+  return ml_pairs(shape, rows) * sizeof(float2) + 2 * static_cast<size_t>(shape.workers) * rows * dim * sizeof(float);
+}
+__device__ __forceinline__ Partials partials_of(const TreeArgs& a, const LineShape& shape) {
+  Partials p;
+  p.rows = slot_rows(shape, a.nodes, a.q_heads, a.kv_heads);
+  p.ml = static_cast<float2*>(a.workspace);
+  p.acc = reinterpret_cast<float*>(p.ml + ml_pairs(shape, p.rows));
+  return p;
+}
+
+// ---- output ------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ bool gate_in_pieces(const TreeArgs& a) {   // of eight channels, 16-byte aligned
+  return a.gate_is_bf16 && a.gate_token % 8 == 0 && a.gate_head % 8 == 0 && (reinterpret_cast<uintptr_t>(a.gate) & 15u) == 0;
+}
+// Eight neighbouring channels of one output row (bf16).
+__device__ __forceinline__ void store_out8(const TreeArgs& a, size_t token, int head, int d, const float (&x)[8], bool gate_pieces) {
+  float y[8];
+  if (a.gate != nullptr && gate_pieces) {
+    const uint4 g = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.gate) + token * a.gate_token +
+                                                    static_cast<size_t>(head) * a.gate_head + d);
+    const float gate[8] = {bf16_lo(g.x), bf16_hi(g.x), bf16_lo(g.y), bf16_hi(g.y), bf16_lo(g.z), bf16_hi(g.z), bf16_lo(g.w), bf16_hi(g.w)};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float factor = sigmoid(gate[i]);
+      y[i] = a.round ? bf16_round(x[i]) * bf16_round(factor) : x[i] * factor;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = tree_output(a, token, head, d + i, x[i]);
+  }
+  *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + (token * a.q_heads + head) * a.dim + d) =
+      make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
+}
+
+// tree_decode_merge.cu: launched behind the kernel that leaves the parts, by programmatic dependent launch
+cudaError_t tree_decode_merge(cudaStream_t stream, const TreeArgs& a, const LineShape& shape);
+
+}  // namespace pluto

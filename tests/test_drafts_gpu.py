@@ -245,7 +245,10 @@ EIGHT, BF16, FP32 = torch.float8_e4m3fn, torch.bfloat16, torch.float32
     (1, 1, 24, 4, 256, 0, 0), (1, 1, 24, 4, 256, 63, 0), (3, 1, 24, 4, 256, 777, 16), (2, 13, 24, 4, 256, 130, 64), (1, 64, 24, 4, 256, 500, 0),
     (2, 128, 12, 2, 256, 70, 16), (1, 1, 40, 8, 128, 64, 0), (5, 1, 40, 8, 128, 2000, 16), (3, 5, 40, 8, 128, 65, 7), (2, 61, 40, 8, 128, 1000, 64),
     (1, 128, 10, 2, 128, 333, 48), (2, 26, 5, 1, 128, 200, 0), (4, 1, 12, 12, 64, 100, 16), (3, 8, 12, 12, 64, 1023, 1), (2, 127, 16, 1, 64, 129, 0),
-    (40, 3, 12, 12, 64, 40, 16), (70, 1, 5, 1, 128, 300, 64)])
+    (40, 3, 12, 12, 64, 40, 16), (70, 1, 5, 1, 128, 300, 64),
+    # few rows per KV head, either side of 8 and 16
+    (3, 3, 40, 8, 128, 500, 16), (2, 8, 8, 8, 128, 129, 0), (2, 9, 4, 4, 128, 1000, 5), (2, 16, 12, 12, 64, 333, 16), (2, 17, 12, 12, 64, 333, 16),
+    (3, 16, 2, 2, 128, 15, 0), (9, 8, 4, 4, 256, 700, 16), (2, 9, 4, 4, 256, 700, 16), (300, 2, 4, 2, 64, 90, 16), (1, 1, 8, 1, 128, 9000, 64)])
 def test_tree_attention(store, batch, nodes, hq, hkv, dim, longest, page):
     attention_case(store, batch, nodes, hq, hkv, dim, longest, page, tree=nodes > 1)
 
@@ -278,7 +281,7 @@ def test_one_node_is_gqa_decode():
 
 
 @pytest.mark.parametrize("store", [EIGHT, BF16, FP32])
-@pytest.mark.parametrize("dim,hq,hkv", [(128, 10, 2), (256, 6, 1), (64, 4, 4)])
+@pytest.mark.parametrize("dim,hq,hkv", [(128, 10, 2), (256, 6, 1), (64, 4, 4), (128, 2, 2), (256, 1, 1), (64, 2, 1)])
 def test_what_a_node_does_not_see_does_not_reach_it(store, dim, hq, hkv):
     """A row of infinities or NaN among the drafts (its keys, its values or both): nodes that see it get NaN, the
     others what they get without it."""
