@@ -81,9 +81,6 @@ bool draft_shape(int batch, int nodes, int q_heads, int kv_heads, int head_dim) 
          head_dim <= 256 && batch <= 65535 && fits_int(batch, nodes, q_heads);
 }
 
-// Rows that share a KV head fit one 16-row tile of mma.sync (at width 256 half of it: registers).
-bool few_rows(int nodes, int q_heads, int kv_heads, int head_dim) { return nodes * (q_heads / kv_heads) <= (head_dim == 256 ? 8 : 16); }
-
 bool tensor_core_shape(const pluto::TreeArgs& a) {
   const size_t element = a.pool.store == pluto::kStoreBf16 ? 2 : 1;
   return a.q_is_bf16 && a.out_is_bf16 && a.pool.store != pluto::kStoreFp32 && (a.dim == 64 || a.dim == 128 || a.dim == 256) &&
@@ -158,8 +155,10 @@ int pluto_draft_prepare(pluto_stream_t stream, const void* q_in, const void* k_i
 size_t pluto_gqa_tree_decode_workspace_bytes(int batch, int nodes, int q_heads, int kv_heads, int head_dim) {
   if (!draft_shape(batch, nodes, q_heads, kv_heads, head_dim) || nodes > pluto::kMaxDraftNodes) return 0;
   if (head_dim != 64 && head_dim != 128 && head_dim != 256) return 16;
-  return few_rows(nodes, q_heads, kv_heads, head_dim) ? pluto::tree_decode_mma_workspace_bytes(nodes, q_heads, kv_heads, head_dim)
-                                            : pluto::tree_decode_tc_workspace_bytes(nodes, q_heads, kv_heads, head_dim);
+  // which kernel runs goes by the cache as well, which is not asked for here
+  const size_t few = pluto::tree_decode_mma_workspace_bytes(nodes, q_heads, kv_heads, head_dim);
+  const size_t many = pluto::tree_decode_tc_workspace_bytes(nodes, q_heads, kv_heads, head_dim);
+  return few > many ? few : many;
 }
 
 int pluto_gqa_tree_decode(pluto_stream_t stream, const void* q, int q_dtype, const void* gate, int gate_dtype,
@@ -190,7 +189,7 @@ int pluto_gqa_tree_decode(pluto_stream_t stream, const void* q, int q_dtype, con
   a.scale = 1.0f / sqrtf(static_cast<float>(head_dim));
   if (int c = take_status(&a.pool.status)) return c;
   return pluto::report_cuda(!tensor_core_shape(a)                    ? pluto::tree_decode_exact(stream, a)
-                            : few_rows(nodes, q_heads, kv_heads, head_dim) ? pluto::tree_decode_mma(stream, a)
+                            : pluto::tree_decode_mma_supported(a) ? pluto::tree_decode_mma(stream, a)
                                                                  : pluto::tree_decode_tc(stream, a),
                             "attention of drafted tokens");
 }

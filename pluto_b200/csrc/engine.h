@@ -295,12 +295,12 @@ struct TreeArgs {
   float scale;
 };
 cudaError_t tree_decode_exact(cudaStream_t stream, const TreeArgs& args);
-// bf16 queries and results over a bf16 or 8-bit cache, width 64, 128 or 256, rows on 16-byte boundaries: by rows per
-// KV head (nodes * query heads per KV head) on one of the two tensor-core kernels
+// bf16 queries and results over a bf16 or 8-bit cache, width 64, 128 or 256, rows on 16-byte boundaries
 size_t tree_decode_tc_workspace_bytes(int nodes, int q_heads, int kv_heads, int dim);
-cudaError_t tree_decode_tc(cudaStream_t stream, const TreeArgs& args);    // tree_decode_sm100.cu: any number of rows
+cudaError_t tree_decode_tc(cudaStream_t stream, const TreeArgs& args);    // tree_decode_sm100.cu: any of them
+bool tree_decode_mma_supported(const TreeArgs& args);                     // tree_decode_mma.cu: few rows per KV head
 size_t tree_decode_mma_workspace_bytes(int nodes, int q_heads, int kv_heads, int dim);
-cudaError_t tree_decode_mma(cudaStream_t stream, const TreeArgs& args);   // tree_decode_mma.cu: at most 16 rows
+cudaError_t tree_decode_mma(cudaStream_t stream, const TreeArgs& args);
 
 // verify.cu
 struct VerifyArgs {

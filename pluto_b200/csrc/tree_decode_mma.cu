@@ -3,8 +3,9 @@
 // rows are one 16-row tile of mma.sync (m16n8k16, fp32 accumulation), and the arithmetic has to stay out of the way.
 //
 // A warp works alone: it streams its range of the line (tree_line.cuh) in steps of sixteen tokens through a ring of its
-// own in shared memory (asynchronous 16-byte copies, up to 160 KB in flight per SM), so its main loop meets no other
-// warp and no barrier.  Pages may have any size, rows any 16-byte stride.
+// own in shared memory, so its main loop meets no other warp.  One lane fetches a step with tiled TMA copies over a
+// map of the page pool (column, KV head, token in page, page); a step lies in one page, which is what limits the
+// kernel to page sizes that sixteen divides and to contiguous caches.
 //
 // The codes of an 8-bit cache become MMA operands in registers, one instruction per two codes and exact.  The order of
 // the channels in a product is free as long as both operands share it, so a lane takes whole 16-byte pieces: of the
@@ -26,40 +27,29 @@ template <int D, bool kEight>
 constexpr int kRowBytes = D * (kEight ? 1 : 2);
 template <int D, bool kEight>
 constexpr int kStageBytes = 2 * kTile * kRowBytes<D, kEight>;   // keys, then values
-// CTAs per SM, and steps in the ring of a warp
+// CTAs per SM, and steps in the ring of a warp: as many warps as their registers allow, and 96 KB or more in flight per SM
 template <int D, bool kEight>
-constexpr int kCtas = D == 256 && !kEight ? 1 : 2;
+constexpr int kCtas = D == 256 ? (kEight ? 2 : 1) : D == 128 ? 3 : 4;
 template <int D, bool kEight>
-constexpr int kStages = D == 256 ? 3 : D == 128 ? (kEight ? 6 : 3) : (kEight ? 8 : 6);
-template <int D, bool kEight>
-constexpr int kWarpBytes = kStages<D, kEight> * (kStageBytes<D, kEight> + 2 * kTile);   // and two scale bytes per token
+constexpr int kStages = D == 256 ? 3 : D == 128 ? (kEight ? 4 : 2) : (kEight ? 6 : 3);
+constexpr int kSegments = 8;   // of a warp's range that its copies are ahead by, at most (a step each)
 
-__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool there) {   // zeros where it is not
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+// What a warp has beside its ring.  Scale bytes come as the aligned words that hold them, [0]: keys, [1]: values, with the
+// byte's place in the word.
+template <int kS, bool kEight>
+struct WarpState {
+  uint64_t full[kS];
+  Cursor ahead;
+  Segment segments[kSegments];
+  uint32_t words[kEight ? kS : 1][32];
+  uint8_t places[kEight ? kS : 1][32];
+};
+
+__device__ __forceinline__ void copy4(uint32_t to, const void* from, bool there) {   // zero where it is not
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(there ? 4 : 0) : "memory");
 }
-__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int kLeft>
-__device__ __forceinline__ void wait_copies() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
-}
-__device__ __forceinline__ uint32_t load_byte(const uint8_t* p, bool there) {   // 127 where it is not
-  uint32_t v;
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\tmov.u32 %0, 127;\n\t@p ld.global.u8 %0, [%1];\n\t}"
-               : "=r"(v) : "l"(p), "r"(static_cast<uint32_t>(there)));
-  return v;
-}
-__device__ __forceinline__ uint32_t lds_b8(uint32_t at) {
-  uint32_t v;
-  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
-  return v;
-}
-__device__ __forceinline__ uint32_t lds_b16(uint32_t at) {
-  uint16_t v;
-  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at) : "memory");
-  return v;
-}
-__device__ __forceinline__ void sts_b8(uint32_t at, uint32_t v) {
-  asm volatile("st.shared.u8 [%0], %1;" ::"r"(at), "r"(v) : "memory");
+__device__ __forceinline__ void arrive_behind_copies(uint64_t* bar) {   // when this thread's copies so far have landed
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 __device__ __forceinline__ uint32_t halves_of(uint32_t codes) {   // two codes in the low 16 bits -> two fp16
   uint32_t r;
@@ -87,28 +77,28 @@ __device__ __forceinline__ bool not_finite(uint32_t pair) {
   return (pair & 0x7f80u) == 0x7f80u || (pair & 0x7f800000u) == 0x7f800000u;
 }
 
-// Byte offset of 16-byte piece c of row r in a tile: pieces are exchanged within 128 bytes so that the reads below, which
-// take the same piece of several rows, hit all banks.
+// Byte offset of 16-byte piece c of row r in a tile: slabs of 128 bytes (64 where a row has no more), swizzled by the copies,
+// so that the reads below, which take the same piece of several rows, hit all banks.
 template <int kBytes>
 __device__ __forceinline__ uint32_t piece_at(int r, int c) {
-  return r * kBytes + (kBytes == 64 ? (c ^ (r >> 1 & 3)) << 4 : ((c & ~7) | ((c ^ r) & 7)) << 4);
+  return kBytes == 64 ? r * 64 + ((c ^ (r >> 1 & 3)) << 4) : (c / 8) * (kTile * 128) + r * 128 + (((c ^ r) & 7) << 4);
 }
 
 template <int D, bool kEight, bool kHalf>   // kHalf: at most eight rows
-__global__ void __launch_bounds__(kWarps * 32, kCtas<D, kEight>) tree_decode_mma_kernel(TreeArgs a, LineShape shape) {
+__global__ void __launch_bounds__(kWarps * 32, kCtas<D, kEight>) tree_decode_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, TreeArgs a, LineShape shape) {
   constexpr int kBytes = kRowBytes<D, kEight>, kPieces = kBytes / 16, kS = kStages<D, kEight>;
   constexpr int kH = kHalf ? 1 : 2;                     // rows of a lane
   constexpr int kC = kHalf ? 2 : 4;                     // values of an accumulator block in a lane
   constexpr int kChunks = kPieces < 4 ? 1 : kPieces / 4, kSteps = kEight ? 4 : 2;   // pieces of a key row per lane, k steps per piece
   constexpr int kBlocks = D / 8;                        // accumulator blocks
   static_assert(kChunks * kSteps == D / 16, "channels");
-  extern __shared__ __align__(128) uint8_t smem[];
+  using State = WarpState<kS, kEight>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const int warp = uniform_warp_index(), lane = threadIdx.x % 32, quad = lane / 4, t4 = lane % 4;
-  const uint32_t ring = smem_u32(smem) + warp * kS * kStageBytes<D, kEight>;
-  const uint32_t scale_ring = smem_u32(smem) + kWarps * kS * kStageBytes<D, kEight> + warp * kS * 2 * kTile;
+  const uint32_t ring = base + warp * kS * kStageBytes<D, kEight>;
+  State* own = reinterpret_cast<State*>(smem_raw + (base - smem_u32(smem_raw)) + kWarps * kS * kStageBytes<D, kEight>) + warp;
   uint32_t* status = a.pool.status;
-  const char* k_base = static_cast<const char*>(a.pool.k);
-  const char* v_base = static_cast<const char*>(a.pool.v);
   const int page_shift = (a.pool.page_size & (a.pool.page_size - 1)) == 0 ? __ffs(a.pool.page_size) - 1 : -1;
   const int group = a.q_heads / a.kv_heads;
   const float scale_log2 = a.scale * 1.4426950408889634f;
@@ -117,76 +107,87 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, kEight>) tree_decode_mma
   pdl_launch_dependents();   // the merge may be placed as SMs free up; it waits for this grid's end
 
   const int worker = blockIdx.x * kWarps + warp;
-  Cursor cursor;
-  cursor.seek(a, shape, worker, lane);
-
-  // ---- copies: the next step to issue, kS - 1 ahead of the one that is worked on
-  Cursor ahead = cursor;
-  Segment load;
-  bool more = ahead.next(a, load);
-  int tile = more ? load.tile0 : 0, page = -1, issued = 0, passed = -1;
-  uint32_t k_byte = 0u, v_byte = 0u;
-  const auto fetch_page = [&]() {   // of row lane % 16 of the next step
-    const int t = tile * kTile + lane % 16;
-    page = -1;
-    if (!more || t >= load.prefix + load.count) return;
-    const int block = page_shift >= 0 ? t >> page_shift : t / a.pool.page_size;
-    if (block >= (a.pool.table ? a.pool.max_blocks : 1)) report_status(status, 48, kBadLength);
-    else page = a.pool.table ? a.pool.table[static_cast<size_t>(load.b) * a.pool.max_blocks + block] : load.b;
+  if (lane == 0) {
+    for (int i = 0; i < kS; ++i) mbar_init(&own->full[i], kEight ? 33 : 1);
+    mbar_fence_init();
+    tma_prefetch_desc(&map_k);
+    tma_prefetch_desc(&map_v);
+  }
+  // ---- copies: the next step to issue, kS - 1 ahead of the one that is worked on; what says which one lives in shared
+  // memory (the registers are the products')
+  {
+    Cursor cursor;
+    cursor.seek(a, shape, worker, lane);
+    if (lane == 0) own->ahead = cursor;
+  }
+  __syncwarp();
+  int tile = 0, last = 0, page = 0, issued = 0, listed = 0;   // of the next step: its tile, the segment's end, its page
+  const auto next_load = [&]() {
+    Cursor cursor = own->ahead;
+    Segment load{};
+    const bool more = cursor.next(a, load);   // (rows 0 behind the last)
+    __syncwarp();
+    if (lane == 0) {
+      own->ahead = cursor;
+      own->segments[listed % kSegments] = load;
+    }
+    __syncwarp();
+    ++listed;
+    tile = more ? load.tile0 : 0;
+    last = more ? load.tile1 : 0;
+  };
+  next_load();
+  const auto block_of = [&](int t) { return page_shift >= 0 ? t >> page_shift : t / a.pool.page_size; };
+  const auto fetch_page = [&]() {   // used by the next issue only
+    if (tile >= last) return;
+    const int b = own->segments[(listed - 1) % kSegments].b, block = block_of(tile * kTile);
+    if (block >= (a.pool.table ? a.pool.max_blocks : 1)) {
+      report_status(status, 48, kBadLength);
+      page = -1;
+    } else {
+      page = a.pool.table ? a.pool.table[static_cast<size_t>(b) * a.pool.max_blocks + block] : b;
+    }
   };
   fetch_page();
   const auto issue = [&]() {
-    if (kEight && passed >= 0) {   // the scale bytes asked for by the last issue have arrived meanwhile
-      if (lane < kTile) {
-        sts_b8(scale_ring + passed * 2 * kTile + lane, k_byte);
-        sts_b8(scale_ring + passed * 2 * kTile + kTile + lane, v_byte);
-      }
-      passed = -1;
+    if (tile >= last) return;
+    const Segment* load = &own->segments[(listed - 1) % kSegments];
+    const int t0 = tile * kTile, slot = issued % kS, inside = t0 - block_of(t0) * a.pool.page_size, kv_head = load->kv_head;
+    if (page < 0 || (a.pool.table && page >= a.pool.num_pages)) {
+      report_status(status, 48, kBadPage);   // (a slot past the pages was reported as such before)
+      page = -1;                             // the copies read zeros there
     }
-    if (more) {
-      const int t = tile * kTile + lane % 16, slot = issued % kS;
-      long long row_at = -1;
-      size_t scale_at = 0;
-      if (t < load.prefix + load.count) {
-        if (page < 0 || (a.pool.table && page >= a.pool.num_pages)) {
-          report_status(status, 48, kBadPage);   // (a slot past the pages was reported as such before)
-        } else {
-          const int inside = t - (page_shift >= 0 ? t >> page_shift << page_shift : t / a.pool.page_size * a.pool.page_size);
-          row_at = static_cast<long long>((static_cast<size_t>(page) * a.pool.page_stride + static_cast<size_t>(inside) * a.pool.token_stride +
-                                           static_cast<size_t>(load.kv_head) * D) * (kEight ? 1 : 2));
-          if (kEight) scale_at = static_cast<size_t>(page) * a.pool.scale_page + static_cast<size_t>(inside) * a.pool.scale_token + load.kv_head;
-        }
-      }
+    if (lane == 0) {
       const uint32_t to = ring + slot * kStageBytes<D, kEight>;
+      constexpr int kSlabs = kBytes == 64 ? 1 : kBytes / 128, kColumns = D / kSlabs, kSlab = kTile * kBytes / kSlabs;
+      mbar_expect_tx(&own->full[slot], kStageBytes<D, kEight>);
 #pragma unroll
-      for (int i = 0; i < kPieces / 2; ++i) {
-        const int row = i * (32 / kPieces) + lane / kPieces, c = lane % kPieces;
-        const long long at = __shfl_sync(0xffffffffu, row_at, row);
-        const uint32_t piece = to + piece_at<kBytes>(row, c);
-        const long long from = at >= 0 ? at + c * 16 : 0;
-        copy16(piece, k_base + from, at >= 0);
-        copy16(piece + kTile * kBytes, v_base + from, at >= 0);
+      for (int i = 0; i < kSlabs; ++i) {
+        tma_load_4d_at(to + i * kSlab, &map_k, i * kColumns, kv_head, inside, page, &own->full[slot]);
+        tma_load_4d_at(to + kTile * kBytes + i * kSlab, &map_v, i * kColumns, kv_head, inside, page, &own->full[slot]);
       }
-      if (kEight) {
-        k_byte = load_byte(a.pool.k_scales + scale_at, row_at >= 0);
-        v_byte = load_byte(a.pool.v_scales + scale_at, row_at >= 0);
-        passed = slot;
-      }
-      ++issued;
-      if (++tile >= load.tile1) {
-        more = ahead.next(a, load);
-        if (more) tile = load.tile0;
-      }
-      fetch_page();
     }
-    commit_copies();
+    if (kEight) {   // lanes 0-15: the keys' scales, 16-31: the values'
+      const int row = lane % kTile;
+      const bool there = page >= 0 && row < load->prefix + load->count - t0;
+      const uint8_t* byte = (lane < kTile ? a.pool.k_scales : a.pool.v_scales) +
+                            (there ? static_cast<size_t>(page) * a.pool.scale_page + static_cast<size_t>(inside + row) * a.pool.scale_token + kv_head : 0);
+      const uintptr_t at = reinterpret_cast<uintptr_t>(byte);
+      own->places[slot][lane] = static_cast<uint8_t>(at & 3u);
+      copy4(smem_u32(&own->words[slot][lane]), reinterpret_cast<const void*>(at & ~static_cast<uintptr_t>(3)), there);
+      arrive_behind_copies(&own->full[slot]);
+    }
+    ++issued;
+    if (++tile >= last) next_load();
+    fetch_page();
   };
 #pragma unroll 1
   for (int i = 0; i < kS - 1; ++i) issue();
 
   int step = 0;   // of the range
-  Segment seg;
-  while (cursor.next(a, seg)) {
+  for (int n = 0;; ++n) {
+    const Segment seg = own->segments[n % kSegments];
+    if (seg.rows == 0) break;
     // ---- the queries: A fragments, columns in the order of the keys' pieces
     uint32_t qf[D / 16][kHalf ? 2 : 4];
     float row_scale[kH];
@@ -257,36 +258,44 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, kEight>) tree_decode_mma
 #pragma unroll 1
     for (int j = seg.tile0; j < seg.tile1; ++j, ++step) {
       issue();
-      wait_copies<kS - 1>();
-      __syncwarp();
       const int slot = step % kS;
+      if (!__all_sync(0xffffffffu, mbar_wait(&own->full[slot], (step / kS) & 1, status, 50))) return;
       const uint32_t k_tile = ring + slot * kStageBytes<D, kEight>, v_tile = k_tile + kTile * kBytes;
-      const uint32_t k_scale = scale_ring + slot * 2 * kTile, v_scale = k_scale + kTile;
       const int behind = j * kTile - seg.prefix;   // of the drafts' first slot
       const bool border = behind > -kTile;         // the step holds drafts, or ends the sequence
+      uint32_t scale = 127u;                       // lanes 0-15: of the keys, 16-31: of the values
+      if (kEight) scale = own->words[slot][lane] >> (8 * own->places[slot][lane]) & 0xffu;
       uint32_t hidden = 0u;                        // tokens whose value row is not finite, among drafts that not every row sees
-      if (border && seg.count > 1) {
-        // Such a row must not meet the zero weights of the rows that do not see it: it becomes zeros, and those that see
-        // it get NaN scores.
-        if (kEight) {
-          const bool bad = lane < kTile && lane + behind >= 0 && lds_b8(v_scale + lane) == 255u;
-          hidden = __ballot_sync(0xffffffffu, bad);
-        } else {
+      if (border) {
+        // Rows behind the last draft hold anything.  Neither they nor value rows that are not finite may meet the zero
+        // weights of the rows that do not see them: they become zeros, and those that see the latter get NaN scores.
+        const int live = seg.count - behind;
+        uint32_t clear = live < kTile ? 0xffffu << live & 0xffffu : 0u;
+        if (seg.count > 1) {
+          if (kEight) {
+            hidden = __ballot_sync(0xffffffffu, lane >= kTile && lane - kTile + behind >= 0 && scale == 255u) >> kTile;
+          } else {
 #pragma unroll 2
-          for (int i = 0; i < kPieces / 2; ++i) {
-            const int row = i * (32 / kPieces) + lane / kPieces;
-            const uint4 w = lds_b32x4(v_tile + piece_at<kBytes>(row, lane % kPieces));
-            if (row + behind >= 0 && (not_finite(w.x) || not_finite(w.y) || not_finite(w.z) || not_finite(w.w))) hidden |= 1u << row;
+            for (int i = 0; i < kPieces / 2; ++i) {
+              const int row = i * (32 / kPieces) + lane / kPieces;
+              const uint4 w = lds_b32x4(v_tile + piece_at<kBytes>(row, lane % kPieces));
+              if (row + behind >= 0 && (not_finite(w.x) || not_finite(w.y) || not_finite(w.z) || not_finite(w.w))) hidden |= 1u << row;
+            }
+            hidden = __reduce_or_sync(0xffffffffu, hidden);
           }
-          hidden = __reduce_or_sync(0xffffffffu, hidden);
+          hidden &= ~clear;
+          clear |= hidden;
         }
-        if (hidden) {
+        if (clear) {
 #pragma unroll 1
           for (int i = lane; i < kTile * kPieces; i += 32)
-            if (hidden >> (i / kPieces) & 1u) sts_b32x4(v_tile + piece_at<kBytes>(i / kPieces, i % kPieces), 0u, 0u, 0u, 0u);
+            if (clear >> (i / kPieces) & 1u) sts_b32x4(v_tile + piece_at<kBytes>(i / kPieces, i % kPieces), 0u, 0u, 0u, 0u);
+          fence_proxy_async();   // (the slot's next copies write behind these stores)
           __syncwarp();
         }
       }
+      // factors: a key row that is not finite makes its scores NaN; the codes of such a value row are NaN, or zeros here
+      const float own_factor = scale == 255u ? (lane < kTile ? __uint_as_float(0x7fc00000u) : 1.0f) : e8m0_value(scale);
       // ---- S = Q K^T: two blocks of eight tokens, two accumulators each (the chain of products is what a step waits for)
       float s[2][kC] = {}, s2[2][kC] = {};
 #pragma unroll
@@ -319,20 +328,14 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, kEight>) tree_decode_mma
       float x[2][kC];
 #pragma unroll
       for (int nb = 0; nb < 2; ++nb) {
-        uint32_t k2 = 0u, v2 = 0u;
-        if (kEight) {
-          k2 = lds_b16(k_scale + nb * 8 + 2 * t4);
-          v2 = lds_b16(v_scale + nb * 8 + 2 * t4);
-        }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int token = nb * 8 + 2 * t4 + e;
           float k_factor = 1.0f, v_power = kSmallest;
           if (kEight) {
-            const uint32_t k = k2 >> (8 * e) & 0xffu, v = v2 >> (8 * e) & 0xffu;
-            k_factor = e8m0_value(k);
-            v_factor[nb][e] = v == 255u ? 1.0f : e8m0_value(v);   // (codes of a row that is not finite are NaN, or zeros here)
-            if (v != 255u) v_power = static_cast<float>(static_cast<int>(v) - 127);
+            k_factor = __shfl_sync(0xffffffffu, own_factor, token);
+            v_factor[nb][e] = __shfl_sync(0xffffffffu, own_factor, kTile + token);
+            v_power = static_cast<float>(static_cast<int>(__float_as_uint(v_factor[nb][e]) >> 23) - 127);
           }
           if (hidden >> token & 1u) k_factor = __uint_as_float(0x7fc00000u);
 #pragma unroll
@@ -488,7 +491,32 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, kEight>) tree_decode_mma
     }
     __syncwarp();
   }
-  wait_copies<0>();
+}
+
+// 4-D map of a page pool: (column, KV head, token in page, page); a box is sixteen tokens of 128 bytes (64 where a row has
+// no more) of one KV head, swizzled; zeros outside the pool.
+bool make_pool_map(CUtensorMap* map, const void* base, const TreeArgs& a) {
+  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static Encode encode = [] {
+    void* symbol = nullptr;
+    cudaDriverEntryPointQueryResult result;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &symbol, cudaEnableDefault, &result) != cudaSuccess ||
+        result != cudaDriverEntryPointSuccess)
+      return static_cast<Encode>(nullptr);
+    return reinterpret_cast<Encode>(symbol);
+  }();
+  if (encode == nullptr) return false;
+  const bool eight = a.pool.store == kStoreE4m3;
+  const cuuint64_t element = eight ? 1 : 2, row = a.dim * element;
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(a.dim), static_cast<cuuint64_t>(a.kv_heads), static_cast<cuuint64_t>(a.pool.page_size),
+                              static_cast<cuuint64_t>(a.pool.table ? a.pool.num_pages : a.batch)};
+  const cuuint64_t strides[3] = {row, a.pool.token_stride * element, a.pool.page_stride * element};
+  const cuuint32_t box[4] = {static_cast<cuuint32_t>((row < 128 ? row : 128) / element), 1, kTile, 1}, steps[4] = {1, 1, 1, 1};
+  return encode(map, eight ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box,
+                steps, CU_TENSOR_MAP_INTERLEAVE_NONE, row < 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <int D, bool kEight>
@@ -499,13 +527,15 @@ constexpr LineShape line_shape() {
 template <int D, bool kEight, bool kHalf>
 cudaError_t launch_rows(cudaStream_t stream, const TreeArgs& a) {
   constexpr LineShape shape = line_shape<D, kEight>();
-  constexpr int kBytes = kWarps * kWarpBytes<D, kEight>;
-  static_assert(kBytes * kCtas<D, kEight> <= 224 * 1024, "shared memory");
+  constexpr int kBytes = kWarps * (kStages<D, kEight> * kStageBytes<D, kEight> + static_cast<int>(sizeof(WarpState<kStages<D, kEight>, kEight>))) + 1024;
+  static_assert((kBytes + 1024) * kCtas<D, kEight> <= 228 * 1024, "shared memory");
+  CUtensorMap map_k, map_v;
+  if (!make_pool_map(&map_k, a.pool.k, a) || !make_pool_map(&map_v, a.pool.v, a)) return cudaErrorInvalidValue;
   const long long tiles = static_cast<long long>(a.batch) * a.kv_heads * ((static_cast<long long>(a.max_prefix) + a.nodes + kTile - 1) / kTile);
   const long long ctas = (tiles + kWarps - 1) / kWarps, most = 148 * kCtas<D, kEight>;
   cudaError_t e = cudaFuncSetAttribute(tree_decode_mma_kernel<D, kEight, kHalf>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
   if (e != cudaSuccess) return e;
-  tree_decode_mma_kernel<D, kEight, kHalf><<<static_cast<unsigned>(ctas < most ? ctas : most), kWarps * 32, kBytes, stream>>>(a, shape);
+  tree_decode_mma_kernel<D, kEight, kHalf><<<static_cast<unsigned>(ctas < most ? ctas : most), kWarps * 32, kBytes, stream>>>(map_k, map_v, a, shape);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   return tree_decode_merge(stream, a, shape);
 }
@@ -518,8 +548,14 @@ cudaError_t launch(cudaStream_t stream, const TreeArgs& a) {
 
 }  // namespace
 
+bool tree_decode_mma_supported(const TreeArgs& a) {
+  const size_t element = a.pool.store == kStoreBf16 ? 2 : 1;
+  return a.nodes * (a.q_heads / a.kv_heads) <= (a.dim == 256 ? 8 : 16) && (a.pool.table == nullptr || a.pool.page_size % kTile == 0) &&
+         a.pool.page_stride * element < (1ull << 40) && a.pool.token_stride * element < (1ull << 40);   // (limits of a tensor map)
+}
+
 size_t tree_decode_mma_workspace_bytes(int nodes, int q_heads, int kv_heads, int dim) {
-  return line_workspace_bytes({kTile, 3, 16, 148 * 2 * kWarps}, nodes, q_heads, kv_heads, dim);   // (one CTA per SM needs less)
+  return line_workspace_bytes({kTile, 3, 16, 148 * (dim == 256 ? 2 : dim == 128 ? 3 : 4) * kWarps}, nodes, q_heads, kv_heads, dim);   // (for either storage)
 }
 
 cudaError_t tree_decode_mma(cudaStream_t stream, const TreeArgs& a) {

@@ -38,10 +38,19 @@ __device__ __forceinline__ long long weight_of(const LineShape& shape, const Seq
 }
 
 struct Line {
-  long long total;
-  int parts;   // workers that take part: no more than there are tiles
+  long long total, base;
+  int parts, longer;   // workers that take part, no more than there are tiles; the first `longer` hold base + 1, the others base
 };
-__device__ __forceinline__ long long range_begin(const Line& line, int c) { return line.total * c / line.parts; }
+__device__ __forceinline__ long long range_begin(const Line& line, int c) { return line.base * c + min(c, line.longer); }
+// (64-bit divisions take a few hundred clocks, and a line is hardly ever that long)
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+  return (a | b) >> 32 ? a / b : static_cast<long long>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b));
+}
+__device__ __forceinline__ int holder_of(const Line& line, long long position) {   // worker whose range it falls into
+  const long long from = static_cast<long long>(line.longer) * (line.base + 1);
+  return position < from ? static_cast<int>(quotient(position, line.base + 1))
+                         : line.longer + static_cast<int>(quotient(position - from, line.base));
+}
 
 // The whole line, by one warp; `before`: the weight of the sequences below `upto`.
 __device__ __forceinline__ Line measure_line(const TreeArgs& a, const LineShape& shape, int lane, int upto, long long& before) {
@@ -60,7 +69,12 @@ __device__ __forceinline__ Line measure_line(const TreeArgs& a, const LineShape&
     below += __shfl_xor_sync(0xffffffffu, below, o);
   }
   before = below;
-  return Line{total, static_cast<int>(max(1ll, min(static_cast<long long>(shape.workers), tiles)))};
+  Line line;
+  line.total = total;
+  line.parts = static_cast<int>(max(1ll, min(static_cast<long long>(shape.workers), tiles)));
+  line.base = quotient(total, line.parts);
+  line.longer = static_cast<int>(total - line.base * line.parts);
+  return line;
 }
 // Sequence that holds `position` < total, and where it starts on the line: by one warp.
 __device__ __forceinline__ int find_sequence(const TreeArgs& a, const LineShape& shape, long long position, int lane, long long& start) {
@@ -113,7 +127,7 @@ struct Cursor {
     b = find_sequence(a, shape, begin, lane, start);
     if (b >= a.batch) return;
     s = sequence_at(a, shape, b);
-    unit = static_cast<int>((begin - start) / (s.tiles + shape.overhead));   // straight to the unit that holds the begin
+    unit = static_cast<int>(quotient(begin - start, s.tiles + shape.overhead));   // straight to the unit that holds the begin
     start += static_cast<long long>(unit) * (s.tiles + shape.overhead);
   }
   __device__ __forceinline__ bool next(const TreeArgs& a, Segment& out) {
