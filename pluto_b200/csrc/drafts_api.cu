@@ -186,11 +186,13 @@ int pluto_gqa_tree_decode(pluto_stream_t stream, const void* q, int q_dtype, con
   a.workspace = workspace;
   a.batch = batch; a.nodes = nodes; a.q_heads = q_heads; a.kv_heads = kv_heads; a.dim = head_dim;
   a.round = round_to_bf16;
+  a.group = q_heads / kv_heads;
   a.scale = 1.0f / sqrtf(static_cast<float>(head_dim));
   if (int c = take_status(&a.pool.status)) return c;
-  return pluto::report_cuda(!tensor_core_shape(a)                    ? pluto::tree_decode_exact(stream, a)
-                            : pluto::tree_decode_mma_supported(a) ? pluto::tree_decode_mma(stream, a)
-                                                                 : pluto::tree_decode_tc(stream, a),
+  const bool tensor_cores = tensor_core_shape(a);
+  return pluto::report_cuda(tensor_cores && pluto::tree_decode_mma_supported(a)  ? pluto::tree_decode_mma(stream, a)
+                            : tensor_cores && pluto::tree_decode_tc_supported(a) ? pluto::tree_decode_tc(stream, a)
+                                                                                 : pluto::tree_decode_exact(stream, a),
                             "attention of drafted tokens");
 }
 

@@ -292,12 +292,14 @@ struct TreeArgs {
   float* lse;                     // optional [batch, nodes, q_heads]
   void* workspace;
   int batch, nodes, q_heads, kv_heads, dim, round;
+  int group;                      // q_heads / kv_heads
   float scale;
 };
 cudaError_t tree_decode_exact(cudaStream_t stream, const TreeArgs& args);
 // bf16 queries and results over a bf16 or 8-bit cache, width 64, 128 or 256, rows on 16-byte boundaries
 size_t tree_decode_tc_workspace_bytes(int nodes, int q_heads, int kv_heads, int dim);
-cudaError_t tree_decode_tc(cudaStream_t stream, const TreeArgs& args);    // tree_decode_sm100.cu: any of them
+bool tree_decode_tc_supported(const TreeArgs& args);                      // tree_decode_sm100.cu: (sizes up to 2^31 tiles)
+cudaError_t tree_decode_tc(cudaStream_t stream, const TreeArgs& args);
 bool tree_decode_mma_supported(const TreeArgs& args);                     // tree_decode_mma.cu: few rows per KV head
 size_t tree_decode_mma_workspace_bytes(int nodes, int q_heads, int kv_heads, int dim);
 cudaError_t tree_decode_mma(cudaStream_t stream, const TreeArgs& args);

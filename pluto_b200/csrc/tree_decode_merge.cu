@@ -18,20 +18,20 @@ __global__ void __launch_bounds__(kWarps * 32) tree_decode_merge_kernel(TreeArgs
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int per_sequence = a.kv_heads * groups_at_most, b = blockIdx.x / per_sequence, unit = blockIdx.x % per_sequence;
   // (lengths and counts were there before the kernel that this one waits for)
-  long long start;
+  unsigned start;
   const Line line = measure_line(a, shape, lane, b, start);
   const Sequence s = sequence_at(a, shape, b);
   pdl_wait();   // the parts are complete and visible from here on
   // the sequence's units in their order, kv_head * groups + group; this block's may not exist
   if (unit >= s.units || line.total == 0) return;
-  start += static_cast<long long>(unit) * (s.tiles + shape.overhead);
-  const long long end = start + s.tiles + shape.overhead;
-  const int group = a.q_heads / a.kv_heads, groups = s.units / a.kv_heads, kv_head = unit / groups;
-  const int row0 = unit % groups * shape.rows, rows = min(shape.rows, s.count * group - row0);
+  start += unit * (s.tiles + shape.overhead);
+  const unsigned end = start + s.tiles + shape.overhead;
+  const int group = a.group, groups = (s.count * group + (1 << shape.rows_shift) - 1) >> shape.rows_shift, kv_head = unit / groups;
+  const int row0 = unit % groups << shape.rows_shift, rows = min(1 << shape.rows_shift, s.count * group - row0);
   const int row = kSplit ? blockIdx.y : blockIdx.y * kWarps + warp;
   if (row >= rows) return;   // (the whole CTA where its warps share a row)
   // the workers that hold tiles of it
-  const int first = holder_of(line, start + shape.overhead), last = holder_of(line, end - 1);
+  const int first = static_cast<int>(holder_of(line, start + shape.overhead)), last = static_cast<int>(holder_of(line, end - 1));
   if (first == last) return;   // one worker holds all of its tiles and has written it out
   const Partials parts = partials_of(a, shape);
   const auto part_at = [&](int c) {
@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(kWarps * 32) tree_decode_merge_kernel(TreeArgs
 }  // namespace
 
 cudaError_t tree_decode_merge(cudaStream_t stream, const TreeArgs& a, const LineShape& shape) {
-  const int groups = (a.nodes * (a.q_heads / a.kv_heads) + shape.rows - 1) / shape.rows;
+  const int groups = (a.nodes * a.group + (1 << shape.rows_shift) - 1) >> shape.rows_shift;
   const int rows = slot_rows(shape, a.nodes, a.q_heads, a.kv_heads);
   const long long units = static_cast<long long>(a.batch) * a.kv_heads * groups;
   const bool many_parts = shape.workers >= 16 * units;   // of a unit, when the line is long enough for all workers

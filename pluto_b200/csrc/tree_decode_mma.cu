@@ -5,7 +5,7 @@
 // A warp works alone: it streams its range of the line (tree_line.cuh) in steps of sixteen tokens through a ring of its
 // own in shared memory, so its main loop meets no other warp.  One lane fetches a step with tiled TMA copies over a
 // map of the page pool (column, KV head, token in page, page); a step lies in one page, which is what limits the
-// kernel to page sizes that sixteen divides and to contiguous caches.
+// kernel to page sizes that sixteen divides and to caches of one page per sequence.
 //
 // The codes of an 8-bit cache become MMA operands in registers, one instruction per two codes and exact.  The order of
 // the channels in a product is free as long as both operands share it, so a lane takes whole 16-byte pieces: of the
@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, kEight>) tree_decode_mma
   State* own = reinterpret_cast<State*>(smem_raw + (base - smem_u32(smem_raw)) + kWarps * kS * kStageBytes<D, kEight>) + warp;
   uint32_t* status = a.pool.status;
   const int page_shift = (a.pool.page_size & (a.pool.page_size - 1)) == 0 ? __ffs(a.pool.page_size) - 1 : -1;
-  const int group = a.q_heads / a.kv_heads;
+  const int group = a.group;
   const float scale_log2 = a.scale * 1.4426950408889634f;
   const Partials parts = partials_of(a, shape);
   const bool gate_pieces = gate_in_pieces(a);
@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, kEight>) tree_decode_mma
   const auto next_load = [&]() {
     Cursor cursor = own->ahead;
     Segment load{};
-    const bool more = cursor.next(a, load);   // (rows 0 behind the last)
+    const bool more = cursor.next(a, shape, load);   // (rows 0 behind the last)
     __syncwarp();
     if (lane == 0) {
       own->ahead = cursor;
@@ -181,16 +181,68 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, kEight>) tree_decode_mma
     if (++tile >= last) next_load();
     fetch_page();
   };
+  // One loop over the steps of the range, so that every piece of code is there once: a range of few steps is as long as
+  // the fetching of its instructions takes.
+  Segment seg{};
+  int primed = 0, step = 0, n = 0, j = 0;
+  uint32_t qf[D / 16][kHalf ? 2 : 4], seen[kH];
+  float row_scale[kH], m_used[kH], m_true[kH], v_used[kH], l[kH], o[kBlocks][kC];
 #pragma unroll 1
-  for (int i = 0; i < kS - 1; ++i) issue();
-
-  int step = 0;   // of the range
-  for (int n = 0;; ++n) {
-    const Segment seg = own->segments[n % kSegments];
+  while (true) {
+    issue();
+    if (primed < kS - 1) {
+      ++primed;
+      continue;
+    }
+    if (j >= seg.tile1) {   // (the first time: 0 >= 0)
+    if (seg.rows > 0) {
+    // ---- the unit's part; its result where the whole unit is here
+    const int slot = 2 * worker + seg.slot;
+    float* acc = parts.acc + static_cast<size_t>(slot) * parts.rows * D;
+#pragma unroll
+    for (int h = 0; h < kH; ++h) {
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+      const int r = quad + 8 * h;
+      if (r >= seg.rows) continue;
+      float* to = acc + r * D;
+      if constexpr (kEight) {
+        constexpr int kWidth = D == 64 ? 8 : 16;   // neighbouring channels of a column
+#pragma unroll
+        for (int set = 0; set < (D == 256 ? 2 : 1); ++set)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int i = 0; i < kWidth; i += 4)
+              *reinterpret_cast<float4*>(to + set * 128 + (2 * t4 + e) * kWidth + i) =
+                  make_float4(o[set * 16 + i][2 * h + e], o[set * 16 + i + 1][2 * h + e], o[set * 16 + i + 2][2 * h + e], o[set * 16 + i + 3][2 * h + e]);
+      } else {
+#pragma unroll
+        for (int nb = 0; nb < kBlocks; ++nb) *reinterpret_cast<float2*>(to + nb * 8 + 2 * t4) = make_float2(o[nb][2 * h], o[nb][2 * h + 1]);
+      }
+      if (t4 == 0) parts.ml[static_cast<size_t>(slot) * parts.rows + r] = make_float2(m_used[h] == -INFINITY ? -INFINITY : m_used[h] + v_used[h], l[h]);
+    }
+    if (seg.whole) {   // (through the slot that the warp has anyway: rows in the order of memory, and one piece of code)
+      __syncwarp();
+      constexpr int kEights = D / 8;
+#pragma unroll 1
+      for (int i = lane; i < seg.rows * kEights; i += 32) {
+        const int r = i / kEights, d = i % kEights * 8, node = r / group, head = seg.kv_head * group + r % group;
+        const size_t token = static_cast<size_t>(seg.b) * a.nodes + node;
+        const float2 ml = parts.ml[static_cast<size_t>(slot) * parts.rows + r];
+        const float inverse = ml.y == 0.0f ? 0.0f : 1.0f / ml.y;
+        const float4 u = *reinterpret_cast<const float4*>(acc + r * D + d), v = *reinterpret_cast<const float4*>(acc + r * D + d + 4);
+        const float x[8] = {u.x * inverse, u.y * inverse, u.z * inverse, u.w * inverse, v.x * inverse, v.y * inverse, v.z * inverse, v.w * inverse};
+        store_out8(a, token, head, d, x, gate_pieces);
+        if (d == 0 && a.lse) a.lse[token * a.q_heads + head] = (ml.x == -INFINITY ? 0.0f : ml.x * 0.6931471805599453f) + logf(ml.y);
+      }
+      __syncwarp();
+    }
+    }
+    seg = own->segments[n++ % kSegments];
     if (seg.rows == 0) break;
+    j = seg.tile0;
     // ---- the queries: A fragments, columns in the order of the keys' pieces
-    uint32_t qf[D / 16][kHalf ? 2 : 4];
-    float row_scale[kH];
 #pragma unroll
     for (int h = 0; h < kH; ++h) {
       const int r = quad + 8 * h, node = r / group, head = seg.kv_head * group + r % group;
@@ -227,23 +279,26 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, kEight>) tree_decode_mma
       }
     }
     // ---- which drafts a row sees: one bit per node
-    uint32_t seen[kH] = {};
-    if (seg.tile1 * kTile > seg.prefix) {
 #pragma unroll
+    for (int h = 0; h < kH; ++h) seen[h] = 0u;
+    if (seg.tile1 * kTile > seg.prefix) {
+#pragma unroll 1
       for (int h = 0; h < kH; ++h) {
         const int r = quad + 8 * h;
-        if (r >= seg.rows) continue;
+        uint32_t bits = 0u;
+        if (r < seg.rows)
         for (int i = r / group; i >= 0;) {
-          seen[h] |= 1u << i;
+          bits |= 1u << i;
           const int up = a.parents ? a.parents[static_cast<size_t>(seg.b) * a.nodes + i] : i - 1;
           if (up < -1 || up >= i) report_status(status, 49, kBadDraft);   // taken as a first token's
           i = up < i ? up : -1;
         }
+        if (h == 0) seen[0] = bits;
+        else seen[kH - 1] = bits;
       }
     }
     // Weights are 2^(score * row_scale - reference), reference = m_used + v_used: for 8-bit caches v_used is the largest
     // exponent of the value rows seen so far, so that a weight times its row's 2^n fits fp16.
-    float m_used[kH], m_true[kH], v_used[kH], l[kH], o[kBlocks][kC];
 #pragma unroll
     for (int h = 0; h < kH; ++h) {
       m_used[h] = m_true[h] = -INFINITY;
@@ -255,9 +310,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, kEight>) tree_decode_mma
 #pragma unroll
       for (int i = 0; i < kC; ++i) o[nb][i] = 0.0f;
 
-#pragma unroll 1
-    for (int j = seg.tile0; j < seg.tile1; ++j, ++step) {
-      issue();
+    }
       const int slot = step % kS;
       if (!__all_sync(0xffffffffu, mbar_wait(&own->full[slot], (step / kS) & 1, status, 50))) return;
       const uint32_t k_tile = ring + slot * kStageBytes<D, kEight>, v_tile = k_tile + kTile * kBytes;
@@ -437,59 +490,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, kEight>) tree_decode_mma
         }
       }
       __syncwarp();   // the slot is free for the next issue
-    }
-
-    // ---- the unit's part, or its result
-    const int slot = 2 * worker + seg.slot;
-#pragma unroll
-    for (int h = 0; h < kH; ++h) {
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-      const int r = quad + 8 * h, node = r / group, head = seg.kv_head * group + r % group;
-      if (r >= seg.rows) continue;
-      const size_t token = static_cast<size_t>(seg.b) * a.nodes + node;
-      const float inverse = l[h] == 0.0f ? 0.0f : 1.0f / l[h];
-      const float reference = m_used[h] == -INFINITY ? -INFINITY : m_used[h] + v_used[h];
-      float* acc = parts.acc + (static_cast<size_t>(slot) * parts.rows + r) * D;
-      if constexpr (kEight) {
-        constexpr int kWidth = D == 64 ? 8 : 16;   // neighbouring channels of a column
-#pragma unroll
-        for (int set = 0; set < (D == 256 ? 2 : 1); ++set)
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-#pragma unroll
-            for (int b = 0; b < kWidth; b += 8) {
-              const int d = set * 128 + (2 * t4 + e) * kWidth + b;
-              float v[8];
-#pragma unroll
-              for (int i = 0; i < 8; ++i) v[i] = o[set * 16 + b + i][2 * h + e];
-              if (seg.whole) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] *= inverse;
-                store_out8(a, token, head, d, v, gate_pieces);
-              } else {
-                reinterpret_cast<float4*>(acc + d)[0] = make_float4(v[0], v[1], v[2], v[3]);
-                reinterpret_cast<float4*>(acc + d)[1] = make_float4(v[4], v[5], v[6], v[7]);
-              }
-            }
-      } else {
-#pragma unroll
-        for (int nb = 0; nb < kBlocks; ++nb) {
-          const int d = nb * 8 + 2 * t4;
-          const float v0 = o[nb][2 * h], v1 = o[nb][2 * h + 1];
-          if (seg.whole)
-            *reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(a.out) + (token * a.q_heads + head) * D + d) =
-                pack_bf16(tree_output(a, token, head, d, v0 * inverse), tree_output(a, token, head, d + 1, v1 * inverse));
-          else
-            *reinterpret_cast<float2*>(acc + d) = make_float2(v0, v1);
-        }
-      }
-      if (t4 == 0) {
-        if (!seg.whole) parts.ml[static_cast<size_t>(slot) * parts.rows + r] = make_float2(reference, l[h]);
-        else if (a.lse) a.lse[token * a.q_heads + head] = (reference == -INFINITY ? 0.0f : reference * 0.6931471805599453f) + logf(l[h]);
-      }
-    }
-    __syncwarp();
+      ++step;
+      ++j;
   }
 }
 
@@ -521,7 +523,7 @@ bool make_pool_map(CUtensorMap* map, const void* base, const TreeArgs& a) {
 
 template <int D, bool kEight>
 constexpr LineShape line_shape() {
-  return {kTile, 3, 16, 148 * kCtas<D, kEight> * kWarps};
+  return {4, 3, 4, 148 * kCtas<D, kEight> * kWarps};
 }
 
 template <int D, bool kEight, bool kHalf>
@@ -543,19 +545,20 @@ cudaError_t launch_rows(cudaStream_t stream, const TreeArgs& a) {
 template <int D, bool kEight>
 cudaError_t launch(cudaStream_t stream, const TreeArgs& a) {
   if constexpr (D == 256) return launch_rows<D, kEight, true>(stream, a);
-  else return a.nodes * (a.q_heads / a.kv_heads) <= 8 ? launch_rows<D, kEight, true>(stream, a) : launch_rows<D, kEight, false>(stream, a);
+  else return a.nodes * a.group <= 8 ? launch_rows<D, kEight, true>(stream, a) : launch_rows<D, kEight, false>(stream, a);
 }
 
 }  // namespace
 
 bool tree_decode_mma_supported(const TreeArgs& a) {
   const size_t element = a.pool.store == kStoreBf16 ? 2 : 1;
-  return a.nodes * (a.q_heads / a.kv_heads) <= (a.dim == 256 ? 8 : 16) && (a.pool.table == nullptr || a.pool.page_size % kTile == 0) &&
-         a.pool.page_stride * element < (1ull << 40) && a.pool.token_stride * element < (1ull << 40);   // (limits of a tensor map)
+  return a.nodes * a.group <= (a.dim == 256 ? 8 : 16) && (a.pool.table == nullptr || a.pool.max_blocks == 1 || a.pool.page_size % kTile == 0) &&
+         a.pool.page_stride * element < (1ull << 40) && a.pool.token_stride * element < (1ull << 40) &&   // (limits of a tensor map)
+         line_fits(a, {4, 3, 4, 0});
 }
 
 size_t tree_decode_mma_workspace_bytes(int nodes, int q_heads, int kv_heads, int dim) {
-  return line_workspace_bytes({kTile, 3, 16, 148 * (dim == 256 ? 2 : dim == 128 ? 3 : 4) * kWarps}, nodes, q_heads, kv_heads, dim);   // (for either storage)
+  return line_workspace_bytes({4, 3, 4, 148 * (dim == 256 ? 2 : dim == 128 ? 3 : 4) * kWarps}, nodes, q_heads, kv_heads, dim);   // (for either storage)
 }
 
 cudaError_t tree_decode_mma(cudaStream_t stream, const TreeArgs& a) {

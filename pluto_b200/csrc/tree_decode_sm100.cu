@@ -439,7 +439,7 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(TreeArg
       for (int n = 0; more; ++n) {
         const int at = n % kSegments;
         Segment seg{};
-        more = cursor.next(a, seg);
+        more = cursor.next(a, shape, seg);
         if (n >= kSegments && !__all_sync(0xffffffffu, mbar_wait(&sh->seg_empty[at], (n / kSegments - 1) & 1, status, 62))) break;
         if (lane == 0) {
           if (!more) seg.rows = 0;
@@ -452,7 +452,7 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(TreeArg
   } else if (warp < 12) {
     if (kEight) asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
     // ------------------------------------------------------------------ softmax, one thread per row
-    const int x = (warp - 4) / 4, quarter = warp & 3, row = quarter * 32 + lane, group = a.q_heads / a.kv_heads;
+    const int x = (warp - 4) / 4, quarter = warp & 3, row = quarter * 32 + lane, group = a.group;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
     const float scale_log2 = a.scale * 1.4426950408889634f;
     const Partials parts = partials_of(a, shape);
@@ -739,12 +739,13 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(TreeArg
   if (warp == 0) tmem_dealloc(tmem, 512);
 }
 
-constexpr LineShape line_shape(int dim) { return {kTile, kUnitTiles, group_rows(dim), kMaxCtas}; }
+constexpr LineShape line_shape(int dim) { return {6, kUnitTiles, dim == 256 ? 7 : 8, kMaxCtas}; }
 
 template <int D, bool kEight>
 cudaError_t launch(cudaStream_t stream, const TreeArgs& a) {
   constexpr LineShape shape = line_shape(D);
-  const long long units = static_cast<long long>(a.batch) * a.kv_heads * ((a.nodes * (a.q_heads / a.kv_heads) + shape.rows - 1) / shape.rows);
+  static_assert(1 << shape.tile_shift == kTile && 1 << shape.rows_shift == group_rows(D), "line");
+  const long long units = static_cast<long long>(a.batch) * a.kv_heads * ((a.nodes * a.group + group_rows(D) - 1) / group_rows(D));
   const long long tiles = units * ((static_cast<long long>(a.max_prefix) + a.nodes + kTile - 1) / kTile);
   constexpr int kBytes = kRingBytes<D, kEight> + static_cast<int>(sizeof(Shared<D, kEight>)) + 1024;
   static_assert(kBytes <= 227 * 1024, "shared memory");
@@ -758,6 +759,8 @@ cudaError_t launch(cudaStream_t stream, const TreeArgs& a) {
 }
 
 }  // namespace
+
+bool tree_decode_tc_supported(const TreeArgs& a) { return line_fits(a, line_shape(a.dim)); }
 
 size_t tree_decode_tc_workspace_bytes(int nodes, int q_heads, int kv_heads, int dim) {
   return line_workspace_bytes(line_shape(dim), nodes, q_heads, kv_heads, dim);

@@ -11,12 +11,19 @@
 
 namespace pluto {
 
+// Positions are 32-bit: line_fits is asked on the host.
 struct LineShape {
-  int tile;       // keys per tile
-  int overhead;   // what a unit costs besides its tiles, in tiles
-  int rows;       // rows of a unit at most
-  int workers;    // at most
+  int tile_shift;   // keys per tile
+  int overhead;     // what a unit costs besides its tiles, in tiles
+  int rows_shift;   // rows of a unit at most
+  int workers;      // at most
 };
+inline bool line_fits(const TreeArgs& a, const LineShape& shape) {
+  const long long groups = (static_cast<long long>(a.nodes) * a.group + (1 << shape.rows_shift) - 1) >> shape.rows_shift;
+  const long long tiles = ((static_cast<long long>(a.max_prefix) + a.nodes) >> shape.tile_shift) + 1 + shape.overhead;
+  return tiles < (1ll << 31) / (a.batch * groups * a.kv_heads + 1);
+}
+
 struct Sequence {
   int prefix, count, tiles, units;
 };
@@ -28,76 +35,46 @@ __device__ __forceinline__ Sequence sequence_at(const TreeArgs& a, const LineSha
     report_status(a.pool.status, 47, kBadLength);
     s.prefix = s.prefix < 0 ? 0 : a.max_prefix;
   }
-  const int rows = s.count * (a.q_heads / a.kv_heads);
-  s.tiles = (s.prefix + s.count + shape.tile - 1) / shape.tile;
-  s.units = a.kv_heads * ((rows + shape.rows - 1) / shape.rows);   // no nodes: no units
+  s.tiles = (s.prefix + s.count + (1 << shape.tile_shift) - 1) >> shape.tile_shift;
+  s.units = a.kv_heads * ((s.count * a.group + (1 << shape.rows_shift) - 1) >> shape.rows_shift);   // no nodes: no units
   return s;
 }
-__device__ __forceinline__ long long weight_of(const LineShape& shape, const Sequence& s) {
-  return static_cast<long long>(s.units) * (s.tiles + shape.overhead);
+__device__ __forceinline__ unsigned weight_of(const LineShape& shape, const Sequence& s) {
+  return static_cast<unsigned>(s.units) * (s.tiles + shape.overhead);
 }
 
 struct Line {
-  long long total, base;
-  int parts, longer;   // workers that take part, no more than there are tiles; the first `longer` hold base + 1, the others base
+  unsigned total, base;
+  unsigned parts, longer;   // workers that take part, no more than there are tiles; the first `longer` hold base + 1, the others base
 };
-__device__ __forceinline__ long long range_begin(const Line& line, int c) { return line.base * c + min(c, line.longer); }
-// (64-bit divisions take a few hundred clocks, and a line is hardly ever that long)
-__device__ __forceinline__ long long quotient(long long a, long long b) {
-  return (a | b) >> 32 ? a / b : static_cast<long long>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b));
+__device__ __forceinline__ unsigned range_begin(const Line& line, unsigned c) { return line.base * c + min(c, line.longer); }
+__device__ __forceinline__ unsigned holder_of(const Line& line, unsigned position) {   // worker whose range it falls into
+  const unsigned from = line.longer * (line.base + 1);
+  return position < from ? position / (line.base + 1) : line.longer + (position - from) / line.base;
 }
-__device__ __forceinline__ int holder_of(const Line& line, long long position) {   // worker whose range it falls into
-  const long long from = static_cast<long long>(line.longer) * (line.base + 1);
-  return position < from ? static_cast<int>(quotient(position, line.base + 1))
-                         : line.longer + static_cast<int>(quotient(position - from, line.base));
+__device__ __forceinline__ Line cut_line(const LineShape& shape, unsigned total, unsigned tiles) {
+  Line line;
+  line.total = total;
+  line.parts = max(1u, min(static_cast<unsigned>(shape.workers), tiles));
+  line.base = total / line.parts;
+  line.longer = total - line.base * line.parts;
+  return line;
 }
 
 // The whole line, by one warp; `before`: the weight of the sequences below `upto`.
-__device__ __forceinline__ Line measure_line(const TreeArgs& a, const LineShape& shape, int lane, int upto, long long& before) {
-  long long total = 0, tiles = 0, below = 0;
+__device__ __forceinline__ Line measure_line(const TreeArgs& a, const LineShape& shape, int lane, int upto, unsigned& before) {
+  unsigned total = 0, tiles = 0, below = 0;
   for (int b = lane; b < a.batch; b += 32) {
     const Sequence s = sequence_at(a, shape, b);
-    const long long weight = weight_of(shape, s);
+    const unsigned weight = weight_of(shape, s);
     total += weight;
-    tiles += static_cast<long long>(s.units) * s.tiles;
+    tiles += s.units * s.tiles;
     if (b < upto) below += weight;
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    total += __shfl_xor_sync(0xffffffffu, total, o);
-    tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
-    below += __shfl_xor_sync(0xffffffffu, below, o);
-  }
-  before = below;
-  Line line;
-  line.total = total;
-  line.parts = static_cast<int>(max(1ll, min(static_cast<long long>(shape.workers), tiles)));
-  line.base = quotient(total, line.parts);
-  line.longer = static_cast<int>(total - line.base * line.parts);
-  return line;
-}
-// Sequence that holds `position` < total, and where it starts on the line: by one warp.
-__device__ __forceinline__ int find_sequence(const TreeArgs& a, const LineShape& shape, long long position, int lane, long long& start) {
-  long long before = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += 32) {
-    const int b = b0 + lane;
-    const long long own = b < a.batch ? weight_of(shape, sequence_at(a, shape, b)) : 0;
-    long long up_to = own;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long other = __shfl_up_sync(0xffffffffu, up_to, o);
-      if (lane >= o) up_to += other;
-    }
-    const unsigned holds = __ballot_sync(0xffffffffu, before + up_to > position);
-    if (holds) {
-      const int at = __ffs(holds) - 1;
-      start = before + __shfl_sync(0xffffffffu, up_to - own, at);
-      return b0 + at;
-    }
-    before += __shfl_sync(0xffffffffu, up_to, 31);
-  }
-  start = before;
-  return a.batch;
+  total = __reduce_add_sync(0xffffffffu, total);
+  tiles = __reduce_add_sync(0xffffffffu, tiles);
+  before = __reduce_add_sync(0xffffffffu, below);
+  return cut_line(shape, total, tiles);
 }
 
 // A worker's part of a unit.
@@ -109,28 +86,48 @@ struct Segment {
 };
 // Walks the segments of a range.
 struct Cursor {
-  LineShape shape;
-  long long begin, end, start;   // of the range; start of the current unit
+  unsigned begin, end, start;   // of the range; start of the current unit
   int b, unit;
   Sequence s;
   // by a whole warp
-  __device__ __forceinline__ void seek(const TreeArgs& a, const LineShape& line_shape, int worker, int lane) {
-    shape = line_shape;
-    long long before;
-    const Line line = measure_line(a, shape, lane, 0, before);
+  __device__ __forceinline__ void seek(const TreeArgs& a, const LineShape& shape, unsigned worker, int lane) {
+    unsigned none;
+    const Line line = measure_line(a, shape, lane, 0, none);
     begin = end = start = 0;
     b = unit = 0;
     s = Sequence{0, 0, 0, 0};
     if (worker >= line.parts || line.total == 0) return;
     begin = range_begin(line, worker);
     end = range_begin(line, worker + 1);
-    b = find_sequence(a, shape, begin, lane, start);
-    if (b >= a.batch) return;
-    s = sequence_at(a, shape, b);
-    unit = static_cast<int>(quotient(begin - start, s.tiles + shape.overhead));   // straight to the unit that holds the begin
-    start += static_cast<long long>(unit) * (s.tiles + shape.overhead);
+    // the sequence that holds the begin
+    unsigned before = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += 32) {
+      const int own_b = min(b0 + lane, a.batch - 1);
+      const Sequence own = sequence_at(a, shape, own_b);
+      const unsigned weight = b0 + lane < a.batch ? weight_of(shape, own) : 0u;
+      unsigned up_to = weight;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned other = __shfl_up_sync(0xffffffffu, up_to, o);
+        if (lane >= o) up_to += other;
+      }
+      const unsigned holds = __ballot_sync(0xffffffffu, before + up_to > begin);
+      if (holds) {
+        const int at = __ffs(holds) - 1;
+        b = b0 + at;
+        start = before + __shfl_sync(0xffffffffu, up_to - weight, at);
+        s.prefix = __shfl_sync(0xffffffffu, own.prefix, at);
+        s.count = __shfl_sync(0xffffffffu, own.count, at);
+        s.tiles = __shfl_sync(0xffffffffu, own.tiles, at);
+        s.units = __shfl_sync(0xffffffffu, own.units, at);
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, up_to, 31);
+    }
+    unit = (begin - start) / (s.tiles + shape.overhead);   // straight to the unit that holds the begin
+    start += unit * (s.tiles + shape.overhead);
   }
-  __device__ __forceinline__ bool next(const TreeArgs& a, Segment& out) {
+  __device__ __forceinline__ bool next(const TreeArgs& a, const LineShape& shape, Segment& out) {
     while (start < end && b < a.batch) {
       if (unit >= s.units) {
         unit = 0;
@@ -138,18 +135,18 @@ struct Cursor {
         s = sequence_at(a, shape, b);
         continue;
       }
-      const long long first = start + shape.overhead;
-      const int tile0 = static_cast<int>(max(0ll, begin - first)), tile1 = static_cast<int>(min(static_cast<long long>(s.tiles), end - first));
+      const unsigned first = start + shape.overhead;
+      const int tile0 = begin > first ? begin - first : 0, tile1 = end > first ? min(static_cast<unsigned>(s.tiles), end - first) : 0u;
       const int own = unit;
-      const long long own_start = start;
+      const unsigned own_start = start;
       ++unit;
       start += s.tiles + shape.overhead;
       if (tile0 >= tile1) continue;
-      const int rows = s.count * (a.q_heads / a.kv_heads), groups = s.units / a.kv_heads;
+      const int rows = s.count * a.group, groups = (rows + (1 << shape.rows_shift) - 1) >> shape.rows_shift;
       out.b = b;
-      out.kv_head = own / groups;
-      out.row0 = own % groups * shape.rows;
-      out.rows = min(shape.rows, rows - out.row0);
+      out.kv_head = groups == 1 ? own : own / groups;
+      out.row0 = (groups == 1 ? 0 : own % groups) << shape.rows_shift;
+      out.rows = min(1 << shape.rows_shift, rows - out.row0);
       out.prefix = s.prefix;
       out.count = s.count;
       out.tile0 = tile0;
@@ -170,7 +167,7 @@ struct Partials {
 };
 __host__ __device__ inline int slot_rows(const LineShape& shape, int nodes, int q_heads, int kv_heads) {
   const int rows = nodes * (q_heads / kv_heads);
-  return rows < shape.rows ? rows : shape.rows;
+  return rows < (1 << shape.rows_shift) ? rows : 1 << shape.rows_shift;
 }
 __host__ __device__ inline size_t ml_pairs(const LineShape& shape, int rows) {   // even: the accumulators stay 16-byte aligned
   return (2 * static_cast<size_t>(shape.workers) * rows + 1) & ~static_cast<size_t>(1);
