@@ -33,17 +33,43 @@ __device__ __forceinline__ RowAt row_at(const Kv8Args& a, unsigned row, uint32_t
   return r;
 }
 
-__device__ __forceinline__ void load8(const void* p, size_t at, int is_bf16, float (&x)[8]) {
-  if (is_bf16) {
-    const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p) + at);
-    x[0] = bf16_lo(w.x); x[1] = bf16_hi(w.x); x[2] = bf16_lo(w.y); x[3] = bf16_hi(w.y);
-    x[4] = bf16_lo(w.z); x[5] = bf16_hi(w.z); x[6] = bf16_lo(w.w); x[7] = bf16_hi(w.w);
-  } else {
-    const float4* f = reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
-    const float4 u = f[0], v = f[1];
-    x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w; x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
+// The rows of a sub-warp: usually neighbouring heads of one token, which share the look-ups.
+__device__ __forceinline__ void rows_at(const Kv8Args& a, unsigned row, uint32_t site, RowAt (&at)[kRows]) {
+  at[0] = row_at(a, row, site);
+  unsigned h = row % a.heads;
+#pragma unroll
+  for (int i = 1; i < kRows; ++i) {
+    if (++h < static_cast<unsigned>(a.heads)) {
+      at[i] = at[i - 1];
+      at[i].data += a.head_stride;
+      at[i].pool += a.dim;
+      at[i].scale += 1;
+    } else {
+      at[i] = row_at(a, row + i, site);
+      h = 0;
+    }
   }
 }
+
+// Eight channels as they lie in memory.
+template <bool kBf16>
+struct Raw8 {
+  uint4 w[kBf16 ? 1 : 2];
+  __device__ __forceinline__ void load(const void* p, size_t at) {
+    const char* from = static_cast<const char*>(p) + at * (kBf16 ? 2 : 4);
+#pragma unroll
+    for (int i = 0; i < (kBf16 ? 1 : 2); ++i) w[i] = __ldcs(reinterpret_cast<const uint4*>(from) + i);
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < (kBf16 ? 1 : 2); ++i) w[i] = make_uint4(0u, 0u, 0u, 0u);
+  }
+  __device__ __forceinline__ void values(float (&x)[8]) const {
+    const uint32_t words[8] = {w[0].x, w[0].y, w[0].z, w[0].w, w[kBf16 ? 0 : 1].x, w[kBf16 ? 0 : 1].y, w[kBf16 ? 0 : 1].z, w[kBf16 ? 0 : 1].w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = !kBf16 ? __uint_as_float(words[i]) : i & 1 ? bf16_hi(words[i / 2]) : bf16_lo(words[i / 2]);
+  }
+};
 
 // The codes of eight channels; a row that is not finite gets NaN codes.
 __device__ __forceinline__ uint2 codes8(const float (&x)[8], uint32_t byte) {
@@ -53,46 +79,38 @@ __device__ __forceinline__ uint2 codes8(const float (&x)[8], uint32_t byte) {
                     e4m3_pair(x[4] * f, x[5] * f) | e4m3_pair(x[6] * f, x[7] * f) << 16);
 }
 
-template <int kLanes>   // lanes per row: dim <= 8 * kLanes
+template <bool kBf16, int kLanes>   // lanes per row: dim <= 8 * kLanes
 __global__ void __launch_bounds__(256) kv8_append_vec(Kv8Args a) {
   const unsigned group = (blockIdx.x * 256u + threadIdx.x) / kLanes, lane = threadIdx.x % kLanes;
   const int c = lane * 8;
-  float k[kRows][8], v[kRows][8];
+  Raw8<kBf16> in[kRows][2];
   RowAt at[kRows];
+  rows_at(a, group * kRows, 40, at);
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
-    at[i] = row_at(a, group * kRows + i, 40);
-#pragma unroll
-    for (int u = 0; u < 8; ++u) k[i][u] = v[i][u] = 0.0f;
+    in[i][0].zero();
+    in[i][1].zero();
     if (at[i].live && c < a.dim) {
-      load8(a.k, at[i].data + c, a.is_bf16, k[i]);
-      load8(a.v, at[i].data + c, a.is_bf16, v[i]);
+      in[i][0].load(a.k, at[i].data + c);
+      in[i][1].load(a.v, at[i].data + c);
     }
   }
 #pragma unroll
-  for (int i = 0; i < kRows; ++i) {
-    uint32_t km = 0u, vm = 0u;
+  for (int i = 0; i < kRows; ++i)
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      km = max(km, __float_as_uint(k[i][u]) & 0x7fffffffu);
-      vm = max(vm, __float_as_uint(v[i][u]) & 0x7fffffffu);
-    }
+    for (int side = 0; side < 2; ++side) {
+      float x[8];
+      in[i][side].values(x);
+      uint32_t largest = 0u;
 #pragma unroll
-    for (int o = kLanes / 2; o > 0; o >>= 1) {
-      km = max(km, __shfl_xor_sync(0xffffffffu, km, o));
-      vm = max(vm, __shfl_xor_sync(0xffffffffu, vm, o));
+      for (int u = 0; u < 8; ++u) largest = max(largest, __float_as_uint(x[u]) & 0x7fffffffu);
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1) largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+      if (!at[i].live) continue;
+      const uint32_t byte = e8m0_of(largest);
+      if (c < a.dim) *reinterpret_cast<uint2*>(static_cast<uint8_t*>(side ? a.pool.v : a.pool.k) + at[i].pool + c) = codes8(x, byte);
+      if (lane == 0) (side ? a.pool.v_scales : a.pool.k_scales)[at[i].scale] = static_cast<uint8_t>(byte);
     }
-    if (!at[i].live) continue;
-    const uint32_t kb = e8m0_of(km), vb = e8m0_of(vm);
-    if (c < a.dim) {
-      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.pool.k) + at[i].pool + c) = codes8(k[i], kb);
-      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.pool.v) + at[i].pool + c) = codes8(v[i], vb);
-    }
-    if (lane == 0) {
-      a.pool.k_scales[at[i].scale] = static_cast<uint8_t>(kb);
-      a.pool.v_scales[at[i].scale] = static_cast<uint8_t>(vb);
-    }
-  }
 }
 
 __device__ __forceinline__ float load1(const void* p, size_t at, int is_bf16) {
@@ -122,7 +140,8 @@ __global__ void __launch_bounds__(256) kv8_append_any(Kv8Args a) {
   }
 }
 
-__device__ __forceinline__ void store8(void* p, size_t at, int is_bf16, uint2 codes, float f) {
+template <bool kBf16>
+__device__ __forceinline__ void store8(void* p, size_t at, uint2 codes, float f) {
   float x[8];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -130,17 +149,17 @@ __device__ __forceinline__ void store8(void* p, size_t at, int is_bf16, uint2 co
     x[2 * i] = pair.x * f;
     x[2 * i + 1] = pair.y * f;
   }
-  if (is_bf16) {
-    *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p) + at) =
-        make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+  if (kBf16) {
+    __stcs(reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p) + at),
+           make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])));
   } else {
     float4* out = reinterpret_cast<float4*>(static_cast<float*>(p) + at);
-    out[0] = make_float4(x[0], x[1], x[2], x[3]);
-    out[1] = make_float4(x[4], x[5], x[6], x[7]);
+    __stcs(out, make_float4(x[0], x[1], x[2], x[3]));
+    __stcs(out + 1, make_float4(x[4], x[5], x[6], x[7]));
   }
 }
 
-template <int kLanes>
+template <bool kBf16, int kLanes>
 __global__ void __launch_bounds__(256) kv8_read_vec(Kv8Args a) {
   const unsigned group = (blockIdx.x * 256u + threadIdx.x) / kLanes, lane = threadIdx.x % kLanes;
   const int c = lane * 8;
@@ -148,9 +167,9 @@ __global__ void __launch_bounds__(256) kv8_read_vec(Kv8Args a) {
   uint2 k[kRows], v[kRows];
   uint32_t kb[kRows], vb[kRows];
   RowAt at[kRows];
+  rows_at(a, group * kRows, 41, at);
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
-    at[i] = row_at(a, group * kRows + i, 41);
     if (at[i].live) {
       k[i] = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.pool.k) + at[i].pool + c);
       v[i] = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.pool.v) + at[i].pool + c);
@@ -161,8 +180,8 @@ __global__ void __launch_bounds__(256) kv8_read_vec(Kv8Args a) {
 #pragma unroll
   for (int i = 0; i < kRows; ++i)
     if (at[i].live) {
-      store8(a.k, at[i].data + c, a.is_bf16, k[i], e8m0_value(kb[i]));
-      store8(a.v, at[i].data + c, a.is_bf16, v[i], e8m0_value(vb[i]));
+      store8<kBf16>(a.k, at[i].data + c, k[i], e8m0_value(kb[i]));
+      store8<kBf16>(a.v, at[i].data + c, v[i], e8m0_value(vb[i]));
     }
 }
 
@@ -255,23 +274,34 @@ __global__ void __launch_bounds__(128) kv_keep_kernel(KeepArgs a, size_t row_byt
   }
 }
 
+template <bool kBf16, int kLanes>
+void launch_vec(cudaStream_t stream, const Kv8Args& a, bool append) {
+  const unsigned blocks = blocks_for(a, kLanes, kRows);
+  if (append) kv8_append_vec<kBf16, kLanes><<<blocks, 256, 0, stream>>>(a);
+  else kv8_read_vec<kBf16, kLanes><<<blocks, 256, 0, stream>>>(a);
+}
+template <bool kBf16>
+void launch_vec(cudaStream_t stream, const Kv8Args& a, bool append) {
+  if (a.dim <= 64) launch_vec<kBf16, 8>(stream, a, append);
+  else if (a.dim <= 128) launch_vec<kBf16, 16>(stream, a, append);
+  else launch_vec<kBf16, 32>(stream, a, append);
+}
+cudaError_t launch_rows(cudaStream_t stream, const Kv8Args& a, bool append) {
+  if (vector_rows(a)) {
+    if (a.is_bf16) launch_vec<true>(stream, a, append);
+    else launch_vec<false>(stream, a, append);
+  } else if (append) {
+    kv8_append_any<<<blocks_for(a, 32, 1), 256, 0, stream>>>(a);
+  } else {
+    kv8_read_any<<<blocks_for(a, 32, 1), 256, 0, stream>>>(a);
+  }
+  return cudaGetLastError();
+}
+
 }  // namespace
 
-cudaError_t kv8_append(cudaStream_t stream, const Kv8Args& a) {
-  if (!vector_rows(a)) kv8_append_any<<<blocks_for(a, 32, 1), 256, 0, stream>>>(a);
-  else if (a.dim <= 64) kv8_append_vec<8><<<blocks_for(a, 8, kRows), 256, 0, stream>>>(a);
-  else if (a.dim <= 128) kv8_append_vec<16><<<blocks_for(a, 16, kRows), 256, 0, stream>>>(a);
-  else kv8_append_vec<32><<<blocks_for(a, 32, kRows), 256, 0, stream>>>(a);
-  return cudaGetLastError();
-}
-
-cudaError_t kv8_read(cudaStream_t stream, const Kv8Args& a) {
-  if (!vector_rows(a)) kv8_read_any<<<blocks_for(a, 32, 1), 256, 0, stream>>>(a);
-  else if (a.dim <= 64) kv8_read_vec<8><<<blocks_for(a, 8, kRows), 256, 0, stream>>>(a);
-  else if (a.dim <= 128) kv8_read_vec<16><<<blocks_for(a, 16, kRows), 256, 0, stream>>>(a);
-  else kv8_read_vec<32><<<blocks_for(a, 32, kRows), 256, 0, stream>>>(a);
-  return cudaGetLastError();
-}
+cudaError_t kv8_append(cudaStream_t stream, const Kv8Args& a) { return launch_rows(stream, a, true); }
+cudaError_t kv8_read(cudaStream_t stream, const Kv8Args& a) { return launch_rows(stream, a, false); }
 
 cudaError_t kv_keep(cudaStream_t stream, const KeepArgs& a) {
   const int element = a.pool.store == kStoreE4m3 ? 1 : a.pool.store == kStoreBf16 ? 2 : 4;

@@ -16,16 +16,18 @@
 // to 1e-16 in any order, so the tokens do not depend on how the row was cut.
 //
 // The tests of all nodes are independent given the p of the drafted tokens, so a thread takes a node and only
-// the walk along the accepted path is serial.  What costs is the one row the last token is drawn from: a cluster
-// of eight CTAs shares it, a warp per contiguous chunk, the chunks' sums meet in distributed shared memory
-// and the CTA whose chunk holds the threshold looks for the token in it.
+// the walk along the accepted path is serial.  What costs is the one row the last token is drawn from (two with
+// `draft`): a cluster of CTAs shares it, a warp per contiguous chunk, and the chunks' sums meet in distributed shared
+// memory.  The CTA whose chunk holds the threshold cuts that chunk over its threads and looks for the token, by sums
+// over threads first.  A pass of the serial parts (tests, walk, scans, two barriers of the cluster) takes longer than
+// the row, so eight CTAs share it only while all clusters are resident at once, else four.
 #include "common.cuh"
 #include "engine.h"
 
 namespace pluto {
 namespace {
 
-constexpr int kParts = 8, kThreads = 512, kWarps = kThreads / 32;
+constexpr int kMaxParts = 8, kThreads = 512, kWarps = kThreads / 32;
 constexpr int kUnroll = 8;
 
 template <bool kBf16>
@@ -55,14 +57,24 @@ __device__ __forceinline__ double left_at(const void* p, size_t p0, const void* 
   return tried != nullptr && (tried[(x - first) >> 5] >> ((x - first) & 31) & 1u) ? 0.0 : value;
 }
 
+// Inclusive sums over the lanes of a warp.
+__device__ __forceinline__ double warp_scan(double x, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double other = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += other;
+  }
+  return x;
+}
+
+// One cluster per sequence, `parts` CTAs; chunk: tokens of a warp, a multiple of 32.
 template <bool kBf16>
-__global__ void __cluster_dims__(kParts, 1, 1) __launch_bounds__(kThreads)
-verify_kernel(VerifyArgs a, int chunk) {   // chunk: tokens of a warp, a multiple of 32
+__global__ void __launch_bounds__(kThreads, 2) verify_kernel(VerifyArgs a, int parts, int chunk) {
   extern __shared__ uint32_t tried[];      // one bit per token of this CTA's slice
-  __shared__ double p_of[kMaxDraftNodes], sums[kWarps], all[kParts * kWarps];
+  __shared__ double p_of[kMaxDraftNodes], sums[2][kWarps], all[kMaxParts * kWarps];
   __shared__ int token_of[kMaxDraftNodes], parent_of[kMaxDraftNodes], child_of[kMaxDraftNodes + 1];
   __shared__ uint8_t good[kMaxDraftNodes], repeated[kMaxDraftNodes];
-  __shared__ int path[kMaxDraftNodes], accepted, last, any_tried;
+  __shared__ int path[kMaxDraftNodes], accepted, last, any_tried, first_over, last_some;
   const int b = blockIdx.y, part = blockIdx.x, warp = threadIdx.x / 32, lane = threadIdx.x % 32, i = threadIdx.x;
   const size_t node0 = static_cast<size_t>(b) * a.nodes, row0 = static_cast<size_t>(b) * (a.nodes + 1);
   int count = a.nodes;
@@ -77,11 +89,15 @@ verify_kernel(VerifyArgs a, int chunk) {   // chunk: tokens of a warp, a multipl
   if (i <= kMaxDraftNodes) child_of[i] = -1;
   bool fits = false;
   double u = 0.0;
+  int token = 0, parent = 0;
+  if (i < a.nodes) {   // (beside the count)
+    token = a.tokens[node0 + i];
+    parent = tree ? a.parents[node0 + i] : i - 1;
+    u = a.accept[node0 + i];
+  }
   if (i < count) {
-    const int token = a.tokens[node0 + i], parent = tree ? a.parents[node0 + i] : i - 1;
     fits = token >= 0 && token < a.vocab && parent >= -1 && parent < i;
     if (!fits) report_status(a.status, 43, kBadDraft);
-    u = a.accept[node0 + i];
     const double p = fits ? static_cast<double>(prob<kBf16>(a.target, (row0 + parent + 1) * a.vocab + token)) : 0.0;
     token_of[i] = fits ? token : -1;
     parent_of[i] = fits ? parent : -2;   // never anybody's child
@@ -121,6 +137,8 @@ verify_kernel(VerifyArgs a, int chunk) {   // chunk: tokens of a warp, a multipl
     accepted = n;
     last = node;
     any_tried = 0;
+    first_over = kThreads;
+    last_some = -1;
   }
   const int first_token = part * kWarps * chunk;
   const bool drop = tree || a.draft == nullptr;
@@ -147,84 +165,125 @@ verify_kernel(VerifyArgs a, int chunk) {   // chunk: tokens of a warp, a multipl
   // what is left after the refusals, or the row itself; then the row itself where nothing is left
   const void* q = !tree && accepted < count ? a.draft : nullptr;
   const uint32_t* gone = drop && any_tried ? tried : nullptr;
-  double total = 0.0;
+  // Sums of the chunks: lane's chunks lane * 4 to + 3 (unused ones hold 0)
+  const int chunks = parts * kWarps;
+  double total = 0.0, own[4], upto = 0.0;
   for (int attempt = 0; attempt < 2; ++attempt) {
     double sum = 0.0;
     for (int x0 = begin + lane; x0 < end; x0 += 32 * kUnroll) {
-      double v[kUnroll];
+      float v[kUnroll], w[kUnroll];
 #pragma unroll
       for (int k = 0; k < kUnroll; ++k) {
         const int x = x0 + 32 * k;
-        v[k] = x < end ? left_at<kBf16>(a.target, p0, q, q0, gone, first_token, x) : 0.0;
+        v[k] = x < end ? prob<kBf16>(a.target, p0 + x) : 0.0f;
+        w[k] = q != nullptr && x < end ? prob<kBf16>(q, q0 + x) : 0.0f;
       }
 #pragma unroll
-      for (int k = 0; k < kUnroll; ++k) sum += v[k];
+      for (int k = 0; k < kUnroll; ++k) {
+        const int x = x0 + 32 * k;
+        if (gone != nullptr && x < end && (gone[(x - first_token) >> 5] >> ((x - first_token) & 31) & 1u)) v[k] = 0.0f;
+        const double rest = static_cast<double>(v[k]) - static_cast<double>(w[k]);
+        sum += q != nullptr && rest < 0.0 ? 0.0 : rest;   // (NaN stays)
+      }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) sums[warp] = sum;
+    if (lane == 0) sums[attempt][warp] = sum;
     cluster_sync();
-    if (i < kParts * kWarps) all[i] = lds_cluster_f64(&sums[i % kWarps], i / kWarps);
-    cluster_sync();   // read by everybody before the next attempt writes, or the CTA leaves
-    total = 0.0;
-    for (int w = 0; w < kParts * kWarps; ++w) total += all[w];
+    if (i < kMaxParts * kWarps) all[i] = i < chunks ? lds_cluster_f64(&sums[attempt][i % kWarps], i / kWarps) : 0.0;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 4; ++k) own[k] = all[lane * 4 + k];
+    upto = warp_scan((own[0] + own[1]) + (own[2] + own[3]), lane);
+    total = __shfl_sync(0xffffffffu, upto, 31);
     if (total > 0.0 || (q == nullptr && gone == nullptr)) break;
     q = nullptr;
     gone = nullptr;
+    __syncthreads();   // all[] is written again
   }
+  cluster_arrive();   // this CTA has read the others' sums; it leaves when they have read its own
   int32_t* out = a.out + static_cast<size_t>(b) * (a.nodes + 1) + accepted;
   if (!(total > 0.0) || isinf(total)) {
     if (part == 0 && i == 0) *out = -1;
+    cluster_wait();
     return;
   }
   // the chunk that holds the threshold (the last one with anything in it where rounding leaves none)
   const double threshold = static_cast<double>(a.sample[b]) * total;
-  double before = 0.0, cum = 0.0;
-  int holder = -1;
-  for (int w = 0; w < kParts * kWarps; ++w) {
-    if (all[w] > 0.0) {
-      holder = w;
-      before = cum;
-    }
-    cum += all[w];
-    if (cum > threshold) break;
-  }
-  if (holder != part * kWarps + warp) return;
-  int found = -1, nonzero = -1;
-  for (int x0 = begin; x0 < end && found < 0; x0 += 32 * kUnroll) {
-    double v[kUnroll];
+  double cum = __shfl_up_sync(0xffffffffu, upto, 1), before = 0.0, before_some = 0.0;   // (kept exactly: no difference of sums)
+  int over = -1, some = -1;
+  if (lane == 0) cum = 0.0;
 #pragma unroll
-    for (int k = 0; k < kUnroll; ++k) {
-      const int x = x0 + 32 * k + lane;
-      v[k] = x < end ? left_at<kBf16>(a.target, p0, q, q0, gone, first_token, x) : 0.0;
-    }
-#pragma unroll
-    for (int k = 0; k < kUnroll; ++k) {
-      double up_to = v[k];
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double other = __shfl_up_sync(0xffffffffu, up_to, o);
-        if (lane >= o) up_to += other;
+  for (int k = 0; k < 4; ++k) {
+    if (own[k] > 0.0) {
+      some = lane * 4 + k;
+      before_some = cum;
+      if (over < 0 && cum + own[k] > threshold) {
+        over = some;
+        before = cum;
       }
-      const unsigned over = __ballot_sync(0xffffffffu, v[k] > 0.0 && before + up_to > threshold);
-      const unsigned some = __ballot_sync(0xffffffffu, v[k] > 0.0);
-      if (found < 0 && over) found = x0 + 32 * k + __ffs(over) - 1;
-      if (some) nonzero = x0 + 32 * k + 31 - __clz(some);
-      before += __shfl_sync(0xffffffffu, up_to, 31);
+    }
+    cum += own[k];
+  }
+  const unsigned overs = __ballot_sync(0xffffffffu, over >= 0), somes = __ballot_sync(0xffffffffu, some >= 0);
+  const int from = overs ? __ffs(overs) - 1 : 31 - __clz(somes);
+  const int holder = __shfl_sync(0xffffffffu, overs ? over : some, from);
+  before = __shfl_sync(0xffffffffu, overs ? before : before_some, from);
+  if (holder / kWarps == part) {
+    // a few neighbouring tokens per thread
+    const int per = (chunk + kThreads - 1) / kThreads;
+    const int stop = min(a.vocab, first_token + (holder % kWarps + 1) * chunk);
+    const int at = min(stop, first_token + holder % kWarps * chunk + i * per), to = min(stop, at + per);
+    double sum = 0.0;
+#pragma unroll 4
+    for (int x = at; x < to; ++x) sum += left_at<kBf16>(a.target, p0, q, q0, gone, first_token, x);
+    const double scanned = warp_scan(sum, lane);
+    double below = __shfl_up_sync(0xffffffffu, scanned, 1);
+    if (lane == 0) below = 0.0;
+    __syncthreads();   // all[] was read by every warp
+    if (lane == 31) all[warp] = scanned;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) before += all[w];
+    below += before;
+    if (sum > 0.0) {
+      atomicMax(&last_some, i);
+      if (below + sum > threshold) atomicMin(&first_over, i);
+    }
+    __syncthreads();
+    if (i == (first_over < kThreads ? first_over : last_some)) {
+      int found = -1;
+      for (int x = at; x < to; ++x) {
+        const double value = left_at<kBf16>(a.target, p0, q, q0, gone, first_token, x);
+        below += value;
+        if (value > 0.0) {
+          found = x;
+          if (below > threshold) break;
+        }
+      }
+      *out = found;
     }
   }
-  if (lane == 0) *out = found >= 0 ? found : nonzero;
+  cluster_wait();
 }
 
 }  // namespace
 
 cudaError_t verify_drafts(cudaStream_t stream, const VerifyArgs& a) {
-  const int per_warp = (a.vocab + kParts * kWarps - 1) / (kParts * kWarps), chunk = (per_warp + 31) / 32 * 32;
-  const size_t bytes = static_cast<size_t>(kWarps) * chunk / 8;
-  const dim3 grid(kParts, a.batch);
-  if (a.is_bf16) verify_kernel<true><<<grid, kThreads, bytes, stream>>>(a, chunk);
-  else verify_kernel<false><<<grid, kThreads, bytes, stream>>>(a, chunk);
-  return cudaGetLastError();
+  const int parts = a.batch * kMaxParts <= 2 * 148 ? kMaxParts : kMaxParts / 2;
+  const int per_warp = (a.vocab + parts * kWarps - 1) / (parts * kWarps), chunk = (per_warp + 31) / 32 * 32;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(parts, a.batch);
+  config.blockDim = dim3(kThreads);
+  config.dynamicSmemBytes = static_cast<size_t>(kWarps) * chunk / 8;
+  config.stream = stream;
+  cudaLaunchAttribute cluster;
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim = {static_cast<unsigned>(parts), 1, 1};
+  config.attrs = &cluster;
+  config.numAttrs = 1;
+  const cudaError_t e = a.is_bf16 ? cudaLaunchKernelEx(&config, verify_kernel<true>, a, parts, chunk)
+                                  : cudaLaunchKernelEx(&config, verify_kernel<false>, a, parts, chunk);
+  return e != cudaSuccess ? e : cudaGetLastError();
 }
 
 }  // namespace pluto
