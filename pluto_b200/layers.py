@@ -702,48 +702,58 @@ class DraftVerdict(NamedTuple):
 _STORAGE = {torch.float32: 0, torch.bfloat16: 1, torch.float8_e4m3fn: 2}
 
 
-def _draft_pool(k_pool, v_pool, block_table, k_scales, v_scales, batch):
+def _draft_pool(k_pool, v_pool, block_table, k_scales, v_scales, batch, device):
     """struct pluto_kv_cache and struct pluto_kv_scales of a page pool of any storage type, as bytes."""
-    code = _STORAGE.get(k_pool.dtype)
+    code, shape, strides = _STORAGE.get(k_pool.dtype), k_pool.shape, k_pool.stride()
     if code is None or v_pool.dtype != k_pool.dtype:
         raise _invalid("a cache pool stores fp32, bf16 or E4M3")
-    strides = k_pool.stride()
-    if (k_pool.dim() != 4 or v_pool.shape != k_pool.shape or v_pool.stride() != strides or strides[3] != 1
-            or strides[2] != k_pool.shape[3]):
+    if len(shape) != 4 or v_pool.shape != shape or v_pool.stride() != strides or strides[3] != 1 or strides[2] != shape[3]:
         raise _invalid("cache pools are [pages, page_size, kv_heads, head_dim] of one shape, heads contiguous")
-    if k_pool.get_device() != _device_index():
+    if k_pool.get_device() != device or v_pool.get_device() != device:
         raise _invalid("the cache is not on the current device")
+    table, blocks = None, 0
     if block_table is None:
-        if k_pool.shape[0] < batch:
+        if shape[0] < batch:
             raise _invalid("a cache without a block table has a page for every sequence")
     else:
-        _check_ints(block_table, (batch, block_table.shape[-1]), "block table")
-    cache = _capi.fast().kv_cache(k_pool.data_ptr(), v_pool.data_ptr(), _ptr(block_table),
-                                  0 if block_table is None else block_table.shape[1], k_pool.shape[1], strides[0], strides[1],
-                                  code, k_pool.shape[0])
-    if (code == 2) != (k_scales is not None) or (code == 2) != (v_scales is not None):
-        raise _invalid("an 8-bit cache needs its scales, and only that")
+        blocks = block_table.shape[-1]
+        _check_ints(block_table, (batch, blocks), "block table", device)
+        table = block_table.data_ptr()
+    L = _capi.fast()
+    cache = L.kv_cache(k_pool.data_ptr(), v_pool.data_ptr(), table, blocks, shape[1], strides[0], strides[1], code, shape[0])
     if code != 2:
+        if k_scales is not None or v_scales is not None:
+            raise _invalid("an 8-bit cache needs its scales, and only that")
         return cache, None
-    if (k_scales.shape != k_pool.shape[:3] or v_scales.shape != k_scales.shape or v_scales.stride() != k_scales.stride()
-            or (k_scales.stride(2) != 1 and k_scales.shape[2] != 1) or k_scales.element_size() != 1
-            or v_scales.element_size() != 1 or k_scales.get_device() != k_pool.get_device()):
+    if k_scales is None or v_scales is None:
+        raise _invalid("an 8-bit cache needs its scales, and only that")
+    strides = k_scales.stride()
+    if (k_scales.shape != shape[:3] or v_scales.shape != shape[:3] or v_scales.stride() != strides
+            or (strides[2] != 1 and shape[2] != 1) or k_scales.element_size() != 1 or v_scales.element_size() != 1
+            or k_scales.get_device() != device or v_scales.get_device() != device):
         raise _invalid("cache scales are one byte each, [pages, page_size, kv_heads], heads contiguous")
-    return cache, _capi.fast().kv_scales(k_scales.data_ptr(), v_scales.data_ptr(), k_scales.stride(0), k_scales.stride(1))
+    return cache, L.kv_scales(k_scales.data_ptr(), v_scales.data_ptr(), strides[0], strides[1])
 
 
 def _device_index() -> int:
     return torch.cuda.current_device() if _current_device is None else _current_device()
 
 
-def _check_ints(t, shape, what: str) -> None:
-    if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous() or not t.is_cuda):
-        raise _invalid(f"{what} must be a contiguous int32 device tensor of shape {list(shape)}")
+def _check_ints(t, shape, what: str, device: int) -> Optional[int]:
+    """The address of an optional int32 argument."""
+    if t is None:
+        return None
+    if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous() or t.get_device() != device:
+        raise _invalid(f"{what} must be a contiguous int32 tensor of shape {list(shape)} on the current device")
+    return t.data_ptr()
 
 
-def _check_rows(t, shape, what: str) -> None:
-    if tuple(t.shape) != tuple(shape) or t.stride(3) != 1 or t.get_device() != _device_index():
+def _check_rows(t, shape, what: str, device: int):
+    """The strides of head rows."""
+    strides = t.stride()
+    if t.shape != shape or strides[3] != 1 or t.get_device() != device:
         raise _invalid(f"{what} must be {list(shape)} on the current device, head rows contiguous")
+    return strides
 
 
 def _call_scratch(device: torch.device, nbytes: int) -> torch.Tensor:
@@ -760,17 +770,16 @@ def kv8_append(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor, v_pool: t
     """Quantises rows k, v [B,T,Hkv,D] (bf16 or fp32) into the slots positions[b] + t (None: t) of an 8-bit page
     pool [pages, page_size, Hkv, D] (float8_e4m3fn) with scales [pages, page_size, Hkv] (one byte each); with
     `counts` int32 [B] only the first counts[b] tokens of sequence b."""
-    B, T, H, D = k.shape
-    cache, scales = _draft_pool(k_pool, v_pool, block_table, k_scales, v_scales, B)
+    (B, T, H, D), device = k.shape, _device_index()
+    cache, scales = _draft_pool(k_pool, v_pool, block_table, k_scales, v_scales, B, device)
     if k.stride(3) != 1 or k.stride() != v.stride():
         k, v = k.contiguous(), v.contiguous()
-    if v.shape != k.shape or v.dtype != k.dtype or k_pool.shape[2:] != k.shape[2:]:
+    strides = _check_rows(k, (B, T, H, D), "cache rows", device)
+    if v.shape != k.shape or v.dtype != k.dtype or v.get_device() != device or k_pool.shape[2:] != (H, D):
         raise _invalid("8-bit cache rows do not match the pool")
-    _check_rows(k, k.shape, "cache rows")
-    _check_ints(positions, (B,), "positions")
-    _check_ints(counts, (B,), "counts")
-    check(_capi.fast().pluto_kv8_append(_stream(), k.data_ptr(), v.data_ptr(), _dt(k), k.stride(0), k.stride(1), k.stride(2),
-                                        cache, scales, _ptr(positions), _ptr(counts), B, T, H, D))
+    check(_capi.fast().pluto_kv8_append(_stream(), k.data_ptr(), v.data_ptr(), _dt(k), strides[0], strides[1], strides[2], cache, scales,
+                                        _check_ints(positions, (B,), "positions", device), _check_ints(counts, (B,), "counts", device),
+                                        B, T, H, D))
 
 
 def kv8_read(k_pool: torch.Tensor, v_pool: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor,
@@ -778,14 +787,15 @@ def kv8_read(k_pool: torch.Tensor, v_pool: torch.Tensor, k_scales: torch.Tensor,
              counts: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.bfloat16):
     """(k, v) [B,tokens,Hkv,D]: the values that the slots positions[b] .. positions[b] + tokens - 1 of an 8-bit
     pool hold (exact in bf16); with `counts` the rows from counts[b] on are zero."""
-    B, (_, _, H, D) = positions.shape[0], k_pool.shape
-    cache, scales = _draft_pool(k_pool, v_pool, block_table, k_scales, v_scales, B)
-    _check_ints(positions, (B,), "positions")
-    _check_ints(counts, (B,), "counts")
+    B, device = positions.shape[0], _device_index()
+    cache, scales = _draft_pool(k_pool, v_pool, block_table, k_scales, v_scales, B, device)
+    _, _, H, D = k_pool.shape
     new = torch.empty if counts is None else torch.zeros
-    k, v = (new((B, tokens, H, D), dtype=dtype, device=k_pool.device) for _ in range(2))
-    check(_capi.fast().pluto_kv8_read(_stream(), k.data_ptr(), v.data_ptr(), _dt(k), k.stride(0), k.stride(1), k.stride(2),
-                                      cache, scales, positions.data_ptr(), _ptr(counts), B, tokens, H, D))
+    k = new((B, tokens, H, D), dtype=dtype, device=k_pool.device)
+    v = new((B, tokens, H, D), dtype=dtype, device=k_pool.device)
+    check(_capi.fast().pluto_kv8_read(_stream(), k.data_ptr(), v.data_ptr(), _dt(k), tokens * H * D, H * D, D, cache, scales,
+                                      _check_ints(positions, (B,), "positions", device), _check_ints(counts, (B,), "counts", device),
+                                      B, tokens, H, D))
     return k, v
 
 
@@ -795,12 +805,10 @@ def kv_keep(k_pool: torch.Tensor, v_pool: torch.Tensor, prefix_lens: torch.Tenso
     """After a verification: the rows of the accepted path move from slots prefix_lens[b] + path[b][i] to slots
     prefix_lens[b] + i, in place, for i < accepted[b]; every other slot keeps its rows.  The caller then adds
     `accepted` to its lengths.  path int32 [B,N], accepted int32 [B], as verify_drafts returns them."""
-    B, N = path.shape
-    cache, scales = _draft_pool(k_pool, v_pool, block_table, k_scales, v_scales, B)
-    _check_ints(prefix_lens, (B,), "prefix lengths")
-    _check_ints(path, (B, N), "path")
-    _check_ints(accepted, (B,), "accepted")
-    check(_capi.fast().pluto_kv_keep(_stream(), cache, scales, prefix_lens.data_ptr(), path.data_ptr(), accepted.data_ptr(), B, N,
+    (B, N), device = path.shape, _device_index()
+    cache, scales = _draft_pool(k_pool, v_pool, block_table, k_scales, v_scales, B, device)
+    check(_capi.fast().pluto_kv_keep(_stream(), cache, scales, _check_ints(prefix_lens, (B,), "prefix lengths", device),
+                                     _check_ints(path, (B, N), "path", device), _check_ints(accepted, (B,), "accepted", device), B, N,
                                      k_pool.shape[2], k_pool.shape[3]))
 
 
@@ -814,28 +822,26 @@ def draft_prepare(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_norm: tor
     strides), k, v [B,N,Hkv,D].  Node i of sequence b is rotated for position prefix_lens[b] + its depth and its
     rows go to slot prefix_lens[b] + i of a pool of any storage type.  Returns the queries [B,N,Hq,D], bf16
     when round_to_bfloat16 and fp32 otherwise.  Without `parents` (a chain, or a whole prompt) any N."""
-    B, N, Hq, D = q.shape
+    (B, N, Hq, D), device = q.shape, _device_index()
+    cache, scales = _draft_pool(k_pool, v_pool, block_table, k_scales, v_scales, B, device)
     Hkv = k_pool.shape[2]
-    cache, scales = _draft_pool(k_pool, v_pool, block_table, k_scales, v_scales, B)
-    if q.stride(3) != 1 or (B > 1 and q.stride(0) != N * q.stride(1)):
+    strides = _check_rows(q, (B, N, Hq, k_pool.shape[3]), "drafted queries", device)
+    if B > 1 and strides[0] != N * strides[1]:
         raise _invalid("attention query must have a contiguous head dimension and batch")
     k, v = k.contiguous(), v.contiguous()
-    _check_rows(q, (B, N, Hq, k_pool.shape[3]), "drafted queries")
-    _check_rows(k, (B, N, Hkv, D), "drafted keys")
-    _check_rows(v, (B, N, Hkv, D), "drafted values")
+    _check_rows(k, (B, N, Hkv, D), "drafted keys", device)
+    _check_rows(v, (B, N, Hkv, D), "drafted values", device)
     if k.dtype != q.dtype or v.dtype != q.dtype:
         raise _invalid("drafted queries, keys and values have one type")
     for norm in (q_norm, k_norm):
-        if norm.dtype != torch.float32 or norm.numel() != D or not norm.is_cuda:
+        if norm.dtype != torch.float32 or norm.numel() != D or norm.get_device() != device or not norm.is_contiguous():
             raise _invalid("Qwen attention norms must be FP32 head-width parameters on its Executor")
-    _check_ints(prefix_lens, (B,), "prefix lengths")
-    _check_ints(parents, (B, N), "parents")
-    _check_ints(counts, (B,), "counts")
     out = torch.empty((B, N, Hq, D), dtype=torch.bfloat16 if round_to_bfloat16 else torch.float32, device=q.device)
     check(_capi.fast().pluto_draft_prepare(
-        _stream(), q.data_ptr(), k.data_ptr(), v.data_ptr(), _dt(q), q.stride(1), q.stride(2), q_norm.data_ptr(),
-        k_norm.data_ptr(), _ptr(prefix_lens), _ptr(parents), _ptr(counts), out.data_ptr(), _dt(out), cache, scales, B, N, Hq,
-        Hkv, D, rotary_dim, rms_norm_epsilon, rope_theta, int(round_to_bfloat16)))
+        _stream(), q.data_ptr(), k.data_ptr(), v.data_ptr(), _dt(q), strides[1], strides[2], q_norm.data_ptr(), k_norm.data_ptr(),
+        _check_ints(prefix_lens, (B,), "prefix lengths", device), _check_ints(parents, (B, N), "parents", device),
+        _check_ints(counts, (B,), "counts", device), out.data_ptr(), _dt(out), cache, scales, B, N, Hq, Hkv, D, rotary_dim,
+        rms_norm_epsilon, rope_theta, int(round_to_bfloat16)))
     return out
 
 
@@ -850,34 +856,34 @@ def gqa_tree_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     prefix_lens[b], its ancestors by `parents` int32 [B,N] (None: a chain) and itself.  `counts` int32 [B]: the
     sequence has that many nodes; the rows of the others are left as they were (zeros without `out`).  One
     node per sequence is gqa_decode.  Returns out [B,N,Hq,D] (and lse [B,N,Hq])."""
-    B, N, Hq, D = q.shape
+    (B, N, Hq, D), device = q.shape, _device_index()
+    cache, scales = _draft_pool(k_pool, v_pool, block_table, k_scales, v_scales, B, device)
     Hkv = k_pool.shape[2]
-    cache, scales = _draft_pool(k_pool, v_pool, block_table, k_scales, v_scales, B)
-    _check_rows(q, (B, N, Hq, k_pool.shape[3]), "drafted queries")
+    _check_rows(q, (B, N, Hq, k_pool.shape[3]), "drafted queries", device)
     if not q.is_contiguous():
         q = q.contiguous()
-    _check_ints(prefix_lens, (B,), "prefix lengths")
-    _check_ints(parents, (B, N), "parents")
-    _check_ints(counts, (B,), "counts")
     new = torch.empty if counts is None else torch.zeros
     if out is None:
         out = new((B, N, Hq, D), dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or not out.is_contiguous() or out.get_device() != q.get_device():
+    elif out.shape != q.shape or not out.is_contiguous() or out.get_device() != device:
         raise _invalid("attention output must be contiguous and of the query's shape")
     lse = new((B, N, Hq), dtype=torch.float32, device=q.device) if want_lse else None
-    gts = ghs = 0
+    gate_at, gate_type, gts, ghs = None, 0, 0, 0
     if gate is not None:
-        _check_rows(gate, q.shape, "attention gate")
-        if B > 1 and gate.stride(0) != N * gate.stride(1):
+        strides = _check_rows(gate, q.shape, "attention gate", device)
+        if B > 1 and strides[0] != N * strides[1]:
             raise _invalid("attention gate must have a contiguous head dimension and batch")
-        gts, ghs = gate.stride(1), gate.stride(2)
+        gate_at, gate_type, gts, ghs = gate.data_ptr(), _dt(gate), strides[1], strides[2]
     L = _capi.fast()
     if workspace is None:
         workspace = _call_scratch(q.device, L.pluto_gqa_tree_decode_workspace_bytes(B, N, Hq, Hkv, D))
-    check(L.pluto_gqa_tree_decode(_stream(), q.data_ptr(), _dt(q), _ptr(gate), 0 if gate is None else _dt(gate), gts, ghs, cache,
-                                  scales, prefix_lens.data_ptr(), max_prefix_len, _ptr(parents), _ptr(counts), out.data_ptr(),
-                                  _dt(out), _ptr(lse), workspace.data_ptr(), workspace.numel() * workspace.element_size(), B, N,
-                                  Hq, Hkv, D, int(round_to_bfloat16)))
+    elif workspace.get_device() != device or not workspace.is_contiguous():
+        raise _invalid("the workspace must be contiguous, on the current device")
+    check(L.pluto_gqa_tree_decode(_stream(), q.data_ptr(), _dt(q), gate_at, gate_type, gts, ghs, cache, scales,
+                                  _check_ints(prefix_lens, (B,), "prefix lengths", device), max_prefix_len,
+                                  _check_ints(parents, (B, N), "parents", device), _check_ints(counts, (B,), "counts", device),
+                                  out.data_ptr(), _dt(out), _ptr(lse), workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+                                  B, N, Hq, Hkv, D, int(round_to_bfloat16)))
     return (out, lse) if want_lse else out
 
 
@@ -893,25 +899,24 @@ def verify_drafts(target_probs: torch.Tensor, tokens: torch.Tensor, accept_unifo
     tree: the children of the last accepted node in index order, child c when u_c * (1 - p of the siblings tried
     before) < p(x_c), a token tried before never; what is left is p without the tried tokens.  The drawn
     token is the smallest x whose running sum exceeds u * total.  Tests and sums are in double."""
-    B, N = tokens.shape
-    V = target_probs.shape[2] if target_probs.dim() == 3 else 0
-    if V == 0 or tuple(target_probs.shape) != (B, N + 1, V) or not target_probs.is_contiguous():
+    (B, N), shape, device = tokens.shape, target_probs.shape, _device_index()
+    V = shape[2] if len(shape) == 3 else 0
+    if V == 0 or shape != (B, N + 1, V) or not target_probs.is_contiguous():
         raise _invalid("target probabilities must be [batch, nodes + 1, vocab], contiguous")
-    if draft_probs is not None and (tuple(draft_probs.shape) != (B, N, V) or not draft_probs.is_contiguous()
-                                    or draft_probs.dtype != target_probs.dtype or not draft_probs.is_cuda):
+    if draft_probs is not None and (draft_probs.shape != (B, N, V) or not draft_probs.is_contiguous()
+                                    or draft_probs.dtype != target_probs.dtype or draft_probs.get_device() != device):
         raise _invalid("draft probabilities must be [batch, nodes, vocab] of the target's type, contiguous")
     for u, shape in ((accept_uniforms, (B, N)), (sample_uniforms, (B,))):
-        if u.dtype != torch.float32 or tuple(u.shape) != shape or not u.is_contiguous() or not u.is_cuda:
+        if u.dtype is not torch.float32 or u.shape != shape or not u.is_contiguous() or u.get_device() != device:
             raise _invalid("uniform numbers must be fp32 [batch, nodes] and [batch], contiguous")
-    if target_probs.get_device() != _device_index():
+    if target_probs.get_device() != device:
         raise _invalid("target probabilities are not on the current device")
-    _check_ints(tokens, (B, N), "drafted tokens")
-    _check_ints(parents, (B, N), "parents")
-    _check_ints(counts, (B,), "counts")
-    accepted, path, out = (torch.empty(shape, dtype=torch.int32, device=target_probs.device) for shape in ((B,), (B, N), (B, N + 1)))
+    at = _check_ints(tokens, (B, N), "drafted tokens", device)
+    accepted, path, out = tokens.new_empty(B), torch.empty_like(tokens), tokens.new_empty((B, N + 1))
     check(_capi.fast().pluto_verify_drafts(
-        _stream(), target_probs.data_ptr(), _ptr(draft_probs), _dt(target_probs), tokens.data_ptr(), accept_uniforms.data_ptr(),
-        sample_uniforms.data_ptr(), _ptr(parents), _ptr(counts), accepted.data_ptr(), path.data_ptr(), out.data_ptr(), B, N, V))
+        _stream(), target_probs.data_ptr(), _ptr(draft_probs), _dt(target_probs), at, accept_uniforms.data_ptr(),
+        sample_uniforms.data_ptr(), _check_ints(parents, (B, N), "parents", device), _check_ints(counts, (B,), "counts", device),
+        accepted.data_ptr(), path.data_ptr(), out.data_ptr(), B, N, V))
     return DraftVerdict(accepted, path, out)
 
 
