@@ -4,15 +4,17 @@
 //
 // The rows of a unit (sequence, KV head) are its nodes times the query heads of the KV head, row = node *
 // group + head, so the cache is read once for all of them.  They are the 128 lanes of the MMA tiles:
-//   S = Q K^T   M 128, N 64 keys, A = Q held in TMEM for the whole unit, B = the key tile (K-major)
+//   S = Q K^T   M 128, N 64 keys, A = Q, B = the key tile (K-major)
 //   O += P V    M 128, N D, A = P (bf16) written over S in TMEM, B = the value tile (MN-major)
 // with one thread per row doing the softmax (running maximum with lazy rescaling of O, fp32 sums).  Few rows leave
 // lanes idle, which costs nothing while the tiles arrive at memory speed: a 64-key tile of width 128 takes
 // 512 clocks of the tensor pipe and 712 (8-bit) or 1424 (bf16) of an SM's share of the HBM rate.
 //
 // Two streams of S, O and softmax warps run side by side so that one's products run under the other's softmax.
-// Up to 128 rows: the streams take the even and the odd key tiles and are merged at the end.  More: each
-// takes 128 rows and both read every tile.  Width 256 (O takes half of TMEM): one O, two buffers of S.
+// Up to 128 rows: the streams take the even and the odd key tiles and are merged at the end.  More (kWide): each
+// takes 128 rows and both read every tile; Q moves to shared memory, which makes room in TMEM for two score buffers
+// per stream, so that the softmax, which bounds this form, does not wait for the product before it.  Width 256 (O takes
+// half of TMEM): one stream with two score buffers.
 //
 // Loading.  Four warps copy the rows into a ring with asynchronous 16-byte copies; pages may have any size and rows any
 // 16-byte stride.  bf16 rows land as the swizzled tiles that the products read.  8-bit codes land as they are (96 KB per
@@ -29,7 +31,7 @@
 namespace pluto {
 namespace {
 
-constexpr int kTile = 64;            // keys
+constexpr int kTile = 64, kHalf = kTile / 2;   // keys of a tile, and of what the softmax takes at a time
 template <bool kEight>
 constexpr int kThreads = kEight ? 768 : 512;   // warps 0-3: MMA issue; 4-11: softmax; 12-15: loads; 16-23: widening
 constexpr int kMaxCtas = 148;
@@ -37,25 +39,28 @@ constexpr int kUnitTiles = 3;        // query load and read-out of a unit, in ti
 constexpr float kRescale = 8.0f;     // O is rescaled when the maximum has grown by more than 2^8
 constexpr float kSmallest = -100.0f; // exponent of the value rows from which smaller ones are taken for as large
 
-template <int D, bool kEight>
-constexpr int kStages = kEight ? (D == 64 ? 6 : D == 128 ? 3 : 2) : (D == 64 ? 10 : D == 128 ? 6 : 3);   // tiles of keys, and of values
-template <int D>
-constexpr int kRawStages = D == 64 ? 8 : D == 128 ? 6 : 2;   // key and value tiles as codes
+// kWide: more than 128 rows may share a pass over the keys (never at width 256)
+template <int D, bool kEight, bool kWide>   // tiles of keys, and of values
+constexpr int kStages = kEight ? (D == 64 ? 6 : D == 128 ? 3 : 2) : (D == 64 ? 10 : D == 128 ? (kWide ? 4 : 6) : 3);
+template <int D, bool kWide>
+constexpr int kRawStages = D == 64 ? 8 : D == 128 ? (kWide ? 3 : 6) : 2;   // key and value tiles as codes
 template <int D>
 constexpr int kTileBytes = kTile * D * 2;
 constexpr int group_rows(int dim) { return dim == 256 ? 128 : 256; }   // rows that share one pass over the keys
 
 // ---- shared memory -------------------------------------------------------------------------------------------
 constexpr int kSegments = 8;         // of the ring
-constexpr int kSegmentReaders = 13;  // warps: MMA issue, eight softmax, four loaders
+template <bool kWide>
+constexpr int kSegmentReaders = kWide ? 14 : 13;   // warps: MMA issue, eight softmax, four loaders
 
-template <int D, bool kEight>
+template <int D, bool kEight, bool kWide>
 struct Shared {
-  static constexpr int kTiles = kStages<D, kEight>, kRaw = kEight ? kRawStages<D> : 1;
+  static constexpr int kTiles = kStages<D, kEight, kWide>, kRaw = kEight ? kRawStages<D, kWide> : 1;
   uint64_t seg_full[kSegments], seg_empty[kSegments];
   uint64_t k_full[kTiles], k_empty[kTiles], v_full[kTiles], v_empty[kTiles];
   uint64_t raw_k[kRaw], raw_v[kRaw], raw_scales[kRaw], raw_empty[kRaw];
-  uint64_t q_full[2], s_full[2], p_half[2], p_full[2], pv_half[2], pv_done[2];   // one phase per tile of the buffer
+  uint64_t q_full[2];
+  uint64_t s_full[2][2], p_half[2][2], p_full[2][2], pv_half[2][2], pv_done[2][2];   // [stream][score buffer]
   uint64_t ml_full, o_read;   // the two streams' meeting points: sums written, O read
   Segment seg[kSegments];
   uint32_t tmem;
@@ -63,12 +68,12 @@ struct Shared {
   // 8-bit caches: the raw tiles' scale bytes and first draft that not every node sees (-1: the range ends)
   uint8_t k_byte[kRaw][kTile], v_byte[kRaw][kTile];
   int draft_row[kRaw];
-  // ... and per tile whether the softmax has to apply the rows' factors; a ring of twice the stages (a tile's scores may
-  // still be read when its key stage has been refilled, but not when the next one has: that product was issued
-  // behind this tile's)
-  alignas(16) float k_factor[2 * kTiles][kTile];   // (read four at a time)
-  float v_factor[2 * kTiles][kTile];
-  int scaled[2 * kTiles], v_largest[2 * kTiles];
+  // ... and per tile whether the softmax has to apply the rows' factors.  A ring of three times the stages: a slot is
+  // written again once the stage of the tile two rounds on is free, and that tile's scores are issued behind the
+  // product of this one, whose softmax has then read them.
+  alignas(16) float k_factor[3 * kTiles][kTile];   // (read four at a time)
+  float v_factor[3 * kTiles][kTile];
+  int scaled[3 * kTiles], v_largest[3 * kTiles];
 };
 
 // The next segment of the range, by every lane of a warp; false at its end (or when a wait ran out).
@@ -111,9 +116,9 @@ __device__ __forceinline__ uint32_t load_byte(const uint8_t* p, bool there) {   
 // Four warps; a warp copies every fourth half tile (32 rows of keys and of values), a lane looking after the page and the
 // scales of its row.  Nothing is used in the step that asks for it: pages are fetched one unit ahead of the
 // copies, scale bytes are passed on one unit later.
-template <int D, bool kEight>
-__device__ __forceinline__ void load_tiles(const TreeArgs& a, Shared<D, kEight>* sh, uint32_t k_ring, uint32_t v_ring, int warp, int lane) {
-  constexpr int kRing = kEight ? kRawStages<D> : kStages<D, kEight>;
+template <int D, bool kEight, bool kWide>
+__device__ __forceinline__ void load_tiles(const TreeArgs& a, Shared<D, kEight, kWide>* sh, uint32_t k_ring, uint32_t v_ring, int warp, int lane) {
+  constexpr int kRing = kEight ? kRawStages<D, kWide> : kStages<D, kEight, kWide>;
   constexpr int kElement = kEight ? 1 : 2, kBytes = kTile * D * kElement, kPieces = D * kElement / 16, kLoads = kPieces;
   uint64_t* k_full = kEight ? sh->raw_k : sh->k_full;
   uint64_t* v_full = kEight ? sh->raw_v : sh->v_full;
@@ -151,8 +156,8 @@ __device__ __forceinline__ void load_tiles(const TreeArgs& a, Shared<D, kEight>*
   for (;; n += 2, tile += 2, settle()) {
     const int slot = n % kRing, use = n / kRing;
     if (!more && !kEight) break;
-    // (with two slots this unit's is the one whose scales are still to be passed on)
-    if (kEight && kRing == 2) pass_scales();
+    // (few slots: this one, or one that its tile waits for, is freed once the last unit's scales have been passed on)
+    if (kEight && kRing <= 3) pass_scales();
     if (use > 0) {
       if (!__all_sync(0xffffffffu, mbar_wait(kEight ? &sh->raw_empty[slot] : &sh->k_empty[slot], (use - 1) & 1, status, 50))) return;
       if (!kEight && !__all_sync(0xffffffffu, mbar_wait(&sh->v_empty[slot], (use - 1) & 1, status, 51))) return;
@@ -236,16 +241,16 @@ __device__ __forceinline__ uint32_t half_power(uint32_t byte) {
 }
 
 // Eight warps: every fourth half of the key tiles, or of the value tiles, each.
-template <int D>
-__device__ __forceinline__ void widen_tiles(Shared<D, true>* sh, uint32_t raw_ring, uint32_t ring, uint32_t* status, int warp, int lane, bool values) {
-  constexpr int kTiles = kStages<D, true>, kRaw = kRawStages<D>, kPieces = D / 16, kStep = 32 / kPieces;   // rows per step
+template <int D, bool kWide>
+__device__ __forceinline__ void widen_tiles(Shared<D, true, kWide>* sh, uint32_t raw_ring, uint32_t ring, uint32_t* status, int warp, int lane, bool values) {
+  constexpr int kTiles = kStages<D, true, kWide>, kRaw = kRawStages<D, kWide>, kPieces = D / 16, kStep = 32 / kPieces;   // rows per step
   const int first_row = (warp & 1) * 32;
   const int row = lane / kPieces, c = lane % kPieces;
   // Channels 16c .. 16c + 15 are pieces 2c and 2c + 1 of the tile's row; odd slabs store the second first, so that eight lanes
   // hit all banks once.  A step is kStep rows, so the swizzle of the two pieces repeats every 8 / kStep steps.
   const int second = c / 4 & 1, slab = c / 4 * (kTile * 128), p0 = (2 * c + second) & 7, p1 = (2 * c + 1 - second) & 7;
   for (int n = warp >> 1;; n += 2) {
-    const int slot = n % kRaw, stage = n % kTiles, use = n / kTiles, scale_slot = n % (2 * kTiles);
+    const int slot = n % kRaw, stage = n % kTiles, use = n / kTiles, scale_slot = n % (3 * kTiles);
     if (!__all_sync(0xffffffffu, mbar_wait(&sh->raw_scales[slot], (n / kRaw) & 1, status, 47))) return;
     const int draft_row = sh->draft_row[slot];
     if (draft_row < 0) return;
@@ -302,34 +307,40 @@ __device__ __forceinline__ void widen_tiles(Shared<D, true>* sh, uint32_t raw_ri
   }
 }
 
-template <int D, bool kEight>
-constexpr int kRingBytes = 2 * kStages<D, kEight> * kTileBytes<D> + (kEight ? 2 * kRawStages<D> * kTile * D : 0);
+template <int D, bool kEight, bool kWide>
+constexpr int kRingBytes = 2 * kStages<D, kEight, kWide> * kTileBytes<D> + (kEight ? 2 * kRawStages<D, kWide> * kTile * D : 0);
+template <int D, bool kWide>
+constexpr int kQueryBytes = kWide ? 128 * D * 2 : 0;   // of a stream, in shared memory
 
-template <int D, bool kEight>
+template <int D, bool kEight, bool kWide>
 __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(TreeArgs a, LineShape shape) {
-  constexpr bool kOneO = D == 256;                       // one accumulator for both score buffers
-  constexpr uint32_t kColO1 = D, kColS = kOneO ? 256 : 2 * D, kColQ = kColS + 128;
-  static_assert(kColQ + (kOneO ? D / 2 : D) <= 512, "tensor memory");
+  constexpr bool kOneO = D == 256;                       // one stream
+  constexpr int kBuffers = kOneO || kWide ? 2 : 1;       // of scores, per stream
+  constexpr uint32_t kColO1 = D, kColS = kOneO ? D : 2 * D, kColQ = kColS + (kOneO ? 1 : 2) * kBuffers * kTile;   // (kWide: the queries lie in shared memory)
+  static_assert(kColQ + (kWide ? 0 : D / 2) <= 512 && !(kOneO && kWide), "tensor memory");
+  const auto buffer_of = [](int t) { return kBuffers == 2 ? t & 1 : 0; };   // of the stream's tile t
+  const auto phase_of = [](int t) { return kBuffers == 2 ? t >> 1 & 1 : t & 1; };
   constexpr uint32_t kBf16 = 1u << 7 | 1u << 10;   // operand types: bf16, or fp16 for 8-bit caches
   constexpr uint32_t kIdescQK = umma_idesc_bf16(128, kTile, false) ^ (kEight ? kBf16 : 0u);
   constexpr uint32_t kIdescPV = umma_idesc_bf16(128, D, true) ^ (kEight ? kBf16 : 0u);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  Shared<D, kEight>* sh = reinterpret_cast<Shared<D, kEight>*>(smem + kRingBytes<D, kEight>);
-  const uint32_t k_ring = smem_u32(smem), v_ring = k_ring + kStages<D, kEight> * kTileBytes<D>;
-  const uint32_t raw_k = v_ring + kStages<D, kEight> * kTileBytes<D>, raw_v = raw_k + kRawStages<D> * kTile * D;   // 8-bit caches
+  Shared<D, kEight, kWide>* sh = reinterpret_cast<Shared<D, kEight, kWide>*>(smem + kRingBytes<D, kEight, kWide> + 2 * kQueryBytes<D, kWide>);
+  const uint32_t k_ring = smem_u32(smem), v_ring = k_ring + kStages<D, kEight, kWide> * kTileBytes<D>;
+  const uint32_t raw_k = v_ring + kStages<D, kEight, kWide> * kTileBytes<D>, raw_v = raw_k + kRawStages<D, kWide> * kTile * D;   // 8-bit caches
+  const uint32_t queries = k_ring + kRingBytes<D, kEight, kWide>;   // slabs of 64 channels, 128 rows of 128 bytes, swizzled
   const int warp = uniform_warp_index(), lane = threadIdx.x % 32;
   pdl_launch_dependents();   // the merge may be placed as SMs free up; it waits for this grid's end
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages<D, kEight>; ++s) {
+    for (int s = 0; s < kStages<D, kEight, kWide>; ++s) {
       mbar_init(&sh->k_full[s], kEight ? 2 : 64);
       mbar_init(&sh->v_full[s], kEight ? 2 : 64);
-      mbar_init(&sh->k_empty[s], 1);
-      mbar_init(&sh->v_empty[s], 1);
+      mbar_init(&sh->k_empty[s], kWide ? 2 : 1);   // (the streams each, or the one that has the tile twice)
+      mbar_init(&sh->v_empty[s], kWide ? 2 : 1);
     }
     if (kEight) {
-      for (int r = 0; r < kRawStages<D>; ++r) {
+      for (int r = 0; r < kRawStages<D, kWide>; ++r) {
         mbar_init(&sh->raw_k[r], 64);
         mbar_init(&sh->raw_v[r], 64);
         mbar_init(&sh->raw_scales[r], 2);
@@ -338,15 +349,17 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(TreeArg
     }
     for (int i = 0; i < kSegments; ++i) {
       mbar_init(&sh->seg_full[i], 1);
-      mbar_init(&sh->seg_empty[i], kSegmentReaders);
+      mbar_init(&sh->seg_empty[i], kSegmentReaders<kWide>);
     }
     for (int x = 0; x < 2; ++x) {
-      mbar_init(&sh->q_full[x], 4);
-      mbar_init(&sh->s_full[x], 1);
-      mbar_init(&sh->p_half[x], 4);
-      mbar_init(&sh->p_full[x], 4);
-      mbar_init(&sh->pv_half[x], 1);
-      mbar_init(&sh->pv_done[x], 1);
+      mbar_init(&sh->q_full[x], x == 0 && !kOneO ? 8 : 4);   // ([0]: both streams' warps have come to the segment)
+      for (int buffer = 0; buffer < 2; ++buffer) {
+        mbar_init(&sh->s_full[x][buffer], 1);
+        mbar_init(&sh->p_half[x][buffer], 4);
+        mbar_init(&sh->p_full[x][buffer], 4);
+        mbar_init(&sh->pv_half[x][buffer], 1);
+        mbar_init(&sh->pv_done[x][buffer], 1);
+      }
     }
     mbar_init(&sh->ml_full, 8);
     mbar_init(&sh->o_read, 8);
@@ -362,74 +375,91 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(TreeArg
   const uint32_t tmem = sh->tmem;
   uint32_t* status = a.pool.status;
 
-  // Register file: 512 threads x 128, nothing to move; or 768 x 80 (of 480 per thread of six warpgroups: issue 40,
+  // Register file: 512 threads x 128, nothing to move; or 768 x 80 (of 480 per thread of six warpgroups: issue 56,
   // softmax 2 x 112, loads 56, widening 2 x 72).
   if (warp < 4) {
-    if (kEight) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-    if (warp == 0) {
+    if (kEight) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 0 || (warp == 2 && kWide)) {
       // ---------------------------------------------------------------- MMA issue
-      int tile_n = 0, q_n[2] = {0, 0}, p_n[2] = {0, 0};   // tiles, queries and P handed over so far
+      // A warp per stream where both read every tile; else warp 0 for both, as every tile has to be awaited in its order (a
+      // parity tells a phase from its neighbours only).
+      int tile_n = 0, own_0 = 0, own_1 = 0, segments = 0, pairs = 0;   // so far: tiles, those of the streams
       bool ok = true;
       int seg_n = 0;
       Segment seg;
       while (ok && next_segment(sh, seg_n, seg, lane, status)) {
         const int tiles = __shfl_sync(0xffffffffu, seg.tile1 - seg.tile0, 0);
-        const bool pair = __shfl_sync(0xffffffffu, seg.rows > 128 ? 1 : 0, 0);
-        const int items = pair ? 2 * tiles : tiles;
-        for (int x = 0; x < (pair ? 2 : 1) && ok; ++x)
-          ok = __all_sync(0xffffffffu, mbar_wait(&sh->q_full[x], q_n[x]++ & 1, status, 52));
+        const bool pair = kWide && __shfl_sync(0xffffffffu, seg.rows > 128 ? 1 : 0, 0), every = pair || kOneO;   // every: all tiles are a stream's
+        ok = __all_sync(0xffffffffu, mbar_wait(&sh->q_full[0], segments++ & 1, status, 52));
+        if (ok && pair && warp) ok = __all_sync(0xffffffffu, mbar_wait(&sh->q_full[1], pairs & 1, status, 52));
+        pairs += pair;
         if (!ok) break;
-        const auto issue_qk = [&](int i) -> bool {
-          const int x = i & 1, n = tile_n + (pair ? i >> 1 : i), stage = n % kStages<D, kEight>;
-          if (!pair || x == 0) {
-            if (!__all_sync(0xffffffffu, mbar_wait(&sh->k_full[stage], (n / kStages<D, kEight>) & 1, status, 53))) return false;
-            fence_proxy_async();   // the loaders' stores, before the tensor cores read them
-          }
+        const uint64_t q_desc = umma_desc_sw128(queries + (pair && warp ? kQueryBytes<D, kWide> : 0), 16, 1024);
+        const auto issue_qk = [&](int x, int u) -> bool {
+          const int n = tile_n + (every ? u : 2 * u + x), stage = n % kStages<D, kEight, kWide>, buffer = buffer_of((x ? own_1 : own_0) + u);
+          if (!__all_sync(0xffffffffu, mbar_wait(&sh->k_full[stage], (n / kStages<D, kEight, kWide>) & 1, status, 53))) return false;
+          fence_proxy_async();   // the loaders' stores, before the tensor cores read them
           tc_fence_after();
           const uint64_t k_desc = umma_desc_sw128(k_ring + stage * kTileBytes<D>, 16, 1024);
-          const uint32_t q = tmem + kColQ + (pair && x ? D / 2 : 0);
+          const uint32_t s_at = tmem + kColS + (kBuffers * x + buffer) * kTile;
           if (elect_one()) {
 #pragma unroll
-            for (int ks = 0; ks < D / 16; ++ks)
-              umma_ts(tmem + kColS + x * kTile, q + ks * 8, k_desc + (((ks / 4) * (kTile * 128) + (ks % 4) * 32) >> 4), kIdescQK, ks > 0);
-            tc_commit(&sh->s_full[x]);
-            if (!pair || x == 1) tc_commit(&sh->k_empty[stage]);
+            for (int ks = 0; ks < D / 16; ++ks) {
+              const uint64_t k_at = k_desc + (((ks / 4) * (kTile * 128) + (ks % 4) * 32) >> 4);
+              if (!kWide) umma_ts(s_at, tmem + kColQ + ks * 8, k_at, kIdescQK, ks > 0);
+              else umma_ss(s_at, q_desc + (((ks / 4) * (128 * 128) + (ks % 4) * 32) >> 4), k_at, kIdescQK, ks > 0);
+            }
+            tc_commit(&sh->s_full[x][buffer]);
+            tc_commit(&sh->k_empty[stage]);
+            if (kWide && !every) tc_commit(&sh->k_empty[stage]);
           }
           __syncwarp();
           return true;
         };
-        const auto issue_pv = [&](int i) -> bool {
-          const int x = i & 1, j = pair ? i >> 1 : i, n = tile_n + j, stage = n % kStages<D, kEight>;
-          if (!pair || x == 0) {
-            if (!__all_sync(0xffffffffu, mbar_wait(&sh->v_full[stage], (n / kStages<D, kEight>) & 1, status, 54))) return false;
-            fence_proxy_async();
-          }
+        const auto issue_pv = [&](int x, int u) -> bool {
+          const int n = tile_n + (every ? u : 2 * u + x), stage = n % kStages<D, kEight, kWide>, t = (x ? own_1 : own_0) + u;
+          const int buffer = buffer_of(t), phase = phase_of(t);
+          if (!__all_sync(0xffffffffu, mbar_wait(&sh->v_full[stage], (n / kStages<D, kEight, kWide>) & 1, status, 54))) return false;
+          fence_proxy_async();
           const uint64_t v_desc = umma_desc_sw128(v_ring + stage * kTileBytes<D>, kTile * 128, 1024);
-          const bool add = kOneO ? i > 0 : pair ? j > 0 : i > 1;
-          const uint32_t phase = p_n[x]++ & 1, o = tmem + (kOneO ? 0u : x * kColO1), p = tmem + kColS + x * kTile;
+          const uint32_t o = tmem + x * kColO1, p = tmem + kColS + (kBuffers * x + buffer) * kTile;
           // the weights come in two halves of the tile's keys; the first half's product runs under the second's softmax
-          if (!__all_sync(0xffffffffu, mbar_wait(&sh->p_half[x], phase, status, 55))) return false;
+          if (!__all_sync(0xffffffffu, mbar_wait(&sh->p_half[x][buffer], phase, status, 55))) return false;
           tc_fence_after();
           if (elect_one()) {
 #pragma unroll
-            for (int ks = 0; ks < kTile / 32; ++ks) umma_ts(o, p + ks * 8, v_desc + ks * (2048 >> 4), kIdescPV, add || ks > 0);
-            tc_commit(&sh->pv_half[x]);
+            for (int ks = 0; ks < kTile / 32; ++ks) umma_ts(o, p + ks * 8, v_desc + ks * (2048 >> 4), kIdescPV, u > 0 || ks > 0);
+            tc_commit(&sh->pv_half[x][buffer]);
           }
           __syncwarp();
-          if (!__all_sync(0xffffffffu, mbar_wait(&sh->p_full[x], phase, status, 55))) return false;
+          if (!__all_sync(0xffffffffu, mbar_wait(&sh->p_full[x][buffer], phase, status, 55))) return false;
           tc_fence_after();
           if (elect_one()) {
 #pragma unroll
             for (int ks = kTile / 32; ks < kTile / 16; ++ks) umma_ts(o, p + ks * 8, v_desc + ks * (2048 >> 4), kIdescPV, true);
-            tc_commit(&sh->pv_done[x]);
-            if (!pair || x == 1) tc_commit(&sh->v_empty[stage]);
+            tc_commit(&sh->pv_done[x][buffer]);
+            tc_commit(&sh->v_empty[stage]);
+            if (kWide && !every) tc_commit(&sh->v_empty[stage]);
           }
           __syncwarp();
           return true;
         };
-        ok = issue_qk(0) && (items < 2 || issue_qk(1));
-        for (int i = 0; i < items && ok; ++i) ok = issue_pv(i) && (i + 2 >= items || issue_qk(i + 2));
+        // Where a stream reads every tile and has two score buffers, the next tile's scores are there when the softmax has
+        // ended one.  (On alternate tiles two would keep four tiles in the rings.)
+        const int ahead = kBuffers == 2 && every ? 2 : 1;
+        const int tiles_0 = every ? tiles : (tiles + 1) / 2, tiles_1 = every ? tiles : tiles / 2;
+        const int first = pair ? warp >> 1 : 0, last = every ? first : warp ? -1 : 1;
+#pragma unroll 1
+        for (int u = 0; u < tiles_0 + ahead && ok; ++u)
+#pragma unroll 1
+          for (int x = first; x <= last && ok; ++x) {
+            const int own = x ? tiles_1 : tiles_0;
+            if (u >= ahead && u - ahead < own) ok = issue_pv(x, u - ahead);
+            if (ok && u < own) ok = issue_qk(x, u);
+          }
         tile_n += tiles;
+        own_0 += tiles_0;
+        own_1 += tiles_1;
       }
     } else if (warp == 1) {
       // ---------------------------------------------------------------- the range's segments
@@ -457,15 +487,15 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(TreeArg
     const float scale_log2 = a.scale * 1.4426950408889634f;
     const Partials parts = partials_of(a, shape);
     const bool gate_pieces = gate_in_pieces(a);
-    // tiles of the range; those of the score buffers 0 and 1; meetings of the streams
-    int tile_n = 0, tiles_0 = 0, tiles_1 = 0, met = 0;
+    // tiles of the range; those of this stream and of the other; meetings of the streams
+    int tile_n = 0, own_n = 0, other_n = 0, met = 0;
     bool ok = true;
     int seg_n = 0;
     Segment seg;
     // (at width 256 the second warpgroup only keeps the ring of segments going)
     while (next_segment(sh, seg_n, seg, lane, status)) {
       if (kOneO && x == 1) continue;
-      const bool pair = seg.rows > 128;
+      const bool pair = kWide && seg.rows > 128;
       const int tiles = seg.tile1 - seg.tile0, own_row = (pair ? x * 128 : 0) + row;
       const bool live = own_row < seg.rows, warp_live = (pair ? x * 128 : 0) + quarter * 32 < seg.rows;
       const int r = seg.row0 + own_row, node = r / group, head = seg.kv_head * group + r % group;
@@ -487,29 +517,40 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(TreeArg
         q_scale = __uint_as_float((254u - e) << 23);
         row_scale = scale_log2 * __uint_as_float(e << 23);
       }
-      // ---- the queries, into TMEM
-      if (pair || x == 0) {
-        if (warp_live) {
+      // ---- the queries, into shared memory or TMEM
+      if (warp_live && (pair || x == 0)) {
 #pragma unroll 1
-          for (int c = 0; c < D / 64; ++c) {
-            uint32_t w[32];
+        for (int c = 0; c < D / 64; ++c) {
+          uint32_t w[32];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const uint4 v = live ? q[c * 8 + i] : make_uint4(0u, 0u, 0u, 0u);
-              w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
-            }
-            if (kEight) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                w[i] = pack_f16(bf16_lo(w[i]) * q_scale, bf16_hi(w[i]) * q_scale);
-            }
-            tmem_st32(lanes + kColQ + (pair ? x * (D / 2) : 0) + c * 32, w);
+          for (int i = 0; i < 8; ++i) {
+            const uint4 v = live ? q[c * 8 + i] : make_uint4(0u, 0u, 0u, 0u);
+            w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
           }
+          if (kEight) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              w[i] = pack_f16(bf16_lo(w[i]) * q_scale, bf16_hi(w[i]) * q_scale);
+          }
+          if (!kWide) {
+            tmem_st32(lanes + kColQ + c * 32, w);
+          } else {
+            const uint32_t to = queries + x * kQueryBytes<D, kWide> + c * (128 * 128) + row * 128;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sts_b32x4(to + ((i ^ (row & 7)) << 4), w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+          }
+        }
+        if (!kWide) {
           tmem_wait_st();
           tc_fence_before();
+        } else {
+          fence_proxy_async();
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh->q_full[pair ? x : 0]);
+      }
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&sh->q_full[0]);
+        if (x == 1 && pair) mbar_arrive(&sh->q_full[1]);
       }
       // ---- which drafts the row sees: one bit per node
       uint64_t seen_lo = 0, seen_hi = 0;
@@ -534,16 +575,16 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(TreeArg
       // Weights are 2^(score * row_scale - reference), reference = m_used * row_scale + v_used: for 8-bit caches v_used is
       // the largest exponent of the value rows so far, so that a weight times its row's 2^n fits fp16.
       float m_used = -INFINITY, m_true = -INFINITY, l = 0.0f, v_used = kEight ? kSmallest : 0.0f;
-      const int step = pair || kOneO ? 1 : 2;
-      int done = 0;
-      for (int j = pair || kOneO ? 0 : x; j < tiles && ok; j += step, ++done) {
-        // A parity tells the phase that is awaited from its two neighbours only: every barrier of a buffer completes once per
-        // tile, and this tile's scores were committed behind the buffer's previous product.
-        const int sb = kOneO ? j & 1 : x, phase = ((sb ? tiles_1 : tiles_0) + (kOneO ? j >> 1 : done)) & 1;
-        ok = __all_sync(0xffffffffu, mbar_wait(&sh->s_full[sb], phase, status, 56));
+      const bool every = pair || kOneO;
+      const int own = every ? tiles : (tiles + 1 - x) / 2;
+      for (int u = 0; u < own && ok; ++u) {
+        // A parity tells the phase that is awaited from its two neighbours only.  Every barrier of a score buffer completes
+        // once per tile in it, and a tile's scores are committed behind the products of the buffer's last tile.
+        const int j = every ? u : 2 * u + x, t = own_n + u, buffer = buffer_of(t);
+        ok = __all_sync(0xffffffffu, mbar_wait(&sh->s_full[x][buffer], phase_of(t), status, 56));
         if (!ok) break;
-        const uint32_t s_at = lanes + kColS + sb * kTile;
-        const int slot = (tile_n + j) % (2 * kStages<D, kEight>);
+        const uint32_t s_at = lanes + kColS + (kBuffers * x + buffer) * kTile;
+        const int slot = (tile_n + j) % (3 * kStages<D, kEight, kWide>);
         const uint32_t k_factor = smem_u32(sh->k_factor[slot]), v_factor = smem_u32(sh->v_factor[slot]);
         const bool scaled = kEight && warp_live && sh->scaled[slot] != 0;   // the rare tile with rows that fp16 does not hold
         const float v_tile = scaled ? fmaxf(v_used, static_cast<float>(sh->v_largest[slot])) : kEight ? fmaxf(v_used, 0.0f) : v_used;
@@ -573,36 +614,12 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(TreeArg
               for (int i = 0; i < 32; ++i)
                 if (!(bits >> i & 1u)) s[i] = 0xff800000u;
             }
+            // The weights are taken relative to the maximum so far, so that their way does not lead through this one's; where it
+            // has grown too far, the half is done again.
             float mx[4] = {m_true, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
             for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
             m_true = max3(mx[0], mx[1], fmaxf(mx[2], mx[3]));
-            const bool grow = (m_true - m_used) * row_scale > kRescale;
-            if (__any_sync(0xffffffffu, grow || v_tile > v_used)) {
-              const float factor = fast_exp2((grow ? (m_used - m_true) * row_scale : 0.0f) + (v_used - v_tile));
-              if (grow) m_used = m_true;
-              v_used = v_tile;
-              l *= factor;
-              if (done > 0 || h == 1) {
-                // every product into this O must have ended: this tile's first half, the other buffer's last tile (one O);
-                // those into an own O before this tile have
-                if (h == 1) ok = __all_sync(0xffffffffu, mbar_wait(&sh->pv_half[sb], phase, status, 57));
-                else if (kOneO) ok = __all_sync(0xffffffffu, mbar_wait(&sh->pv_done[sb ^ 1], ((sb ? tiles_0 : tiles_1) + ((j - 1) >> 1)) & 1, status, 57));
-                if (!ok) break;
-                tc_fence_after();
-#pragma unroll 1
-                for (int c = 0; c < D / 16; ++c) {
-                  uint32_t o[16];
-                  const uint32_t o_at = lanes + (kOneO ? 0u : x * kColO1) + c * 16;
-                  tmem_ld16(o_at, o);
-                  tmem_wait_ld();
-#pragma unroll
-                  for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
-                  tmem_st16(o_at, o);
-                }
-                tmem_wait_st();
-              }
-            }
             const float reference = (m_used == -INFINITY ? 0.0f : m_used * row_scale) + v_used;   // (nothing seen yet: any)
             const uint64_t scale2 = f2_pack(row_scale, row_scale), neg2 = f2_pack(-reference, -reference);
             uint64_t sum2[2] = {0ull, 0ull};
@@ -621,6 +638,32 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(TreeArg
                 packed[i / 2] = pack_bf16(p0, p1);
               }
             }
+            const bool grow = (m_true - m_used) * row_scale > kRescale;
+            if (__any_sync(0xffffffffu, grow || v_tile > v_used)) {
+              const float factor = fast_exp2((grow ? (m_used - m_true) * row_scale : 0.0f) + (v_used - v_tile));
+              if (grow) m_used = m_true;
+              v_used = v_tile;
+              l *= factor;
+              if (u > 0 || h == 1) {
+                // every product into this O must have ended: the first half's, or the previous tile's second
+                ok = __all_sync(0xffffffffu, mbar_wait(h ? &sh->pv_half[x][buffer] : &sh->pv_done[x][buffer_of(t - 1)], phase_of(h ? t : t - 1), status, 57));
+                if (!ok) break;
+                tc_fence_after();
+#pragma unroll 1
+                for (int c = 0; c < D / 16; ++c) {
+                  uint32_t o[16];
+                  const uint32_t o_at = lanes + x * kColO1 + c * 16;
+                  tmem_ld16(o_at, o);
+                  tmem_wait_ld();
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
+                  tmem_st16(o_at, o);
+                }
+                tmem_wait_st();
+              }
+              --h;
+              continue;
+            }
             if (scaled) {
 #pragma unroll
               for (int i = 0; i < 32; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) * lds_f32(v_factor + (h * 32 + i) * 4));
@@ -638,17 +681,16 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(TreeArg
             tc_fence_before();
           }
           __syncwarp();
-          if (lane == 0) mbar_arrive(h ? &sh->p_full[sb] : &sh->p_half[sb]);
+          if (lane == 0) mbar_arrive(h ? &sh->p_full[x][buffer] : &sh->p_half[x][buffer]);
         }
       }
       if (!ok) break;
       const bool merged = !pair && !kOneO;
       tile_n += tiles;
-      tiles_0 += pair ? tiles : (tiles + 1) / 2;
-      tiles_1 += pair ? tiles : tiles / 2;
-      // this stream's last product (one O: the last tile's, which ends behind all others)
-      const int last = kOneO ? (tiles - 1) & 1 : x;
-      if (kOneO || done > 0) ok = __all_sync(0xffffffffu, mbar_wait(&sh->pv_done[last], ((last ? tiles_1 : tiles_0) - 1) & 1, status, 58));
+      own_n += own;
+      other_n += every ? tiles : tiles - own;
+      // this stream's last product
+      if (own > 0) ok = __all_sync(0xffffffffu, mbar_wait(&sh->pv_done[x][buffer_of(own_n - 1)], phase_of(own_n - 1), status, 58));
       if (!ok) break;
       tc_fence_after();
       // ---- read-out: rows of one stream, or the two streams' halves of the keys merged, half of the channels each
@@ -661,7 +703,7 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(TreeArg
         ok = __all_sync(0xffffffffu, mbar_wait(&sh->ml_full, met & 1, status, 59));
         // (the other stream has seen its last product end before it arrived there: this returns at once)
         if (ok && (x == 1 || tiles > 1))
-          ok = __all_sync(0xffffffffu, mbar_wait(&sh->pv_done[1 - x], ((x ? tiles_0 : tiles_1) - 1) & 1, status, 58));
+          ok = __all_sync(0xffffffffu, mbar_wait(&sh->pv_done[1 - x][buffer_of(other_n - 1)], phase_of(other_n - 1), status, 58));
         if (!ok) break;
         tc_fence_after();
         const float2 one = sh->ml[0][row], two = sh->ml[1][row];
@@ -680,7 +722,7 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(TreeArg
 #pragma unroll 1
         for (int c = c0; c < c1; ++c) {
           uint32_t o[16];
-          tmem_ld16(lanes + (merged || kOneO ? 0u : x * kColO1) + c * 16, o);
+          tmem_ld16(lanes + (merged ? 0u : x * kColO1) + c * 16, o);
           if (both) {
             uint32_t o2[16];
             tmem_ld16(lanes + kColO1 + c * 16, o2);
@@ -724,12 +766,12 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(TreeArg
     // ------------------------------------------------------------------ loads, widening
     if (warp < 16) {
       if (kEight) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-      load_tiles<D, kEight>(a, sh, kEight ? raw_k : k_ring, kEight ? raw_v : v_ring, warp - 12, lane);
+      load_tiles<D, kEight, kWide>(a, sh, kEight ? raw_k : k_ring, kEight ? raw_v : v_ring, warp - 12, lane);
       asm volatile("cp.async.wait_all;" ::: "memory");   // (landed long ago unless a wait ran out)
     } else {
       if constexpr (kEight) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        widen_tiles<D>(sh, warp < 20 ? raw_k : raw_v, warp < 20 ? k_ring : v_ring, status, warp & 3, lane, warp >= 20);
+        widen_tiles<D, kWide>(sh, warp < 20 ? raw_k : raw_v, warp < 20 ? k_ring : v_ring, status, warp & 3, lane, warp >= 20);
       }
     }
   }
@@ -741,21 +783,29 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(TreeArg
 
 constexpr LineShape line_shape(int dim) { return {6, kUnitTiles, dim == 256 ? 7 : 8, kMaxCtas}; }
 
-template <int D, bool kEight>
-cudaError_t launch(cudaStream_t stream, const TreeArgs& a) {
+template <int D, bool kEight, bool kWide>
+cudaError_t launch_kernel(cudaStream_t stream, const TreeArgs& a) {
   constexpr LineShape shape = line_shape(D);
   static_assert(1 << shape.tile_shift == kTile && 1 << shape.rows_shift == group_rows(D), "line");
   const long long units = static_cast<long long>(a.batch) * a.kv_heads * ((a.nodes * a.group + group_rows(D) - 1) / group_rows(D));
   const long long tiles = units * ((static_cast<long long>(a.max_prefix) + a.nodes + kTile - 1) / kTile);
-  constexpr int kBytes = kRingBytes<D, kEight> + static_cast<int>(sizeof(Shared<D, kEight>)) + 1024;
+  constexpr int kBytes = kRingBytes<D, kEight, kWide> + 2 * kQueryBytes<D, kWide> + static_cast<int>(sizeof(Shared<D, kEight, kWide>)) + 1024;
   static_assert(kBytes <= 227 * 1024, "shared memory");
-  using S = Shared<D, kEight>;
+  using S = Shared<D, kEight, kWide>;
   static_assert(offsetof(S, k_factor) % 16 == 0 && offsetof(S, ml) % 8 == 0 && alignof(S) == 16, "alignment");
-  cudaError_t e = cudaFuncSetAttribute(tree_decode_sm100<D, kEight>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+  cudaError_t e = cudaFuncSetAttribute(tree_decode_sm100<D, kEight, kWide>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
   if (e != cudaSuccess) return e;
-  tree_decode_sm100<D, kEight><<<static_cast<unsigned>(tiles < kMaxCtas ? tiles : kMaxCtas), kThreads<kEight>, kBytes, stream>>>(a, shape);
+  tree_decode_sm100<D, kEight, kWide><<<static_cast<unsigned>(tiles < kMaxCtas ? tiles : kMaxCtas), kThreads<kEight>, kBytes, stream>>>(a, shape);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   return tree_decode_merge(stream, a, shape);
+}
+
+template <int D, bool kEight>
+cudaError_t launch(cudaStream_t stream, const TreeArgs& a) {
+  if constexpr (D < 256) {
+    if (a.nodes * a.group > 128) return launch_kernel<D, kEight, true>(stream, a);
+  }
+  return launch_kernel<D, kEight, false>(stream, a);
 }
 
 }  // namespace
