@@ -56,18 +56,20 @@ __device__ __forceinline__ uint32_t halves_of(uint32_t codes) {   // two codes i
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<uint16_t>(codes)));
   return r;
 }
-// d (+)= a b: rows lane / 4 (d[0], d[1]) and, unless kHalf, lane / 4 + 8
-template <bool kEight, bool kHalf>
-__device__ __forceinline__ void mma(float (&d)[kHalf ? 2 : 4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  float x = 0.0f, y = 0.0f;
-  float& d2 = kHalf ? x : d[kHalf ? 0 : 2];
-  float& d3 = kHalf ? y : d[kHalf ? 0 : 3];
+// d += a b: a 16 x 16, b 16 x 8
+template <bool kEight>
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   if (kEight)
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d2), "+f"(d3) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   else
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d2), "+f"(d3) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {   // of an 8 x 8 matrix of 16-bit values, a row per four lanes
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
 }
 __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -87,10 +89,9 @@ __device__ __forceinline__ uint32_t piece_at(int r, int c) {
 template <int D, bool kEight, bool kHalf>   // kHalf: at most eight rows
 __global__ void __launch_bounds__(kWarps * 32, kCtas<D, kEight>) tree_decode_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, TreeArgs a, LineShape shape) {
   constexpr int kBytes = kRowBytes<D, kEight>, kPieces = kBytes / 16, kS = kStages<D, kEight>;
-  constexpr int kH = kHalf ? 1 : 2;                     // rows of a lane
-  constexpr int kC = kHalf ? 2 : 4;                     // values of an accumulator block in a lane
+  constexpr int kN = kHalf ? 1 : 2, kR = 2 * kN;        // blocks of eight rows; rows of a lane: 8 n + 2 t4 + e
   constexpr int kChunks = kPieces < 4 ? 1 : kPieces / 4, kSteps = kEight ? 4 : 2;   // pieces of a key row per lane, k steps per piece
-  constexpr int kBlocks = D / 8;                        // accumulator blocks
+  constexpr int kBlocks = D / 16;                       // accumulator blocks of sixteen channels
   static_assert(kChunks * kSteps == D / 16, "channels");
   using State = WarpState<kS, kEight>;
   extern __shared__ uint8_t smem_raw[];
@@ -121,7 +122,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, kEight>) tree_decode_mma
     if (lane == 0) own->ahead = cursor;
   }
   __syncwarp();
-  int tile = 0, last = 0, page = 0, issued = 0, listed = 0;   // of the next step: its tile, the segment's end, its page
+  int tile = 0, last = 0, page = 0, to_slot = 0, listed = 0;   // of the next step: its tile, the segment's end, its page, its slot
+  int load_b = 0, load_head = 0, load_end = 0;                 // of the segment: sequence, KV head, tokens
   const auto next_load = [&]() {
     Cursor cursor = own->ahead;
     Segment load{};
@@ -135,58 +137,60 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, kEight>) tree_decode_mma
     ++listed;
     tile = more ? load.tile0 : 0;
     last = more ? load.tile1 : 0;
+    load_b = load.b;
+    load_head = load.kv_head;
+    load_end = load.prefix + load.count;
   };
   next_load();
   const auto block_of = [&](int t) { return page_shift >= 0 ? t >> page_shift : t / a.pool.page_size; };
   const auto fetch_page = [&]() {   // used by the next issue only
     if (tile >= last) return;
-    const int b = own->segments[(listed - 1) % kSegments].b, block = block_of(tile * kTile);
+    const int block = block_of(tile * kTile);
     if (block >= (a.pool.table ? a.pool.max_blocks : 1)) {
       report_status(status, 48, kBadLength);
       page = -1;
     } else {
-      page = a.pool.table ? a.pool.table[static_cast<size_t>(b) * a.pool.max_blocks + block] : b;
+      page = a.pool.table ? a.pool.table[static_cast<size_t>(load_b) * a.pool.max_blocks + block] : load_b;
     }
   };
   fetch_page();
+  const uint8_t* scales = lane < kTile ? a.pool.k_scales : a.pool.v_scales;   // lanes 0-15: the keys', 16-31: the values'
   const auto issue = [&]() {
     if (tile >= last) return;
-    const Segment* load = &own->segments[(listed - 1) % kSegments];
-    const int t0 = tile * kTile, slot = issued % kS, inside = t0 - block_of(t0) * a.pool.page_size, kv_head = load->kv_head;
+    const int t0 = tile * kTile, inside = t0 - block_of(t0) * a.pool.page_size;
     if (page < 0 || (a.pool.table && page >= a.pool.num_pages)) {
       report_status(status, 48, kBadPage);   // (a slot past the pages was reported as such before)
       page = -1;                             // the copies read zeros there
     }
     if (lane == 0) {
-      const uint32_t to = ring + slot * kStageBytes<D, kEight>;
+      const uint32_t to = ring + to_slot * kStageBytes<D, kEight>;
       constexpr int kSlabs = kBytes == 64 ? 1 : kBytes / 128, kColumns = D / kSlabs, kSlab = kTile * kBytes / kSlabs;
-      mbar_expect_tx(&own->full[slot], kStageBytes<D, kEight>);
+      mbar_expect_tx(&own->full[to_slot], kStageBytes<D, kEight>);
 #pragma unroll
       for (int i = 0; i < kSlabs; ++i) {
-        tma_load_4d_at(to + i * kSlab, &map_k, i * kColumns, kv_head, inside, page, &own->full[slot]);
-        tma_load_4d_at(to + kTile * kBytes + i * kSlab, &map_v, i * kColumns, kv_head, inside, page, &own->full[slot]);
+        tma_load_4d_at(to + i * kSlab, &map_k, i * kColumns, load_head, inside, page, &own->full[to_slot]);
+        tma_load_4d_at(to + kTile * kBytes + i * kSlab, &map_v, i * kColumns, load_head, inside, page, &own->full[to_slot]);
       }
     }
-    if (kEight) {   // lanes 0-15: the keys' scales, 16-31: the values'
+    if (kEight) {
       const int row = lane % kTile;
-      const bool there = page >= 0 && row < load->prefix + load->count - t0;
-      const uint8_t* byte = (lane < kTile ? a.pool.k_scales : a.pool.v_scales) +
-                            (there ? static_cast<size_t>(page) * a.pool.scale_page + static_cast<size_t>(inside + row) * a.pool.scale_token + kv_head : 0);
+      const bool there = page >= 0 && t0 + row < load_end;
+      const uint8_t* byte = scales + load_head + (there ? static_cast<size_t>(page) * a.pool.scale_page + static_cast<size_t>(inside + row) * a.pool.scale_token : 0);
       const uintptr_t at = reinterpret_cast<uintptr_t>(byte);
-      own->places[slot][lane] = static_cast<uint8_t>(at & 3u);
-      copy4(smem_u32(&own->words[slot][lane]), reinterpret_cast<const void*>(at & ~static_cast<uintptr_t>(3)), there);
-      arrive_behind_copies(&own->full[slot]);
+      own->places[to_slot][lane] = static_cast<uint8_t>(at & 3u);
+      copy4(smem_u32(&own->words[to_slot][lane]), reinterpret_cast<const void*>(at & ~static_cast<uintptr_t>(3)), there);
+      arrive_behind_copies(&own->full[to_slot]);
     }
-    ++issued;
+    to_slot = to_slot + 1 == kS ? 0 : to_slot + 1;
     if (++tile >= last) next_load();
     fetch_page();
   };
   // One loop over the steps of the range, so that every piece of code is there once: a range of few steps is as long as
   // the fetching of its instructions takes.
   Segment seg{};
-  int primed = 0, step = 0, n = 0, j = 0;
-  uint32_t qf[D / 16][kHalf ? 2 : 4], seen[kH];
-  float row_scale[kH], m_used[kH], m_true[kH], v_used[kH], l[kH], o[kBlocks][kC];
+  int primed = 0, slot = 0, round = 0, n = 0, j = 0;   // slot and round of the ring
+  uint32_t qf[D / 16][kN][2], seen[kR];
+  float row_scale[kR], m_used[kR], v_used[kR], l[kR], o[kBlocks][kN][4], v_low = 0.0f;
 #pragma unroll 1
   while (true) {
     issue();
@@ -197,30 +201,32 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, kEight>) tree_decode_mma
     if (j >= seg.tile1) {   // (the first time: 0 >= 0)
     if (seg.rows > 0) {
     // ---- the unit's part; its result where the whole unit is here
-    const int slot = 2 * worker + seg.slot;
-    float* acc = parts.acc + static_cast<size_t>(slot) * parts.rows * D;
+    const int part = 2 * worker + seg.slot;
+    float* acc = parts.acc + static_cast<size_t>(part) * parts.rows * D;
 #pragma unroll
-    for (int h = 0; h < kH; ++h) {
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-      const int r = quad + 8 * h;
+    for (int i = 0; i < kR; ++i) {
+#pragma unroll
+      for (int lanes = 4; lanes < 32; lanes *= 2) l[i] += __shfl_xor_sync(0xffffffffu, l[i], lanes);
+      const int nb = i / 2, e = i % 2, r = nb * 8 + 2 * t4 + e;
       if (r >= seg.rows) continue;
       float* to = acc + r * D;
       if constexpr (kEight) {
-        constexpr int kWidth = D == 64 ? 8 : 16;   // neighbouring channels of a column
+        constexpr int kWidth = D == 64 ? 8 : 16;   // neighbouring channels of a lane
 #pragma unroll
         for (int set = 0; set < (D == 256 ? 2 : 1); ++set)
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
-#pragma unroll
-            for (int i = 0; i < kWidth; i += 4)
-              *reinterpret_cast<float4*>(to + set * 128 + (2 * t4 + e) * kWidth + i) =
-                  make_float4(o[set * 16 + i][2 * h + e], o[set * 16 + i + 1][2 * h + e], o[set * 16 + i + 2][2 * h + e], o[set * 16 + i + 3][2 * h + e]);
+          for (int k = 0; k < kWidth; k += 4) {
+            const int m = set * 8 + k / 2;
+            *reinterpret_cast<float4*>(to + set * 128 + quad * kWidth + k) = make_float4(o[m][nb][e], o[m][nb][2 + e], o[m + 1][nb][e], o[m + 1][nb][2 + e]);
+          }
       } else {
 #pragma unroll
-        for (int nb = 0; nb < kBlocks; ++nb) *reinterpret_cast<float2*>(to + nb * 8 + 2 * t4) = make_float2(o[nb][2 * h], o[nb][2 * h + 1]);
+        for (int m = 0; m < kBlocks; ++m) {
+          to[m * 16 + quad] = o[m][nb][e];
+          to[m * 16 + 8 + quad] = o[m][nb][2 + e];
+        }
       }
-      if (t4 == 0) parts.ml[static_cast<size_t>(slot) * parts.rows + r] = make_float2(m_used[h] == -INFINITY ? -INFINITY : m_used[h] + v_used[h], l[h]);
+      if (quad == 0) parts.ml[static_cast<size_t>(part) * parts.rows + r] = make_float2(m_used[i] == -INFINITY ? -INFINITY : m_used[i] + v_used[i], l[i]);
     }
     if (seg.whole) {   // (through the slot that the warp has anyway: rows in the order of memory, and one piece of code)
       __syncwarp();
@@ -229,7 +235,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, kEight>) tree_decode_mma
       for (int i = lane; i < seg.rows * kEights; i += 32) {
         const int r = i / kEights, d = i % kEights * 8, node = r / group, head = seg.kv_head * group + r % group;
         const size_t token = static_cast<size_t>(seg.b) * a.nodes + node;
-        const float2 ml = parts.ml[static_cast<size_t>(slot) * parts.rows + r];
+        const float2 ml = parts.ml[static_cast<size_t>(part) * parts.rows + r];
         const float inverse = ml.y == 0.0f ? 0.0f : 1.0f / ml.y;
         const float4 u = *reinterpret_cast<const float4*>(acc + r * D + d), v = *reinterpret_cast<const float4*>(acc + r * D + d + 4);
         const float x[8] = {u.x * inverse, u.y * inverse, u.z * inverse, u.w * inverse, v.x * inverse, v.y * inverse, v.z * inverse, v.w * inverse};
@@ -242,25 +248,27 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, kEight>) tree_decode_mma
     seg = own->segments[n++ % kSegments];
     if (seg.rows == 0) break;
     j = seg.tile0;
-    // ---- the queries: A fragments, columns in the order of the keys' pieces
+    // ---- the queries: B fragments of row 8 nb + quad, channels in the order of the keys' pieces
+    float of_row[kN];       // scale of the row's scores
+    uint32_t bits_of[kN];   // which drafts it sees: one bit per node
 #pragma unroll
-    for (int h = 0; h < kH; ++h) {
-      const int r = quad + 8 * h, node = r / group, head = seg.kv_head * group + r % group;
+    for (int nb = 0; nb < kN; ++nb) {
+      const int r = nb * 8 + quad, node = r / group, head = seg.kv_head * group + r % group;
       const bool live = r < seg.rows;
       const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) + ((static_cast<size_t>(seg.b) * a.nodes + node) * a.q_heads + head) * D;
       uint32_t largest = 0u;
 #pragma unroll
-      for (int j = 0; j < kChunks; ++j) {
-        const int c = kPieces < 8 ? t4 : 2 * t4 + (j & 1) + 8 * (j >> 1);
+      for (int i = 0; i < kChunks; ++i) {
+        const int c = kPieces < 8 ? t4 : 2 * t4 + (i & 1) + 8 * (i >> 1);
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-          const uint2 w = live ? *reinterpret_cast<const uint2*>(q + c * (kEight ? 16 : 8) + 4 * s) : make_uint2(0u, 0u);
-          qf[j * kSteps + s][h] = w.x;
-          qf[j * kSteps + s][kH + h] = w.y;
+        for (int k = 0; k < kSteps; ++k) {
+          const uint2 w = live ? *reinterpret_cast<const uint2*>(q + c * (kEight ? 16 : 8) + 4 * k) : make_uint2(0u, 0u);
+          qf[i * kSteps + k][nb][0] = w.x;
+          qf[i * kSteps + k][nb][1] = w.y;
           largest = max(largest, max(max(w.x & 0x7fffu, w.y & 0x7fffu), max(w.x & 0x7fff0000u, w.y & 0x7fff0000u) >> 16));
         }
       }
-      row_scale[h] = scale_log2;
+      of_row[nb] = scale_log2;
       if (kEight) {
         // fp16 holds the row exactly once its largest value is between 1 and 2 (what is below 2^-14 of that loses bits
         // beyond those that the row's scores have); the scores get the power of two back
@@ -268,51 +276,46 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, kEight>) tree_decode_mma
         largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
         const uint32_t e = min(max(largest >> 7, 2u), 252u);
         const float down = __uint_as_float((254u - e) << 23);
-        row_scale[h] = scale_log2 * __uint_as_float(e << 23);
+        of_row[nb] = scale_log2 * __uint_as_float(e << 23);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            uint32_t& w = qf[k][u * kH + h];
+            uint32_t& w = qf[k][nb][u];
             w = pack_f16(bf16_lo(w) * down, bf16_hi(w) * down);
           }
       }
-    }
-    // ---- which drafts a row sees: one bit per node
-#pragma unroll
-    for (int h = 0; h < kH; ++h) seen[h] = 0u;
-    if (seg.tile1 * kTile > seg.prefix) {
+      bits_of[nb] = 0u;
+      if (seg.tile1 * kTile > seg.prefix && live) {
 #pragma unroll 1
-      for (int h = 0; h < kH; ++h) {
-        const int r = quad + 8 * h;
-        uint32_t bits = 0u;
-        if (r < seg.rows)
-        for (int i = r / group; i >= 0;) {
-          bits |= 1u << i;
+        for (int i = node; i >= 0;) {
+          bits_of[nb] |= 1u << i;
           const int up = a.parents ? a.parents[static_cast<size_t>(seg.b) * a.nodes + i] : i - 1;
           if (up < -1 || up >= i) report_status(status, 49, kBadDraft);   // taken as a first token's
           i = up < i ? up : -1;
         }
-        if (h == 0) seen[0] = bits;
-        else seen[kH - 1] = bits;
       }
     }
+    __syncwarp();
     // Weights are 2^(score * row_scale - reference), reference = m_used + v_used: for 8-bit caches v_used is the largest
     // exponent of the value rows seen so far, so that a weight times its row's 2^n fits fp16.
 #pragma unroll
-    for (int h = 0; h < kH; ++h) {
-      m_used[h] = m_true[h] = -INFINITY;
-      v_used[h] = kEight ? kSmallest : 0.0f;
-      l[h] = 0.0f;
+    for (int i = 0; i < kR; ++i) {
+      row_scale[i] = __shfl_sync(0xffffffffu, of_row[i / 2], (2 * t4 + i % 2) * 4);
+      seen[i] = __shfl_sync(0xffffffffu, bits_of[i / 2], (2 * t4 + i % 2) * 4);
+      m_used[i] = -INFINITY;
+      v_used[i] = kEight ? kSmallest : 0.0f;
+      l[i] = 0.0f;
     }
+    v_low = kSmallest;
 #pragma unroll
-    for (int nb = 0; nb < kBlocks; ++nb)
+    for (int m = 0; m < kBlocks; ++m)
 #pragma unroll
-      for (int i = 0; i < kC; ++i) o[nb][i] = 0.0f;
-
+      for (int nb = 0; nb < kN; ++nb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[m][nb][i] = 0.0f;
     }
-      const int slot = step % kS;
-      if (!__all_sync(0xffffffffu, mbar_wait(&own->full[slot], (step / kS) & 1, status, 50))) return;
+      if (!__all_sync(0xffffffffu, mbar_wait(&own->full[slot], round & 1, status, 50))) return;
       const uint32_t k_tile = ring + slot * kStageBytes<D, kEight>, v_tile = k_tile + kTile * kBytes;
       const int behind = j * kTile - seg.prefix;   // of the drafts' first slot
       const bool border = behind > -kTile;         // the step holds drafts, or ends the sequence
@@ -349,110 +352,120 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, kEight>) tree_decode_mma
       }
       // factors: a key row that is not finite makes its scores NaN; the codes of such a value row are NaN, or zeros here
       const float own_factor = scale == 255u ? (lane < kTile ? __uint_as_float(0x7fc00000u) : 1.0f) : e8m0_value(scale);
-      // ---- S = Q K^T: two blocks of eight tokens, two accumulators each (the chain of products is what a step waits for)
-      float s[2][kC] = {}, s2[2][kC] = {};
+      // ---- S^T = K Q^T: sixteen tokens by the rows, two accumulators each (the chain of products is what a step waits for)
+      float st[kN][4] = {}, st2[kN][4] = {};
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
         const int c = kPieces < 8 ? t4 : 2 * t4 + (i & 1) + 8 * (i >> 1);
+        const uint4 w0 = lds_b32x4(k_tile + piece_at<kBytes>(quad, c)), w1 = lds_b32x4(k_tile + piece_at<kBytes>(8 + quad, c));
 #pragma unroll
-        for (int nb = 0; nb < 2; ++nb) {
-          const uint4 w = lds_b32x4(k_tile + piece_at<kBytes>(nb * 8 + quad, c));
-#pragma unroll
-          for (int k = 0; k < kSteps; ++k) {
-            uint32_t b0, b1;
-            if (kEight) {
-              const uint32_t codes = k == 0 ? w.x : k == 1 ? w.y : k == 2 ? w.z : w.w;
-              b0 = halves_of(codes);
-              b1 = halves_of(codes >> 16);
-            } else {
-              b0 = k == 0 ? w.x : w.z;
-              b1 = k == 0 ? w.y : w.w;
-            }
-            const uint32_t(&q)[kHalf ? 2 : 4] = qf[i * kSteps + k];
-            mma<kEight, kHalf>(k & 1 ? s2[nb] : s[nb], q[0], kHalf ? 0u : q[kHalf ? 0 : 1], q[kHalf ? 1 : 2], kHalf ? 0u : q[kHalf ? 0 : 3], b0, b1);
-          }
-        }
-      }
-      // ---- the tokens of this lane: nb * 8 + 2 t4 + e
-      float v_factor[2][2];
-      float v_tile_max[kH];
-#pragma unroll
-      for (int h = 0; h < kH; ++h) v_tile_max[h] = v_used[h];
-      float x[2][kC];
-#pragma unroll
-      for (int nb = 0; nb < 2; ++nb) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int token = nb * 8 + 2 * t4 + e;
-          float k_factor = 1.0f, v_power = kSmallest;
+        for (int k = 0; k < kSteps; ++k) {
+          uint32_t a0, a1, a2, a3;
           if (kEight) {
-            k_factor = __shfl_sync(0xffffffffu, own_factor, token);
-            v_factor[nb][e] = __shfl_sync(0xffffffffu, own_factor, kTile + token);
-            v_power = static_cast<float>(static_cast<int>(__float_as_uint(v_factor[nb][e]) >> 23) - 127);
-          }
-          if (hidden >> token & 1u) k_factor = __uint_as_float(0x7fc00000u);
-#pragma unroll
-          for (int h = 0; h < kH; ++h) {
-            float score = (s[nb][2 * h + e] + s2[nb][2 * h + e]) * row_scale[h];
-            if (kEight || border) score *= k_factor;
-            const bool sees = !border || token + behind < 0 || (token + behind < 16 && (seen[h] >> (token + behind) & 1u));
-            x[nb][2 * h + e] = sees ? score : -INFINITY;
-            if (kEight && sees) v_tile_max[h] = fmaxf(v_tile_max[h], v_power);
-          }
-        }
-      }
-      // ---- running maximum, rescaled rarely
-      bool grow[kH], any = false;
-#pragma unroll
-      for (int h = 0; h < kH; ++h) {
-        float m = fmaxf(fmaxf(x[0][2 * h], x[0][2 * h + 1]), fmaxf(x[1][2 * h], x[1][2 * h + 1]));
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        m_true[h] = fmaxf(m_true[h], m);
-        if (kEight) {
-          v_tile_max[h] = fmaxf(v_tile_max[h], __shfl_xor_sync(0xffffffffu, v_tile_max[h], 1));
-          v_tile_max[h] = fmaxf(v_tile_max[h], __shfl_xor_sync(0xffffffffu, v_tile_max[h], 2));
-        }
-        grow[h] = m_true[h] - m_used[h] > kRescale;
-        any = any || grow[h] || v_tile_max[h] > v_used[h];
-      }
-      if (__any_sync(0xffffffffu, any)) {
-#pragma unroll
-        for (int h = 0; h < kH; ++h) {
-          const float factor = fast_exp2((grow[h] ? m_used[h] - m_true[h] : 0.0f) + (v_used[h] - v_tile_max[h]));
-          if (grow[h]) m_used[h] = m_true[h];
-          v_used[h] = v_tile_max[h];
-          l[h] *= factor;
-#pragma unroll
-          for (int nb = 0; nb < kBlocks; ++nb) {
-            o[nb][2 * h] *= factor;
-            o[nb][2 * h + 1] *= factor;
-          }
-        }
-      }
-      uint32_t p[2][2], rest[2][2];   // [h][tokens 0-7, 8-15]
-#pragma unroll
-      for (int h = 0; h < kH; ++h) {
-        const float reference = (m_used[h] == -INFINITY ? 0.0f : m_used[h]) + v_used[h];   // (nothing seen yet: any)
-#pragma unroll
-        for (int nb = 0; nb < 2; ++nb) {
-          float p0 = fast_exp2(x[nb][2 * h] - reference), p1 = fast_exp2(x[nb][2 * h + 1] - reference);
-          l[h] += p0 + p1;
-          if (kEight) {
-            p[h][nb] = pack_f16(p0 * v_factor[nb][0], p1 * v_factor[nb][1]);
+            const uint32_t lo = k == 0 ? w0.x : k == 1 ? w0.y : k == 2 ? w0.z : w0.w, hi = k == 0 ? w1.x : k == 1 ? w1.y : k == 2 ? w1.z : w1.w;
+            a0 = halves_of(lo);
+            a1 = halves_of(hi);
+            a2 = halves_of(lo >> 16);
+            a3 = halves_of(hi >> 16);
           } else {
-            p[h][nb] = pack_bf16(p0, p1);
-            rest[h][nb] = pack_bf16(p0 - bf16_lo(p[h][nb]), p1 - bf16_hi(p[h][nb]));
+            a0 = k == 0 ? w0.x : w0.z;
+            a1 = k == 0 ? w1.x : w1.z;
+            a2 = k == 0 ? w0.y : w0.w;
+            a3 = k == 0 ? w1.y : w1.w;
+          }
+#pragma unroll
+          for (int nb = 0; nb < kN; ++nb) mma<kEight>(k & 1 ? st2[nb] : st[nb], a0, a1, a2, a3, qf[i * kSteps + k][nb][0], qf[i * kSteps + k][nb][1]);
+        }
+      }
+      // ---- the tokens of this lane: quad and quad + 8; its rows: 8 nb + 2 t4 + e
+      float k_factor[2] = {1.0f, 1.0f}, v_factor[2] = {1.0f, 1.0f};
+      if (kEight) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          k_factor[u] = __shfl_sync(0xffffffffu, own_factor, 8 * u + quad);
+          v_factor[u] = __shfl_sync(0xffffffffu, own_factor, kTile + 8 * u + quad);
+        }
+      }
+      float x[kR][2];
+#pragma unroll
+      for (int i = 0; i < kR; ++i)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          x[i][u] = (st[i / 2][2 * u + i % 2] + st2[i / 2][2 * u + i % 2]) * row_scale[i];
+          if (kEight) x[i][u] *= k_factor[u];
+        }
+      if (border) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int token = 8 * u + quad, draft = token + behind;
+#pragma unroll
+          for (int i = 0; i < kR; ++i) {
+            if (hidden >> token & 1u) x[i][u] = __uint_as_float(0x7fc00000u);
+            if (draft >= 0 && (draft >= 16 || !(seen[i] >> draft & 1u))) x[i][u] = -INFINITY;
           }
         }
       }
-      // ---- O += P V
+      // ---- the references are moved rarely: when a score, or the exponent of a value row, has grown beyond them
+      const float v_power[2] = {static_cast<float>(static_cast<int>(__float_as_uint(v_factor[0]) >> 23) - 127),
+                                static_cast<float>(static_cast<int>(__float_as_uint(v_factor[1]) >> 23) - 127)};
+      bool move = kEight && fmaxf(v_power[0], v_power[1]) > v_low;
+#pragma unroll
+      for (int i = 0; i < kR; ++i) move = move || fmaxf(x[i][0], x[i][1]) - m_used[i] > kRescale;
+      if (__any_sync(0xffffffffu, move)) {
+        v_low = INFINITY;
+#pragma unroll
+        for (int i = 0; i < kR; ++i) {
+          float m = fmaxf(x[i][0], x[i][1]), v = v_used[i];
+          if (kEight) {
+            if (x[i][0] != -INFINITY) v = fmaxf(v, v_power[0]);   // (of the rows that are seen)
+            if (x[i][1] != -INFINITY) v = fmaxf(v, v_power[1]);
+          }
+#pragma unroll
+          for (int lanes = 4; lanes < 32; lanes *= 2) {
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, lanes));
+            if (kEight) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, lanes));
+          }
+          const bool grow = m - m_used[i] > kRescale;
+          const float factor = fast_exp2((grow ? m_used[i] - m : 0.0f) + (v_used[i] - v));
+          if (grow) m_used[i] = m;
+          v_used[i] = v;
+          v_low = fminf(v_low, v);
+          l[i] *= factor;
+#pragma unroll
+          for (int k = 0; k < kBlocks; ++k) {
+            o[k][i / 2][i % 2] *= factor;
+            o[k][i / 2][2 + i % 2] *= factor;
+          }
+        }
+      }
+      uint32_t p[kN][2], rest[kN][2];   // [rows][tokens 0-7, 8-15]: B fragments
+#pragma unroll
+      for (int nb = 0; nb < kN; ++nb)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          float w[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int i = 2 * nb + e;
+            w[e] = fast_exp2(x[i][u] - ((m_used[i] == -INFINITY ? 0.0f : m_used[i]) + v_used[i]));   // (nothing seen yet: any)
+            l[i] += w[e];
+          }
+          if (kEight) {
+            p[nb][u] = transposed(pack_f16(w[0] * v_factor[u], w[1] * v_factor[u]));
+          } else {
+            const uint32_t most = pack_bf16(w[0], w[1]);
+            p[nb][u] = transposed(most);
+            rest[nb][u] = transposed(pack_bf16(w[0] - bf16_lo(most), w[1] - bf16_hi(most)));
+          }
+        }
+      // ---- O^T += V^T P^T
       if constexpr (kEight) {
-        // block nb of 128 channels (of 64): column n is channel 16 n + nb (8 n + nb) of the tile's rows 2 t4, 2 t4 + 1, and 8 further
-        constexpr int kWide = D == 64 ? 2 : 4;   // words of a row a lane takes
+        // rows quad and quad + 8 of block m are channels 16 quad + 2 m and 2 m + 1 (8 quad at width 64), columns the tokens
+        // 2 t4, 2 t4 + 1 and 8 further
+        constexpr int kWords = D == 64 ? 2 : 4;   // words of a row a lane takes
 #pragma unroll
         for (int set = 0; set < (D == 256 ? 2 : 1); ++set) {
-          uint32_t w[4][kWide];
+          uint32_t w[4][kWords];
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
             const int row = 2 * t4 + (u & 1) + 8 * (u >> 1);
@@ -466,31 +479,32 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, kEight>) tree_decode_mma
             }
           }
 #pragma unroll
-          for (int k = 0; k < kWide; ++k)
+          for (int k = 0; k < kWords; ++k)
 #pragma unroll
             for (int pair = 0; pair < 2; ++pair) {   // bytes 0, 1 and 2, 3 of the word
               const uint32_t ab = __byte_perm(w[0][k], w[1][k], pair ? 0x7362 : 0x5140), cd = __byte_perm(w[2][k], w[3][k], pair ? 0x7362 : 0x5140);
+              const uint32_t a0 = halves_of(ab), a1 = halves_of(ab >> 16), a2 = halves_of(cd), a3 = halves_of(cd >> 16);
 #pragma unroll
-              for (int e = 0; e < 2; ++e)
-                mma<kEight, kHalf>(o[set * 16 + 4 * k + 2 * pair + e], p[0][0], kHalf ? 0u : p[kHalf ? 0 : 1][0], p[0][1],
-                                   kHalf ? 0u : p[kHalf ? 0 : 1][1], halves_of(e ? ab >> 16 : ab), halves_of(e ? cd >> 16 : cd));
+              for (int nb = 0; nb < kN; ++nb) mma<kEight>(o[set * 8 + 2 * k + pair][nb], a0, a1, a2, a3, p[nb][0], p[nb][1]);
             }
         }
       } else {
 #pragma unroll
-        for (int np = 0; np < D / 16; ++np) {
+        for (int m = 0; m < kBlocks; ++m) {
           uint32_t vf[4];
-          ldmatrix_x4_trans(vf, v_tile + piece_at<kBytes>((lane / 8 & 1) * 8 + lane % 8, np * 2 + lane / 16));
+          ldmatrix_x4_trans(vf, v_tile + piece_at<kBytes>((lane / 16) * 8 + lane % 8, m * 2 + (lane / 8 & 1)));
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            mma<kEight, kHalf>(o[2 * np + u], p[0][0], kHalf ? 0u : p[kHalf ? 0 : 1][0], p[0][1], kHalf ? 0u : p[kHalf ? 0 : 1][1], vf[2 * u], vf[2 * u + 1]);
-            mma<kEight, kHalf>(o[2 * np + u], rest[0][0], kHalf ? 0u : rest[kHalf ? 0 : 1][0], rest[0][1], kHalf ? 0u : rest[kHalf ? 0 : 1][1], vf[2 * u],
-                               vf[2 * u + 1]);
+          for (int nb = 0; nb < kN; ++nb) {
+            mma<kEight>(o[m][nb], vf[0], vf[1], vf[2], vf[3], p[nb][0], p[nb][1]);
+            mma<kEight>(o[m][nb], vf[0], vf[1], vf[2], vf[3], rest[nb][0], rest[nb][1]);
           }
         }
       }
       __syncwarp();   // the slot is free for the next issue
-      ++step;
+      if (++slot == kS) {
+        slot = 0;
+        ++round;
+      }
       ++j;
   }
 }
