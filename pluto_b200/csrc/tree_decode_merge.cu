@@ -23,19 +23,20 @@ __global__ void __launch_bounds__(kWarps * 32) tree_decode_merge_kernel(TreeArgs
   const Sequence s = sequence_at(a, shape, b);
   pdl_wait();   // the parts are complete and visible from here on
   // the sequence's units in their order, kv_head * groups + group; this block's may not exist
-  if (unit >= s.units || line.total == 0) return;
-  start += unit * (s.tiles + shape.overhead);
+  const int group = a.group, groups = (s.count * group + (1 << shape.rows_shift) - 1) >> shape.rows_shift;
+  if (unit >= a.kv_heads * groups || line.total == 0) return;
+  const int kv_head = unit / groups;
+  start += (shape.side > 1 ? unit % groups : unit) * (s.tiles + shape.overhead);
   const unsigned end = start + s.tiles + shape.overhead;
-  const int group = a.group, groups = (s.count * group + (1 << shape.rows_shift) - 1) >> shape.rows_shift, kv_head = unit / groups;
   const int row0 = unit % groups << shape.rows_shift, rows = min(1 << shape.rows_shift, s.count * group - row0);
   const int row = kSplit ? blockIdx.y : blockIdx.y * kWarps + warp;
   if (row >= rows) return;   // (the whole CTA where its warps share a row)
-  // the workers that hold tiles of it
+  // the ranges that hold tiles of it
   const int first = static_cast<int>(holder_of(line, start + shape.overhead)), last = static_cast<int>(holder_of(line, end - 1));
   if (first == last) return;   // one worker holds all of its tiles and has written it out
   const Partials parts = partials_of(a, shape);
   const auto part_at = [&](int c) {
-    return static_cast<size_t>(2 * c + (start < range_begin(line, c) ? 0 : 1)) * parts.rows + row;
+    return static_cast<size_t>(2 * (c * shape.side + (shape.side > 1 ? kv_head : 0)) + (start < range_begin(line, c) ? 0 : 1)) * parts.rows + row;
   };
   float m = -INFINITY;
   for (int c = first + lane; c <= last; c += 32) m = fmaxf(m, parts.ml[part_at(c)].x);

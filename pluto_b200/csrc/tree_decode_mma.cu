@@ -51,6 +51,10 @@ __device__ __forceinline__ void copy4(uint32_t to, const void* from, bool there)
 __device__ __forceinline__ void arrive_behind_copies(uint64_t* bar) {   // when this thread's copies so far have landed
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+__device__ __forceinline__ void bulk_load_at(uint32_t to, const void* from, uint32_t bytes, uint64_t* bar) {   // all multiples of 16
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to), "l"(from), "r"(bytes),
+               "r"(smem_u32(bar)) : "memory");
+}
 __device__ __forceinline__ uint32_t halves_of(uint32_t codes) {   // two codes in the low 16 bits -> two fp16
   uint32_t r;
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<uint16_t>(codes)));
@@ -122,68 +126,83 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, kEight>) tree_decode_mma
     if (lane == 0) own->ahead = cursor;
   }
   __syncwarp();
-  int tile = 0, last = 0, page = 0, to_slot = 0, listed = 0;   // of the next step: its tile, the segment's end, its page, its slot
-  int load_b = 0, load_head = 0, load_end = 0;                 // of the segment: sequence, KV head, tokens
-  const auto next_load = [&]() {
-    Cursor cursor = own->ahead;
-    Segment load{};
-    const bool more = cursor.next(a, shape, load);   // (rows 0 behind the last)
-    __syncwarp();
-    if (lane == 0) {
-      own->ahead = cursor;
-      own->segments[listed % kSegments] = load;
+  bool started = false;
+  int tile = 0, last = 0, page = 0, inside = 0, to_slot = 0, listed = 0;   // of the next step: its tile, the segment's end, its page and place in it, its slot
+  int load_b = 0, load_head = 0, load_end = 0, load_rows = 0;              // of the segment: sequence, KV head, tokens, rows still to be fetched
+  const unsigned pages = a.pool.table ? a.pool.num_pages : a.batch, blocks = a.pool.table ? a.pool.max_blocks : 1;
+  const uint8_t* scales = lane < kTile ? a.pool.k_scales : a.pool.v_scales;   // lanes 0-15: the keys', 16-31: the values'
+  const uint32_t scale_page = static_cast<uint32_t>(a.pool.scale_page), scale_token = static_cast<uint32_t>(a.pool.scale_token);
+  const auto issue = [&]() {   // (the first call only finds the first step)
+    if (started) {
+      if (tile >= last) return;
+      const int slot_now = to_slot;
+      to_slot = to_slot + 1 == kS ? 0 : to_slot + 1;
+      if (load_rows > 0) {   // the queries come first, through the ring as well: a load would wait behind all copies of the SM
+        const int nodes = load_rows / group, bytes = group * D * 2;
+        if (lane == 0) mbar_expect_tx(&own->full[slot_now], nodes * bytes);
+        __syncwarp();
+        if (lane < nodes)
+          bulk_load_at(ring + slot_now * kStageBytes<D, kEight> + lane * bytes,
+                    static_cast<const __nv_bfloat16*>(a.q) + ((static_cast<size_t>(load_b) * a.nodes + lane) * a.q_heads + load_head * group) * D, bytes,
+                    &own->full[slot_now]);
+        if (kEight) mbar_arrive(&own->full[slot_now]);
+        load_rows = 0;
+        return;
+      }
+      if (static_cast<unsigned>(page) >= pages) {
+        report_status(status, 48, kBadPage);   // (a slot past the pages was reported as such before)
+        page = -1;                             // the copies read zeros there
+      }
+      if (lane == 0) {
+        const uint32_t to = ring + slot_now * kStageBytes<D, kEight>;
+        constexpr int kSlabs = kBytes == 64 ? 1 : kBytes / 128, kColumns = D / kSlabs, kSlab = kTile * kBytes / kSlabs;
+        mbar_expect_tx(&own->full[slot_now], kStageBytes<D, kEight>);
+#pragma unroll
+        for (int i = 0; i < kSlabs; ++i) {
+          tma_load_4d_at(to + i * kSlab, &map_k, i * kColumns, load_head, inside, page, &own->full[slot_now]);
+          tma_load_4d_at(to + kTile * kBytes + i * kSlab, &map_v, i * kColumns, load_head, inside, page, &own->full[slot_now]);
+        }
+      }
+      if (kEight) {
+        const int row = lane % kTile;
+        const bool there = page >= 0 && tile * kTile + row < load_end;
+        const uint8_t* byte = scales + load_head;
+        if (there) byte += static_cast<uint64_t>(static_cast<uint32_t>(page)) * scale_page + static_cast<uint64_t>(static_cast<uint32_t>(inside + row)) * scale_token;
+        const uintptr_t at = reinterpret_cast<uintptr_t>(byte);
+        own->places[slot_now][lane] = static_cast<uint8_t>(at & 3u);
+        copy4(smem_u32(&own->words[slot_now][lane]), reinterpret_cast<const void*>(at & ~static_cast<uintptr_t>(3)), there);
+        arrive_behind_copies(&own->full[slot_now]);
+      }
+      ++tile;
     }
-    __syncwarp();
-    ++listed;
-    tile = more ? load.tile0 : 0;
-    last = more ? load.tile1 : 0;
-    load_b = load.b;
-    load_head = load.kv_head;
-    load_end = load.prefix + load.count;
-  };
-  next_load();
-  const auto block_of = [&](int t) { return page_shift >= 0 ? t >> page_shift : t / a.pool.page_size; };
-  const auto fetch_page = [&]() {   // used by the next issue only
-    if (tile >= last) return;
-    const int block = block_of(tile * kTile);
-    if (block >= (a.pool.table ? a.pool.max_blocks : 1)) {
+    started = true;
+    if (tile >= last) {   // the next segment
+      Cursor cursor = own->ahead;
+      Segment load{};
+      const bool more = cursor.next(a, shape, load);   // (rows 0 behind the last)
+      __syncwarp();
+      if (lane == 0) {
+        own->ahead = cursor;
+        own->segments[listed % kSegments] = load;
+      }
+      __syncwarp();
+      ++listed;
+      tile = more ? load.tile0 : 0;
+      last = more ? load.tile1 : 0;
+      load_b = load.b;
+      load_head = load.kv_head;
+      load_end = load.prefix + load.count;
+      if (!more) return;
+      load_rows = load.rows;
+    }
+    const int t0 = tile * kTile, block = page_shift >= 0 ? t0 >> page_shift : t0 / a.pool.page_size;
+    inside = t0 - block * a.pool.page_size;
+    if (static_cast<unsigned>(block) >= blocks) {
       report_status(status, 48, kBadLength);
       page = -1;
     } else {
       page = a.pool.table ? a.pool.table[static_cast<size_t>(load_b) * a.pool.max_blocks + block] : load_b;
     }
-  };
-  fetch_page();
-  const uint8_t* scales = lane < kTile ? a.pool.k_scales : a.pool.v_scales;   // lanes 0-15: the keys', 16-31: the values'
-  const auto issue = [&]() {
-    if (tile >= last) return;
-    const int t0 = tile * kTile, inside = t0 - block_of(t0) * a.pool.page_size;
-    if (page < 0 || (a.pool.table && page >= a.pool.num_pages)) {
-      report_status(status, 48, kBadPage);   // (a slot past the pages was reported as such before)
-      page = -1;                             // the copies read zeros there
-    }
-    if (lane == 0) {
-      const uint32_t to = ring + to_slot * kStageBytes<D, kEight>;
-      constexpr int kSlabs = kBytes == 64 ? 1 : kBytes / 128, kColumns = D / kSlabs, kSlab = kTile * kBytes / kSlabs;
-      mbar_expect_tx(&own->full[to_slot], kStageBytes<D, kEight>);
-#pragma unroll
-      for (int i = 0; i < kSlabs; ++i) {
-        tma_load_4d_at(to + i * kSlab, &map_k, i * kColumns, load_head, inside, page, &own->full[to_slot]);
-        tma_load_4d_at(to + kTile * kBytes + i * kSlab, &map_v, i * kColumns, load_head, inside, page, &own->full[to_slot]);
-      }
-    }
-    if (kEight) {
-      const int row = lane % kTile;
-      const bool there = page >= 0 && t0 + row < load_end;
-      const uint8_t* byte = scales + load_head + (there ? static_cast<size_t>(page) * a.pool.scale_page + static_cast<size_t>(inside + row) * a.pool.scale_token : 0);
-      const uintptr_t at = reinterpret_cast<uintptr_t>(byte);
-      own->places[to_slot][lane] = static_cast<uint8_t>(at & 3u);
-      copy4(smem_u32(&own->words[to_slot][lane]), reinterpret_cast<const void*>(at & ~static_cast<uintptr_t>(3)), there);
-      arrive_behind_copies(&own->full[to_slot]);
-    }
-    to_slot = to_slot + 1 == kS ? 0 : to_slot + 1;
-    if (++tile >= last) next_load();
-    fetch_page();
   };
   // One loop over the steps of the range, so that every piece of code is there once: a range of few steps is as long as
   // the fetching of its instructions takes.
@@ -194,7 +213,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, kEight>) tree_decode_mma
 #pragma unroll 1
   while (true) {
     issue();
-    if (primed < kS - 1) {
+    if (primed < kS) {   // (a call without a step, and steps but one of the ring)
       ++primed;
       continue;
     }
@@ -248,24 +267,26 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, kEight>) tree_decode_mma
     seg = own->segments[n++ % kSegments];
     if (seg.rows == 0) break;
     j = seg.tile0;
+    if (!__all_sync(0xffffffffu, mbar_wait(&own->full[slot], round & 1, status, 50))) return;
+    const uint32_t rows_at = ring + slot * kStageBytes<D, kEight>;
     // ---- the queries: B fragments of row 8 nb + quad, channels in the order of the keys' pieces
     float of_row[kN];       // scale of the row's scores
     uint32_t bits_of[kN];   // which drafts it sees: one bit per node
 #pragma unroll
     for (int nb = 0; nb < kN; ++nb) {
-      const int r = nb * 8 + quad, node = r / group, head = seg.kv_head * group + r % group;
+      const int r = nb * 8 + quad;
       const bool live = r < seg.rows;
-      const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) + ((static_cast<size_t>(seg.b) * a.nodes + node) * a.q_heads + head) * D;
       uint32_t largest = 0u;
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
         const int c = kPieces < 8 ? t4 : 2 * t4 + (i & 1) + 8 * (i >> 1);
 #pragma unroll
         for (int k = 0; k < kSteps; ++k) {
-          const uint2 w = live ? *reinterpret_cast<const uint2*>(q + c * (kEight ? 16 : 8) + 4 * k) : make_uint2(0u, 0u);
-          qf[i * kSteps + k][nb][0] = w.x;
-          qf[i * kSteps + k][nb][1] = w.y;
-          largest = max(largest, max(max(w.x & 0x7fffu, w.y & 0x7fffu), max(w.x & 0x7fff0000u, w.y & 0x7fff0000u) >> 16));
+          const uint64_t w = live ? lds_b64(rows_at + (r * D + c * (kEight ? 16 : 8) + 4 * k) * 2) : 0ull;
+          const uint32_t lo = static_cast<uint32_t>(w), hi = static_cast<uint32_t>(w >> 32);
+          qf[i * kSteps + k][nb][0] = lo;
+          qf[i * kSteps + k][nb][1] = hi;
+          largest = max(largest, max(max(lo & 0x7fffu, hi & 0x7fffu), max(lo & 0x7fff0000u, hi & 0x7fff0000u) >> 16));
         }
       }
       of_row[nb] = scale_log2;
@@ -288,7 +309,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, kEight>) tree_decode_mma
       bits_of[nb] = 0u;
       if (seg.tile1 * kTile > seg.prefix && live) {
 #pragma unroll 1
-        for (int i = node; i >= 0;) {
+        for (int i = r / group; i >= 0;) {
           bits_of[nb] |= 1u << i;
           const int up = a.parents ? a.parents[static_cast<size_t>(seg.b) * a.nodes + i] : i - 1;
           if (up < -1 || up >= i) report_status(status, 49, kBadDraft);   // taken as a first token's
@@ -314,6 +335,11 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, kEight>) tree_decode_mma
       for (int nb = 0; nb < kN; ++nb)
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[m][nb][i] = 0.0f;
+    if (++slot == kS) {
+      slot = 0;
+      ++round;
+    }
+    continue;
     }
       if (!__all_sync(0xffffffffu, mbar_wait(&own->full[slot], round & 1, status, 50))) return;
       const uint32_t k_tile = ring + slot * kStageBytes<D, kEight>, v_tile = k_tile + kTile * kBytes;
@@ -536,13 +562,13 @@ bool make_pool_map(CUtensorMap* map, const void* base, const TreeArgs& a) {
 }
 
 template <int D, bool kEight>
-constexpr LineShape line_shape() {
-  return {4, 3, 4, 148 * kCtas<D, kEight> * kWarps};
+LineShape line_shape(const TreeArgs& a) {   // (many heads would leave workers over)
+  return {4, 3, 4, 148 * kCtas<D, kEight> * kWarps, a.kv_heads <= 64 ? a.kv_heads : 1};
 }
 
 template <int D, bool kEight, bool kHalf>
 cudaError_t launch_rows(cudaStream_t stream, const TreeArgs& a) {
-  constexpr LineShape shape = line_shape<D, kEight>();
+  const LineShape shape = line_shape<D, kEight>(a);
   constexpr int kBytes = kWarps * (kStages<D, kEight> * kStageBytes<D, kEight> + static_cast<int>(sizeof(WarpState<kStages<D, kEight>, kEight>))) + 1024;
   static_assert((kBytes + 1024) * kCtas<D, kEight> <= 228 * 1024, "shared memory");
   CUtensorMap map_k, map_v;
@@ -568,11 +594,12 @@ bool tree_decode_mma_supported(const TreeArgs& a) {
   const size_t element = a.pool.store == kStoreBf16 ? 2 : 1;
   return a.nodes * a.group <= (a.dim == 256 ? 8 : 16) && (a.pool.table == nullptr || a.pool.max_blocks == 1 || a.pool.page_size % kTile == 0) &&
          a.pool.page_stride * element < (1ull << 40) && a.pool.token_stride * element < (1ull << 40) &&   // (limits of a tensor map)
-         line_fits(a, {4, 3, 4, 0});
+         a.pool.scale_page < (1ull << 32) && a.pool.scale_token < (1ull << 32) &&
+         line_fits(a, {4, 3, 4, 0, 1});
 }
 
 size_t tree_decode_mma_workspace_bytes(int nodes, int q_heads, int kv_heads, int dim) {
-  return line_workspace_bytes({4, 3, 4, 148 * (dim == 256 ? 2 : dim == 128 ? 3 : 4) * kWarps}, nodes, q_heads, kv_heads, dim);   // (for either storage)
+  return line_workspace_bytes({4, 3, 4, 148 * (dim == 256 ? 2 : dim == 128 ? 3 : 4) * kWarps, 1}, nodes, q_heads, kv_heads, dim);   // (for either storage)
 }
 
 cudaError_t tree_decode_mma(cudaStream_t stream, const TreeArgs& a) {

@@ -781,7 +781,7 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(TreeArg
   if (warp == 0) tmem_dealloc(tmem, 512);
 }
 
-constexpr LineShape line_shape(int dim) { return {6, kUnitTiles, dim == 256 ? 7 : 8, kMaxCtas}; }
+constexpr LineShape line_shape(int dim) { return {6, kUnitTiles, dim == 256 ? 7 : 8, kMaxCtas, 1}; }
 
 template <int D, bool kEight, bool kWide>
 cudaError_t launch_kernel(cudaStream_t stream, const TreeArgs& a) {

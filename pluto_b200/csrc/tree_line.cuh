@@ -11,12 +11,14 @@
 
 namespace pluto {
 
-// Positions are 32-bit: line_fits is asked on the host.
+// Positions are 32-bit: line_fits is asked on the host.  A cache row holds all KV heads of a token, so workers that walk
+// the heads side by side read whole rows of it between them.
 struct LineShape {
   int tile_shift;   // keys per tile
   int overhead;     // what a unit costs besides its tiles, in tiles
   int rows_shift;   // rows of a unit at most
   int workers;      // at most
+  int side;         // KV heads walked side by side, by neighbouring workers over the same range: all of them, or 1
 };
 inline bool line_fits(const TreeArgs& a, const LineShape& shape) {
   const long long groups = (static_cast<long long>(a.nodes) * a.group + (1 << shape.rows_shift) - 1) >> shape.rows_shift;
@@ -36,7 +38,7 @@ __device__ __forceinline__ Sequence sequence_at(const TreeArgs& a, const LineSha
     s.prefix = s.prefix < 0 ? 0 : a.max_prefix;
   }
   s.tiles = (s.prefix + s.count + (1 << shape.tile_shift) - 1) >> shape.tile_shift;
-  s.units = a.kv_heads * ((s.count * a.group + (1 << shape.rows_shift) - 1) >> shape.rows_shift);   // no nodes: no units
+  s.units = a.kv_heads / shape.side * ((s.count * a.group + (1 << shape.rows_shift) - 1) >> shape.rows_shift);   // no nodes: no units
   return s;
 }
 __device__ __forceinline__ unsigned weight_of(const LineShape& shape, const Sequence& s) {
@@ -45,17 +47,17 @@ __device__ __forceinline__ unsigned weight_of(const LineShape& shape, const Sequ
 
 struct Line {
   unsigned total, base;
-  unsigned parts, longer;   // workers that take part, no more than there are tiles; the first `longer` hold base + 1, the others base
+  unsigned parts, longer;   // ranges, no more than there are tiles; the first `longer` hold base + 1, the others base
 };
 __device__ __forceinline__ unsigned range_begin(const Line& line, unsigned c) { return line.base * c + min(c, line.longer); }
-__device__ __forceinline__ unsigned holder_of(const Line& line, unsigned position) {   // worker whose range it falls into
+__device__ __forceinline__ unsigned holder_of(const Line& line, unsigned position) {   // range it falls into
   const unsigned from = line.longer * (line.base + 1);
   return position < from ? position / (line.base + 1) : line.longer + (position - from) / line.base;
 }
 __device__ __forceinline__ Line cut_line(const LineShape& shape, unsigned total, unsigned tiles) {
   Line line;
   line.total = total;
-  line.parts = max(1u, min(static_cast<unsigned>(shape.workers), tiles));
+  line.parts = max(1u, min(static_cast<unsigned>(shape.workers / shape.side), tiles));
   line.base = total / line.parts;
   line.longer = total - line.base * line.parts;
   return line;
@@ -87,7 +89,7 @@ struct Segment {
 // Walks the segments of a range.
 struct Cursor {
   unsigned begin, end, start;   // of the range; start of the current unit
-  int b, unit;
+  int b, unit, head;             // head: the worker's, where they are walked side by side
   Sequence s;
   // by a whole warp
   __device__ __forceinline__ void seek(const TreeArgs& a, const LineShape& shape, unsigned worker, int lane) {
@@ -96,9 +98,11 @@ struct Cursor {
     begin = end = start = 0;
     b = unit = 0;
     s = Sequence{0, 0, 0, 0};
-    if (worker >= line.parts || line.total == 0) return;
-    begin = range_begin(line, worker);
-    end = range_begin(line, worker + 1);
+    const unsigned range = worker / shape.side;
+    head = worker % shape.side;
+    if (range >= line.parts || line.total == 0) return;
+    begin = range_begin(line, range);
+    end = range_begin(line, range + 1);
     // the sequence that holds the begin
     unsigned before = 0;
     for (int b0 = 0; b0 < a.batch; b0 += 32) {
@@ -144,7 +148,7 @@ struct Cursor {
       if (tile0 >= tile1) continue;
       const int rows = s.count * a.group, groups = (rows + (1 << shape.rows_shift) - 1) >> shape.rows_shift;
       out.b = b;
-      out.kv_head = groups == 1 ? own : own / groups;
+      out.kv_head = shape.side > 1 ? head : groups == 1 ? own : own / groups;
       out.row0 = (groups == 1 ? 0 : own % groups) << shape.rows_shift;
       out.rows = min(1 << shape.rows_shift, rows - out.row0);
       out.prefix = s.prefix;
