@@ -3,15 +3,15 @@
 // Few units, of up to a few hundred parts (a short batch): a CTA per row, its eight warps take every eighth part each and
 // their sums meet in shared memory (one sequence of 777 tokens, 46 parts: 10 us, 35 with a warp per row).  Many units,
 // of a few parts: a warp per row (288 units of 4 parts, 8 rows: 8 us, 26 with a CTA per row).  Either way a lane owns
-// eight channels and four parts are in flight; the order of the additions is fixed.
+// eight channels and eight parts are in flight; the order of the additions is fixed.
 #include "tree_line.cuh"
 
 namespace pluto {
 namespace {
 
-constexpr int kWarps = 8, kAhead = 4;
+constexpr int kWarps = 8;
 
-template <bool kSplit>
+template <bool kSplit, int kAhead>   // kAhead: parts in flight
 __global__ void __launch_bounds__(kWarps * 32) tree_decode_merge_kernel(TreeArgs a, LineShape shape, int groups_at_most) {
   __shared__ float sums[kSplit ? kWarps : 1][256];
   __shared__ float sum_of_weights[kSplit ? kWarps : 1];
@@ -29,71 +29,79 @@ __global__ void __launch_bounds__(kWarps * 32) tree_decode_merge_kernel(TreeArgs
   start += (shape.side > 1 ? unit % groups : unit) * (s.tiles + shape.overhead);
   const unsigned end = start + s.tiles + shape.overhead;
   const int row0 = unit % groups << shape.rows_shift, rows = min(1 << shape.rows_shift, s.count * group - row0);
-  const int row = kSplit ? blockIdx.y : blockIdx.y * kWarps + warp;
-  if (row >= rows) return;   // (the whole CTA where its warps share a row)
   // the ranges that hold tiles of it
   const int first = static_cast<int>(holder_of(line, start + shape.overhead)), last = static_cast<int>(holder_of(line, end - 1));
   if (first == last) return;   // one worker holds all of its tiles and has written it out
   const Partials parts = partials_of(a, shape);
-  const auto part_at = [&](int c) {
-    return static_cast<size_t>(2 * (c * shape.side + (shape.side > 1 ? kv_head : 0)) + (start < range_begin(line, c) ? 0 : 1)) * parts.rows + row;
-  };
-  float m = -INFINITY;
-  for (int c = first + lane; c <= last; c += 32) m = fmaxf(m, parts.ml[part_at(c)].x);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const float m_safe = m == -INFINITY ? 0.0f : m;
-  float l = 0.0f, acc[8] = {};
-  const int D = a.dim, step = kSplit ? kWarps : 1;
-  const bool owns = lane * 8 < D;
-  for (int c0 = first + (kSplit ? warp : 0); c0 <= last; c0 += kAhead * step) {
+  // (the whole CTA has a row, or none, where its warps share it)
+  for (int row = kSplit ? blockIdx.y : blockIdx.y * kWarps + warp; row < rows; row += kSplit ? rows : gridDim.y * kWarps) {
+    const auto part_at = [&](int c) {
+      return static_cast<size_t>(2 * (c * shape.side + (shape.side > 1 ? kv_head : 0)) + (start < range_begin(line, c) ? 0 : 1)) * parts.rows + row;
+    };
+    const int D = a.dim, step = kSplit ? kWarps : 1;
+    const bool owns = lane * 8 < D;
     float4 x[kAhead][2];
     float2 ml[kAhead];
+    const auto load = [&](int c0) {
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const int c = c0 + u * step;
-      const size_t at = part_at(min(c, last));
-      ml[u] = c <= last ? parts.ml[at] : make_float2(-INFINITY, 0.0f);
-      const float4* from = reinterpret_cast<const float4*>(parts.acc + at * D + (owns ? lane * 8 : 0));
-      x[u][0] = from[0];
-      x[u][1] = from[1];
+      for (int u = 0; u < kAhead; ++u) {
+        const int c = c0 + u * step;
+        if (c > last) break;
+        const size_t at = part_at(c);
+        ml[u] = parts.ml[at];
+        const float4* from = reinterpret_cast<const float4*>(parts.acc + at * D + (owns ? lane * 8 : 0));
+        x[u][0] = from[0];
+        x[u][1] = from[1];
+      }
+    };
+    int c0 = first + (kSplit ? warp : 0);
+    load(c0);   // (before the maximum is known, which takes as long)
+    float m = -INFINITY;
+    for (int c = first + lane; c <= last; c += 32) m = fmaxf(m, parts.ml[part_at(c)].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float m_safe = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f, acc[8] = {};
+    while (c0 <= last) {
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if (c0 + u * step > last) break;   // (a weight of zero would not do: nothing was read)
+        const float w = fast_exp2(ml[u].x - m_safe);
+        l = fmaf(ml[u].y, w, l);
+        acc[0] = fmaf(x[u][0].x, w, acc[0]); acc[1] = fmaf(x[u][0].y, w, acc[1]);
+        acc[2] = fmaf(x[u][0].z, w, acc[2]); acc[3] = fmaf(x[u][0].w, w, acc[3]);
+        acc[4] = fmaf(x[u][1].x, w, acc[4]); acc[5] = fmaf(x[u][1].y, w, acc[5]);
+        acc[6] = fmaf(x[u][1].z, w, acc[6]); acc[7] = fmaf(x[u][1].w, w, acc[7]);
+      }
+      c0 += kAhead * step;
+      load(c0);
     }
+    const int r = row0 + row, node = r / group, head = kv_head * group + r % group;
+    const size_t token = static_cast<size_t>(b) * a.nodes + node;
+    if (kSplit) {
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      if (c0 + u * step > last) continue;   // (a weight of zero would not do: what was read may be anything)
-      const float w = fast_exp2(ml[u].x - m_safe);
-      l = fmaf(ml[u].y, w, l);
-      acc[0] = fmaf(x[u][0].x, w, acc[0]); acc[1] = fmaf(x[u][0].y, w, acc[1]);
-      acc[2] = fmaf(x[u][0].z, w, acc[2]); acc[3] = fmaf(x[u][0].w, w, acc[3]);
-      acc[4] = fmaf(x[u][1].x, w, acc[4]); acc[5] = fmaf(x[u][1].y, w, acc[5]);
-      acc[6] = fmaf(x[u][1].z, w, acc[6]); acc[7] = fmaf(x[u][1].w, w, acc[7]);
+      for (int i = 0; i < 8; ++i)
+        if (owns) sums[warp][lane * 8 + i] = acc[i];
+      if (lane == 0) sum_of_weights[warp] = l;
+      __syncthreads();
+      if (warp > 0) return;
+      l = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[i] = 0.0f;
+      for (int w = 0; w < kWarps; ++w) {
+        l += sum_of_weights[w];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[i] += owns ? sums[w][lane * 8 + i] : 0.0f;
+      }
     }
-  }
-  const int r = row0 + row, node = r / group, head = kv_head * group + r % group;
-  const size_t token = static_cast<size_t>(b) * a.nodes + node;
-  if (kSplit) {
+    const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
+    if (owns) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (owns) sums[warp][lane * 8 + i] = acc[i];
-    if (lane == 0) sum_of_weights[warp] = l;
-    __syncthreads();
-    if (warp > 0) return;
-    l = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) acc[i] = 0.0f;
-    for (int w = 0; w < kWarps; ++w) {
-      l += sum_of_weights[w];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) acc[i] += owns ? sums[w][lane * 8 + i] : 0.0f;
+      for (int i = 0; i < 8; ++i) acc[i] *= inverse;
+      store_out8(a, token, head, lane * 8, acc, gate_in_pieces(a));
     }
+    if (lane == 0 && a.lse) a.lse[token * a.q_heads + head] = m_safe * 0.6931471805599453f + logf(l);
   }
-  const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
-  if (owns) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) acc[i] *= inverse;
-    store_out8(a, token, head, lane * 8, acc, gate_in_pieces(a));
-  }
-  if (lane == 0 && a.lse) a.lse[token * a.q_heads + head] = m_safe * 0.6931471805599453f + logf(l);
 }
 
 }  // namespace
@@ -102,9 +110,11 @@ cudaError_t tree_decode_merge(cudaStream_t stream, const TreeArgs& a, const Line
   const int groups = (a.nodes * a.group + (1 << shape.rows_shift) - 1) >> shape.rows_shift;
   const int rows = slot_rows(shape, a.nodes, a.q_heads, a.kv_heads);
   const long long units = static_cast<long long>(a.batch) * a.kv_heads * groups;
-  const bool many_parts = shape.workers >= 16 * units;   // of a unit, when the line is long enough for all workers
+  // parts of a unit, when the line is long enough for all workers
+  const bool many_parts = shape.workers >= 16 * units, few_parts = shape.workers < 2 * units;
+  const int row_groups = (rows + kWarps - 1) / kWarps, resident = static_cast<int>(148 * 16 / units) + 1;
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(static_cast<unsigned>(a.batch) * a.kv_heads * groups, many_parts ? rows : (rows + kWarps - 1) / kWarps);
+  config.gridDim = dim3(static_cast<unsigned>(units), many_parts ? rows : row_groups < resident ? row_groups : resident);
   config.blockDim = dim3(kWarps * 32);
   config.stream = stream;
   cudaLaunchAttribute attribute;
@@ -112,8 +122,9 @@ cudaError_t tree_decode_merge(cudaStream_t stream, const TreeArgs& a, const Line
   attribute.val.programmaticStreamSerializationAllowed = 1;
   config.attrs = &attribute;
   config.numAttrs = 1;
-  return many_parts ? cudaLaunchKernelEx(&config, tree_decode_merge_kernel<true>, a, shape, groups)
-                    : cudaLaunchKernelEx(&config, tree_decode_merge_kernel<false>, a, shape, groups);
+  return many_parts  ? cudaLaunchKernelEx(&config, tree_decode_merge_kernel<true, 8>, a, shape, groups)
+         : few_parts ? cudaLaunchKernelEx(&config, tree_decode_merge_kernel<false, 2>, a, shape, groups)
+                     : cudaLaunchKernelEx(&config, tree_decode_merge_kernel<false, 8>, a, shape, groups);
 }
 
 }  // namespace pluto
