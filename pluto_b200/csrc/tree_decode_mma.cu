@@ -204,6 +204,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, kEight>) tree_decode_mma
       page = a.pool.table ? a.pool.table[static_cast<size_t>(load_b) * a.pool.max_blocks + block] : load_b;
     }
   };
+  // A wait that runs out is reported and the warp goes on: the results are worth nothing then, but every copy has been waited
+  // for when its memory is given up.
   // One loop over the steps of the range, so that every piece of code is there once: a range of few steps is as long as
   // the fetching of its instructions takes.
   Segment seg{};
@@ -267,7 +269,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, kEight>) tree_decode_mma
     seg = own->segments[n++ % kSegments];
     if (seg.rows == 0) break;
     j = seg.tile0;
-    if (!__all_sync(0xffffffffu, mbar_wait(&own->full[slot], round & 1, status, 50))) return;
+    mbar_wait(&own->full[slot], round & 1, status, 50);
+    __syncwarp();
     const uint32_t rows_at = ring + slot * kStageBytes<D, kEight>;
     // ---- the queries: B fragments of row 8 nb + quad, channels in the order of the keys' pieces
     float of_row[kN];       // scale of the row's scores
@@ -341,7 +344,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, kEight>) tree_decode_mma
     }
     continue;
     }
-      if (!__all_sync(0xffffffffu, mbar_wait(&own->full[slot], round & 1, status, 50))) return;
+      mbar_wait(&own->full[slot], round & 1, status, 50);
+      __syncwarp();
       const uint32_t k_tile = ring + slot * kStageBytes<D, kEight>, v_tile = k_tile + kTile * kBytes;
       const int behind = j * kTile - seg.prefix;   // of the drafts' first slot
       const bool border = behind > -kTile;         // the step holds drafts, or ends the sequence
