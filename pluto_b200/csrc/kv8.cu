@@ -51,6 +51,12 @@ __device__ __forceinline__ void rows_at(const Kv8Args& a, unsigned row, uint32_t
   }
 }
 
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
 // Eight channels as they lie in memory.
 template <bool kBf16>
 struct Raw8 {
@@ -71,10 +77,35 @@ struct Raw8 {
   }
 };
 
+// Largest magnitude of a row as the bits of an fp32 value (its lanes each hold eight channels).  Magnitudes order as
+// integers; bf16 ones are compared two at a time.
+template <bool kBf16, int kLanes>
+__device__ __forceinline__ uint32_t row_largest(const Raw8<kBf16>& x) {
+  if constexpr (kBf16) {
+    constexpr uint32_t kAbs = 0x7fff7fffu;
+    uint32_t m = max_u16x2(max_u16x2(x.w[0].x & kAbs, x.w[0].y & kAbs), max_u16x2(x.w[0].z & kAbs, x.w[0].w & kAbs));
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) m = max_u16x2(m, __shfl_xor_sync(0xffffffffu, m, o));
+    return max(m & 0xffff0000u, m << 16);
+  } else {
+    float v[8];
+    x.values(v);
+    uint32_t m = 0u;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) m = max(m, __float_as_uint(v[u]) & 0x7fffffffu);
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    return m;
+  }
+}
+
 // The codes of eight channels; a row that is not finite gets NaN codes.
-__device__ __forceinline__ uint2 codes8(const float (&x)[8], uint32_t byte) {
+template <bool kBf16>
+__device__ __forceinline__ uint2 codes8(const Raw8<kBf16>& in, uint32_t byte) {
   if (byte == 255u) return make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu);
   const float f = e8m0_inverse(byte);
+  float x[8];
+  in.values(x);
   return make_uint2(e4m3_pair(x[0] * f, x[1] * f) | e4m3_pair(x[2] * f, x[3] * f) << 16,
                     e4m3_pair(x[4] * f, x[5] * f) | e4m3_pair(x[6] * f, x[7] * f) << 16);
 }
@@ -99,16 +130,9 @@ __global__ void __launch_bounds__(256) kv8_append_vec(Kv8Args a) {
   for (int i = 0; i < kRows; ++i)
 #pragma unroll
     for (int side = 0; side < 2; ++side) {
-      float x[8];
-      in[i][side].values(x);
-      uint32_t largest = 0u;
-#pragma unroll
-      for (int u = 0; u < 8; ++u) largest = max(largest, __float_as_uint(x[u]) & 0x7fffffffu);
-#pragma unroll
-      for (int o = kLanes / 2; o > 0; o >>= 1) largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+      const uint32_t byte = e8m0_of(row_largest<kBf16, kLanes>(in[i][side]));
       if (!at[i].live) continue;
-      const uint32_t byte = e8m0_of(largest);
-      if (c < a.dim) *reinterpret_cast<uint2*>(static_cast<uint8_t*>(side ? a.pool.v : a.pool.k) + at[i].pool + c) = codes8(x, byte);
+      if (c < a.dim) *reinterpret_cast<uint2*>(static_cast<uint8_t*>(side ? a.pool.v : a.pool.k) + at[i].pool + c) = codes8(in[i][side], byte);
       if (lane == 0) (side ? a.pool.v_scales : a.pool.k_scales)[at[i].scale] = static_cast<uint8_t>(byte);
     }
 }
