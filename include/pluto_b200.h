@@ -386,7 +386,7 @@ int pluto_cached_attention_step(pluto_stream_t stream, const void* q_gate, const
  * holds an infinity or a NaN gets scale byte 255 and reads back as NaN.  `scales` is NULL for the other two. */
 enum { PLUTO_E4M3 = 2 };
 typedef struct pluto_kv_scales {
-  uint8_t* k; /* device */
+  uint8_t* k; /* device; the attention reads scale bytes by the aligned 4-byte word they lie in */
   uint8_t* v;
   size_t page_stride;  /* elements */
   size_t token_stride; /* elements, >= kv_heads */
@@ -407,18 +407,19 @@ int pluto_kv8_read(pluto_stream_t stream, void* k, void* v, int dtype, size_t ba
                    const pluto_kv_scales* scales /* host */, const int32_t* positions,
                    const int32_t* counts, int batch, int tokens, int kv_heads, int head_dim);
 
-/* After a verification (in the place of KeyValueCache::Advance, src/llm/key_value_cache.h:25-57): for i < accepted[b] the key and value rows (and scales) of slot prefix_lens[b] +
- * path[b][i] move to slot prefix_lens[b] + i, in place; path is int32 [batch, nodes], rising, accepted int32
- * [batch] in [0, nodes].  Every other slot keeps its rows.  Any of the three storage types. */
+/* After a verification (in the place of KeyValueCache::Advance, src/llm/key_value_cache.h:25-57): for i < accepted[b]
+ * the key and value rows (and scales) of slot prefix_lens[b] + path[b][i] move to slot prefix_lens[b] + i, in place;
+ * path is int32 [batch, nodes], rising, accepted int32 [batch] in [0, nodes].  Every other slot keeps its rows.  Any
+ * of the three storage types. */
 int pluto_kv_keep(pluto_stream_t stream, const pluto_kv_cache* cache /* host */,
                   const pluto_kv_scales* scales /* host */, const int32_t* prefix_lens, const int32_t* path,
                   const int32_t* accepted, int batch, int nodes, int kv_heads, int head_dim);
 
-/* pluto_qk_prepare (src/llm/layers/util/cached_attention_ops.cc:30-79) for drafted tokens: q_in, k_in, v_in as there with tokens = nodes.  Node i of sequence b is
- * rotated for position prefix_lens[b] + (number of its ancestors) and its K/V row goes to slot
- * prefix_lens[b] + i of a cache of any storage type; queries and rows are those of pluto_qk_prepare bit for
- * bit (8-bit rows: those of pluto_kv8_append of them).  parents NULL (a chain, or a prompt): any number of
- * tokens; prefix_lens NULL: 0. */
+/* pluto_qk_prepare (src/llm/layers/util/cached_attention_ops.cc:30-79) for drafted tokens: q_in, k_in, v_in as there with
+ * tokens = nodes.  Node i of sequence b is rotated for position prefix_lens[b] + (number of its ancestors) and its K/V
+ * row goes to slot prefix_lens[b] + i of a cache of any storage type; queries and rows are those of
+ * pluto_qk_prepare bit for bit (8-bit rows: those of pluto_kv8_append of them).  parents NULL (a chain, or a prompt): any
+ * number of tokens; prefix_lens NULL: 0. */
 int pluto_draft_prepare(pluto_stream_t stream, const void* q_in, const void* k_in, const void* v_in,
                         int in_dtype, size_t q_token_stride, size_t q_head_stride, const float* q_norm,
                         const float* k_norm, const int32_t* prefix_lens, const int32_t* parents,
@@ -434,14 +435,20 @@ int pluto_draft_prepare(pluto_stream_t stream, const void* q_in, const void* k_i
  *   q            [batch, nodes, q_heads, head_dim] prepared queries (q_dtype)
  *   gate         optional; element (b, i, h, d) at gate + (b * nodes + i) * gate_token_stride + h *
  *                gate_head_stride + d
- *   max_prefix_len  host upper bound of prefix_lens
- *   out          [batch, nodes, q_heads, head_dim] (out_dtype);  lse optional fp32 [batch, nodes, q_heads]
+ *   max_prefix_len  host upper bound of prefix_lens, <= 2^31 - 1025
+ *   out          [batch, nodes, q_heads, head_dim] (out_dtype), apart from every input;  lse optional fp32
+ *                [batch, nodes, q_heads]
  *   workspace    >= pluto_gqa_tree_decode_workspace_bytes(...) bytes, 16-byte aligned; overwritten, so calls that
  *                share one are ordered on one stream
  * What a node does not see does not reach its output, whatever it holds; a node that sees a row with an
  * infinity or a NaN gets NaN.
- * bf16 queries with a bf16 result over a bf16 or 8-bit cache, head_dim 64, 128 or 256, rows on 16-byte
- * boundaries, run on the tensor cores (probabilities enter P V as bf16); everything else in fp32 arithmetic. */
+ * bf16 queries with a bf16 result over a bf16 or 8-bit cache, head_dim 64, 128 or 256, rows on 16-byte boundaries, run on
+ * the tensor cores; everything else in fp32 arithmetic.  On the tensor cores sums are in fp32 and what enters a product
+ * is exact but for the softmax weights:
+ *   bf16 cache   few rows (nodes * q_heads / kv_heads <= 16, at width 256 <= 8; pages that 16 divides, or one page per
+ *                sequence): weights to 16 bits; more rows, or other pages: to bf16
+ *   8-bit cache  weights to fp16, relative to the largest scale 2^n among the value rows that a query sees: value rows of a
+ *                much smaller scale lose weights below 2^-25 of that */
 size_t pluto_gqa_tree_decode_workspace_bytes(int batch, int nodes, int q_heads, int kv_heads, int head_dim);
 int pluto_gqa_tree_decode(pluto_stream_t stream, const void* q, int q_dtype, const void* gate, int gate_dtype,
                           size_t gate_token_stride, size_t gate_head_stride,

@@ -15,6 +15,7 @@ namespace {
 using pluto::report;
 
 bool aligned_to(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+size_t bytes_of(int dtype) { return dtype == PLUTO_FP32 ? 4 : 2; }   // of an activation type
 bool activation(int dtype) { return dtype == PLUTO_FP32 || dtype == PLUTO_BF16; }
 bool fits_int(long long a, long long b, long long c) { return a * b <= 0x7fffffff && a * b * c <= 0x7fffffff; }
 
@@ -29,7 +30,7 @@ int fill_pool(pluto::DraftPool* p, const pluto_kv_cache* cache, const pluto_kv_s
   const size_t element = cache->dtype == PLUTO_FP32 ? 4 : cache->dtype == PLUTO_BF16 ? 2 : 1;
   if (cache->page_size <= 0 || (cache->block_table && (cache->max_blocks <= 0 || cache->num_pages <= 0)) ||
       cache->token_stride < static_cast<size_t>(kv_heads) * head_dim || cache->page_stride < cache->token_stride ||
-      !aligned_to(cache->k_base, element) || !aligned_to(cache->v_base, element))
+      !aligned_to(cache->k_base, element) || !aligned_to(cache->v_base, element) || !aligned_to(cache->block_table, 4))
     return report(PLUTO_E_INVALID, "attention cache shape or capacity does not match parameters");
   if ((cache->dtype == PLUTO_E4M3) != (scales != nullptr))
     return report(PLUTO_E_INVALID, "an 8-bit cache needs its scales, and only that");
@@ -64,7 +65,7 @@ int fill_kv8(pluto::Kv8Args* a, const void* k, const void* v, int dtype, size_t 
   if (cache && cache->dtype != PLUTO_E4M3) return report(PLUTO_E_INVALID, "the cache is not an 8-bit one");
   if (!k || !v) return report(PLUTO_E_INVALID, "attention requires non-null device pointers");
   const size_t element = dtype == PLUTO_BF16 ? 2 : 4;
-  if (!aligned_to(k, element) || !aligned_to(v, element) || (kv_heads > 1 && head_stride < static_cast<size_t>(head_dim)))
+  if (!aligned_to(k, element) || !aligned_to(v, element) || !aligned_to(positions, 4) || !aligned_to(counts, 4) || (kv_heads > 1 && head_stride < static_cast<size_t>(head_dim)))
     return report(PLUTO_E_INVALID, "invalid 8-bit cache dimensions or parameters");
   *a = pluto::Kv8Args{};
   if (int c = fill_pool(&a->pool, cache, scales, kv_heads, head_dim)) return c;
@@ -119,6 +120,8 @@ int pluto_kv_keep(pluto_stream_t stream, const pluto_kv_cache* cache, const plut
   pluto::KeepArgs a{};
   if (int c = fill_pool(&a.pool, cache, scales, kv_heads, head_dim)) return c;
   if (!prefix_lens || !path || !accepted) return report(PLUTO_E_INVALID, "attention requires non-null device pointers");
+  if (!aligned_to(prefix_lens, 4) || !aligned_to(path, 4) || !aligned_to(accepted, 4))
+    return report(PLUTO_E_INVALID, "attention tensors are not aligned to their elements");
   a.prefix = prefix_lens; a.path = path; a.accepted = accepted;
   a.batch = batch; a.nodes = nodes; a.heads = kv_heads; a.dim = head_dim;
   if (int c = take_status(&a.pool.status)) return c;
@@ -139,6 +142,10 @@ int pluto_draft_prepare(pluto_stream_t stream, const void* q_in, const void* k_i
   if (int c = fill_pool(&d.pool, cache, scales, kv_heads, head_dim)) return c;
   if (!q_in || !k_in || !v_in || !q_norm || !k_norm || !q_out)
     return report(PLUTO_E_INVALID, "attention requires non-null device pointers");
+  if (!aligned_to(q_in, bytes_of(in_dtype)) || !aligned_to(k_in, bytes_of(in_dtype)) || !aligned_to(v_in, bytes_of(in_dtype)) ||
+      !aligned_to(q_out, bytes_of(q_out_dtype)) || !aligned_to(q_norm, 4) || !aligned_to(k_norm, 4) || !aligned_to(prefix_lens, 4) ||
+      !aligned_to(parents, 4) || !aligned_to(counts, 4))
+    return report(PLUTO_E_INVALID, "attention tensors are not aligned to their elements");
   pluto::PrepareArgs& a = d.p;
   a.q_in = q_in; a.k_in = k_in; a.v_in = v_in; a.in_is_bf16 = in_dtype == PLUTO_BF16;
   a.q_token = q_token_stride; a.q_head = q_head_stride;
@@ -168,12 +175,16 @@ int pluto_gqa_tree_decode(pluto_stream_t stream, const void* q, int q_dtype, con
                           size_t workspace_bytes, int batch, int nodes, int q_heads, int kv_heads, int head_dim,
                           int round_to_bf16) {
   if (!draft_shape(batch, nodes, q_heads, kv_heads, head_dim) || nodes > pluto::kMaxDraftNodes || max_prefix_len < 0 ||
-      max_prefix_len > 0x7fffffff - pluto::kMaxDraftNodes || !activation(q_dtype) || !activation(out_dtype) ||
+      max_prefix_len > 0x7fffffff - 1024 ||   // (slots rounded up to whole tiles stay 32-bit)
+       !activation(q_dtype) || !activation(out_dtype) ||
       (gate && !activation(gate_dtype)))
     return report(PLUTO_E_INVALID, "invalid full-attention dimensions or parameters");
   pluto::TreeArgs a{};
   if (int c = fill_pool(&a.pool, cache, scales, kv_heads, head_dim)) return c;
   if (!q || !prefix_lens || !out || !workspace) return report(PLUTO_E_INVALID, "attention requires non-null device pointers");
+  if (!aligned_to(q, bytes_of(q_dtype)) || !aligned_to(out, bytes_of(out_dtype)) || (gate && !aligned_to(gate, bytes_of(gate_dtype))) ||
+      !aligned_to(lse, 4) || !aligned_to(prefix_lens, 4) || !aligned_to(parents, 4) || !aligned_to(counts, 4))
+    return report(PLUTO_E_INVALID, "attention tensors are not aligned to their elements");
   if (workspace_bytes < pluto_gqa_tree_decode_workspace_bytes(batch, nodes, q_heads, kv_heads, head_dim) ||
       !aligned_to(workspace, 16))
     return report(PLUTO_E_INVALID, "attention decode workspace is too small or misaligned");
@@ -207,6 +218,10 @@ int pluto_verify_drafts(pluto_stream_t stream, const void* target_probs, const v
     return report(PLUTO_E_UNIMPLEMENTED, "draft probabilities are taken for chains, not for trees");
   if (!target_probs || !tokens || !accept_uniforms || !sample_uniforms || !accepted || !path || !out_tokens)
     return report(PLUTO_E_INVALID, "draft verification requires non-null device pointers");
+  if (!aligned_to(target_probs, bytes_of(dtype)) || !aligned_to(draft_probs, bytes_of(dtype)) || !aligned_to(tokens, 4) ||
+      !aligned_to(accept_uniforms, 4) || !aligned_to(sample_uniforms, 4) || !aligned_to(parents, 4) || !aligned_to(counts, 4) ||
+      !aligned_to(accepted, 4) || !aligned_to(path, 4) || !aligned_to(out_tokens, 4))
+    return report(PLUTO_E_INVALID, "draft verification tensors are not aligned to their elements");
   pluto::VerifyArgs a{};
   a.target = target_probs; a.draft = draft_probs; a.is_bf16 = dtype == PLUTO_BF16;
   a.tokens = tokens; a.parents = parents; a.counts = counts;

@@ -6,7 +6,9 @@
 // ones each (16 bytes of bf16 in, 8 of codes out), so the row maximum is a butterfly over at most 32 lanes
 // and no shared memory is used; a sub-warp takes the key and the value row of kRows (token, head) pairs at
 // a time, which keeps 2 * kRows loads per lane in flight.  Widths that 8 does not divide and rows off the
-// 16-byte boundary take single channels, a warp per row.
+// 16-byte boundary take single channels, a warp per row.  Measured (B200, 16 x 8191 tokens, 8 heads of 128, bf16): append
+// 154 us, 5.2 TB/s, bound by the issue of its instructions; read 126 us, 6.4 TB/s.  Scale bytes gathered into words
+// took longer (177), four rows at a time no less.
 #include "draft_rows.cuh"
 
 namespace pluto {

@@ -7,7 +7,7 @@
 // A CTA owns a (node, query head).  Its warps take every eighth key, a lane owns up to eight channels, the
 // running maximum, sum and accumulator of a warp stay in registers, and the warps' states are merged in
 // order.  Keys that a node does not see are skipped, so nothing they hold can reach it.  Nodes from counts[b]
-// on are left as they were.  Shapes of the tensor cores take tree_decode_sm100.cu.
+// on are left as they were.  Shapes of the tensor cores take tree_decode_mma.cu or tree_decode_sm100.cu.
 #include "draft_rows.cuh"
 
 namespace pluto {

@@ -1,9 +1,11 @@
 // Merges the parts of the units that the cuts of the line (tree_line.cuh) fall into, in the order of the keys:
 //   out = sum_c 2^(m_c - m) acc_c / sum_c 2^(m_c - m) l_c,   m = max_c m_c.
-// Few units, of up to a few hundred parts (a short batch): a CTA per row, its eight warps take every eighth part each and
-// their sums meet in shared memory (one sequence of 777 tokens, 46 parts: 10 us, 35 with a warp per row).  Many units,
-// of a few parts: a warp per row (288 units of 4 parts, 8 rows: 8 us, 26 with a CTA per row).  Either way a lane owns
-// eight channels and eight parts are in flight; the order of the additions is fixed.
+// A lane owns eight channels; the order of the additions is fixed.  Few units, of up to a few hundred parts (a short
+// batch): a CTA per row, its eight warps take every eighth part each and their sums meet in shared memory (one
+// sequence of 777 tokens, 46 parts: 7 us, 35 with a warp per row).  Many units: a warp per row, eight parts in flight
+// (192 units of 9 parts, 5 rows: 7 us, 11 with four); units of a part or two: two in flight, for more warps per SM, and
+// no more CTAs than fit, as a CTA's look-ups take longer than a row (39040 rows: 26 us, 55 with a warp for every row and
+// eight parts).
 #include "tree_line.cuh"
 
 namespace pluto {

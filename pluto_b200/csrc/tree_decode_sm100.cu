@@ -17,13 +17,17 @@
 // half of TMEM): one stream with two score buffers.
 //
 // Loading.  Four warps copy the rows into a ring with asynchronous 16-byte copies; pages may have any size and rows any
-// 16-byte stride.  bf16 rows land as the swizzled tiles that the products read.  8-bit codes land as they are (96 KB per
-// SM in flight at width 128) and eight more warps widen them to fp16 tiles, one instruction per two codes and exact,
+// 16-byte stride.  bf16 rows land as the swizzled tiles that the products read.  8-bit codes land as they are (up to 96 KB
+// per SM in flight) and eight more warps widen them to fp16 tiles, one instruction per two codes and exact,
 // and multiply them by their row's 2^n where fp16 holds every product (-15 <= n <= 7, values from 2^-24 to 57344);
 // a tile with other rows keeps its codes and the softmax multiplies scores and weights by the rows' factors.  P then
 // carries 11 bits, over bf16 caches 8.
 //
 // Work is cut evenly over the SMs as tree_line.cuh says, one CTA per SM.
+//
+// Measured (B200, 16 sequences of 8000 tokens, 40 and 8 heads of 128): 40 rows per KV head, bf16 114 us, 4.6 TB/s of
+// cache, 8-bit 135; 100 rows 130 and 147; 305 rows 303 and 402, where the softmax bounds it: one warp's chain of loads,
+// maxima, exponentials and stores, two such warps per scheduler.
 #include <stddef.h>
 
 #include "tree_line.cuh"
@@ -37,7 +41,8 @@ constexpr int kThreads = kEight ? 768 : 512;   // warps 0-3: MMA issue; 4-11: so
 constexpr int kMaxCtas = 148;
 constexpr int kUnitTiles = 3;        // query load and read-out of a unit, in tiles
 constexpr float kRescale = 8.0f;     // O is rescaled when the maximum has grown by more than 2^8
-constexpr float kSmallest = -100.0f; // exponent of the value rows from which smaller ones are taken for as large
+constexpr float kSmallest = -90.0f;    // exponent of the value rows from which smaller ones are taken for as large: sums of weights
+                                       // of up to 2^(90 + 8) stay finite for any number of tokens
 
 // kWide: more than 128 rows may share a pass over the keys (never at width 256)
 template <int D, bool kEight, bool kWide>   // tiles of keys, and of values
