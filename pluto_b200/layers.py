@@ -790,9 +790,8 @@ def kv8_read(k_pool: torch.Tensor, v_pool: torch.Tensor, k_scales: torch.Tensor,
     B, device = positions.shape[0], _device_index()
     cache, scales = _draft_pool(k_pool, v_pool, block_table, k_scales, v_scales, B, device)
     _, _, H, D = k_pool.shape
-    new = torch.empty if counts is None else torch.zeros
-    k = new((B, tokens, H, D), dtype=dtype, device=k_pool.device)
-    v = new((B, tokens, H, D), dtype=dtype, device=k_pool.device)
+    k = k_pool.new_empty((B, tokens, H, D), dtype=dtype) if counts is None else k_pool.new_zeros((B, tokens, H, D), dtype=dtype)
+    v = torch.empty_like(k) if counts is None else torch.zeros_like(k)
     check(_capi.fast().pluto_kv8_read(_stream(), k.data_ptr(), v.data_ptr(), _dt(k), tokens * H * D, H * D, D, cache, scales,
                                       _check_ints(positions, (B,), "positions", device), _check_ints(counts, (B,), "counts", device),
                                       B, tokens, H, D))
