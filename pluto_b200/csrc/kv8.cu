@@ -114,7 +114,7 @@ __device__ __forceinline__ uint2 codes8(const Raw8<kBf16>& in, uint32_t byte) {
 
 template <bool kBf16, int kLanes>   // lanes per row: dim <= 8 * kLanes
 __global__ void __launch_bounds__(256) kv8_append_vec(Kv8Args a) {
-  const unsigned group = (blockIdx.x * 256u + threadIdx.x) / kLanes, lane = threadIdx.x % kLanes;
+  const unsigned group = blockIdx.x * (256u / kLanes) + threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
   const int c = lane * 8;
   Raw8<kBf16> in[kRows][2];
   RowAt at[kRows];
@@ -149,7 +149,7 @@ __device__ __forceinline__ void store1(void* p, size_t at, int is_bf16, float x)
 
 __global__ void __launch_bounds__(256) kv8_append_any(Kv8Args a) {
   const int lane = threadIdx.x % 32;
-  const RowAt at = row_at(a, (blockIdx.x * 256u + threadIdx.x) / 32, 40);
+  const RowAt at = row_at(a, blockIdx.x * 8u + threadIdx.x / 32, 40);
   if (!at.live) return;
 #pragma unroll
   for (int side = 0; side < 2; ++side) {
@@ -187,7 +187,7 @@ __device__ __forceinline__ void store8(void* p, size_t at, uint2 codes, float f)
 
 template <bool kBf16, int kLanes>
 __global__ void __launch_bounds__(256) kv8_read_vec(Kv8Args a) {
-  const unsigned group = (blockIdx.x * 256u + threadIdx.x) / kLanes, lane = threadIdx.x % kLanes;
+  const unsigned group = blockIdx.x * (256u / kLanes) + threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
   const int c = lane * 8;
   if (c >= a.dim) return;
   uint2 k[kRows], v[kRows];
@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(256) kv8_read_vec(Kv8Args a) {
 
 __global__ void __launch_bounds__(256) kv8_read_any(Kv8Args a) {
   const int lane = threadIdx.x % 32;
-  const RowAt at = row_at(a, (blockIdx.x * 256u + threadIdx.x) / 32, 41);
+  const RowAt at = row_at(a, blockIdx.x * 8u + threadIdx.x / 32, 41);
   if (!at.live) return;
   const float kf = e8m0_value(a.pool.k_scales[at.scale]), vf = e8m0_value(a.pool.v_scales[at.scale]);
   for (int c = lane; c < a.dim; c += 32) {
