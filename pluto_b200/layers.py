@@ -381,7 +381,6 @@ class KeyValueCache:
             self.value_scales_ = torch.zeros_like(self.key_scales_)
         self.position_ = 0
         self.packed_ = None
-        self.length_ = None
 
     @staticmethod
     def Create(capacity: int, key_value_heads: int, head_dim: int,
@@ -409,10 +408,8 @@ class KeyValueCache:
                     v_scales=part(self.value_scales_))
 
     def device_position(self) -> torch.Tensor:
-        """The position as an int32 [1] device tensor, set on the current stream."""
-        if self.length_ is None or self.length_.device != self.keys_.device:
-            self.length_ = torch.empty((1,), dtype=torch.int32, device=self.keys_.device)
-        return self.length_.fill_(self.position_)
+        """The position as a new int32 [1] device tensor, set on the current stream."""
+        return torch.full((1,), self.position_, dtype=torch.int32, device=self.keys_.device)
 
     def Keep(self, path: torch.Tensor, accepted: torch.Tensor) -> int:
         """After CachedDraftStep and a verification: the rows of the accepted path (int32 [nodes] and [1], as
