@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, kEight>) tree_decode_mma
     seg = own->segments[n++ % kSegments];
     if (seg.rows == 0) break;
     j = seg.tile0;
-    mbar_wait(&own->full[slot], round & 1, status, 50);
+    tree_wait(&own->full[slot], round & 1, status, 50);
     __syncwarp();
     const uint32_t rows_at = ring + slot * kStageBytes<D, kEight>;
     // ---- the queries: B fragments of row 8 nb + quad, channels in the order of the keys' pieces
@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, kEight>) tree_decode_mma
     }
     continue;
     }
-      mbar_wait(&own->full[slot], round & 1, status, 50);
+      tree_wait(&own->full[slot], round & 1, status, 50);
       __syncwarp();
       const uint32_t k_tile = ring + slot * kStageBytes<D, kEight>, v_tile = k_tile + kTile * kBytes;
       const int behind = j * kTile - seg.prefix;   // of the drafts' first slot

@@ -85,7 +85,7 @@ struct Shared {
 template <typename S>
 __device__ __forceinline__ bool next_segment(S* sh, int& n, Segment& seg, int lane, uint32_t* status) {
   const int at = n % kSegments;
-  if (!__all_sync(0xffffffffu, mbar_wait(&sh->seg_full[at], (n / kSegments) & 1, status, 61))) return false;
+  if (!__all_sync(0xffffffffu, tree_wait(&sh->seg_full[at], (n / kSegments) & 1, status, 61))) return false;
   seg = sh->seg[at];
   ++n;
   __syncwarp();
@@ -164,8 +164,8 @@ __device__ __forceinline__ void load_tiles(const TreeArgs& a, Shared<D, kEight, 
     // (few slots: this one, or one that its tile waits for, is freed once the last unit's scales have been passed on)
     if (kEight && kRing <= 3) pass_scales();
     if (use > 0) {
-      if (!__all_sync(0xffffffffu, mbar_wait(kEight ? &sh->raw_empty[slot] : &sh->k_empty[slot], (use - 1) & 1, status, 50))) return;
-      if (!kEight && !__all_sync(0xffffffffu, mbar_wait(&sh->v_empty[slot], (use - 1) & 1, status, 51))) return;
+      if (!__all_sync(0xffffffffu, tree_wait(kEight ? &sh->raw_empty[slot] : &sh->k_empty[slot], (use - 1) & 1, status, 50))) return;
+      if (!kEight && !__all_sync(0xffffffffu, tree_wait(&sh->v_empty[slot], (use - 1) & 1, status, 51))) return;
     }
     if (!more) {   // the range ends, for the widening warps of this half and parity as well
       if (first_row == 0 && lane == 0) sh->draft_row[slot] = -1;
@@ -256,7 +256,7 @@ __device__ __forceinline__ void widen_tiles(Shared<D, true, kWide>* sh, uint32_t
   const int second = c / 4 & 1, slab = c / 4 * (kTile * 128), p0 = (2 * c + second) & 7, p1 = (2 * c + 1 - second) & 7;
   for (int n = warp >> 1;; n += 2) {
     const int slot = n % kRaw, stage = n % kTiles, use = n / kTiles, scale_slot = n % (3 * kTiles);
-    if (!__all_sync(0xffffffffu, mbar_wait(&sh->raw_scales[slot], (n / kRaw) & 1, status, 47))) return;
+    if (!__all_sync(0xffffffffu, tree_wait(&sh->raw_scales[slot], (n / kRaw) & 1, status, 47))) return;
     const int draft_row = sh->draft_row[slot];
     if (draft_row < 0) return;
     // the rows' factors: in the codes for all rows of the tile or for none
@@ -270,7 +270,7 @@ __device__ __forceinline__ void widen_tiles(Shared<D, true, kWide>* sh, uint32_t
     const bool hidden = own_v == 255u && first_row + lane >= draft_row;
     if (!values && hidden) factor = 0x7fff7fffu;
     const unsigned zeros = __ballot_sync(0xffffffffu, values && hidden);
-    if (use > 0 && !__all_sync(0xffffffffu, mbar_wait(values ? &sh->v_empty[stage] : &sh->k_empty[stage], (use - 1) & 1, status, values ? 46 : 45))) return;
+    if (use > 0 && !__all_sync(0xffffffffu, tree_wait(values ? &sh->v_empty[stage] : &sh->k_empty[stage], (use - 1) & 1, status, values ? 46 : 45))) return;
     if (!values && first_row == 0) {
       uint32_t largest = 127u;
       if (!k_fits || !v_fits) {
@@ -286,7 +286,7 @@ __device__ __forceinline__ void widen_tiles(Shared<D, true, kWide>* sh, uint32_t
         sh->v_largest[scale_slot] = static_cast<int>(largest) - 127;
       }
     }
-    if (!__all_sync(0xffffffffu, mbar_wait(values ? &sh->raw_v[slot] : &sh->raw_k[slot], (n / kRaw) & 1, status, 44))) return;
+    if (!__all_sync(0xffffffffu, tree_wait(values ? &sh->raw_v[slot] : &sh->raw_k[slot], (n / kRaw) & 1, status, 44))) return;
     uint32_t from = raw_ring + slot * (kTile * D) + (first_row + row) * D + c * 16;
     uint32_t to = ring + stage * kTileBytes<D> + slab + (first_row + row) * 128;
 #pragma unroll 4
@@ -395,14 +395,14 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(TreeArg
       while (ok && next_segment(sh, seg_n, seg, lane, status)) {
         const int tiles = __shfl_sync(0xffffffffu, seg.tile1 - seg.tile0, 0);
         const bool pair = kWide && __shfl_sync(0xffffffffu, seg.rows > 128 ? 1 : 0, 0), every = pair || kOneO;   // every: all tiles are a stream's
-        ok = __all_sync(0xffffffffu, mbar_wait(&sh->q_full[0], segments++ & 1, status, 52));
-        if (ok && pair && warp) ok = __all_sync(0xffffffffu, mbar_wait(&sh->q_full[1], pairs & 1, status, 52));
+        ok = __all_sync(0xffffffffu, tree_wait(&sh->q_full[0], segments++ & 1, status, 52));
+        if (ok && pair && warp) ok = __all_sync(0xffffffffu, tree_wait(&sh->q_full[1], pairs & 1, status, 52));
         pairs += pair;
         if (!ok) break;
         const uint64_t q_desc = umma_desc_sw128(queries + (pair && warp ? kQueryBytes<D, kWide> : 0), 16, 1024);
         const auto issue_qk = [&](int x, int u) -> bool {
           const int n = tile_n + (every ? u : 2 * u + x), stage = n % kStages<D, kEight, kWide>, buffer = buffer_of((x ? own_1 : own_0) + u);
-          if (!__all_sync(0xffffffffu, mbar_wait(&sh->k_full[stage], (n / kStages<D, kEight, kWide>) & 1, status, 53))) return false;
+          if (!__all_sync(0xffffffffu, tree_wait(&sh->k_full[stage], (n / kStages<D, kEight, kWide>) & 1, status, 53))) return false;
           fence_proxy_async();   // the loaders' stores, before the tensor cores read them
           tc_fence_after();
           const uint64_t k_desc = umma_desc_sw128(k_ring + stage * kTileBytes<D>, 16, 1024);
@@ -424,12 +424,12 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(TreeArg
         const auto issue_pv = [&](int x, int u) -> bool {
           const int n = tile_n + (every ? u : 2 * u + x), stage = n % kStages<D, kEight, kWide>, t = (x ? own_1 : own_0) + u;
           const int buffer = buffer_of(t), phase = phase_of(t);
-          if (!__all_sync(0xffffffffu, mbar_wait(&sh->v_full[stage], (n / kStages<D, kEight, kWide>) & 1, status, 54))) return false;
+          if (!__all_sync(0xffffffffu, tree_wait(&sh->v_full[stage], (n / kStages<D, kEight, kWide>) & 1, status, 54))) return false;
           fence_proxy_async();
           const uint64_t v_desc = umma_desc_sw128(v_ring + stage * kTileBytes<D>, kTile * 128, 1024);
           const uint32_t o = tmem + x * kColO1, p = tmem + kColS + (kBuffers * x + buffer) * kTile;
           // the weights come in two halves of the tile's keys; the first half's product runs under the second's softmax
-          if (!__all_sync(0xffffffffu, mbar_wait(&sh->p_half[x][buffer], phase, status, 55))) return false;
+          if (!__all_sync(0xffffffffu, tree_wait(&sh->p_half[x][buffer], phase, status, 55))) return false;
           tc_fence_after();
           if (elect_one()) {
 #pragma unroll
@@ -437,7 +437,7 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(TreeArg
             tc_commit(&sh->pv_half[x][buffer]);
           }
           __syncwarp();
-          if (!__all_sync(0xffffffffu, mbar_wait(&sh->p_full[x][buffer], phase, status, 55))) return false;
+          if (!__all_sync(0xffffffffu, tree_wait(&sh->p_full[x][buffer], phase, status, 55))) return false;
           tc_fence_after();
           if (elect_one()) {
 #pragma unroll
@@ -475,7 +475,7 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(TreeArg
         const int at = n % kSegments;
         Segment seg{};
         more = cursor.next(a, shape, seg);
-        if (n >= kSegments && !__all_sync(0xffffffffu, mbar_wait(&sh->seg_empty[at], (n / kSegments - 1) & 1, status, 62))) break;
+        if (n >= kSegments && !__all_sync(0xffffffffu, tree_wait(&sh->seg_empty[at], (n / kSegments - 1) & 1, status, 62))) break;
         if (lane == 0) {
           if (!more) seg.rows = 0;
           sh->seg[at] = seg;
@@ -586,7 +586,7 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(TreeArg
         // A parity tells the phase that is awaited from its two neighbours only.  Every barrier of a score buffer completes
         // once per tile in it, and a tile's scores are committed behind the products of the buffer's last tile.
         const int j = every ? u : 2 * u + x, t = own_n + u, buffer = buffer_of(t);
-        ok = __all_sync(0xffffffffu, mbar_wait(&sh->s_full[x][buffer], phase_of(t), status, 56));
+        ok = __all_sync(0xffffffffu, tree_wait(&sh->s_full[x][buffer], phase_of(t), status, 56));
         if (!ok) break;
         const uint32_t s_at = lanes + kColS + (kBuffers * x + buffer) * kTile;
         const int slot = (tile_n + j) % (3 * kStages<D, kEight, kWide>);
@@ -651,7 +651,7 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(TreeArg
               l *= factor;
               if (u > 0 || h == 1) {
                 // every product into this O must have ended: the first half's, or the previous tile's second
-                ok = __all_sync(0xffffffffu, mbar_wait(h ? &sh->pv_half[x][buffer] : &sh->pv_done[x][buffer_of(t - 1)], phase_of(h ? t : t - 1), status, 57));
+                ok = __all_sync(0xffffffffu, tree_wait(h ? &sh->pv_half[x][buffer] : &sh->pv_done[x][buffer_of(t - 1)], phase_of(h ? t : t - 1), status, 57));
                 if (!ok) break;
                 tc_fence_after();
 #pragma unroll 1
@@ -695,7 +695,7 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(TreeArg
       own_n += own;
       other_n += every ? tiles : tiles - own;
       // this stream's last product
-      if (own > 0) ok = __all_sync(0xffffffffu, mbar_wait(&sh->pv_done[x][buffer_of(own_n - 1)], phase_of(own_n - 1), status, 58));
+      if (own > 0) ok = __all_sync(0xffffffffu, tree_wait(&sh->pv_done[x][buffer_of(own_n - 1)], phase_of(own_n - 1), status, 58));
       if (!ok) break;
       tc_fence_after();
       // ---- read-out: rows of one stream, or the two streams' halves of the keys merged, half of the channels each
@@ -705,10 +705,10 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(TreeArg
         sh->ml[x][row] = make_float2(m, l);
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh->ml_full);
-        ok = __all_sync(0xffffffffu, mbar_wait(&sh->ml_full, met & 1, status, 59));
+        ok = __all_sync(0xffffffffu, tree_wait(&sh->ml_full, met & 1, status, 59));
         // (the other stream has seen its last product end before it arrived there: this returns at once)
         if (ok && (x == 1 || tiles > 1))
-          ok = __all_sync(0xffffffffu, mbar_wait(&sh->pv_done[1 - x][buffer_of(other_n - 1)], phase_of(other_n - 1), status, 58));
+          ok = __all_sync(0xffffffffu, tree_wait(&sh->pv_done[1 - x][buffer_of(other_n - 1)], phase_of(other_n - 1), status, 58));
         if (!ok) break;
         tc_fence_after();
         const float2 one = sh->ml[0][row], two = sh->ml[1][row];
@@ -763,7 +763,7 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(TreeArg
       if (merged) {   // both have read both accumulators (and sums) before either stream's next product
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh->o_read);
-        ok = __all_sync(0xffffffffu, mbar_wait(&sh->o_read, met++ & 1, status, 60));
+        ok = __all_sync(0xffffffffu, tree_wait(&sh->o_read, met++ & 1, status, 60));
         if (!ok) break;
       }
     }

@@ -188,6 +188,24 @@ __device__ __forceinline__ Partials partials_of(const TreeArgs& a, const LineSha
   return p;
 }
 
+// Bounded wait on a phase parity, as mbar_wait, that gives up for a wait that ran out and for nothing else: what a call
+// reports about its data stays in the status word until it is read, and the next calls are right all the same.
+__device__ __forceinline__ bool tree_wait(uint64_t* bar, uint32_t parity, uint32_t* status, uint32_t site) {
+  if (mbar_test(bar, parity)) return true;
+  const uint64_t start = global_timer_ns();
+  uint32_t spins = 0;
+  while (!mbar_test(bar, parity)) {
+    if ((++spins & 0x3ffu) == 0) {
+      if ((*reinterpret_cast<volatile uint32_t*>(status) & 0xffu) == kWaitTimeout) return false;   // someone else gave up
+      if (global_timer_ns() - start > kWaitLimitNs) {
+        atomicExch(status, (site << 8) | kWaitTimeout);
+        return false;
+      }
+    }
+  }
+  return true;
+}
+
 // ---- output ------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   uint32_t r;

@@ -188,6 +188,24 @@ def test_a_captured_speculative_step():
     assert _capi.kernel_status() == 0
 
 
+def test_a_report_that_nobody_has_read_does_not_touch_later_calls():
+    """A bad draft is reported; the attention calls behind it are those of a healthy status word."""
+    gen, rnd = random(6)
+    calls = []
+    for nodes, hq, hkv, dim, store in ((61, 40, 8, 128, EIGHT), (40, 24, 4, 256, torch.bfloat16), (1, 40, 8, 128, EIGHT), (30, 12, 12, 64, torch.bfloat16)):
+        q, at = rnd(4, nodes, hq, dim).bfloat16(), torch.tensor([9000, 100, 8000, 4000], **INT)
+        rows = [rnd(4, 9100, hkv, dim).to(store) for _ in range(2)]
+        scales = [torch.full((4, 9100, hkv), 127, dtype=torch.uint8, device="cuda") if store == EIGHT else None for _ in range(2)]
+        calls.append(lambda q=q, r=rows, s=scales, at=at: gqa_tree_decode(q, r[0], r[1], at, 9000, k_scales=s[0], v_scales=s[1]))
+    want = [call() for call in calls]
+    assert _capi.kernel_status() == 0
+    verify_drafts(torch.full((1, 2, 4), 0.25, device="cuda"), torch.full((1, 1), 7, **INT), torch.zeros(1, 1, device="cuda"), torch.zeros(1, device="cuda"))
+    for _ in range(20):
+        for call, clean in zip(calls, want):
+            assert torch.equal(call(), clean)
+    assert _capi.kernel_status() & 0xff == 5 and _capi.kernel_status() == 0
+
+
 def test_tensors_elsewhere_are_refused():
     k = torch.zeros(2, 16, 2, 64, dtype=EIGHT, device="cuda")
     s = torch.zeros(2, 16, 2, dtype=torch.uint8, device="cuda")
