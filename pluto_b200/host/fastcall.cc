@@ -9,6 +9,7 @@
 #include <Python.h>
 
 #include <cstdint>
+#include <cstdio>
 #include <tuple>
 #include <type_traits>
 #include <utility>
@@ -88,16 +89,166 @@ PyObject* kv_cache(PyObject*, PyObject* const* args, Py_ssize_t count) {
   return PyBytes_FromStringAndSize(reinterpret_cast<const char*>(&c), sizeof(c));
 }
 
-// kv_scales(k, v, page_stride, token_stride) -> bytes: struct pluto_kv_scales.
-PyObject* kv_scales(PyObject*, PyObject* const* args, Py_ssize_t count) {
-  if (count != 4) {
-    PyErr_SetString(PyExc_TypeError, "kv_scales takes 4 arguments");
+// ---- tensors, by the attributes that a Python caller would ask for ---------------------------------------------
+struct Names {
+  PyObject *shape, *stride, *dtype, *data_ptr, *get_device, *is_contiguous, *element_size;
+};
+Names names;
+PyObject* refusal;    // class of the error: (code name, message, code)
+PyObject* dtypes[4];  // fp32, bf16, E4M3, int32
+constexpr int kInt32 = 3;
+
+// bind_tensors(error class, fp32, bf16, E4M3, int32): the objects that the functions below compare with and raise.
+PyObject* bind_tensors(PyObject*, PyObject* const* args, Py_ssize_t count) {
+  if (count != 5) {
+    PyErr_SetString(PyExc_TypeError, "bind_tensors takes 5 arguments");
     return nullptr;
   }
-  pluto_kv_scales s = {};
-  if (!convert(args[0], s.k) || !convert(args[1], s.v) || !convert(args[2], s.page_stride) || !convert(args[3], s.token_stride))
+  names = {PyUnicode_InternFromString("shape"), PyUnicode_InternFromString("stride"), PyUnicode_InternFromString("dtype"),
+           PyUnicode_InternFromString("data_ptr"), PyUnicode_InternFromString("get_device"), PyUnicode_InternFromString("is_contiguous"),
+           PyUnicode_InternFromString("element_size")};
+  for (int i = 0; i < 5; ++i) Py_INCREF(args[i]);
+  refusal = args[0];
+  for (int i = 0; i < 4; ++i) dtypes[i] = args[1 + i];
+  Py_RETURN_NONE;
+}
+
+bool refuse(const char* message) {   // false, with the error set
+  if (PyErr_Occurred()) return false;
+  if (PyObject* e = PyObject_CallFunction(refusal, "ssi", "InvalidArgument", message, -1)) {
+    PyErr_SetObject(refusal, e);
+    Py_DECREF(e);
+  }
+  return false;
+}
+
+struct Sizes {
+  Py_ssize_t rank;
+  long long n[4];
+  bool operator==(const Sizes& o) const {
+    if (rank != o.rank) return false;
+    for (Py_ssize_t i = 0; i < rank && i < 4; ++i)
+      if (n[i] != o.n[i]) return false;
+    return true;
+  }
+};
+bool take_sizes(PyObject* tuple, Sizes& out) {   // takes the reference; at most four dimensions are kept
+  if (tuple == nullptr) return false;
+  out.rank = PyTuple_Check(tuple) ? PyTuple_GET_SIZE(tuple) : 0;
+  for (Py_ssize_t i = 0; i < out.rank && i < 4; ++i) out.n[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(tuple, i));
+  Py_DECREF(tuple);
+  return !PyErr_Occurred();
+}
+bool shape_of(PyObject* t, Sizes& out) { return take_sizes(PyObject_GetAttr(t, names.shape), out); }
+bool strides_of(PyObject* t, Sizes& out) { return take_sizes(PyObject_CallMethodNoArgs(t, names.stride), out); }
+long long number_of(PyObject* t, PyObject* method) {   // -2 with an error set
+  PyObject* v = PyObject_CallMethodNoArgs(t, method);
+  if (v == nullptr) return -2;
+  const long long n = PyLong_AsLongLong(v);
+  Py_DECREF(v);
+  return PyErr_Occurred() ? -2 : n;
+}
+template <typename T>
+bool address_of(PyObject* t, T*& out) {
+  PyObject* v = PyObject_CallMethodNoArgs(t, names.data_ptr);
+  if (v == nullptr) return false;
+  out = reinterpret_cast<T*>(static_cast<uintptr_t>(PyLong_AsUnsignedLongLong(v)));
+  Py_DECREF(v);
+  return !PyErr_Occurred();
+}
+int dtype_of(PyObject* t) {   // index into dtypes, -1 for others, -2 with an error set
+  PyObject* d = PyObject_GetAttr(t, names.dtype);
+  if (d == nullptr) return -2;
+  Py_DECREF(d);   // (torch keeps its dtypes alive)
+  for (int i = 0; i < 4; ++i)
+    if (d == dtypes[i]) return i;
+  return -1;
+}
+// A contiguous int32 tensor of the given shape on the device; its address.
+bool int32_of(PyObject* t, const Sizes& want, long long device, const char* what, const int32_t*& out) {
+  Sizes shape;
+  if (dtype_of(t) == kInt32 && shape_of(t, shape) && shape == want && number_of(t, names.get_device) == device && number_of(t, names.is_contiguous) == 1)
+    return address_of(t, out);
+  char message[160];
+  if (want.rank == 1) snprintf(message, sizeof(message), "%s must be a contiguous int32 tensor of shape [%lld] on the current device", what, want.n[0]);
+  else snprintf(message, sizeof(message), "%s must be a contiguous int32 tensor of shape [%lld, %lld] on the current device", what, want.n[0], want.n[1]);
+  return refuse(message);
+}
+
+// int32_address(t, device, what, n0[, n1]) -> address of an optional contiguous int32 tensor of that shape, or None.
+PyObject* int32_address(PyObject*, PyObject* const* args, Py_ssize_t count) {
+  if (count != 4 && count != 5) {
+    PyErr_SetString(PyExc_TypeError, "int32_address takes 4 or 5 arguments");
     return nullptr;
-  return PyBytes_FromStringAndSize(reinterpret_cast<const char*>(&s), sizeof(s));
+  }
+  if (args[0] == Py_None) Py_RETURN_NONE;
+  Sizes want{count - 3, {}};
+  long long device;
+  if (!convert(args[1], device) || !convert(args[3], want.n[0]) || (count == 5 && !convert(args[4], want.n[1]))) return nullptr;
+  const char* what = PyUnicode_AsUTF8(args[2]);
+  const int32_t* out;
+  if (what == nullptr || !int32_of(args[0], want, device, what, out)) return nullptr;
+  return PyLong_FromVoidPtr(const_cast<int32_t*>(out));
+}
+
+bool fill_draft_pool(PyObject* const* args, pluto_kv_cache& c, pluto_kv_scales& s) {
+  PyObject *k = args[0], *v = args[1], *table = args[2];
+  long long batch, device;
+  if (!convert(args[5], batch) || !convert(args[6], device)) return false;
+  const int code = dtype_of(k);
+  if (code < 0 || code > PLUTO_E4M3 || dtype_of(v) != code) return refuse("a cache pool stores fp32, bf16 or E4M3");
+  Sizes shape, other, strides, other_strides;
+  if (!shape_of(k, shape) || !shape_of(v, other) || !strides_of(k, strides) || !strides_of(v, other_strides)) return false;
+  if (shape.rank != 4 || !(other == shape) || !(other_strides == strides) || strides.n[3] != 1 || strides.n[2] != shape.n[3])
+    return refuse("cache pools are [pages, page_size, kv_heads, head_dim] of one shape, heads contiguous");
+  if (number_of(k, names.get_device) != device || number_of(v, names.get_device) != device) return refuse("the cache is not on the current device");
+  c.dtype = code;
+  if (shape.n[0] > INT32_MAX || shape.n[1] > INT32_MAX) return refuse("cache pools have at most 2^31 - 1 pages of as many slots");
+  c.num_pages = static_cast<int>(shape.n[0]);
+  c.page_size = static_cast<int>(shape.n[1]);
+  c.page_stride = static_cast<size_t>(strides.n[0]);
+  c.token_stride = static_cast<size_t>(strides.n[1]);
+  if (!address_of(k, c.k_base) || !address_of(v, c.v_base)) return false;
+  if (table == Py_None) {
+    if (shape.n[0] < batch) return refuse("a cache without a block table has a page for every sequence");
+  } else {
+    Sizes blocks;
+    if (!shape_of(table, blocks)) return false;
+    if (blocks.rank != 2 || blocks.n[1] > INT32_MAX) return refuse("a block table is [batch, blocks]");
+    if (!int32_of(table, Sizes{2, {batch, blocks.n[1]}}, device, "block table", c.block_table)) return false;
+    c.max_blocks = static_cast<int>(blocks.n[1]);
+  }
+  if ((code == PLUTO_E4M3) != (args[3] != Py_None) || (code == PLUTO_E4M3) != (args[4] != Py_None))
+    return refuse("an 8-bit cache needs its scales, and only that");
+  if (code != PLUTO_E4M3) return true;
+  const Sizes rows{3, {shape.n[0], shape.n[1], shape.n[2]}};
+  uint8_t** bases[2] = {&s.k, &s.v};
+  for (int side = 0; side < 2; ++side) {
+    PyObject* t = args[3 + side];
+    if (!shape_of(t, other) || !strides_of(t, side ? other_strides : strides)) return false;
+    if (!(other == rows) || number_of(t, names.element_size) != 1 || number_of(t, names.get_device) != device ||
+        (side ? !(other_strides == strides) : strides.n[2] != 1 && shape.n[2] != 1))
+      return refuse("cache scales are one byte each, [pages, page_size, kv_heads], heads contiguous");
+    if (!address_of(t, *bases[side])) return false;
+  }
+  s.page_stride = static_cast<size_t>(strides.n[0]);
+  s.token_stride = static_cast<size_t>(strides.n[1]);
+  return true;
+}
+
+// draft_pool(k_pool, v_pool, block_table, k_scales, v_scales, batch, device) -> (bytes of struct pluto_kv_cache, bytes of
+// struct pluto_kv_scales or None): the pool that the functions of drafted tokens take, after every check of its tensors.
+PyObject* draft_pool(PyObject*, PyObject* const* args, Py_ssize_t count) {
+  if (count != 7) {
+    PyErr_SetString(PyExc_TypeError, "draft_pool takes 7 arguments");
+    return nullptr;
+  }
+  pluto_kv_cache c = {};
+  pluto_kv_scales s = {};
+  if (!fill_draft_pool(args, c, s)) return nullptr;
+  return c.dtype != PLUTO_E4M3 ? Py_BuildValue("y#O", reinterpret_cast<const char*>(&c), static_cast<Py_ssize_t>(sizeof(c)), Py_None)
+                               : Py_BuildValue("y#y#", reinterpret_cast<const char*>(&c), static_cast<Py_ssize_t>(sizeof(c)),
+                                               reinterpret_cast<const char*>(&s), static_cast<Py_ssize_t>(sizeof(s)));
 }
 
 template <auto Function>
@@ -154,7 +305,9 @@ PyMethodDef methods[] = {
     ENTRY(pluto_block_linear_workspace_bytes),
     ENTRY(pluto_dequantize_matrix),
     {"kv_cache", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&kv_cache)), METH_FASTCALL, nullptr},
-    {"kv_scales", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&kv_scales)), METH_FASTCALL, nullptr},
+    {"bind_tensors", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&bind_tensors)), METH_FASTCALL, nullptr},
+    {"int32_address", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&int32_address)), METH_FASTCALL, nullptr},
+    {"draft_pool", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&draft_pool)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fastcall", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

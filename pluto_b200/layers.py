@@ -696,53 +696,21 @@ class DraftVerdict(NamedTuple):
     tokens: torch.Tensor     # [B, N + 1] its tokens, the drawn token, then -1
 
 
-_STORAGE = {torch.float32: 0, torch.bfloat16: 1, torch.float8_e4m3fn: 2}
+_tensor_calls = None
 
 
-def _draft_pool(k_pool, v_pool, block_table, k_scales, v_scales, batch, device):
-    """struct pluto_kv_cache and struct pluto_kv_scales of a page pool of any storage type, as bytes."""
-    code, shape, strides = _STORAGE.get(k_pool.dtype), k_pool.shape, k_pool.stride()
-    if code is None or v_pool.dtype != k_pool.dtype:
-        raise _invalid("a cache pool stores fp32, bf16 or E4M3")
-    if len(shape) != 4 or v_pool.shape != shape or v_pool.stride() != strides or strides[3] != 1 or strides[2] != shape[3]:
-        raise _invalid("cache pools are [pages, page_size, kv_heads, head_dim] of one shape, heads contiguous")
-    if k_pool.get_device() != device or v_pool.get_device() != device:
-        raise _invalid("the cache is not on the current device")
-    table, blocks = None, 0
-    if block_table is None:
-        if shape[0] < batch:
-            raise _invalid("a cache without a block table has a page for every sequence")
-    else:
-        blocks = block_table.shape[-1]
-        _check_ints(block_table, (batch, blocks), "block table", device)
-        table = block_table.data_ptr()
-    L = _capi.fast()
-    cache = L.kv_cache(k_pool.data_ptr(), v_pool.data_ptr(), table, blocks, shape[1], strides[0], strides[1], code, shape[0])
-    if code != 2:
-        if k_scales is not None or v_scales is not None:
-            raise _invalid("an 8-bit cache needs its scales, and only that")
-        return cache, None
-    if k_scales is None or v_scales is None:
-        raise _invalid("an 8-bit cache needs its scales, and only that")
-    strides = k_scales.stride()
-    if (k_scales.shape != shape[:3] or v_scales.shape != shape[:3] or v_scales.stride() != strides
-            or (strides[2] != 1 and shape[2] != 1) or k_scales.element_size() != 1 or v_scales.element_size() != 1
-            or k_scales.get_device() != device or v_scales.get_device() != device):
-        raise _invalid("cache scales are one byte each, [pages, page_size, kv_heads], heads contiguous")
-    return cache, L.kv_scales(k_scales.data_ptr(), v_scales.data_ptr(), strides[0], strides[1])
+def _draft_calls():
+    """The vectorcall binding, with the objects that its checks of tensors compare with and raise."""
+    global _tensor_calls
+    if _tensor_calls is None:
+        calls = _capi.fast()
+        calls.bind_tensors(PlutoStatusError, torch.float32, torch.bfloat16, torch.float8_e4m3fn, torch.int32)
+        _tensor_calls = calls
+    return _tensor_calls
 
 
 def _device_index() -> int:
     return torch.cuda.current_device() if _current_device is None else _current_device()
-
-
-def _check_ints(t, shape, what: str, device: int) -> Optional[int]:
-    """The address of an optional int32 argument."""
-    if t is None:
-        return None
-    if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous() or t.get_device() != device:
-        raise _invalid(f"{what} must be a contiguous int32 tensor of shape {list(shape)} on the current device")
-    return t.data_ptr()
 
 
 def _check_rows(t, shape, what: str, device: int):
@@ -768,14 +736,15 @@ def kv8_append(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor, v_pool: t
     pool [pages, page_size, Hkv, D] (float8_e4m3fn) with scales [pages, page_size, Hkv] (one byte each); with
     `counts` int32 [B] only the first counts[b] tokens of sequence b."""
     (B, T, H, D), device = k.shape, _device_index()
-    cache, scales = _draft_pool(k_pool, v_pool, block_table, k_scales, v_scales, B, device)
+    L = _draft_calls()
+    cache, scales = L.draft_pool(k_pool, v_pool, block_table, k_scales, v_scales, B, device)
     if k.stride(3) != 1 or k.stride() != v.stride():
         k, v = k.contiguous(), v.contiguous()
     strides = _check_rows(k, (B, T, H, D), "cache rows", device)
     if v.shape != k.shape or v.dtype != k.dtype or v.get_device() != device or k_pool.shape[2:] != (H, D):
         raise _invalid("8-bit cache rows do not match the pool")
-    check(_capi.fast().pluto_kv8_append(_stream(), k.data_ptr(), v.data_ptr(), _dt(k), strides[0], strides[1], strides[2], cache, scales,
-                                        _check_ints(positions, (B,), "positions", device), _check_ints(counts, (B,), "counts", device),
+    check(L.pluto_kv8_append(_stream(), k.data_ptr(), v.data_ptr(), _dt(k), strides[0], strides[1], strides[2], cache, scales,
+                                        L.int32_address(positions, device, "positions", B), L.int32_address(counts, device, "counts", B),
                                         B, T, H, D))
 
 
@@ -785,12 +754,13 @@ def kv8_read(k_pool: torch.Tensor, v_pool: torch.Tensor, k_scales: torch.Tensor,
     """(k, v) [B,tokens,Hkv,D]: the values that the slots positions[b] .. positions[b] + tokens - 1 of an 8-bit
     pool hold (exact in bf16); with `counts` the rows from counts[b] on are zero."""
     B, device = positions.shape[0], _device_index()
-    cache, scales = _draft_pool(k_pool, v_pool, block_table, k_scales, v_scales, B, device)
+    L = _draft_calls()
+    cache, scales = L.draft_pool(k_pool, v_pool, block_table, k_scales, v_scales, B, device)
     _, _, H, D = k_pool.shape
     k = k_pool.new_empty((B, tokens, H, D), dtype=dtype) if counts is None else k_pool.new_zeros((B, tokens, H, D), dtype=dtype)
     v = torch.empty_like(k) if counts is None else torch.zeros_like(k)
-    check(_capi.fast().pluto_kv8_read(_stream(), k.data_ptr(), v.data_ptr(), _dt(k), tokens * H * D, H * D, D, cache, scales,
-                                      _check_ints(positions, (B,), "positions", device), _check_ints(counts, (B,), "counts", device),
+    check(L.pluto_kv8_read(_stream(), k.data_ptr(), v.data_ptr(), _dt(k), tokens * H * D, H * D, D, cache, scales,
+                                      L.int32_address(positions, device, "positions", B), L.int32_address(counts, device, "counts", B),
                                       B, tokens, H, D))
     return k, v
 
@@ -802,9 +772,10 @@ def kv_keep(k_pool: torch.Tensor, v_pool: torch.Tensor, prefix_lens: torch.Tenso
     prefix_lens[b] + i, in place, for i < accepted[b]; every other slot keeps its rows.  The caller then adds
     `accepted` to its lengths.  path int32 [B,N], accepted int32 [B], as verify_drafts returns them."""
     (B, N), device = path.shape, _device_index()
-    cache, scales = _draft_pool(k_pool, v_pool, block_table, k_scales, v_scales, B, device)
-    check(_capi.fast().pluto_kv_keep(_stream(), cache, scales, _check_ints(prefix_lens, (B,), "prefix lengths", device),
-                                     _check_ints(path, (B, N), "path", device), _check_ints(accepted, (B,), "accepted", device), B, N,
+    L = _draft_calls()
+    cache, scales = L.draft_pool(k_pool, v_pool, block_table, k_scales, v_scales, B, device)
+    check(L.pluto_kv_keep(_stream(), cache, scales, L.int32_address(prefix_lens, device, "prefix lengths", B),
+                                     L.int32_address(path, device, "path", B, N), L.int32_address(accepted, device, "accepted", B), B, N,
                                      k_pool.shape[2], k_pool.shape[3]))
 
 
@@ -819,7 +790,8 @@ def draft_prepare(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_norm: tor
     rows go to slot prefix_lens[b] + i of a pool of any storage type.  Returns the queries [B,N,Hq,D], bf16
     when round_to_bfloat16 and fp32 otherwise.  Without `parents` (a chain, or a whole prompt) any N."""
     (B, N, Hq, D), device = q.shape, _device_index()
-    cache, scales = _draft_pool(k_pool, v_pool, block_table, k_scales, v_scales, B, device)
+    L = _draft_calls()
+    cache, scales = L.draft_pool(k_pool, v_pool, block_table, k_scales, v_scales, B, device)
     Hkv = k_pool.shape[2]
     strides = _check_rows(q, (B, N, Hq, k_pool.shape[3]), "drafted queries", device)
     if B > 1 and strides[0] != N * strides[1]:
@@ -833,10 +805,10 @@ def draft_prepare(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_norm: tor
         if norm.dtype != torch.float32 or norm.numel() != D or norm.get_device() != device or not norm.is_contiguous():
             raise _invalid("Qwen attention norms must be FP32 head-width parameters on its Executor")
     out = torch.empty((B, N, Hq, D), dtype=torch.bfloat16 if round_to_bfloat16 else torch.float32, device=q.device)
-    check(_capi.fast().pluto_draft_prepare(
+    check(L.pluto_draft_prepare(
         _stream(), q.data_ptr(), k.data_ptr(), v.data_ptr(), _dt(q), strides[1], strides[2], q_norm.data_ptr(), k_norm.data_ptr(),
-        _check_ints(prefix_lens, (B,), "prefix lengths", device), _check_ints(parents, (B, N), "parents", device),
-        _check_ints(counts, (B,), "counts", device), out.data_ptr(), _dt(out), cache, scales, B, N, Hq, Hkv, D, rotary_dim,
+        L.int32_address(prefix_lens, device, "prefix lengths", B), L.int32_address(parents, device, "parents", B, N),
+        L.int32_address(counts, device, "counts", B), out.data_ptr(), _dt(out), cache, scales, B, N, Hq, Hkv, D, rotary_dim,
         rms_norm_epsilon, rope_theta, int(round_to_bfloat16)))
     return out
 
@@ -853,7 +825,8 @@ def gqa_tree_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     sequence has that many nodes; the rows of the others are left as they were (zeros without `out`).  One
     node per sequence is gqa_decode.  Returns out [B,N,Hq,D] (and lse [B,N,Hq])."""
     (B, N, Hq, D), device = q.shape, _device_index()
-    cache, scales = _draft_pool(k_pool, v_pool, block_table, k_scales, v_scales, B, device)
+    L = _draft_calls()
+    cache, scales = L.draft_pool(k_pool, v_pool, block_table, k_scales, v_scales, B, device)
     Hkv = k_pool.shape[2]
     _check_rows(q, (B, N, Hq, k_pool.shape[3]), "drafted queries", device)
     if not q.is_contiguous():
@@ -870,14 +843,13 @@ def gqa_tree_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
         if B > 1 and strides[0] != N * strides[1]:
             raise _invalid("attention gate must have a contiguous head dimension and batch")
         gate_at, gate_type, gts, ghs = gate.data_ptr(), _dt(gate), strides[1], strides[2]
-    L = _capi.fast()
     if workspace is None:
         workspace = _call_scratch(q.device, L.pluto_gqa_tree_decode_workspace_bytes(B, N, Hq, Hkv, D))
     elif workspace.get_device() != device or not workspace.is_contiguous():
         raise _invalid("the workspace must be contiguous, on the current device")
     check(L.pluto_gqa_tree_decode(_stream(), q.data_ptr(), _dt(q), gate_at, gate_type, gts, ghs, cache, scales,
-                                  _check_ints(prefix_lens, (B,), "prefix lengths", device), max_prefix_len,
-                                  _check_ints(parents, (B, N), "parents", device), _check_ints(counts, (B,), "counts", device),
+                                  L.int32_address(prefix_lens, device, "prefix lengths", B), max_prefix_len,
+                                  L.int32_address(parents, device, "parents", B, N), L.int32_address(counts, device, "counts", B),
                                   out.data_ptr(), _dt(out), _ptr(lse), workspace.data_ptr(), workspace.numel() * workspace.element_size(),
                                   B, N, Hq, Hkv, D, int(round_to_bfloat16)))
     return (out, lse) if want_lse else out
@@ -907,11 +879,12 @@ def verify_drafts(target_probs: torch.Tensor, tokens: torch.Tensor, accept_unifo
             raise _invalid("uniform numbers must be fp32 [batch, nodes] and [batch], contiguous")
     if target_probs.get_device() != device:
         raise _invalid("target probabilities are not on the current device")
-    at = _check_ints(tokens, (B, N), "drafted tokens", device)
+    L = _draft_calls()
+    at = L.int32_address(tokens, device, "drafted tokens", B, N)
     accepted, path, out = tokens.new_empty(B), torch.empty_like(tokens), tokens.new_empty((B, N + 1))
-    check(_capi.fast().pluto_verify_drafts(
+    check(L.pluto_verify_drafts(
         _stream(), target_probs.data_ptr(), _ptr(draft_probs), _dt(target_probs), at, accept_uniforms.data_ptr(),
-        sample_uniforms.data_ptr(), _check_ints(parents, (B, N), "parents", device), _check_ints(counts, (B,), "counts", device),
+        sample_uniforms.data_ptr(), L.int32_address(parents, device, "parents", B, N), L.int32_address(counts, device, "counts", B),
         accepted.data_ptr(), path.data_ptr(), out.data_ptr(), B, N, V))
     return DraftVerdict(accepted, path, out)
 
