@@ -382,8 +382,9 @@ int pluto_cached_attention_step(pluto_stream_t stream, const void* q_gate, const
  * elements) and one scale byte per (token, head) row in `scales`, at element
  *     page * page_stride + (t % page_size) * token_stride + head        (strides of pluto_kv_scales)
  * A row x is stored with the smallest n >= -127 for which max|x| <= 448 * 2^n: scale byte n + 127 (E8M0), codes
- * the E4M3 values nearest to x * 2^-n (ties to even).  Every value read back is exact in bf16.  A row that
- * holds an infinity or a NaN gets scale byte 255 and reads back as NaN.  `scales` is NULL for the other two. */
+ * the E4M3 values nearest to x * 2^-n (ties to even).  Every value read back is exact in bf16 (one that rounds to 2^128
+ * reads back as infinity).  A row that holds an infinity or a NaN gets scale byte 255 and reads back as NaN.
+ * `scales` is NULL for the other two. */
 enum { PLUTO_E4M3 = 2 };
 typedef struct pluto_kv_scales {
   uint8_t* k; /* device; the attention reads scale bytes by the aligned 4-byte word they lie in */

@@ -86,6 +86,28 @@ def test_rows_that_are_not_finite_in_the_prefix(store, nodes, hq, hkv, dim):
     assert _capi.kernel_status() == 0
 
 
+@pytest.mark.parametrize("kind", ["fp32", "odd", "slice"])
+@pytest.mark.parametrize("nodes,hq,hkv,dim", SHAPES)
+def test_gates_of_other_types_and_strides(nodes, hq, hkv, dim, kind):
+    gen, rnd = random(nodes)
+    k, v, q = rnd(2, 150, hkv, dim).bfloat16(), rnd(2, 150, hkv, dim).bfloat16(), rnd(2, nodes, hq, dim).bfloat16()
+    if kind == "fp32":
+        gate = rnd(2, nodes, hq, dim)
+    elif kind == "odd":
+        gate = rnd(2, nodes, hq, dim + 1).bfloat16()[..., 1:]
+    else:
+        gate = rnd(2, nodes, hq + 3, 2, dim).bfloat16()[:, :, 2:hq + 2, 1]
+    at = torch.tensor([150 - nodes, 11], **INT)
+    got = gqa_tree_decode(q, k, v, at, 150, gate=gate, round_to_bfloat16=False)
+    for b in range(2):
+        n = int(at[b])
+        want, mean, _ = tree_attention(q[b].double(), k[b, :n + nodes].double(), v[b, :n + nodes].double(), n, list(range(-1, nodes - 1)))
+        factor = torch.sigmoid(gate[b].double())
+        # weights rounded to bf16 (2^-8 of a mean of |v|) or better, the result rounded once
+        assert ((got[b].double() - want * factor).abs() <= (mean * 2.0 ** -8 * (1 + 2.0 ** -7) + 2.0 ** -8 * 1.01 * want.abs()) * factor + 1e-6).all()
+    assert _capi.kernel_status() == 0
+
+
 @pytest.mark.parametrize("nodes,dim,hkv,group", [(1, 64, 72, 1), (2, 128, 65, 2), (1, 128, 64, 1), (2, 64, 3, 2), (1, 256, 5, 3), (9, 64, 70, 1)])
 def test_many_and_odd_numbers_of_kv_heads(nodes, dim, hkv, group):
     """Heads side by side and one after the other; 8-bit scales at odd addresses."""
