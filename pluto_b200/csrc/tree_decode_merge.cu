@@ -108,6 +108,37 @@ __global__ void __launch_bounds__(kWarps * 32) tree_decode_merge_kernel(TreeArgs
 
 }  // namespace
 
+bool tree_pool_fits(const TreeArgs& a, int tokens) {
+  const size_t element = a.pool.store == kStoreBf16 ? 2 : 1;
+  return (a.pool.table == nullptr || a.pool.max_blocks == 1 || a.pool.page_size % tokens == 0) &&
+         a.pool.page_stride * element < (1ull << 40) && a.pool.token_stride * element < (1ull << 40);
+}
+
+bool tree_pool_map(CUtensorMap* map, const void* base, const TreeArgs& a, int tokens, int columns, int swizzle) {
+  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static Encode encode = [] {
+    void* symbol = nullptr;
+    cudaDriverEntryPointQueryResult result;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &symbol, cudaEnableDefault, &result) != cudaSuccess ||
+        result != cudaDriverEntryPointSuccess)
+      return static_cast<Encode>(nullptr);
+    return reinterpret_cast<Encode>(symbol);
+  }();
+  if (encode == nullptr) return false;
+  const bool eight = a.pool.store == kStoreE4m3;
+  const cuuint64_t element = eight ? 1 : 2;
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(a.dim), static_cast<cuuint64_t>(a.kv_heads), static_cast<cuuint64_t>(a.pool.page_size),
+                              static_cast<cuuint64_t>(a.pool.table ? a.pool.num_pages : a.batch)};
+  const cuuint64_t strides[3] = {a.dim * element, a.pool.token_stride * element, a.pool.page_stride * element};
+  const cuuint32_t box[4] = {static_cast<cuuint32_t>(columns), 1, static_cast<cuuint32_t>(tokens), 1}, steps[4] = {1, 1, 1, 1};
+  return encode(map, eight ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box,
+                steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                swizzle == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : swizzle == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 cudaError_t tree_decode_merge(cudaStream_t stream, const TreeArgs& a, const LineShape& shape) {
   const int groups = (a.nodes * a.group + (1 << shape.rows_shift) - 1) >> shape.rows_shift;
   const int rows = slot_rows(shape, a.nodes, a.q_heads, a.kv_heads);

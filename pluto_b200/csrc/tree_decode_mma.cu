@@ -550,32 +550,6 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, kEight>) tree_decode_mma
   }
 }
 
-// 4-D map of a page pool: (column, KV head, token in page, page); a box is sixteen tokens of 128 bytes (64 where a row has
-// no more) of one KV head, swizzled; zeros outside the pool.
-bool make_pool_map(CUtensorMap* map, const void* base, const TreeArgs& a) {
-  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-  static Encode encode = [] {
-    void* symbol = nullptr;
-    cudaDriverEntryPointQueryResult result;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &symbol, cudaEnableDefault, &result) != cudaSuccess ||
-        result != cudaDriverEntryPointSuccess)
-      return static_cast<Encode>(nullptr);
-    return reinterpret_cast<Encode>(symbol);
-  }();
-  if (encode == nullptr) return false;
-  const bool eight = a.pool.store == kStoreE4m3;
-  const cuuint64_t element = eight ? 1 : 2, row = a.dim * element;
-  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(a.dim), static_cast<cuuint64_t>(a.kv_heads), static_cast<cuuint64_t>(a.pool.page_size),
-                              static_cast<cuuint64_t>(a.pool.table ? a.pool.num_pages : a.batch)};
-  const cuuint64_t strides[3] = {row, a.pool.token_stride * element, a.pool.page_stride * element};
-  const cuuint32_t box[4] = {static_cast<cuuint32_t>((row < 128 ? row : 128) / element), 1, kTile, 1}, steps[4] = {1, 1, 1, 1};
-  return encode(map, eight ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box,
-                steps, CU_TENSOR_MAP_INTERLEAVE_NONE, row < 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
-                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <int D, bool kEight>
 LineShape line_shape(const TreeArgs& a) {   // (many heads would leave workers over)
   return {4, 3, 4, 148 * kCtas<D, kEight> * kWarps, a.kv_heads <= 64 ? a.kv_heads : 1};
@@ -587,7 +561,9 @@ cudaError_t launch_rows(cudaStream_t stream, const TreeArgs& a) {
   constexpr int kBytes = kWarps * (kStages<D, kEight> * kStageBytes<D, kEight> + static_cast<int>(sizeof(WarpState<kStages<D, kEight>, kEight>))) + 1024;
   static_assert((kBytes + 1024) * kCtas<D, kEight> <= 228 * 1024, "shared memory");
   CUtensorMap map_k, map_v;
-  if (!make_pool_map(&map_k, a.pool.k, a) || !make_pool_map(&map_v, a.pool.v, a)) return cudaErrorInvalidValue;
+  constexpr int kColumns = (kRowBytes<D, kEight> < 128 ? kRowBytes<D, kEight> : 128) / (kEight ? 1 : 2);
+  if (!tree_pool_map(&map_k, a.pool.k, a, kTile, kColumns, kColumns * (kEight ? 1 : 2)) || !tree_pool_map(&map_v, a.pool.v, a, kTile, kColumns, kColumns * (kEight ? 1 : 2)))
+    return cudaErrorInvalidValue;
   const long long tiles = static_cast<long long>(a.batch) * a.kv_heads * ((static_cast<long long>(a.max_prefix) + a.nodes + kTile - 1) / kTile);
   const long long ctas = (tiles + kWarps - 1) / kWarps, most = 148 * kCtas<D, kEight>;
   cudaError_t e = cudaFuncSetAttribute(tree_decode_mma_kernel<D, kEight, kHalf>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
@@ -606,9 +582,7 @@ cudaError_t launch(cudaStream_t stream, const TreeArgs& a) {
 }  // namespace
 
 bool tree_decode_mma_supported(const TreeArgs& a) {
-  const size_t element = a.pool.store == kStoreBf16 ? 2 : 1;
-  return a.nodes * a.group <= (a.dim == 256 ? 8 : 16) && (a.pool.table == nullptr || a.pool.max_blocks == 1 || a.pool.page_size % kTile == 0) &&
-         a.pool.page_stride * element < (1ull << 40) && a.pool.token_stride * element < (1ull << 40) &&   // (limits of a tensor map)
+  return a.nodes * a.group <= (a.dim == 256 ? 8 : 16) && tree_pool_fits(a, kTile) &&
          a.pool.scale_page < (1ull << 32) && a.pool.scale_token < (1ull << 32) &&
          line_fits(a, {4, 3, 4, 0, 1});
 }

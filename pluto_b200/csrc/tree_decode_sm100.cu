@@ -17,7 +17,8 @@
 // half of TMEM): one stream with two score buffers.
 //
 // Loading.  Four warps copy the rows into a ring with asynchronous 16-byte copies; pages may have any size and rows any
-// 16-byte stride.  bf16 rows land as the swizzled tiles that the products read.  8-bit codes land as they are (up to 96 KB
+// 16-byte stride.  Whole tiles of bf16 rows (and 8-bit ones of width 256) in pages of a multiple of 16 come by tiled copies
+// instead, one lane's work; the tiles with drafts and the last one do not, since what lies behind must be zeros.  bf16 rows land as the swizzled tiles that the products read.  8-bit codes land as they are (up to 96 KB
 // per SM in flight) and eight more warps widen them to fp16 tiles, one instruction per two codes and exact,
 // and multiply them by their row's 2^n where fp16 holds every product (-15 <= n <= 7, values from 2^-24 to 57344);
 // a tile with other rows keeps its codes and the softmax multiplies scores and weights by the rows' factors.  P then
@@ -25,8 +26,8 @@
 //
 // Work is cut evenly over the SMs as tree_line.cuh says, one CTA per SM.
 //
-// Measured (B200, 16 sequences of 8000 tokens, 40 and 8 heads of 128): 40 rows per KV head, bf16 114 us, 4.6 TB/s of
-// cache, 8-bit 135; 100 rows 130 and 147; 305 rows 303 and 402, where the softmax bounds it: one warp's chain of loads,
+// Measured (B200, 16 sequences of 8000 tokens, 40 and 8 heads of 128): 40 rows per KV head, bf16 102 us, 5.1 TB/s of
+// cache, 8-bit 136; 100 rows 114 and 147; 305 rows 300 and 402, where the softmax bounds it: one warp's chain of loads,
 // maxima, exponentials and stores, two such warps per scheduler.
 #include <stddef.h>
 
@@ -52,6 +53,11 @@ constexpr int kRawStages = D == 64 ? 8 : D == 128 ? (kWide ? 3 : 6) : 2;   // ke
 template <int D>
 constexpr int kTileBytes = kTile * D * 2;
 constexpr int group_rows(int dim) { return dim == 256 ? 128 : 256; }   // rows that share one pass over the keys
+
+// Tiled copies where pages allow them: 40 rows of width 128, bf16: 114 -> 102 us; 48 rows of width 256, 8-bit: 78 -> 74.  Narrower
+// 8-bit tiles are no faster by them (135 -> 139): widening bounds those.
+template <int D, bool kEight>
+constexpr bool kBoxes = !kEight || D == 256;
 
 // ---- shared memory -------------------------------------------------------------------------------------------
 constexpr int kSegments = 8;         // of the ring
@@ -122,7 +128,7 @@ __device__ __forceinline__ uint32_t load_byte(const uint8_t* p, bool there) {   
 // scales of its row.  Nothing is used in the step that asks for it: pages are fetched one unit ahead of the
 // copies, scale bytes are passed on one unit later.
 template <int D, bool kEight, bool kWide>
-__device__ __forceinline__ void load_tiles(const TreeArgs& a, Shared<D, kEight, kWide>* sh, uint32_t k_ring, uint32_t v_ring, int warp, int lane) {
+__device__ __forceinline__ void load_tiles(const TreeArgs& a, const CUtensorMap& map_k, const CUtensorMap& map_v, int box, Shared<D, kEight, kWide>* sh, uint32_t k_ring, uint32_t v_ring, int warp, int lane) {
   constexpr int kRing = kEight ? kRawStages<D, kWide> : kStages<D, kEight, kWide>;
   constexpr int kElement = kEight ? 1 : 2, kBytes = kTile * D * kElement, kPieces = D * kElement / 16, kLoads = kPieces;
   uint64_t* k_full = kEight ? sh->raw_k : sh->k_full;
@@ -164,8 +170,13 @@ __device__ __forceinline__ void load_tiles(const TreeArgs& a, Shared<D, kEight, 
     // (few slots: this one, or one that its tile waits for, is freed once the last unit's scales have been passed on)
     if (kEight && kRing <= 3) pass_scales();
     if (use > 0) {
-      if (!__all_sync(0xffffffffu, tree_wait(kEight ? &sh->raw_empty[slot] : &sh->k_empty[slot], (use - 1) & 1, status, 50))) return;
-      if (!kEight && !__all_sync(0xffffffffu, tree_wait(&sh->v_empty[slot], (use - 1) & 1, status, 51))) return;
+      bool ok = __all_sync(0xffffffffu, tree_wait(kEight ? &sh->raw_empty[slot] : &sh->k_empty[slot], (use - 1) & 1, status, 50));
+      if (!kEight) ok = ok && __all_sync(0xffffffffu, tree_wait(&sh->v_empty[slot], (use - 1) & 1, status, 51));
+      if (!ok) {   // the copies in flight land (or a limit of tries passes) before their memory is given up
+        for (int m = n - 2; m >= 0 && m > n - kRing; m -= 2)
+          for (int tries = 0; tries < (1 << 16) && !(mbar_test(&k_full[m % kRing], m / kRing & 1) && mbar_test(&v_full[m % kRing], m / kRing & 1)); ++tries) {}
+        return;
+      }
     }
     if (!more) {   // the range ends, for the widening warps of this half and parity as well
       if (first_row == 0 && lane == 0) sh->draft_row[slot] = -1;
@@ -186,8 +197,36 @@ __device__ __forceinline__ void load_tiles(const TreeArgs& a, Shared<D, kEight, 
         if (kEight) scale_at = static_cast<size_t>(page) * a.pool.scale_page + static_cast<size_t>(inside) * a.pool.scale_token + seg.kv_head;
       }
     }
+    // A tile before the drafts, in pages that boxes divide, comes by tiled copies of one lane.  (Rows behind the last
+    // draft must be zeros, which the lanes' own copies write.)
+    const bool whole = kBoxes<D, kEight> && box > 0 && (tile + 1) * kTile <= seg.prefix;
+    if (whole) {
+      const int inside = t - (page_shift >= 0 ? t >> page_shift << page_shift : t / a.pool.page_size * a.pool.page_size);
+      const unsigned pages = a.pool.table ? a.pool.num_pages : a.batch;
+      const int from = static_cast<unsigned>(page) < pages ? page : -1;   // (reported above; zeros)
+      constexpr int kSlabs = kEight ? 1 : D / 64, kSlab = kTile * 128;
+      if (lane == 0) {
+        mbar_expect_tx(&k_full[slot], kBytes / 2);
+        mbar_expect_tx(&v_full[slot], kBytes / 2);
+      } else {
+        mbar_arrive(&k_full[slot]);
+        mbar_arrive(&v_full[slot]);
+      }
+      for (int r0 = 0; r0 < 32; r0 += box) {
+        const int box_page = __shfl_sync(0xffffffffu, from, r0), box_inside = __shfl_sync(0xffffffffu, inside, r0);
+        if (lane == 0) {
 #pragma unroll
-    for (int side = 0; side < 2; ++side) {
+          for (int i = 0; i < kSlabs; ++i) {
+            const uint32_t at = slot * kBytes + i * kSlab + (first_row + r0) * (kEight ? D : 128);
+            tma_load_4d_at(k_ring + at, &map_k, i * 64, seg.kv_head, box_inside, box_page, &k_full[slot]);
+            tma_load_4d_at(v_ring + at, &map_v, i * 64, seg.kv_head, box_inside, box_page, &v_full[slot]);
+          }
+        }
+      }
+      __syncwarp();
+    }
+#pragma unroll
+    for (int side = 0; side < 2 && !whole; ++side) {
       const uint32_t to = (side ? v_ring : k_ring) + slot * kBytes;
       const char* base = static_cast<const char*>(side ? a.pool.v : a.pool.k);
 #pragma unroll 4
@@ -198,7 +237,7 @@ __device__ __forceinline__ void load_tiles(const TreeArgs& a, Shared<D, kEight, 
       }
       if (kEight || draft_row >= first_row + 32) arrive_behind_copies(side ? &v_full[slot] : &k_full[slot]);
     }
-    if (!kEight && draft_row < first_row + 32) {
+    if (!kEight && !whole && draft_row < first_row + 32) {
       // Drafts that not every node sees: a value row that is not finite must not meet the zero weights of those that do
       // not see it.  It becomes zeros, and the key row NaN, which gives those that see it NaN scores and touches no
       // other node.  (8-bit rows: their scale byte says so, when they are widened.)  A lane looks at its own copies.
@@ -318,7 +357,7 @@ template <int D, bool kWide>
 constexpr int kQueryBytes = kWide ? 128 * D * 2 : 0;   // of a stream, in shared memory
 
 template <int D, bool kEight, bool kWide>
-__global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(TreeArgs a, LineShape shape) {
+__global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, int box, TreeArgs a, LineShape shape) {
   constexpr bool kOneO = D == 256;                       // one stream
   constexpr int kBuffers = kOneO || kWide ? 2 : 1;       // of scores, per stream
   constexpr uint32_t kColO1 = D, kColS = kOneO ? D : 2 * D, kColQ = kColS + (kOneO ? 1 : 2) * kBuffers * kTile;   // (kWide: the queries lie in shared memory)
@@ -771,7 +810,7 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(TreeArg
     // ------------------------------------------------------------------ loads, widening
     if (warp < 16) {
       if (kEight) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-      load_tiles<D, kEight, kWide>(a, sh, kEight ? raw_k : k_ring, kEight ? raw_v : v_ring, warp - 12, lane);
+      load_tiles<D, kEight, kWide>(a, map_k, map_v, box, sh, kEight ? raw_k : k_ring, kEight ? raw_v : v_ring, warp - 12, lane);
       asm volatile("cp.async.wait_all;" ::: "memory");   // (landed long ago unless a wait ran out)
     } else {
       if constexpr (kEight) {
@@ -798,9 +837,14 @@ cudaError_t launch_kernel(cudaStream_t stream, const TreeArgs& a) {
   static_assert(kBytes <= 227 * 1024, "shared memory");
   using S = Shared<D, kEight, kWide>;
   static_assert(offsetof(S, k_factor) % 16 == 0 && offsetof(S, ml) % 8 == 0 && alignof(S) == 16, "alignment");
+  // tokens of a tiled copy; 0: rows by the lanes' own copies
+  const int box = !kBoxes<D, kEight> ? 0 : tree_pool_fits(a, kHalf) ? kHalf : tree_pool_fits(a, kHalf / 2) ? kHalf / 2 : 0;
+  CUtensorMap map_k{}, map_v{};
+  if (box > 0 && (!tree_pool_map(&map_k, a.pool.k, a, box, kEight ? D : 64, kEight ? 0 : 128) || !tree_pool_map(&map_v, a.pool.v, a, box, kEight ? D : 64, kEight ? 0 : 128)))
+    return cudaErrorInvalidValue;
   cudaError_t e = cudaFuncSetAttribute(tree_decode_sm100<D, kEight, kWide>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
   if (e != cudaSuccess) return e;
-  tree_decode_sm100<D, kEight, kWide><<<static_cast<unsigned>(tiles < kMaxCtas ? tiles : kMaxCtas), kThreads<kEight>, kBytes, stream>>>(a, shape);
+  tree_decode_sm100<D, kEight, kWide><<<static_cast<unsigned>(tiles < kMaxCtas ? tiles : kMaxCtas), kThreads<kEight>, kBytes, stream>>>(map_k, map_v, box, a, shape);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   return tree_decode_merge(stream, a, shape);
 }

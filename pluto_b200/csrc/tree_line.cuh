@@ -235,6 +235,12 @@ __device__ __forceinline__ void store_out8(const TreeArgs& a, size_t token, int 
       make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
 }
 
+// tree_decode_merge.cu: 4-D map of a page pool (column, KV head, token in page, page); a box is `tokens` tokens of `columns`
+// channels of one KV head, swizzled over 128 or 64 bytes or not (0); zeros outside the pool.  It takes pools whose
+// pages `tokens` divides, or one page per sequence, with strides that a map can hold.
+bool tree_pool_fits(const TreeArgs& a, int tokens);
+bool tree_pool_map(CUtensorMap* map, const void* base, const TreeArgs& a, int tokens, int columns, int swizzle);
+
 // tree_decode_merge.cu: launched behind the kernel that leaves the parts, by programmatic dependent launch
 cudaError_t tree_decode_merge(cudaStream_t stream, const TreeArgs& a, const LineShape& shape);
 

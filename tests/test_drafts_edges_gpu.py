@@ -139,6 +139,42 @@ def test_no_sequence_has_a_node(nodes):
     assert _capi.kernel_status() == 0
 
 
+@pytest.mark.parametrize("store", [EIGHT, torch.bfloat16])
+@pytest.mark.parametrize("nodes,hq,hkv,dim", SHAPES)
+@pytest.mark.parametrize("page", [16, 32, 64, 10])
+def test_bad_pages_in_the_prefix(store, nodes, hq, hkv, dim, page):
+    """Pages outside the pool are reported and read as zeros; the other sequences are as with good ones."""
+    gen, rnd = random(page)
+    blocks = -(-(210 + nodes) // page)
+    table = torch.randperm(3 * blocks, device="cuda", generator=gen).int().view(3, blocks)
+    k, v = (rnd(3 * blocks, page, hkv, dim).to(store) for _ in range(2))
+    scales = [torch.full((3 * blocks, page, hkv), 127, dtype=torch.uint8, device="cuda") if store == EIGHT else None for _ in range(2)]
+    q, at = rnd(3, nodes, hq, dim).bfloat16(), torch.tensor([210, 205, 190], **INT)
+    call = lambda t, k, v: gqa_tree_decode(q, k, v, at, 210, block_table=t, k_scales=scales[0], v_scales=scales[1])  # noqa: E731
+    good = call(table, k, v)
+    assert _capi.kernel_status() == 0
+    for bad in (-1, 3 * blocks, 2 ** 31 - 1, -2 ** 31):
+        wrong = table.clone()
+        wrong[1, 1], wrong[1, 128 // page] = bad, bad
+        got = call(wrong, k, v)
+        assert _capi.kernel_status() & 0xff == 3
+        zeros = [x.clone() for x in (k, v)]
+        for x in zeros:
+            x.view(torch.uint8)[table[1, 1].item()] = 0
+            x.view(torch.uint8)[table[1, 128 // page].item()] = 0
+        assert torch.equal(got[0], good[0]) and torch.equal(got[2], good[2])
+        want = call(table, *zeros)
+        if store == EIGHT:
+            # The rows that read as zeros have scale byte 0, those of the pool of zeros 127.  Where a range of the line holds nothing
+            # else, its weights are relative to another power of two, and the merge's 2^(m_c - m) differs by the 2^-22 that
+            # ex2.approx is off: 2^-20 of a result below max|v| (448 at scale 2^0, here below 8), then its rounding to bf16, which
+            # may fall to the other side: a step, 2^-7 of the result.
+            assert ((got.float() - want.float()).abs() <= 2.0 ** -7 * want.float().abs() + 8 * 2.0 ** -20).all()
+        else:
+            assert torch.equal(got, want)
+    assert _capi.kernel_status() == 0
+
+
 def test_pools_beyond_32_bits():
     """Pages whose rows lie more than 2^32 elements into the pool."""
     gen, rnd = random(4)
