@@ -47,9 +47,12 @@ constexpr float kSmallest = -90.0f;    // exponent of the value rows from which 
 
 // kWide: more than 128 rows may share a pass over the keys (never at width 256)
 template <int D, bool kEight, bool kWide>   // tiles of keys, and of values
-constexpr int kStages = kEight ? (D == 64 ? 6 : D == 128 ? 3 : 2) : (D == 64 ? 10 : D == 128 ? (kWide ? 4 : 6) : 3);
+constexpr int kStages = kEight ? (D == 64 ? 6 : D == 128 && !kWide ? 3 : 2) : (D == 64 ? 10 : D == 128 ? (kWide ? 4 : 6) : 3);
+// Key and value tiles as codes.  An even number: warps load and widen every other tile, and a parity tells a phase from its two
+// neighbours only, so a warp has to meet every use of its slots (three slots gave a wrong result in one of a thousand calls).
+// The products release the widened tiles in their order, whoever fills them, so those rings may have any length.
 template <int D, bool kWide>
-constexpr int kRawStages = D == 64 ? 8 : D == 128 ? (kWide ? 3 : 6) : 2;   // key and value tiles as codes
+constexpr int kRawStages = D == 64 ? 8 : D == 128 ? (kWide ? 4 : 6) : 2;
 template <int D>
 constexpr int kTileBytes = kTile * D * 2;
 constexpr int group_rows(int dim) { return dim == 256 ? 128 : 256; }   // rows that share one pass over the keys
@@ -67,6 +70,7 @@ constexpr int kSegmentReaders = kWide ? 14 : 13;   // warps: MMA issue, eight so
 template <int D, bool kEight, bool kWide>
 struct Shared {
   static constexpr int kTiles = kStages<D, kEight, kWide>, kRaw = kEight ? kRawStages<D, kWide> : 1;
+  static_assert(kRawStages<D, kWide> % 2 == 0, "a warp meets every use of its slots");
   uint64_t seg_full[kSegments], seg_empty[kSegments];
   uint64_t k_full[kTiles], k_empty[kTiles], v_full[kTiles], v_empty[kTiles];
   uint64_t raw_k[kRaw], raw_v[kRaw], raw_scales[kRaw], raw_empty[kRaw];
@@ -167,8 +171,8 @@ __device__ __forceinline__ void load_tiles(const TreeArgs& a, const CUtensorMap&
   for (;; n += 2, tile += 2, settle()) {
     const int slot = n % kRing, use = n / kRing;
     if (!more && !kEight) break;
-    // (few slots: this one, or one that its tile waits for, is freed once the last unit's scales have been passed on)
-    if (kEight && kRing <= 3) pass_scales();
+    // (two slots: this one is freed once the last unit's scales have been passed on)
+    if (kEight && kRing == 2) pass_scales();
     if (use > 0) {
       bool ok = __all_sync(0xffffffffu, tree_wait(kEight ? &sh->raw_empty[slot] : &sh->k_empty[slot], (use - 1) & 1, status, 50));
       if (!kEight) ok = ok && __all_sync(0xffffffffu, tree_wait(&sh->v_empty[slot], (use - 1) & 1, status, 51));
@@ -434,9 +438,9 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(const _
       while (ok && next_segment(sh, seg_n, seg, lane, status)) {
         const int tiles = __shfl_sync(0xffffffffu, seg.tile1 - seg.tile0, 0);
         const bool pair = kWide && __shfl_sync(0xffffffffu, seg.rows > 128 ? 1 : 0, 0), every = pair || kOneO;   // every: all tiles are a stream's
-        ok = __all_sync(0xffffffffu, tree_wait(&sh->q_full[0], segments++ & 1, status, 52));
-        if (ok && pair && warp) ok = __all_sync(0xffffffffu, tree_wait(&sh->q_full[1], pairs & 1, status, 52));
-        pairs += pair;
+        // (the second stream's warp has a part in pairs only, and awaits what is theirs only: nothing goes on without it there)
+        if (warp == 0) ok = __all_sync(0xffffffffu, tree_wait(&sh->q_full[0], segments++ & 1, status, 52));
+        else if (pair) ok = __all_sync(0xffffffffu, tree_wait(&sh->q_full[1], pairs++ & 1, status, 52));
         if (!ok) break;
         const uint64_t q_desc = umma_desc_sw128(queries + (pair && warp ? kQueryBytes<D, kWide> : 0), 16, 1024);
         const auto issue_qk = [&](int x, int u) -> bool {

@@ -127,6 +127,31 @@ def test_many_and_odd_numbers_of_kv_heads(nodes, dim, hkv, group):
     assert _capi.kernel_status() == 0
 
 
+@pytest.mark.parametrize("store", [EIGHT, torch.bfloat16])
+@pytest.mark.parametrize("nodes,hq,hkv,dim,longest", [(61, 40, 8, 128, 4000), (61, 40, 8, 128, 200), (40, 20, 4, 64, 3000), (20, 40, 8, 128, 3000), (20, 24, 4, 256, 2000), (3, 10, 2, 128, 3000)])
+def test_many_calls_agree(store, nodes, hq, hkv, dim, longest):
+    """The order of every sum is fixed, so calls repeat bit for bit whatever the warps' timing."""
+    gen, rnd = random(nodes + longest)
+    k, v = (rnd(8, longest + nodes, hkv, dim) for _ in range(2))
+    scales = [None, None]
+    if store == EIGHT:
+        rows = [torch.zeros(8, longest + nodes, hkv, dim, dtype=EIGHT, device="cuda") for _ in range(2)]
+        rows += [torch.zeros(8, longest + nodes, hkv, dtype=torch.uint8, device="cuda") for _ in range(2)]
+        kv8_append(k * 2.0 ** torch.randint(-4, 4, k.shape[:3] + (1,), device="cuda", generator=gen), v * 2.0 ** torch.randint(-4, 4, v.shape[:3] + (1,), device="cuda", generator=gen), *rows)
+        k, v, *scales = rows
+    else:
+        k, v = k.bfloat16(), v.bfloat16()
+    q = rnd(8, nodes, hq, dim).bfloat16()
+    at = torch.randint(0, longest + 1, (8,), device="cuda", generator=gen).int()
+    counts = torch.randint(nodes // 2, nodes + 1, (8,), device="cuda", generator=gen).int()
+    out = torch.zeros_like(q)
+    call = lambda: gqa_tree_decode(q, k, v, at, longest, counts=counts, k_scales=scales[0], v_scales=scales[1], out=out)  # noqa: E731
+    first, off = call().clone(), torch.zeros((), device="cuda")
+    for _ in range(1500):
+        off += (call() != first).any()
+    assert off.item() == 0 and _capi.kernel_status() == 0
+
+
 @pytest.mark.parametrize("nodes", [1, 20, 60])
 def test_no_sequence_has_a_node(nodes):
     gen, rnd = random(2)
