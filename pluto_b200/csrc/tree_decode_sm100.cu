@@ -74,7 +74,10 @@ struct Shared {
   uint64_t seg_full[kSegments], seg_empty[kSegments];
   uint64_t k_full[kTiles], k_empty[kTiles], v_full[kTiles], v_empty[kTiles];
   uint64_t raw_k[kRaw], raw_v[kRaw], raw_scales[kRaw], raw_empty[kRaw];
-  uint64_t q_full[2];
+  // Softmax warps have come to a segment, with its queries: the first stream's; the second's in a pair; the second's otherwise.
+  // Three, as neither stream may come to a barrier's next phase before the other has come to this one: in pairs they pass
+  // a segment alone.
+  uint64_t q_full[3];
   uint64_t s_full[2][2], p_half[2][2], p_full[2][2], pv_half[2][2], pv_done[2][2];   // [stream][score buffer]
   uint64_t ml_full, o_read;   // the two streams' meeting points: sums written, O read
   Segment seg[kSegments];
@@ -400,7 +403,6 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(const _
       mbar_init(&sh->seg_empty[i], kSegmentReaders<kWide>);
     }
     for (int x = 0; x < 2; ++x) {
-      mbar_init(&sh->q_full[x], x == 0 && !kOneO ? 8 : 4);   // ([0]: both streams' warps have come to the segment)
       for (int buffer = 0; buffer < 2; ++buffer) {
         mbar_init(&sh->s_full[x][buffer], 1);
         mbar_init(&sh->p_half[x][buffer], 4);
@@ -409,6 +411,7 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(const _
         mbar_init(&sh->pv_done[x][buffer], 1);
       }
     }
+    for (int i = 0; i < 3; ++i) mbar_init(&sh->q_full[i], 4);
     mbar_init(&sh->ml_full, 8);
     mbar_init(&sh->o_read, 8);
     mbar_fence_init();
@@ -431,16 +434,19 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(const _
       // ---------------------------------------------------------------- MMA issue
       // A warp per stream where both read every tile; else warp 0 for both, as every tile has to be awaited in its order (a
       // parity tells a phase from its neighbours only).
-      int tile_n = 0, own_0 = 0, own_1 = 0, segments = 0, pairs = 0;   // so far: tiles, those of the streams
+      int tile_n = 0, own_0 = 0, own_1 = 0, segments = 0, pairs = 0, others = 0;   // so far: tiles, those of the streams, ...
       bool ok = true;
       int seg_n = 0;
       Segment seg;
       while (ok && next_segment(sh, seg_n, seg, lane, status)) {
         const int tiles = __shfl_sync(0xffffffffu, seg.tile1 - seg.tile0, 0);
         const bool pair = kWide && __shfl_sync(0xffffffffu, seg.rows > 128 ? 1 : 0, 0), every = pair || kOneO;   // every: all tiles are a stream's
-        // (the second stream's warp has a part in pairs only, and awaits what is theirs only: nothing goes on without it there)
-        if (warp == 0) ok = __all_sync(0xffffffffu, tree_wait(&sh->q_full[0], segments++ & 1, status, 52));
-        else if (pair) ok = __all_sync(0xffffffffu, tree_wait(&sh->q_full[1], pairs++ & 1, status, 52));
+        if (warp == 0) {
+          ok = __all_sync(0xffffffffu, tree_wait(&sh->q_full[0], segments++ & 1, status, 52));
+          if (ok && !every) ok = __all_sync(0xffffffffu, tree_wait(&sh->q_full[2], others++ & 1, status, 52));
+        } else if (pair) {
+          ok = __all_sync(0xffffffffu, tree_wait(&sh->q_full[1], pairs++ & 1, status, 52));
+        }
         if (!ok) break;
         const uint64_t q_desc = umma_desc_sw128(queries + (pair && warp ? kQueryBytes<D, kWide> : 0), 16, 1024);
         const auto issue_qk = [&](int x, int u) -> bool {
@@ -596,10 +602,7 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(const _
         }
       }
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&sh->q_full[0]);
-        if (x == 1 && pair) mbar_arrive(&sh->q_full[1]);
-      }
+      if (lane == 0) mbar_arrive(&sh->q_full[x == 0 ? 0 : pair ? 1 : 2]);
       // ---- which drafts the row sees: one bit per node
       uint64_t seen_lo = 0, seen_hi = 0;
       if (seg.tile1 * kTile > seg.prefix) {
