@@ -152,6 +152,26 @@ def test_many_calls_agree(store, nodes, hq, hkv, dim, longest):
     assert off.item() == 0 and _capi.kernel_status() == 0
 
 
+@pytest.mark.parametrize("store", [EIGHT, torch.bfloat16])
+def test_short_pieces_of_units_agree(store):
+    """Many ragged sequences, cut so that some pieces hold a tile or two: calls repeat bit for bit."""
+    gen, rnd = random(5)
+    off = torch.zeros((), device="cuda")
+    for turn in range(24):
+        batch, nodes, longest = (24, 16)[turn % 2], (31, 40, 62)[turn % 3], (2664, 900, 300)[turn % 3]
+        k, v = (rnd(batch, longest + nodes, 12, 128).to(store) for _ in range(2))
+        scales = [torch.randint(124, 129, k.shape[:3], device="cuda", generator=gen).to(torch.uint8) if store == EIGHT else None for _ in range(2)]
+        q = rnd(batch, nodes, 60, 128).bfloat16()
+        at = torch.randint(0, longest + 1, (batch,), device="cuda", generator=gen).int()
+        counts = torch.randint(0, nodes + 1, (batch,), device="cuda", generator=gen).int()
+        out = torch.zeros_like(q)
+        call = lambda: gqa_tree_decode(q, k, v, at, longest, counts=counts, k_scales=scales[0], v_scales=scales[1], out=out)  # noqa: E731
+        first = call().clone()
+        for _ in range(60):
+            off += (call() != first).any()
+    assert off.item() == 0 and _capi.kernel_status() == 0
+
+
 @pytest.mark.parametrize("nodes", [1, 20, 60])
 def test_no_sequence_has_a_node(nodes):
     gen, rnd = random(2)
