@@ -214,7 +214,8 @@ bool fill_draft_pool(PyObject* const* args, pluto_kv_cache& c, pluto_kv_scales& 
   } else {
     Sizes blocks;
     if (!shape_of(table, blocks)) return false;
-    if (blocks.rank != 2 || blocks.n[1] > INT32_MAX) return refuse("a block table is [batch, blocks]");
+    // (a table without columns has no address, which would pass for no table: a page of its own for every sequence)
+    if (blocks.rank != 2 || blocks.n[1] < 1 || blocks.n[1] > INT32_MAX) return refuse("a block table is [batch, blocks], of one block or more");
     if (!int32_of(table, Sizes{2, {batch, blocks.n[1]}}, device, "block table", c.block_table)) return false;
     c.max_blocks = static_cast<int>(blocks.n[1]);
   }
