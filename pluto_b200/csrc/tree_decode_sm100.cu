@@ -19,10 +19,11 @@
 // Loading.  Four warps copy the rows into a ring with asynchronous 16-byte copies; pages may have any size and rows any
 // 16-byte stride.  Whole tiles of bf16 rows (and 8-bit ones of width 256) in pages of a multiple of 16 come by tiled copies
 // instead, one lane's work; the tiles with drafts and the last one do not, since what lies behind must be zeros.  bf16 rows land as the swizzled tiles that the products read.  8-bit codes land as they are (up to 96 KB
-// per SM in flight) and eight more warps widen them to fp16 tiles, one instruction per two codes and exact,
-// and multiply them by their row's 2^n where fp16 holds every product (-15 <= n <= 7, values from 2^-24 to 57344);
-// a tile with other rows keeps its codes and the softmax multiplies scores and weights by the rows' factors.  P then
-// carries 11 bits, over bf16 caches 8.
+// per SM in flight) and eight more warps widen them to fp16 tiles, one instruction per two codes and exact.
+// Keys are multiplied by their row's 2^n where fp16 holds every product (-15 <= n <= 7, values from 2^-24 to 57344); values by
+// 2^(n - N), 2^N the largest of the tile, where n >= N - 15 for all of its rows and none of them is a draft.  Tiles with
+// other rows keep their codes and the softmax multiplies scores and weights by the rows' factors.  P carries 11 bits, over
+// bf16 caches 8.
 //
 // Work is cut evenly over the SMs as tree_line.cuh says, one CTA per SM.
 //
@@ -44,6 +45,8 @@ constexpr int kUnitTiles = 3;        // query load and read-out of a unit, in ti
 constexpr float kRescale = 8.0f;     // O is rescaled when the maximum has grown by more than 2^8
 constexpr float kSmallest = -90.0f;    // exponent of the value rows from which smaller ones are taken for as large: sums of weights
                                        // of up to 2^(90 + 8) stay finite for any number of tokens
+constexpr float kApart = 60.0f;        // exponents between value rows beyond which the smaller ones' weights are zero in fp16, far
+                                       // from where their sum would lose them
 
 // kWide: more than 128 rows may share a pass over the keys (never at width 256)
 template <int D, bool kEight, bool kWide>   // tiles of keys, and of values
@@ -85,13 +88,13 @@ struct Shared {
   float2 ml[2][128];
   // 8-bit caches: the raw tiles' scale bytes and first draft that not every node sees (-1: the range ends)
   uint8_t k_byte[kRaw][kTile], v_byte[kRaw][kTile];
-  int draft_row[kRaw];
-  // ... and per tile whether the softmax has to apply the rows' factors.  A ring of three times the stages: a slot is
-  // written again once the stage of the tile two rounds on is free, and that tile's scores are issued behind the
-  // product of this one, whose softmax has then read them.
+  int draft_row[kRaw], border[kRaw];   // (border: the tile holds drafts)
+  // ... and per tile whether the softmax has to apply the rows' factors, and the largest exponent of its value rows.  A ring
+  // of three times the stages: a slot is written again once the stage of the tile two rounds on is free, and that
+  // tile's scores are issued behind the product of this one, whose softmax has then read them.
   alignas(16) float k_factor[3 * kTiles][kTile];   // (read four at a time)
   float v_factor[3 * kTiles][kTile];
-  int scaled[3 * kTiles], v_largest[3 * kTiles];
+  int scaled[3 * kTiles], v_largest[3 * kTiles];   // scaled: kKeysScaled, kValuesScaled
 };
 
 // The next segment of the range, by every lane of a warp; false at its end (or when a wait ran out).
@@ -124,10 +127,10 @@ __device__ __forceinline__ uint32_t tile_piece(uint32_t tile, int r, int piece) 
   return tile + (piece / 8) * (kTile * 128) + r * 128 + (((piece & 7) ^ (r & 7)) << 4);
 }
 
-__device__ __forceinline__ uint32_t load_byte(const uint8_t* p, bool there) {   // 127 where it is not
+__device__ __forceinline__ uint32_t load_byte(const uint8_t* p, bool there, uint32_t otherwise) {
   uint32_t v;
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\tmov.u32 %0, 127;\n\t@p ld.global.u8 %0, [%1];\n\t}"
-               : "=r"(v) : "l"(p), "r"(static_cast<uint32_t>(there)));
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\tmov.u32 %0, %3;\n\t@p ld.global.u8 %0, [%1];\n\t}"
+               : "=r"(v) : "l"(p), "r"(static_cast<uint32_t>(there)), "r"(otherwise));
   return v;
 }
 
@@ -262,10 +265,14 @@ __device__ __forceinline__ void load_tiles(const TreeArgs& a, const CUtensorMap&
     }
     if (kEight) {
       pass_scales();
-      k_byte = load_byte(a.pool.k_scales + scale_at, row_at >= 0);
-      v_byte = load_byte(a.pool.v_scales + scale_at, row_at >= 0);
+      // rows that are not there: keys of an ordinary scale, values of the smallest, which no reference is taken from
+      k_byte = load_byte(a.pool.k_scales + scale_at, row_at >= 0, 127u);
+      v_byte = load_byte(a.pool.v_scales + scale_at, row_at >= 0, 0u);
       passed = slot;
-      if (first_row == 0 && lane == 0) sh->draft_row[slot] = draft_row;
+      if (first_row == 0 && lane == 0) {
+        sh->draft_row[slot] = draft_row;
+        sh->border[slot] = (tile + 1) * kTile > seg.prefix;
+      }
     }
   }
   if (kEight) pass_scales();
@@ -277,6 +284,9 @@ __device__ __forceinline__ uint32_t halves_of(uint32_t codes) {   // two codes i
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<uint16_t>(codes)));
   return r;
 }
+__device__ __forceinline__ float power_of_two(float n) {   // n whole, -126 to 127
+  return __uint_as_float(static_cast<uint32_t>(static_cast<int>(n) + 127) << 23);
+}
 __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
   uint32_t r;
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -284,6 +294,7 @@ __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
 }
 // A row's scale byte: 2^n times any of its codes is exact in fp16 for -15 <= n <= 7 (2^-24 to 57344; n = 0 stands in for
 // rows that are not finite, whose codes are NaN).
+enum : int { kKeysScaled = 1, kValuesScaled = 2 };   // by the softmax
 constexpr uint32_t kHalfOne = 0x3c003c00u;
 __device__ __forceinline__ bool fits_fp16(uint32_t byte) { return byte == 255u || (byte >= 112u && byte <= 134u); }
 __device__ __forceinline__ uint32_t half_power(uint32_t byte) {
@@ -305,31 +316,28 @@ __device__ __forceinline__ void widen_tiles(Shared<D, true, kWide>* sh, uint32_t
     if (!__all_sync(0xffffffffu, tree_wait(&sh->raw_scales[slot], (n / kRaw) & 1, status, 47))) return;
     const int draft_row = sh->draft_row[slot];
     if (draft_row < 0) return;
-    // the rows' factors: in the codes for all rows of the tile or for none
+    // the rows' factors: in the codes for all rows of the tile or for none, the values' relative to the largest (`top`)
     const uint32_t k[2] = {sh->k_byte[slot][lane], sh->k_byte[slot][lane + 32]}, v[2] = {sh->v_byte[slot][lane], sh->v_byte[slot][lane + 32]};
     const bool k_fits = __all_sync(0xffffffffu, fits_fp16(k[0]) && fits_fp16(k[1]));
-    const bool v_fits = __all_sync(0xffffffffu, fits_fp16(v[0]) && fits_fp16(v[1]));
+    const uint32_t top = __reduce_max_sync(0xffffffffu, max(v[0] == 255u ? 0u : v[0], v[1] == 255u ? 0u : v[1]));
+    const bool v_fits = sh->border[slot] == 0 && __all_sync(0xffffffffu, min(v[0], v[1]) + 15u >= top);
     const uint32_t own_k = first_row ? k[1] : k[0], own_v = first_row ? v[1] : v[0];   // of row first_row + lane
     uint32_t factor = kHalfOne;
-    if (values ? v_fits : k_fits) factor = half_power(values ? own_v : own_k);
+    if (values ? v_fits : k_fits) factor = half_power(!values ? own_k : own_v == 255u ? 255u : own_v + 127u - top);
     // Of drafts that not every node sees, values that are not finite are stored as zeros and their keys as NaN (see above).
     const bool hidden = own_v == 255u && first_row + lane >= draft_row;
     if (!values && hidden) factor = 0x7fff7fffu;
     const unsigned zeros = __ballot_sync(0xffffffffu, values && hidden);
     if (use > 0 && !__all_sync(0xffffffffu, tree_wait(values ? &sh->v_empty[stage] : &sh->k_empty[stage], (use - 1) & 1, status, values ? 46 : 45))) return;
     if (!values && first_row == 0) {
-      uint32_t largest = 127u;
-      if (!k_fits || !v_fits) {
 #pragma unroll
-        for (int o = 0; o < 2; ++o) {
-          sh->k_factor[scale_slot][lane + 32 * o] = k_fits || k[o] == 255u ? 1.0f : e8m0_value(k[o]);
-          sh->v_factor[scale_slot][lane + 32 * o] = v_fits || v[o] == 255u ? 1.0f : e8m0_value(v[o]);
-        }
-        if (!v_fits) largest = __reduce_max_sync(0xffffffffu, max(v[0] == 255u ? 0u : v[0], v[1] == 255u ? 0u : v[1]));
+      for (int o = 0; o < 2; ++o) {
+        if (!k_fits) sh->k_factor[scale_slot][lane + 32 * o] = k[o] == 255u ? 1.0f : e8m0_value(k[o]);
+        if (!v_fits) sh->v_factor[scale_slot][lane + 32 * o] = v[o] == 255u ? 1.0f : e8m0_value(v[o]);
       }
       if (lane == 0) {
-        sh->scaled[scale_slot] = !k_fits || !v_fits;
-        sh->v_largest[scale_slot] = static_cast<int>(largest) - 127;
+        sh->scaled[scale_slot] = (k_fits ? 0 : kKeysScaled) | (v_fits ? 0 : kValuesScaled);
+        sh->v_largest[scale_slot] = static_cast<int>(top) - 127;
       }
     }
     if (!__all_sync(0xffffffffu, tree_wait(values ? &sh->raw_v[slot] : &sh->raw_k[slot], (n / kRaw) & 1, status, 44))) return;
@@ -623,8 +631,9 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(const _
         }
       }
       // ---- the tiles of this stream
-      // Weights are 2^(score * row_scale - reference), reference = m_used * row_scale + v_used: for 8-bit caches v_used is
-      // the largest exponent of the value rows so far, so that a weight times its row's 2^n fits fp16.
+      // Weights are w = 2^(score * row_scale - m_used * row_scale), and l their sum.  For 8-bit caches v_used is the largest
+      // exponent of the value rows so far and O is kept relative to 2^v_used, so that a weight times its row's 2^n, which is
+      // what enters the product, fits fp16.
       float m_used = -INFINITY, m_true = -INFINITY, l = 0.0f, v_used = kEight ? kSmallest : 0.0f;
       const bool every = pair || kOneO;
       const int own = every ? tiles : (tiles + 1 - x) / 2;
@@ -637,8 +646,13 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(const _
         const uint32_t s_at = lanes + kColS + (kBuffers * x + buffer) * kTile;
         const int slot = (tile_n + j) % (3 * kStages<D, kEight, kWide>);
         const uint32_t k_factor = smem_u32(sh->k_factor[slot]), v_factor = smem_u32(sh->v_factor[slot]);
-        const bool scaled = kEight && warp_live && sh->scaled[slot] != 0;   // the rare tile with rows that fp16 does not hold
-        const float v_tile = scaled ? fmaxf(v_used, static_cast<float>(sh->v_largest[slot])) : kEight ? fmaxf(v_used, 0.0f) : v_used;
+        const int scaled = kEight && warp_live ? sh->scaled[slot] : 0;   // tiles with drafts, and the rare one that fp16 does not hold
+        const float v_largest = kEight ? static_cast<float>(sh->v_largest[slot]) : 0.0f, v_tile = fmaxf(v_used, v_largest);
+        // Whole tiles' weights are taken times 2^-below; where nothing of that would be left in fp16, or the rows differ, the
+        // weights get their factors behind the sum.
+        const float below = v_tile - v_largest;
+        const bool apart = kEight && ((scaled & kValuesScaled) != 0 || below > kApart);
+        const float shift = apart ? 0.0f : below;
         const int behind = (seg.tile0 + j) * kTile - seg.prefix;   // of the drafts' first slot
         uint64_t seen = ~0ull;
         if (behind > -kTile)
@@ -655,7 +669,7 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(const _
             uint32_t s[32];
             tmem_ld32(s_at + h * 32, s);
             tmem_wait_ld();
-            if (scaled) {
+            if (scaled & kKeysScaled) {
 #pragma unroll
               for (int i = 0; i < 32; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) * lds_f32(k_factor + (h * 32 + i) * 4));
             }
@@ -671,7 +685,7 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(const _
 #pragma unroll
             for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
             m_true = max3(mx[0], mx[1], fmaxf(mx[2], mx[3]));
-            const float reference = (m_used == -INFINITY ? 0.0f : m_used * row_scale) + v_used;   // (nothing seen yet: any)
+            const float reference = (m_used == -INFINITY ? 0.0f : m_used * row_scale) + shift;   // (nothing seen yet: any)
             const uint64_t scale2 = f2_pack(row_scale, row_scale), neg2 = f2_pack(-reference, -reference);
             uint64_t sum2[2] = {0ull, 0ull};
             uint32_t packed[16];
@@ -691,10 +705,10 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(const _
             }
             const bool grow = (m_true - m_used) * row_scale > kRescale;
             if (__any_sync(0xffffffffu, grow || v_tile > v_used)) {
-              const float factor = fast_exp2((grow ? (m_used - m_true) * row_scale : 0.0f) + (v_used - v_tile));
+              const float less = grow ? (m_used - m_true) * row_scale : 0.0f, factor = fast_exp2(less + (v_used - v_tile));
               if (grow) m_used = m_true;
               v_used = v_tile;
-              l *= factor;
+              l *= kEight ? fast_exp2(less) : factor;
               if (u > 0 || h == 1) {
                 // every product into this O must have ended: the first half's, or the previous tile's second
                 ok = __all_sync(0xffffffffu, tree_wait(h ? &sh->pv_half[x][buffer] : &sh->pv_done[x][buffer_of(t - 1)], phase_of(h ? t : t - 1), status, 57));
@@ -715,9 +729,11 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(const _
               --h;
               continue;
             }
-            if (scaled) {
+            if (apart) {
+              const float down = scaled & kValuesScaled ? power_of_two(-v_tile) : 0.0f;
 #pragma unroll
-              for (int i = 0; i < 32; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) * lds_f32(v_factor + (h * 32 + i) * 4));
+              for (int i = 0; i < 32; ++i)
+                s[i] = __float_as_uint(__uint_as_float(s[i]) * (scaled & kValuesScaled ? lds_f32(v_factor + (h * 32 + i) * 4) * down : 0.0f));
             }
             if (kEight) {
 #pragma unroll
@@ -727,7 +743,7 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(const _
             float a0, a1, b0, b1;
             f2_unpack(sum2[0], a0, a1);
             f2_unpack(sum2[1], b0, b1);
-            l += (a0 + a1) + (b0 + b1);
+            l += kEight ? ((a0 + a1) + (b0 + b1)) * power_of_two(shift) : (a0 + a1) + (b0 + b1);
             tmem_wait_st();
             tc_fence_before();
           }
@@ -746,6 +762,7 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(const _
       tc_fence_after();
       // ---- read-out: rows of one stream, or the two streams' halves of the keys merged, half of the channels each
       float m = m_used == -INFINITY ? m_used : m_used * row_scale + v_used, f0 = 1.0f, f1 = 0.0f;   // log2 units from here
+      if (kEight) l *= power_of_two(-v_used);   // (of O's unit from here)
       bool both = false;
       if (merged) {
         sh->ml[x][row] = make_float2(m, l);
