@@ -86,6 +86,7 @@ struct Shared {
   Segment seg[kSegments];
   uint32_t tmem;
   float2 ml[2][128];
+  float unit[2][kEight ? 128 : 1];   // v_used of the rows
   // 8-bit caches: the raw tiles' scale bytes and first draft that not every node sees (-1: the range ends)
   uint8_t k_byte[kRaw][kTile], v_byte[kRaw][kTile];
   int draft_row[kRaw], border[kRaw];   // (border: the tile holds drafts)
@@ -632,8 +633,8 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(const _
       }
       // ---- the tiles of this stream
       // Weights are w = 2^(score * row_scale - m_used * row_scale), and l their sum.  For 8-bit caches v_used is the largest
-      // exponent of the value rows so far and O is kept relative to 2^v_used, so that a weight times its row's 2^n, which is
-      // what enters the product, fits fp16.
+      // exponent of the value rows that the row has seen so far and O is kept relative to 2^v_used, so that a weight times its
+      // value row's 2^n, which is what enters the product, fits fp16.
       float m_used = -INFINITY, m_true = -INFINITY, l = 0.0f, v_used = kEight ? kSmallest : 0.0f;
       const bool every = pair || kOneO;
       const int own = every ? tiles : (tiles + 1 - x) / 2;
@@ -647,12 +648,6 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(const _
         const int slot = (tile_n + j) % (3 * kStages<D, kEight, kWide>);
         const uint32_t k_factor = smem_u32(sh->k_factor[slot]), v_factor = smem_u32(sh->v_factor[slot]);
         const int scaled = kEight && warp_live ? sh->scaled[slot] : 0;   // tiles with drafts, and the rare one that fp16 does not hold
-        const float v_largest = kEight ? static_cast<float>(sh->v_largest[slot]) : 0.0f, v_tile = fmaxf(v_used, v_largest);
-        // Whole tiles' weights are taken times 2^-below; where nothing of that would be left in fp16, or the rows differ, the
-        // weights get their factors behind the sum.
-        const float below = v_tile - v_largest;
-        const bool apart = kEight && ((scaled & kValuesScaled) != 0 || below > kApart);
-        const float shift = apart ? 0.0f : below;
         const int behind = (seg.tile0 + j) * kTile - seg.prefix;   // of the drafts' first slot
         uint64_t seen = ~0ull;
         if (behind > -kTile)
@@ -660,6 +655,22 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(const _
                  : behind > 0  ? seen_lo >> behind | seen_hi << (64 - behind)
                  : behind == 0 ? seen_lo
                                : seen_lo << -behind | ((1ull << -behind) - 1);
+        float v_largest = kEight ? static_cast<float>(sh->v_largest[slot]) : 0.0f;
+        if (kEight && behind > -kTile && v_largest > v_used && warp_live) {   // of the drafts' tiles only rows that this one sees count
+          uint32_t most = 0u;
+#pragma unroll 4
+          for (int i = 0; i < kTile; ++i) {
+            const uint32_t factor = __float_as_uint(lds_f32(v_factor + i * 4));
+            if (seen >> i & 1u) most = max(most, factor);
+          }
+          v_largest = static_cast<float>(static_cast<int>(most >> 23) - 127);
+        }
+        const float v_tile = fmaxf(v_used, v_largest);
+        // Whole tiles' weights are taken times 2^-below; where nothing of that would be left in fp16, or the rows differ, the
+        // weights get their factors behind the sum.
+        const float below = v_tile - v_largest;
+        const bool apart = kEight && ((scaled & kValuesScaled) != 0 || below > kApart);
+        const float shift = apart ? 0.0f : below;
         // Half of the tile's keys at a time, in a loop: its code then fits the instruction caches beside the other
         // warps' (straight-line code of 64 columns took twice as long), and the first half's product starts earlier.
 #pragma unroll 1
@@ -730,10 +741,10 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(const _
               continue;
             }
             if (apart) {
-              const float down = scaled & kValuesScaled ? power_of_two(-v_tile) : 0.0f;
+              const float down = scaled & kValuesScaled ? power_of_two(-v_tile) : 0.0f;   // (beyond 1: rows with weights of zero)
 #pragma unroll
               for (int i = 0; i < 32; ++i)
-                s[i] = __float_as_uint(__uint_as_float(s[i]) * (scaled & kValuesScaled ? lds_f32(v_factor + (h * 32 + i) * 4) * down : 0.0f));
+                s[i] = __float_as_uint(__uint_as_float(s[i]) * (scaled & kValuesScaled ? fminf(lds_f32(v_factor + (h * 32 + i) * 4) * down, 1.0f) : 0.0f));
             }
             if (kEight) {
 #pragma unroll
@@ -761,11 +772,12 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(const _
       if (!ok) break;
       tc_fence_after();
       // ---- read-out: rows of one stream, or the two streams' halves of the keys merged, half of the channels each
-      float m = m_used == -INFINITY ? m_used : m_used * row_scale + v_used, f0 = 1.0f, f1 = 0.0f;   // log2 units from here
-      if (kEight) l *= power_of_two(-v_used);   // (of O's unit from here)
+      // log2 units from here: sums relative to 2^m, O to 2^(m + v)
+      float m = m_used == -INFINITY ? m_used : m_used * row_scale, f0 = 1.0f, f1 = 0.0f, v = v_used;
       bool both = false;
       if (merged) {
         sh->ml[x][row] = make_float2(m, l);
+        if (kEight) sh->unit[x][row] = v_used;
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh->ml_full);
         ok = __all_sync(0xffffffffu, tree_wait(&sh->ml_full, met & 1, status, 59));
@@ -781,10 +793,20 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(const _
         f0 = fast_exp2(one.x - m_safe);
         f1 = both ? fast_exp2(two.x - m_safe) : 0.0f;
         l = both ? one.y * f0 + two.y * f1 : one.y * f0;
+        if (kEight) {   // O in the larger of the two units
+          const float v0 = sh->unit[0][row], v1 = both ? sh->unit[1][row] : v0, step = (two.x - one.x) + (v1 - v0);
+          const bool second = both && two.x != -INFINITY && step > 0.0f;
+          f0 = second ? fast_exp2(-step) : 1.0f;
+          f1 = second ? 1.0f : both && two.x != -INFINITY ? fast_exp2(step) : 0.0f;
+          v = second ? v1 + (two.x - m) : one.x == -INFINITY ? v0 : v0 + (one.x - m);
+        }
       }
       if (warp_live) {
         const int slot = 2 * blockIdx.x + seg.slot;
-        const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
+        // A part leaves in the unit of its values, which every part shares, and scaled so that its weights sum to less than
+        // 2^-11: sums over parts stay finite as far as values do.
+        const float drop = kEight && !seg.whole && l > 0.0f ? fminf(static_cast<float>(static_cast<int>(__float_as_uint(l) >> 23) - 127 + 12), 126.0f) : 0.0f;
+        const float inverse = seg.whole ? (l == 0.0f ? 0.0f : 1.0f / l) : power_of_two(-drop), up = kEight ? exp2f(v) : 1.0f;
         float* acc = parts.acc + (static_cast<size_t>(slot) * parts.rows + own_row) * D;
         const int c0 = merged ? x * (D / 32) : 0, c1 = merged ? c0 + D / 32 : D / 16;
 #pragma unroll 1
@@ -807,10 +829,14 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(const _
             for (int h = 0; h < 2; ++h) {
               float v[8];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(o[8 * h + i]) * inverse;
+              for (int i = 0; i < 8; ++i) v[i] = kEight ? __uint_as_float(o[8 * h + i]) * inverse * up : __uint_as_float(o[8 * h + i]) * inverse;
               store_out8(a, token, head, c * 16 + 8 * h, v, gate_pieces);
             }
           } else {
+            if (kEight) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * inverse * up);
+            }
 #pragma unroll
             for (int i = 0; i < 4; ++i)
               reinterpret_cast<uint4*>(acc + c * 16)[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
@@ -818,7 +844,7 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(const _
           __syncwarp();
         }
         if (live && (x == 0 || pair)) {
-          if (!seg.whole) parts.ml[static_cast<size_t>(slot) * parts.rows + own_row] = make_float2(m, l);
+          if (!seg.whole) parts.ml[static_cast<size_t>(slot) * parts.rows + own_row] = make_float2(m + drop, l * power_of_two(-drop));
           else if (a.lse) a.lse[token * a.q_heads + head] = (m == -INFINITY ? 0.0f : m * 0.6931471805599453f) + logf(l);
         }
         tc_fence_before();

@@ -83,3 +83,29 @@ def test_scales_that_change_along_the_keys(nodes, hq, hkv, dim, powers, places):
     q, k, v, ks, vs, parents = case(nodes, hq, hkv, dim, 333, [powers[0]], nodes)
     vs[0, 64 if places == "first tile" else 300:] = 127 + powers[1]
     hold_to_the_model(q, k, v, ks, vs, 333, parents)
+
+
+@pytest.mark.parametrize("prefix", [0, 1, 30, 64, 100, 333])
+@pytest.mark.parametrize("powers", [[-20, -18], [-90, -70], [-15, -22], [30, 27], [0, 40], [-50, 60]])
+@pytest.mark.parametrize("nodes,hq,hkv,dim", SHAPES)
+def test_scales_that_differ_from_row_to_row(nodes, hq, hkv, dim, powers, prefix):
+    q, k, v, ks, vs, parents = case(nodes, hq, hkv, dim, prefix, powers, nodes + prefix)
+    hold_to_the_model(q, k, v, ks, vs, prefix, parents, at_least=0.3)
+
+
+@pytest.mark.parametrize("prefix", [0, 3, 60, 62, 130, 1000])
+@pytest.mark.parametrize("k_power,v_power", [(0, 30), (0, 80), (30, 0), (80, 40), (-40, 9), (0, -40)])
+@pytest.mark.parametrize("hq,hkv,dim", [(10, 2, 128), (6, 1, 256), (4, 4, 64), (2, 2, 128), (1, 1, 256), (40, 2, 64), (40, 1, 128)])
+def test_a_finite_row_that_a_node_does_not_see_does_not_reach_it(hq, hkv, dim, k_power, v_power, prefix):
+    """A draft whose rows have other scales than all others: bit for bit what its neighbours get beside an ordinary one."""
+    up = [-1, 0, 0, 1, -1, 4, 2, 3]
+    q, k, v, ks, vs, _ = case(8, hq, hkv, dim, prefix, [-7], dim + prefix)
+    parents = torch.tensor([up], **INT)
+    clean = hold_to_the_model(q, k, v, ks, vs, prefix, parents, at_least=0.8)
+    ks[0, prefix + 1], vs[0, prefix + 1] = 127 + k_power, 127 + v_power
+    if k_power <= 0:
+        got = hold_to_the_model(q, k, v, ks, vs, prefix, parents, at_least=0.0)
+    else:   # (scores that fp32 holds to some units only: of no interest beside their neighbours)
+        got = gqa_tree_decode(q, k, v, torch.tensor([prefix], **INT), prefix, parents=parents, k_scales=ks, v_scales=vs, round_to_bfloat16=False)
+    for node in (0, 2, 4, 5, 6):
+        assert torch.equal(got[0, node], clean[0, node]), node
