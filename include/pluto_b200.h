@@ -448,7 +448,7 @@ int pluto_draft_prepare(pluto_stream_t stream, const void* q_in, const void* k_i
  * is exact but for the softmax weights:
  *   bf16 cache   few rows (nodes * q_heads / kv_heads <= 16, at width 256 <= 8; pages that 16 divides, or one page per
  *                sequence): weights to 16 bits; more rows, or other pages: to bf16
- *   8-bit cache  weights to fp16, relative to the largest scale 2^n among the value rows that a query sees (2^-90 where
+ *   8-bit cache  weights to fp16, relative to the largest scale 2^n among the value rows that a query sees (2^-118 where
  *                all are smaller): value rows of a much smaller scale lose weights below 2^-25 of that */
 size_t pluto_gqa_tree_decode_workspace_bytes(int batch, int nodes, int q_heads, int kv_heads, int head_dim);
 int pluto_gqa_tree_decode(pluto_stream_t stream, const void* q, int q_dtype, const void* gate, int gate_dtype,

@@ -15,8 +15,8 @@
 // The codes of an 8-bit cache become MMA operands in registers, one instruction per two codes and exact.  The order of
 // the channels in a product is free as long as both operands share it, so a lane takes whole 16-byte pieces: of the
 // keys the pieces of its rows, of the values the piece of its channels from four rows, paired by byte permutes.  The
-// rows' powers of two stay out of the products: a key's multiplies its scores, a value's its weights, relative to
-// the largest so far so that the products fit fp16 (P carries 11 bits).  Over bf16 caches P enters as a bf16 part and
+// rows' powers of two stay out of the products: a key's multiplies its scores, a value's its weights behind their
+// sum, relative to the largest so far so that the products fit fp16 (P carries 11 bits).  Over bf16 caches P enters as a bf16 part and
 // its bf16 remainder, 16 bits, as in gqa_decode.cu.  P^T leaves the score layout by movmatrix, and a lane compares its
 // scores with the reference of their rows by itself: the maximum is reduced over lanes only when one has to move.
 //
@@ -31,8 +31,8 @@ namespace {
 constexpr int kTile = 16;          // tokens of a step
 constexpr int kWarps = 4;
 constexpr float kRescale = 8.0f;   // the accumulator is rescaled when the maximum has grown by more than 2^8
-constexpr float kSmallest = -90.0f;    // exponent of the value rows from which smaller ones are taken for as large: sums of weights
-                                       // of up to 2^(90 + 8) stay finite for any number of tokens
+constexpr float kSmallest = -118.0f;   // exponent of the value rows from which smaller ones are taken for as large: weights of up
+                                       // to 2^8 times 2^118 stay finite
 
 template <int D, bool kEight>
 constexpr int kRowBytes = D * (kEight ? 1 : 2);
@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, kEight>) tree_decode_mma
   Segment seg{};
   int primed = 0, slot = 0, round = 0, n = 0, j = 0;   // slot and round of the ring
   uint32_t qf[D / 16][kN][2], seen[kR];
-  float row_scale[kR], m_used[kR], v_used[kR], l[kR], o[kBlocks][kN][4], v_low = 0.0f;
+  float row_scale[kR], m_used[kR], v_used[kEight ? kR : 1], l[kR], o[kBlocks][kN][4], v_low = 0.0f;
 #pragma unroll 1
   while (true) {
     issue();
@@ -244,8 +244,17 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, kEight>) tree_decode_mma
       const int nb = i / 2, e = i % 2, r = nb * 8 + 2 * t4 + e;
       if (r >= seg.rows) continue;
       float* to = acc + r * D;
+      float drop = 0.0f;
       if constexpr (kEight) {
         constexpr int kWidth = D == 64 ? 8 : 16;   // neighbouring channels of a lane
+        drop = part_drop(l[i]);
+        const float down = power_of_two(-drop), up = power_of_two(v_used[i]);
+        l[i] *= down;
+#pragma unroll
+        for (int m = 0; m < kBlocks; ++m) {
+          o[m][nb][e] = o[m][nb][e] * down * up;
+          o[m][nb][2 + e] = o[m][nb][2 + e] * down * up;
+        }
 #pragma unroll
         for (int set = 0; set < (D == 256 ? 2 : 1); ++set)
 #pragma unroll
@@ -260,7 +269,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, kEight>) tree_decode_mma
           to[m * 16 + 8 + quad] = o[m][nb][2 + e];
         }
       }
-      if (quad == 0) parts.ml[static_cast<size_t>(part) * parts.rows + r] = make_float2(m_used[i] == -INFINITY ? -INFINITY : m_used[i] + v_used[i], l[i]);
+      if (quad == 0) parts.ml[static_cast<size_t>(part) * parts.rows + r] = make_float2(m_used[i] + drop, l[i]);
     }
     if (seg.whole) {   // (through the slot that the warp has anyway: rows in the order of memory, and one piece of code)
       __syncwarp();
@@ -334,17 +343,17 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, kEight>) tree_decode_mma
       }
     }
     __syncwarp();
-    // Weights are 2^(score * row_scale - reference), reference = m_used + v_used: for 8-bit caches v_used is the largest
-    // exponent of the value rows seen so far, so that a weight times its row's 2^n fits fp16.
+    // Weights are 2^(score * row_scale - m_used).  For 8-bit caches v_used is the largest exponent of the value rows seen so far
+    // and O is kept relative to 2^v_used, so that a weight times its value row's 2^n, which is what enters the product, fits fp16.
 #pragma unroll
     for (int i = 0; i < kR; ++i) {
       row_scale[i] = __shfl_sync(0xffffffffu, of_row[i / 2], (2 * t4 + i % 2) * 4);
       seen[i] = __shfl_sync(0xffffffffu, bits_of[i / 2], (2 * t4 + i % 2) * 4);
       m_used[i] = -INFINITY;
-      v_used[i] = kEight ? kSmallest : 0.0f;
+      if (kEight) v_used[i] = kSmallest;
       l[i] = 0.0f;
     }
-    v_low = kSmallest;
+    if (kEight) v_low = kSmallest;
 #pragma unroll
     for (int m = 0; m < kBlocks; ++m)
 #pragma unroll
@@ -455,11 +464,12 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, kEight>) tree_decode_mma
 #pragma unroll
       for (int i = 0; i < kR; ++i) move = move || fmaxf(x[i][0], x[i][1]) - m_used[i] > kRescale;
       if (__any_sync(0xffffffffu, move)) {
-        v_low = INFINITY;
+        if (kEight) v_low = INFINITY;
 #pragma unroll
         for (int i = 0; i < kR; ++i) {
-          float m = fmaxf(x[i][0], x[i][1]), v = v_used[i];
+          float m = fmaxf(x[i][0], x[i][1]), v = 0.0f;
           if (kEight) {
+            v = v_used[i];
             if (x[i][0] != -INFINITY) v = fmaxf(v, v_power[0]);   // (of the rows that are seen)
             if (x[i][1] != -INFINITY) v = fmaxf(v, v_power[1]);
           }
@@ -469,11 +479,13 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, kEight>) tree_decode_mma
             if (kEight) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, lanes));
           }
           const bool grow = m - m_used[i] > kRescale;
-          const float factor = fast_exp2((grow ? m_used[i] - m : 0.0f) + (v_used[i] - v));
+          const float less = grow ? m_used[i] - m : 0.0f, factor = fast_exp2(kEight ? less + (v_used[i] - v) : less);
           if (grow) m_used[i] = m;
-          v_used[i] = v;
-          v_low = fminf(v_low, v);
-          l[i] *= factor;
+          l[i] *= kEight ? fast_exp2(less) : factor;
+          if (kEight) {
+            v_used[i] = v;
+            v_low = fminf(v_low, v);
+          }
 #pragma unroll
           for (int k = 0; k < kBlocks; ++k) {
             o[k][i / 2][i % 2] *= factor;
@@ -490,11 +502,12 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, kEight>) tree_decode_mma
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int i = 2 * nb + e;
-            w[e] = fast_exp2(x[i][u] - ((m_used[i] == -INFINITY ? 0.0f : m_used[i]) + v_used[i]));   // (nothing seen yet: any)
+            w[e] = fast_exp2(x[i][u] - (m_used[i] == -INFINITY ? 0.0f : m_used[i]));   // (nothing seen yet: any)
             l[i] += w[e];
+            if (kEight) w[e] = w[e] * power_of_two(-v_used[i]) * v_factor[u];
           }
           if (kEight) {
-            p[nb][u] = transposed(pack_f16(w[0] * v_factor[u], w[1] * v_factor[u]));
+            p[nb][u] = transposed(pack_f16(w[0], w[1]));
           } else {
             const uint32_t most = pack_bf16(w[0], w[1]);
             p[nb][u] = transposed(most);

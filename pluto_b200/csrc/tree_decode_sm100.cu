@@ -43,8 +43,8 @@ constexpr int kThreads = kEight ? 768 : 512;   // warps 0-3: MMA issue; 4-11: so
 constexpr int kMaxCtas = 148;
 constexpr int kUnitTiles = 3;        // query load and read-out of a unit, in tiles
 constexpr float kRescale = 8.0f;     // O is rescaled when the maximum has grown by more than 2^8
-constexpr float kSmallest = -90.0f;    // exponent of the value rows from which smaller ones are taken for as large: sums of weights
-                                       // of up to 2^(90 + 8) stay finite for any number of tokens
+constexpr float kSmallest = -118.0f;   // exponent of the value rows from which smaller ones are taken for as large: weights of up
+                                       // to 2^8 times 2^118 stay finite
 constexpr float kApart = 60.0f;        // exponents between value rows beyond which the smaller ones' weights are zero in fp16, far
                                        // from where their sum would lose them
 
@@ -284,9 +284,6 @@ __device__ __forceinline__ uint32_t halves_of(uint32_t codes) {   // two codes i
   uint32_t r;
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<uint16_t>(codes)));
   return r;
-}
-__device__ __forceinline__ float power_of_two(float n) {   // n whole, -126 to 127
-  return __uint_as_float(static_cast<uint32_t>(static_cast<int>(n) + 127) << 23);
 }
 __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
   uint32_t r;
@@ -803,9 +800,7 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(const _
       }
       if (warp_live) {
         const int slot = 2 * blockIdx.x + seg.slot;
-        // A part leaves in the unit of its values, which every part shares, and scaled so that its weights sum to less than
-        // 2^-11: sums over parts stay finite as far as values do.
-        const float drop = kEight && !seg.whole && l > 0.0f ? fminf(static_cast<float>(static_cast<int>(__float_as_uint(l) >> 23) - 127 + 12), 126.0f) : 0.0f;
+        const float drop = kEight && !seg.whole ? part_drop(l) : 0.0f;
         const float inverse = seg.whole ? (l == 0.0f ? 0.0f : 1.0f / l) : power_of_two(-drop), up = kEight ? exp2f(v) : 1.0f;
         float* acc = parts.acc + (static_cast<size_t>(slot) * parts.rows + own_row) * D;
         const int c0 = merged ? x * (D / 32) : 0, c1 = merged ? c0 + D / 32 : D / 16;

@@ -188,6 +188,15 @@ __device__ __forceinline__ Partials partials_of(const TreeArgs& a, const LineSha
   return p;
 }
 
+__device__ __forceinline__ float power_of_two(float n) {   // n whole, -126 to 127
+  return __uint_as_float(static_cast<uint32_t>(static_cast<int>(n) + 127) << 23);
+}
+// Parts over 8-bit caches leave in the unit of the values, which all parts share, and times 2^-drop, so that a part's weights
+// sum to less than 2^-11: sums over parts are finite wherever the values are.
+__device__ __forceinline__ float part_drop(float l) {
+  return l > 0.0f ? fminf(static_cast<float>(static_cast<int>(__float_as_uint(l) >> 23) - 127 + 12), 126.0f) : 0.0f;
+}
+
 // Bounded wait on a phase parity, as mbar_wait, that gives up for a wait that ran out and for nothing else: what a call
 // reports about its data stays in the status word until it is read, and the next calls are right all the same.
 __device__ __forceinline__ bool tree_wait(uint64_t* bar, uint32_t parity, uint32_t* status, uint32_t site) {

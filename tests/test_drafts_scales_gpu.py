@@ -86,7 +86,7 @@ def test_scales_that_change_along_the_keys(nodes, hq, hkv, dim, powers, places):
 
 
 @pytest.mark.parametrize("prefix", [0, 1, 30, 64, 100, 333])
-@pytest.mark.parametrize("powers", [[-20, -18], [-90, -70], [-15, -22], [30, 27], [0, 40], [-50, 60]])
+@pytest.mark.parametrize("powers", [[-20, -18], [-90, -70], [-110, -118], [-15, -22], [30, 27], [0, 40], [-50, 60]])
 @pytest.mark.parametrize("nodes,hq,hkv,dim", SHAPES)
 def test_scales_that_differ_from_row_to_row(nodes, hq, hkv, dim, powers, prefix):
     q, k, v, ks, vs, parents = case(nodes, hq, hkv, dim, prefix, powers, nodes + prefix)
@@ -94,7 +94,7 @@ def test_scales_that_differ_from_row_to_row(nodes, hq, hkv, dim, powers, prefix)
 
 
 @pytest.mark.parametrize("prefix", [0, 3, 60, 62, 130, 1000])
-@pytest.mark.parametrize("k_power,v_power", [(0, 30), (0, 80), (30, 0), (80, 40), (-40, 9), (0, -40)])
+@pytest.mark.parametrize("k_power,v_power", [(0, 30), (0, 80), (0, 119), (30, 0), (80, 40), (-40, 9), (0, -40)])
 @pytest.mark.parametrize("hq,hkv,dim", [(10, 2, 128), (6, 1, 256), (4, 4, 64), (2, 2, 128), (1, 1, 256), (40, 2, 64), (40, 1, 128)])
 def test_a_finite_row_that_a_node_does_not_see_does_not_reach_it(hq, hkv, dim, k_power, v_power, prefix):
     """A draft whose rows have other scales than all others: bit for bit what its neighbours get beside an ordinary one."""
@@ -109,3 +109,12 @@ def test_a_finite_row_that_a_node_does_not_see_does_not_reach_it(hq, hkv, dim, k
         got = gqa_tree_decode(q, k, v, torch.tensor([prefix], **INT), prefix, parents=parents, k_scales=ks, v_scales=vs, round_to_bfloat16=False)
     for node in (0, 2, 4, 5, 6):
         assert torch.equal(got[0, node], clean[0, node]), node
+
+
+@pytest.mark.parametrize("prefix", [10, 700, 2500])
+@pytest.mark.parametrize("powers", [[119], [100], [119, 112], [118, -90], [60, -60]])
+@pytest.mark.parametrize("nodes,hq,hkv,dim", SHAPES)
+def test_the_largest_scales_keep_small_weights(nodes, hq, hkv, dim, powers, prefix):
+    """Weights over six powers of e, which add up to more than the largest does."""
+    q, k, v, ks, vs, parents = case(nodes, hq, hkv, dim, prefix, powers, nodes + prefix, spread=2.0)
+    hold_to_the_model(q, k, v, ks, vs, prefix, parents, at_least=0.3)
