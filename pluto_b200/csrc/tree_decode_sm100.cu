@@ -45,6 +45,7 @@ constexpr int kUnitTiles = 3;        // query load and read-out of a unit, in ti
 constexpr float kRescale = 8.0f;     // O is rescaled when the maximum has grown by more than 2^8
 constexpr float kSmallest = -118.0f;   // exponent of the value rows from which smaller ones are taken for as large: weights of up
                                        // to 2^8 times 2^118 stay finite
+constexpr float kLargeScore = 1048576.0f;   // scores (in powers of two) whose own rounding is less than 2^-4
 constexpr float kApart = 60.0f;        // exponents between value rows beyond which the smaller ones' weights are zero in fp16, far
                                        // from where their sum would lose them
 
@@ -677,23 +678,38 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(const _
             uint32_t s[32];
             tmem_ld32(s_at + h * 32, s);
             tmem_wait_ld();
-            if (scaled & kKeysScaled) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) * lds_f32(k_factor + (h * 32 + i) * 4));
-            }
-            if (behind > -kTile) {
-              const uint32_t bits = static_cast<uint32_t>(seen >> (h * 32));
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (!(bits >> i & 1u)) s[i] = 0xff800000u;
-            }
             // The weights are taken relative to the maximum so far, so that their way does not lead through this one's; where it
             // has grown too far, the half is done again.
-            float mx[4] = {m_true, -INFINITY, -INFINITY, -INFINITY};
+            const auto take_maximum = [&]() {
+              float mx[4] = {m_true, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
-            m_true = max3(mx[0], mx[1], fmaxf(mx[2], mx[3]));
-            const float reference = (m_used == -INFINITY ? 0.0f : m_used * row_scale) + shift;   // (nothing seen yet: any)
+              for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+              m_true = max3(mx[0], mx[1], fmaxf(mx[2], mx[3]));
+            };
+            float reference = m_used == -INFINITY ? 0.0f : m_used * row_scale;   // (nothing seen yet: any)
+            const bool large = fabsf(reference) > kLargeScore;                   // its rounding would be an exponent
+            // (one branch: a warp's way through its tile is what this form waits for)
+            if ((scaled & kKeysScaled) != 0 || behind > -kTile || large) {
+              if (scaled & kKeysScaled) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) * lds_f32(k_factor + (h * 32 + i) * 4));
+              }
+              if (behind > -kTile) {
+                const uint32_t bits = static_cast<uint32_t>(seen >> (h * 32));
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                  if (!(bits >> i & 1u)) s[i] = 0xff800000u;
+              }
+              take_maximum();
+              if (large) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) - m_used);
+                reference = 0.0f;
+              }
+            } else {
+              take_maximum();
+            }
+            reference += shift;
             const uint64_t scale2 = f2_pack(row_scale, row_scale), neg2 = f2_pack(-reference, -reference);
             uint64_t sum2[2] = {0ull, 0ull};
             uint32_t packed[16];
@@ -712,36 +728,38 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(const _
               }
             }
             const bool grow = (m_true - m_used) * row_scale > kRescale;
-            if (__any_sync(0xffffffffu, grow || v_tile > v_used)) {
-              const float less = grow ? (m_used - m_true) * row_scale : 0.0f, factor = fast_exp2(less + (v_used - v_tile));
-              if (grow) m_used = m_true;
-              v_used = v_tile;
-              l *= kEight ? fast_exp2(less) : factor;
-              if (u > 0 || h == 1) {
-                // every product into this O must have ended: the first half's, or the previous tile's second
-                ok = __all_sync(0xffffffffu, tree_wait(h ? &sh->pv_half[x][buffer] : &sh->pv_done[x][buffer_of(t - 1)], phase_of(h ? t : t - 1), status, 57));
-                if (!ok) break;
-                tc_fence_after();
+            if (__any_sync(0xffffffffu, grow || v_tile > v_used || apart)) {
+              if (!kEight || __any_sync(0xffffffffu, grow || v_tile > v_used)) {
+                const float less = grow ? (m_used - m_true) * row_scale : 0.0f, factor = fast_exp2(less + (v_used - v_tile));
+                if (grow) m_used = m_true;
+                v_used = v_tile;
+                l *= kEight ? fast_exp2(less) : factor;
+                if (u > 0 || h == 1) {
+                  // every product into this O must have ended: the first half's, or the previous tile's second
+                  ok = __all_sync(0xffffffffu, tree_wait(h ? &sh->pv_half[x][buffer] : &sh->pv_done[x][buffer_of(t - 1)], phase_of(h ? t : t - 1), status, 57));
+                  if (!ok) break;
+                  tc_fence_after();
 #pragma unroll 1
-                for (int c = 0; c < D / 16; ++c) {
-                  uint32_t o[16];
-                  const uint32_t o_at = lanes + x * kColO1 + c * 16;
-                  tmem_ld16(o_at, o);
-                  tmem_wait_ld();
+                  for (int c = 0; c < D / 16; ++c) {
+                    uint32_t o[16];
+                    const uint32_t o_at = lanes + x * kColO1 + c * 16;
+                    tmem_ld16(o_at, o);
+                    tmem_wait_ld();
 #pragma unroll
-                  for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
-                  tmem_st16(o_at, o);
+                    for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
+                    tmem_st16(o_at, o);
+                  }
+                  tmem_wait_st();
                 }
-                tmem_wait_st();
+                --h;
+                continue;
               }
-              --h;
-              continue;
-            }
-            if (apart) {
-              const float down = scaled & kValuesScaled ? power_of_two(-v_tile) : 0.0f;   // (beyond 1: rows with weights of zero)
+              if (apart) {
+                const float down = scaled & kValuesScaled ? power_of_two(-v_tile) : 0.0f;   // (beyond 1: rows with weights of zero)
 #pragma unroll
-              for (int i = 0; i < 32; ++i)
-                s[i] = __float_as_uint(__uint_as_float(s[i]) * (scaled & kValuesScaled ? fminf(lds_f32(v_factor + (h * 32 + i) * 4) * down, 1.0f) : 0.0f));
+                for (int i = 0; i < 32; ++i)
+                  s[i] = __float_as_uint(__uint_as_float(s[i]) * (scaled & kValuesScaled ? fminf(lds_f32(v_factor + (h * 32 + i) * 4) * down, 1.0f) : 0.0f));
+              }
             }
             if (kEight) {
 #pragma unroll
