@@ -164,8 +164,6 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, kEight>) tree_decode_mma
         report_status(status, 48, kBadPage);   // (a slot past the pages was reported as such before)
         page = -1;                             // the copies read zeros there
       }
-      // One page per sequence may end inside a step: the copies read zeros behind it, and no scale is read there.
-      if (inside + min(kTile, load_end - tile * kTile) > a.pool.page_size) report_status(status, 48, kBadLength);
       if (lane == 0) {
         const uint32_t to = ring + slot_now * kStageBytes<D, kEight>;
         constexpr int kSlabs = kBytes == 64 ? 1 : kBytes / 128, kColumns = D / kSlabs, kSlab = kTile * kBytes / kSlabs;
@@ -178,7 +176,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, kEight>) tree_decode_mma
       }
       if (kEight) {
         const int row = lane % kTile;
-        const bool there = page >= 0 && tile * kTile + row < load_end && inside + row < a.pool.page_size;
+        const bool there = page >= 0 && tile * kTile + row < load_end;
         const uint8_t* byte = scales + load_head;
         if (there) byte += static_cast<uint64_t>(static_cast<uint32_t>(page)) * scale_page + static_cast<uint64_t>(static_cast<uint32_t>(inside + row)) * scale_token;
         const uintptr_t at = reinterpret_cast<uintptr_t>(byte);
@@ -205,6 +203,10 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<D, kEight>) tree_decode_mma
       load_b = load.b;
       load_head = load.kv_head;
       load_end = load.prefix + load.count;
+      if (blocks == 1u && load_end > a.pool.page_size) {   // the only page may end inside a step: the copies read zeros behind it,
+        report_status(status, 48, kBadLength);             // and no scale is read there
+        load_end = a.pool.page_size;
+      }
       if (!more) return;
       load_rows = load.rows;
     }
