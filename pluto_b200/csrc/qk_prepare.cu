@@ -160,8 +160,8 @@ __global__ void __launch_bounds__(256) draft_prepare_kernel(DraftPrepareArgs d) 
     __syncthreads();
     if (threadIdx.x == 0) {
       int n = 0;
-      for (int i = t, up; (up = parents[i]) >= 0; i = up, ++n)
-        if (up >= i) {   // taken as a first token
+      for (int i = t, up; (up = parents[i]) != -1; i = up, ++n)
+        if (up < -1 || up >= i) {   // taken as a first token
           report_status(d.pool.status, 46, kBadDraft);
           break;
         }
