@@ -788,7 +788,7 @@ def draft_prepare(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_norm: tor
     """Norm and rotation of drafted tokens and the append of their K/V rows: q [B,N,Hq,D] (any token and head
     strides), k, v [B,N,Hkv,D].  Node i of sequence b is rotated for position prefix_lens[b] + its depth and its
     rows go to slot prefix_lens[b] + i of a pool of any storage type.  Returns the queries [B,N,Hq,D], bf16
-    when round_to_bfloat16 and fp32 otherwise.  Without `parents` (a chain, or a whole prompt) any N."""
+    when round_to_bfloat16 and fp32 otherwise; with `counts` those of the nodes from counts[b] on are zeros.  Without `parents` (a chain, or a whole prompt) any N."""
     (B, N, Hq, D), device = q.shape, _device_index()
     L = _draft_calls()
     cache, scales = L.draft_pool(k_pool, v_pool, block_table, k_scales, v_scales, B, device)
@@ -804,7 +804,8 @@ def draft_prepare(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_norm: tor
     for norm in (q_norm, k_norm):
         if norm.dtype != torch.float32 or norm.numel() != D or norm.get_device() != device or not norm.is_contiguous():
             raise _invalid("Qwen attention norms must be FP32 head-width parameters on its Executor")
-    out = torch.empty((B, N, Hq, D), dtype=torch.bfloat16 if round_to_bfloat16 else torch.float32, device=q.device)
+    new = torch.empty if counts is None else torch.zeros
+    out = new((B, N, Hq, D), dtype=torch.bfloat16 if round_to_bfloat16 else torch.float32, device=q.device)
     check(L.pluto_draft_prepare(
         _stream(), q.data_ptr(), k.data_ptr(), v.data_ptr(), _dt(q), strides[1], strides[2], q_norm.data_ptr(), k_norm.data_ptr(),
         L.int32_address(prefix_lens, device, "prefix lengths", B), L.int32_address(parents, device, "parents", B, N),

@@ -28,3 +28,14 @@ def test_parents_out_of_range_are_reported_and_taken_as_first_tokens(bad):
     assert _capi.kernel_status() == 0
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+def test_queries_of_nodes_that_a_sequence_does_not_have_are_zeros():
+    want = prepare(None)[0]
+    torch.use_deterministic_algorithms(True)   # (new memory then holds NaN)
+    try:
+        got = prepare(None, counts=[4, 1])[0]
+    finally:
+        torch.use_deterministic_algorithms(False)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1, :1], want[1, :1]) and not got[1, 1:].any()
+    assert _capi.kernel_status() == 0
