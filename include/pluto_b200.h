@@ -441,8 +441,10 @@ int pluto_draft_prepare(pluto_stream_t stream, const void* q_in, const void* k_i
  *                [batch, nodes, q_heads]
  *   workspace    >= pluto_gqa_tree_decode_workspace_bytes(...) bytes, 16-byte aligned; overwritten, so calls that
  *                share one are ordered on one stream
- * What a node does not see does not reach its output, whatever it holds; a node that sees a row with an
- * infinity or a NaN gets NaN.
+ * What a node does not see does not reach its output, whatever it holds.  What it sees: 8-bit rows that held an
+ * infinity or a NaN make it NaN.  In bf16 and fp32 caches a key row gives a score as IEEE arithmetic has it; -infinity is a
+ * weight of 0 (a query with no other score gets zeros and an lse of -infinity), +infinity and NaN make the result NaN.
+ * A value row leaves nothing finite in the channels that are not (drafts: possibly in no channel).
  * bf16 queries with a bf16 result over a bf16 or 8-bit cache, head_dim 64, 128 or 256, rows on 16-byte boundaries, run on
  * the tensor cores; everything else in fp32 arithmetic.  On the tensor cores sums are in fp32 and what enters a product
  * is exact but for the softmax weights:

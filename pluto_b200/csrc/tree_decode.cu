@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(kWarps * 32) tree_decode_exact_kernel(TreeArgs
   for (int d = threadIdx.x; d < D; d += kWarps * 32) {
     float sum = 0.0f;
     for (int w = 0; w < kWarps; ++w) sum += acc_of[w][d] * expf(ml_of[w][0] - m_safe);
-    float value = sum / l_all;
+    float value = l_all == 0.0f ? 0.0f : sum / l_all;   // (nothing but scores of -infinity)
     value = tree_output(a, static_cast<size_t>(b) * a.nodes + node, head, d, value);
     if (a.out_is_bf16) static_cast<__nv_bfloat16*>(a.out)[row * D + d] = __float2bfloat16_rn(value);
     else static_cast<float*>(a.out)[row * D + d] = value;
