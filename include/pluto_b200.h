@@ -446,8 +446,9 @@ int pluto_draft_prepare(pluto_stream_t stream, const void* q_in, const void* k_i
  * weight of 0 (a query with no other score gets zeros and an lse of -infinity), +infinity and NaN make the result NaN.
  * A value row leaves nothing finite in the channels that are not (drafts: possibly in no channel).
  * bf16 queries with a bf16 result over a bf16 or 8-bit cache, head_dim 64, 128 or 256, rows on 16-byte boundaries, run on
- * the tensor cores; everything else in fp32 arithmetic.  On the tensor cores sums are in fp32 and what enters a product
- * is exact but for the softmax weights:
+ * the tensor cores; everything else in fp32 arithmetic.  On the tensor cores sums over keys stay in their fp32 accumulators, which
+ * truncate (about 2e-8 of a result per 16 keys that a worker adds up), and what enters a product is exact but for the softmax
+ * weights:
  *   bf16 cache   few rows (nodes * q_heads / kv_heads <= 16, at width 256 <= 8; pages that 16 divides, or one page per
  *                sequence): weights to 16 bits; more rows, or other pages: to bf16
  *   8-bit cache  weights to fp16, relative to the largest scale 2^n among the value rows that a query sees (2^-118 where

@@ -21,8 +21,8 @@
 // scores with the reference of their rows by itself: the maximum is reduced over lanes only when one has to move.
 //
 // Measured (B200, 16 sequences of 8000 tokens, 40 and 8 heads of 128, one token): bf16 90 us, 5.8 TB/s of cache; 8-bit
-// 56 us, 4.7 TB/s, bound by the issue of its instructions (47 % of the cycles with three warps per scheduler).  Four CTAs
-// per SM at 128 registers took 60.
+// 56 us, 4.7 TB/s.  There, three warps per scheduler issue in half of the cycles, the rest are fixed latencies between dependent
+// instructions, and DRAM stands at 61 %.  Four CTAs per SM at 128 registers took 60.
 #include "tree_line.cuh"
 
 namespace pluto {
@@ -598,6 +598,10 @@ cudaError_t launch(cudaStream_t stream, const TreeArgs& a) {
 
 }  // namespace
 
+// Up to sixteen rows, the columns of two products (eight at width 256, whose accumulators fill the registers then), in pages
+// that a step divides.  16 x 8000 tokens, bf16 and 8-bit, us here against tree_decode_sm100: width 128, 1 row 87 : 105 and
+// 54 : 134, 8 rows 91 : 107 and 58 : 136, 16 rows 98 : 107 and 79 : 136; width 256, 6 rows 92 : 91 and 62 : 110; 24 x 4000, width 64,
+// 16 rows 68 : 116 and 65 : 144.  Other pages (of 24) leave 5 rows of width 128 to the latter: 117 and 136 against 90 and 56.
 bool tree_decode_mma_supported(const TreeArgs& a) {
   return a.nodes * a.group <= (a.dim == 256 ? 8 : 16) && tree_pool_fits(a, kTile) &&
          a.pool.scale_page < (1ull << 32) && a.pool.scale_token < (1ull << 32) &&

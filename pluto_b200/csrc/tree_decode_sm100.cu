@@ -27,9 +27,9 @@
 //
 // Work is cut evenly over the SMs as tree_line.cuh says, one CTA per SM.
 //
-// Measured (B200, 16 sequences of 8000 tokens, 40 and 8 heads of 128): 40 rows per KV head, bf16 102 us, 5.1 TB/s of
-// cache, 8-bit 136; 100 rows 114 and 147; 305 rows 300 and 402, where the softmax bounds it: one warp's chain of loads,
-// maxima, exponentials and stores, two such warps per scheduler.
+// Measured (B200, 16 sequences of 8000 tokens, 40 and 8 heads of 128, with the merge): 40 rows per KV head, bf16 113 us, 8-bit
+// 140; 100 rows 125 and 151; 305 rows 294 and 395, where the softmax bounds it: one warp's chain of loads, maxima, exponentials and
+// stores, two such warps per scheduler.  Up to 128 rows the 8-bit form is the slower one: its codes pass shared memory twice.
 #include <stddef.h>
 
 #include "tree_line.cuh"

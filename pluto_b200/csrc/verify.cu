@@ -13,16 +13,17 @@
 // from; where nothing is left of it, the target's row itself; -1 where that row's sum is not positive and finite.
 //
 // Comparisons and sums are in double: products of two fp32 numbers are exact there, and sums of a row agree
-// to 1e-16 in any order, so the tokens do not depend on how the row was cut.
+// to 1e-16 in any order, so the token does not depend on how the row was cut (by the batch) unless a running sum comes that
+// close to the threshold.
 //
 // The tests of all nodes are independent given the p of the drafted tokens, so a thread takes a node and only
 // the walk along the accepted path is serial.  What costs is the one row the last token is drawn from (two with
 // `draft`): a cluster of CTAs shares it, a warp per contiguous chunk, and the chunks' sums meet in distributed shared
 // memory.  The CTA whose chunk holds the threshold cuts that chunk over its threads and looks for the token, by sums
 // over threads first.  A pass of the serial parts (tests, walk, scans, two barriers of the cluster) takes longer than
-// the row, so eight CTAs share it only while all clusters are resident at once, else four.  64 chains of 8, 131071
-// tokens: 22 us (76 with eight CTAs in two waves and the sums added one by one), 3.0 TB/s of the two rows; one chain of
-// 5, 50257 tokens: 6.7 us.
+// the row, so eight CTAs share it only while all clusters are resident at once, else four.  Chains of 8, 131071 tokens, us with
+// eight against four: 1 chain 8.6 : 11.7, 32 chains 12.4 : 12.8, 38 17.6 : 17.3, 64 25 : 20, 128 53 : 42.  64 chains are 3.3 TB/s of
+// the two rows; one chain of 5, 50257 tokens: 7.0 us.
 #include "common.cuh"
 #include "engine.h"
 
