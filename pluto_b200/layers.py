@@ -450,6 +450,7 @@ class KeyValueCache:
 def kv_layout(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: Optional[torch.Tensor],
               page_size: int, page_stride: int, token_stride: int) -> "_capi.KvCacheStruct":
     _wide_cache(k_pool)
+    _table_columns(block_table)
     s = _capi.KvCacheStruct()
     s.k_base, s.v_base = k_pool.data_ptr(), v_pool.data_ptr()
     s.block_table = None if block_table is None else block_table.data_ptr()
@@ -465,9 +466,16 @@ def _wide_cache(pool: torch.Tensor) -> None:
         raise _unimplemented("an 8-bit cache is attended with gqa_tree_decode and CachedAttentionStep")
 
 
+def _table_columns(block_table: Optional[torch.Tensor]) -> None:
+    """A table without columns has no address, which would pass for no table at all."""
+    if block_table is not None and block_table.shape[1] < 1:
+        raise _invalid("a block table is [batch, blocks], of one block or more")
+
+
 def _pack_cache(k_pool, v_pool, block_table, page_size, page_stride, token_stride) -> bytes:
     """kv_layout as the bytes the vectorcall binding takes."""
     _wide_cache(k_pool)
+    _table_columns(block_table)
     return _capi.fast().kv_cache(k_pool.data_ptr(), v_pool.data_ptr(),
                                  None if block_table is None else block_table.data_ptr(),
                                  0 if block_table is None else block_table.shape[1], page_size, page_stride,

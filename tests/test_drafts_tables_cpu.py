@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from pluto_b200 import PlutoStatusError
-from pluto_b200.layers import _draft_calls
+from pluto_b200.layers import _draft_calls, gqa_decode, kv_layout
 
 
 def pool_of(pages, table, batch, dtype=torch.bfloat16):
@@ -29,3 +29,12 @@ def test_tables_of_other_shapes(engine):
     assert scales is None and len(cache) > 0
     with pytest.raises(PlutoStatusError, match="a page for every sequence"):
         pool_of(1, None, 2)
+
+
+def test_the_other_paged_functions_refuse_such_a_table_too(engine):
+    k, table = torch.zeros(1, 16, 2, 64, dtype=torch.bfloat16), torch.zeros(4, 0, dtype=torch.int32)
+    q, lengths = torch.zeros(4, 4, 64, dtype=torch.bfloat16), torch.ones(4, dtype=torch.int32)
+    with pytest.raises(PlutoStatusError, match="block table"):
+        kv_layout(k, k, table, 16, 2048, 128)
+    with pytest.raises(PlutoStatusError, match="block table"):
+        gqa_decode(q, k, k, lengths, 16, block_table=table)
