@@ -28,7 +28,7 @@
 // Work is cut evenly over the SMs as tree_line.cuh says, one CTA per SM.
 //
 // Measured (B200, 16 sequences of 8000 tokens, 40 and 8 heads of 128, with the merge): 40 rows per KV head, bf16 113 us, 8-bit
-// 140; 100 rows 125 and 151; 305 rows 294 and 395, where the softmax bounds it: one warp's chain of loads, maxima, exponentials and
+// 141; 100 rows 125 and 152; 305 rows 296 and 407, where the softmax bounds it: one warp's chain of loads, maxima, exponentials and
 // stores, two such warps per scheduler.  Up to 128 rows the 8-bit form is the slower one: its codes pass shared memory twice.
 #include <stddef.h>
 
@@ -97,6 +97,7 @@ struct Shared {
   alignas(16) float k_factor[3 * kTiles][kTile];   // (read four at a time)
   float v_factor[3 * kTiles][kTile];
   int scaled[3 * kTiles], v_largest[3 * kTiles];   // scaled: kKeysScaled, kValuesScaled
+  uint32_t v_top[3 * kTiles][2];                   // the rows that have it
 };
 
 // The next segment of the range, by every lane of a warp; false at its end (or when a wait ran out).
@@ -332,7 +333,9 @@ __device__ __forceinline__ void widen_tiles(Shared<D, true, kWide>* sh, uint32_t
 #pragma unroll
       for (int o = 0; o < 2; ++o) {
         if (!k_fits) sh->k_factor[scale_slot][lane + 32 * o] = k[o] == 255u ? 1.0f : e8m0_value(k[o]);
-        if (!v_fits) sh->v_factor[scale_slot][lane + 32 * o] = v[o] == 255u ? 1.0f : e8m0_value(v[o]);
+        sh->v_factor[scale_slot][lane + 32 * o] = v_fits || v[o] == 255u ? 1.0f : e8m0_value(v[o]);
+        const unsigned at_top = __ballot_sync(0xffffffffu, v[o] == top);
+        if (lane == 0) sh->v_top[scale_slot][o] = at_top;
       }
       if (lane == 0) {
         sh->scaled[scale_slot] = (k_fits ? 0 : kKeysScaled) | (v_fits ? 0 : kValuesScaled);
@@ -655,13 +658,16 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(const _
                                : seen_lo << -behind | ((1ull << -behind) - 1);
         float v_largest = kEight ? static_cast<float>(sh->v_largest[slot]) : 0.0f;
         if (kEight && behind > -kTile && v_largest > v_used && warp_live) {   // of the drafts' tiles only rows that this one sees count
-          uint32_t most = 0u;
-#pragma unroll 4
-          for (int i = 0; i < kTile; ++i) {
-            const uint32_t factor = __float_as_uint(lds_f32(v_factor + i * 4));
-            if (seen >> i & 1u) most = max(most, factor);
+          if (((static_cast<uint32_t>(seen) & sh->v_top[slot][0]) | (static_cast<uint32_t>(seen >> 32) & sh->v_top[slot][1])) == 0u) {
+            uint32_t most = 0u;
+#pragma unroll 2
+            for (int i = 0; i < kTile; i += 4) {
+              const uint4 factor = lds_b32x4(v_factor + i * 4);
+              const uint32_t bits = static_cast<uint32_t>(seen >> i);
+              most = max(max(most, bits & 1u ? factor.x : 0u), max(bits & 2u ? factor.y : 0u, max(bits & 4u ? factor.z : 0u, bits & 8u ? factor.w : 0u)));
+            }
+            v_largest = static_cast<float>(static_cast<int>(most >> 23) - 127);
           }
-          v_largest = static_cast<float>(static_cast<int>(most >> 23) - 127);
         }
         const float v_tile = fmaxf(v_used, v_largest);
         // Whole tiles' weights are taken times 2^-below; where nothing of that would be left in fp16, or the rows differ, the
@@ -755,10 +761,15 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(const _
                 continue;
               }
               if (apart) {
-                const float down = scaled & kValuesScaled ? power_of_two(-v_tile) : 0.0f;   // (beyond 1: rows with weights of zero)
+                const float down = scaled & kValuesScaled ? power_of_two(-v_tile) : 0.0f;
 #pragma unroll
-                for (int i = 0; i < 32; ++i)
-                  s[i] = __float_as_uint(__uint_as_float(s[i]) * (scaled & kValuesScaled ? fminf(lds_f32(v_factor + (h * 32 + i) * 4) * down, 1.0f) : 0.0f));
+                for (int i = 0; i < 32; i += 4) {
+                  const uint4 factor = lds_b32x4(v_factor + (h * 32 + i) * 4);
+                  s[i] = __float_as_uint(__uint_as_float(s[i]) * down * __uint_as_float(factor.x));
+                  s[i + 1] = __float_as_uint(__uint_as_float(s[i + 1]) * down * __uint_as_float(factor.y));
+                  s[i + 2] = __float_as_uint(__uint_as_float(s[i + 2]) * down * __uint_as_float(factor.z));
+                  s[i + 3] = __float_as_uint(__uint_as_float(s[i + 3]) * down * __uint_as_float(factor.w));
+                }
               }
             }
             if (kEight) {
@@ -819,7 +830,13 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(const _
       if (warp_live) {
         const int slot = 2 * blockIdx.x + seg.slot;
         const float drop = kEight && !seg.whole ? part_drop(l) : 0.0f;
-        const float inverse = seg.whole ? (l == 0.0f ? 0.0f : 1.0f / l) : power_of_two(-drop), up = kEight ? exp2f(v) : 1.0f;
+        float inverse = seg.whole ? (l == 0.0f ? 0.0f : 1.0f / l) : power_of_two(-drop);
+        if (kEight) {   // O's unit, with either factor: beside small values the product of both might not be a normal number
+          const float unit = exp2f(v);
+          f0 *= v < -60.0f ? unit : 1.0f;
+          f1 *= v < -60.0f ? unit : 1.0f;
+          inverse *= v < -60.0f ? 1.0f : unit;
+        }
         float* acc = parts.acc + (static_cast<size_t>(slot) * parts.rows + own_row) * D;
         const int c0 = merged ? x * (D / 32) : 0, c1 = merged ? c0 + D / 32 : D / 16;
 #pragma unroll 1
@@ -834,6 +851,10 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(const _
             for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f0 + __uint_as_float(o2[i]) * f1);
           } else {
             tmem_wait_ld();
+            if (kEight) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f0);
+            }
           }
           if (!live) {
             // (a lane without a row only takes part in the reads)
@@ -842,13 +863,13 @@ __global__ void __launch_bounds__(kThreads<kEight>, 1) tree_decode_sm100(const _
             for (int h = 0; h < 2; ++h) {
               float v[8];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) v[i] = kEight ? __uint_as_float(o[8 * h + i]) * inverse * up : __uint_as_float(o[8 * h + i]) * inverse;
+              for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(o[8 * h + i]) * inverse;
               store_out8(a, token, head, c * 16 + 8 * h, v, gate_pieces);
             }
           } else {
             if (kEight) {
 #pragma unroll
-              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * inverse * up);
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * inverse);
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i)
